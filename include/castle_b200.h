@@ -32,7 +32,7 @@ extern "C" {
 enum { CASTLE_BF16 = 0, CASTLE_F16 = 1, CASTLE_F32 = 2 };
 
 /* status-word bits written by kernels */
-enum { CASTLE_STATUS_OK = 0, CASTLE_STATUS_WAIT_TIMEOUT = 1, CASTLE_STATUS_BAD_LAUNCH = 2 };
+enum { CASTLE_STATUS_OK = 0, CASTLE_STATUS_WAIT_TIMEOUT = 1, CASTLE_STATUS_BAD_LAUNCH = 2, CASTLE_STATUS_BAD_INDEX = 4 };
 
 typedef struct {
   void* ptr;
@@ -145,6 +145,33 @@ int castle_rmsnorm_fwd(int32_t dtype, int64_t rows, int32_t dim, const void* x, 
 size_t castle_rmsnorm_bwd_workspace_bytes(int64_t rows, int32_t dim);
 int castle_rmsnorm_bwd(int32_t dtype, int64_t rows, int32_t dim, const void* dy, const void* x, const void* weight,
                        const float* rstd, void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- layer norm ---------------------------------------------------------------------------------
+ * y = (x - mean) * rsqrt(var + eps) * weight + bias over rows of `dim` elements (any number), row_stride elements apart; weight
+ * and bias may be NULL (one, zero); y contiguous; all of `dtype`, sums in fp32.  `stats` (fp32, rows x 2, may be NULL) gets each
+ * row's mean and 1 / standard deviation, which the backward takes.  Backward: dx (rows x dim, contiguous), dweight and dbias (dim),
+ * each NULL if not wanted; the last two need the workspace, and are the same from call to call.
+ */
+int castle_layernorm_fwd(int32_t dtype, int64_t rows, int32_t dim, const void* x, int64_t row_stride, const void* weight,
+                         const void* bias, float eps, void* y, float* stats, void* stream);
+size_t castle_layernorm_bwd_workspace_bytes(int64_t rows, int32_t dim);
+int castle_layernorm_bwd(int32_t dtype, int64_t rows, int32_t dim, const void* dy, int64_t dy_stride, const void* x,
+                         int64_t row_stride, const void* weight, const float* stats, void* dx, void* dweight, void* dbias,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- token lookup (the input of the model that the reference trains: token embedding of train_triton.py:73-175) -----
+ * y[i] = scale * weight[index[i]] for `tokens` indices of index_bytes (4 or 8) each; weight: `vocab` rows of `dim` elements,
+ * row_stride elements apart; y contiguous.  An index outside the table gives a row of NaN and sets CASTLE_STATUS_BAD_INDEX.
+ * Backward: dweight (vocab x dim, contiguous, every row written) = scale * the sum of each row's dy in the order of the
+ * positions, in fp32; indices equal to padding_idx (-1: none) and those outside the table are left out, the latter set
+ * CASTLE_STATUS_BAD_INDEX.
+ */
+int castle_embedding_fwd(int32_t dtype, int32_t index_bytes, int64_t tokens, int64_t vocab, int32_t dim, const void* index,
+                         const void* weight, int64_t row_stride, float scale, void* y, int32_t* status, void* stream);
+size_t castle_embedding_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int32_t dim);
+int castle_embedding_bwd(int32_t dtype, int32_t index_bytes, int64_t tokens, int64_t vocab, int32_t dim, const void* index,
+                         int64_t padding_idx, const void* dy, int64_t dy_stride, float scale, void* dweight, void* workspace,
+                         size_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---- parallel backward ---------------------------------------------------
  * Replaces CastleAttentionFunction.backward

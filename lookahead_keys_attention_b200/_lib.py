@@ -15,7 +15,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libcastle_b200.so"
-SOURCES = ["api.cu", "decode.cu", "selftest.cu", "convert.cu", "transform.cu", "token_linear.cu", "token_layer.cu", "linear.cu", "norm.cu", "fwd.cu", "bwd.cu", "bwd128.cu"]
+SOURCES = ["api.cu", "decode.cu", "selftest.cu", "convert.cu", "transform.cu", "token_linear.cu", "token_layer.cu", "linear.cu", "norm.cu", "layernorm.cu", "embedding.cu", "fwd.cu", "bwd.cu", "bwd128.cu"]
 
 BF16, F16, F32 = 0, 1, 2
 
@@ -52,6 +52,7 @@ STAMP_PATH = PKG_DIR / "libcastle_b200.so.stamp"
 HOST_PATH = PKG_DIR / "_host.so"
 HOST_STAMP_PATH = PKG_DIR / "_host.so.stamp"
 HOST_SOURCE = CSRC / "host.cpp"
+HOST_PARTS = [HOST_SOURCE, CSRC / "host_lm.h"]
 
 
 def _deps():
@@ -94,7 +95,7 @@ def _host_hash() -> str:
     import sys
     import torch
     h = hashlib.sha256(f"{torch.__version__} {sys.version}".encode())
-    for d in (HOST_SOURCE, PKG_DIR.parent / "include" / "castle_b200.h"):
+    for d in (*HOST_PARTS, PKG_DIR.parent / "include" / "castle_b200.h"):
         h.update(d.read_bytes())
     return h.hexdigest()
 
@@ -184,6 +185,13 @@ _SIGNATURES = {
     "castle_rmsnorm_fwd": (ctypes.c_int, [_i32, ctypes.c_int64, _i32, _vp, _vp, ctypes.c_float, _vp, _vp, _vp]),
     "castle_rmsnorm_bwd_workspace_bytes": (_sz, [ctypes.c_int64, _i32]),
     "castle_rmsnorm_bwd": (ctypes.c_int, [_i32, ctypes.c_int64, _i32] + [_vp] * 7 + [_sz, _vp]),
+    "castle_layernorm_fwd": (ctypes.c_int, [_i32, ctypes.c_int64, _i32, _vp, ctypes.c_int64, _vp, _vp, ctypes.c_float, _vp, _vp, _vp]),
+    "castle_layernorm_bwd_workspace_bytes": (_sz, [ctypes.c_int64, _i32]),
+    "castle_layernorm_bwd": (ctypes.c_int, [_i32, ctypes.c_int64, _i32] + [_vp, ctypes.c_int64] * 2 + [_vp] * 6 + [_sz, _vp]),
+    "castle_embedding_fwd": (ctypes.c_int, [_i32, _i32, ctypes.c_int64, ctypes.c_int64, _i32, _vp, _vp, ctypes.c_int64, ctypes.c_float, _vp, _vp, _vp]),
+    "castle_embedding_bwd_workspace_bytes": (_sz, [ctypes.c_int64, ctypes.c_int64, _i32]),
+    "castle_embedding_bwd": (ctypes.c_int, [_i32, _i32, ctypes.c_int64, ctypes.c_int64, _i32, _vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_float,
+                                            _vp, _vp, _sz, _vp, _vp]),
     "castle_bwd_workspace_bytes": (_sz, [_PR]),
     "castle_bwd": (ctypes.c_int, [_PR] + [_T] * 8 + [_vp, _vp] + [_T] * 6 + [_vp, _sz, _vp, _vp]),
     "castle_decode_workspace_bytes": (_sz, [_PR, _i32]),

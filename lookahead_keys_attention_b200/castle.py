@@ -4,7 +4,7 @@ arguments, state-dict keys (`to_all_qkv.weight`, `combine_heads.weight`,
 `norm.weight`), `forward(x, cache=None, return_next_cache=None)` conventions
 and `Cache` tuple.  The attention cores run as sm_100a kernels through the
 C-ABI library, rotary embedding included.  A plain layer is one native call
-(csrc/host.cpp): RMSNorm and the projections of a few tokens are kernels of this
+(csrc/host.cpp): the norm and the projections of a few tokens are kernels of this
 package, the other projections library products, and the gradient one autograd
 node.  Where a submodule was replaced, wrapped or hooked, or something records or
 replaces torch functions, the submodules are called as modules instead.
@@ -106,7 +106,10 @@ class Castle(nn.Module):
         # package's kernels in the place of Triton.  It selects nothing: there is one code path.
         self.use_triton = bool(use_triton) if use_triton is not None else torch.cuda.is_available()
         self.scale = dim_head ** -0.5
-        self.norm = nn.RMSNorm(dim) if prenorm else nn.Identity()
+        # prenorm: RMSNorm as in the reference, or "layer" for a layer norm.  (A layer norm that the caller puts in the place of
+        # another norm is called as a module.)
+        self._layer_norm = prenorm == "layer"
+        self.norm = nn.LayerNorm(dim) if self._layer_norm else nn.RMSNorm(dim) if prenorm else nn.Identity()
         self.rotary_emb = _Rotary(dim_head) if rotary_emb else None
         self.to_all_qkv = nn.Linear(dim, dim_inner * 6, bias=False)
         self.combine_heads = nn.Linear(dim_inner, dim, bias=False)
@@ -155,9 +158,9 @@ class Castle(nn.Module):
         return fresh
 
     def _plain_layer(self):
-        """What the native path takes of this layer: norm weight and eps, the two projection weights and the head
-        sizes; or None where a submodule was replaced, has a bias, hooks or a forward of its own (how offloading wraps
-        it), so that it must be called as a module."""
+        """What the native path takes of this layer: norm weight and eps, the two projection weights, the head sizes, whether
+        the norm is a layer norm, and its bias; or None where a submodule was replaced, has a bias (but the norm), hooks or a
+        forward of its own (how offloading wraps it), so that it must be called as a module."""
         mods = self._modules
         norm, qkv, combine = mods["norm"], mods["to_all_qkv"], mods["combine_heads"]
         if type(qkv) is not nn.Linear or type(combine) is not nn.Linear or _has_any_global_hook():
@@ -172,9 +175,12 @@ class Castle(nn.Module):
             if wq["bias"] is not None or wc["bias"] is not None:
                 return None
             if type(norm) is nn.Identity:
-                return None, None, wq["weight"], wc["weight"], self.heads, self.dim_head
+                return None, None, wq["weight"], wc["weight"], self.heads, self.dim_head, False, None
             if type(norm) is nn.RMSNorm and norm._parameters["weight"] is not None and len(norm.normalized_shape) == 1:
-                return norm._parameters["weight"], norm.eps, wq["weight"], wc["weight"], self.heads, self.dim_head
+                return norm._parameters["weight"], norm.eps, wq["weight"], wc["weight"], self.heads, self.dim_head, False, None
+            if getattr(self, "_layer_norm", False) and type(norm) is nn.LayerNorm and norm._parameters["weight"] is not None and len(norm.normalized_shape) == 1:
+                return (norm._parameters["weight"], norm.eps, wq["weight"], wc["weight"], self.heads, self.dim_head, True,
+                        norm._parameters["bias"])
         except KeyError:   # a data-parallel replica holds its weights as plain attributes
             pass
         return None

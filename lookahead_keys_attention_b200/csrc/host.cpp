@@ -67,6 +67,12 @@ struct Api {
   decltype(&castle_token_layer_fits) token_layer_fits;
   decltype(&castle_token_layer_workspace_bytes) token_layer_workspace_bytes;
   decltype(&castle_token_layer) token_layer;
+  decltype(&castle_layernorm_fwd) layernorm_fwd;
+  decltype(&castle_layernorm_bwd_workspace_bytes) layernorm_bwd_workspace_bytes;
+  decltype(&castle_layernorm_bwd) layernorm_bwd;
+  decltype(&castle_embedding_fwd) embedding_fwd;
+  decltype(&castle_embedding_bwd_workspace_bytes) embedding_bwd_workspace_bytes;
+  decltype(&castle_embedding_bwd) embedding_bwd;
 } api{};
 
 void check(int rc, const char* what) {
@@ -637,9 +643,12 @@ Tensor decode_step(const Tensor* news, const Tensor* caches, int64_t t, double s
   return decode_core(nd, caches, news[0].size(0), news[0].size(1), news[0].size(3), dtype, t, scale, Rotary{}, news[0].device());
 }
 
+#include "host_lm.h"
+
 // ------------------------------------------------------------------------------------------------ the plain module
 struct Layer {
-  Tensor norm, to_qkv, combine;   // norm may be undefined
+  Tensor norm, norm_bias, to_qkv, combine;   // norm and its bias may be undefined
+  bool layer_norm = false;                   // the norm is a layer norm, not RMSNorm
   std::optional<double> eps;
   int64_t heads = 0, dim_head = 0;
 };
@@ -654,7 +663,8 @@ bool plain_layer(const Tensor& x, const Layer& l) {
   const int64_t inner = l.heads * l.dim_head;
   return x.dim() == 3 && x.is_cuda() && x.numel() > 0 && x.layout() == at::kStrided && !x.is_neg() && !x.unsafeGetTensorImpl()->is_python_dispatch() && !has_tangent(x) &&
          dtype_code(x.scalar_type()) >= 0 && x.size(2) % 8 == 0 && plain(l.to_qkv) && plain(l.combine) &&
-         (!l.norm.defined() || (plain(l.norm) && l.norm.dim() == 1 && l.norm.size(0) == x.size(2))) && l.to_qkv.dim() == 2 &&
+         (!l.norm.defined() || (plain(l.norm) && l.norm.dim() == 1 && l.norm.size(0) == x.size(2))) &&
+         (!l.norm_bias.defined() || (plain(l.norm_bias) && l.norm_bias.dim() == 1 && l.norm_bias.size(0) == x.size(2))) && l.to_qkv.dim() == 2 &&
          l.to_qkv.size(0) == 6 * inner && l.to_qkv.size(1) == x.size(2) && l.combine.dim() == 2 && l.combine.size(1) == inner &&
          !at::autocast::is_autocast_enabled(at::kCUDA) && !c10::impl::dispatch_mode_enabled();
 }
@@ -699,7 +709,7 @@ Tensor product(int layout, const Tensor& a, const Tensor& b, int64_t rows) {
 // and the core) cost 250 us of host time per training step where the kernels of a small one take 120.
 struct LayerBackward : public Node {
   int64_t dim = 0;
-  bool has_norm = false, separate_h = false, separate_merged = false;
+  bool has_norm = false, layer_norm = false, has_bias = false, separate_h = false, separate_merged = false;
   at::ScalarType dtype = at::kFloat;
   std::vector<int64_t> x_sizes;
   // Like autograd over the single operations would, each kept only where a gradient that was asked for needs it, and
@@ -717,10 +727,11 @@ struct LayerBackward : public Node {
   }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
-    variable_list result(has_norm ? 4 : 3);
+    variable_list result(has_bias ? 5 : has_norm ? 4 : 3);
     if (grads.empty() || !grads[0].defined()) return result;
     const bool need_x = task_should_compute_output(0), need_qkv = task_should_compute_output(1), need_combine = task_should_compute_output(2),
-               need_norm = has_norm && task_should_compute_output(3);
+               need_weight = has_norm && task_should_compute_output(3), need_bias = has_bias && task_should_compute_output(4),
+               need_norm = need_weight || need_bias;
     const bool need_core = need_x || need_qkv || need_norm, need_out = need_combine && !separate_merged;
     const Problem& p = core.p;
     const int64_t rows = p.B * p.N, inner = p.H * p.d;
@@ -754,14 +765,19 @@ struct LayerBackward : public Node {
       return result;
     }
     const Tensor xc = aligned_contiguous(xs), wn = restored_contiguous(ws_norm, {dim}, dtype, dev),
-                 rs = restored_contiguous(rs_norm, {rows}, at::kFloat, dev);
+                 rs = layer_norm ? restored_contiguous(rs_norm, {rows, 2}, at::kFloat, dev) : restored_contiguous(rs_norm, {rows}, at::kFloat, dev);
     if (need_x) result[0] = at::empty(x_sizes, dh.options());
-    if (need_norm) result[3] = at::empty({dim}, dh.options());
+    if (need_weight) result[3] = at::empty({dim}, dh.options());
+    if (layer_norm) {
+      if (need_bias) result[4] = at::empty({dim}, dh.options());
+      launch_layernorm_bwd(as_rows(dh, rows, dim), xc.view({rows, dim}), wn, rs, result[0], result[3], has_bias ? result[4] : Tensor(), stream);
+      return result;
+    }
     const size_t bytes = api.rmsnorm_bwd_workspace_bytes(rows, (int32_t)dim);
     StreamUse use(stream);
     const Tensor ws = use.scratch(bytes);
     check(api.rmsnorm_bwd(dtype_code(dtype), rows, (int32_t)dim, dh.data_ptr(), xc.data_ptr(), wn.data_ptr(), rs.data_ptr<float>(),
-                          need_x ? result[0].data_ptr() : nullptr, need_norm ? result[3].data_ptr() : nullptr, ws.data_ptr(), ws.numel(),
+                          need_x ? result[0].data_ptr() : nullptr, need_weight ? result[3].data_ptr() : nullptr, ws.data_ptr(), ws.numel(),
                           stream.stream()), "castle_rmsnorm_bwd");
     return result;
   }
@@ -771,7 +787,7 @@ struct LayerBackward : public Node {
 Tensor layer_native(const Tensor& x, const Layer& l, Options o) {
   const bool grad = at::GradMode::is_enabled(), has_norm = l.norm.defined();
   const bool need_x = grad && x.requires_grad(), need_qkv = grad && l.to_qkv.requires_grad(), need_combine = grad && l.combine.requires_grad(),
-             need_norm = grad && has_norm && l.norm.requires_grad();
+             need_norm = grad && has_norm && (l.norm.requires_grad() || (l.norm_bias.defined() && l.norm_bias.requires_grad()));
   o.need_grad = need_x || need_qkv || need_norm;
   const int64_t B = x.size(0), N = x.size(1), dim = x.size(2), rows = B * N, inner = l.heads * l.dim_head;
   const Problem p = make_problem({B, l.heads, N, l.dim_head}, x.scalar_type(), o.long_seq);
@@ -786,9 +802,14 @@ Tensor layer_native(const Tensor& x, const Layer& l, Options o) {
     if (has_norm) {
       const Tensor src = aligned_contiguous(h);
       h = at::empty({rows, dim}, x.options().requires_grad(false));
+      if (l.layer_norm) {
+        if (o.need_grad) rstd = at::empty({rows, 2}, x.options().dtype(at::kFloat).requires_grad(false));   // mean and 1 / deviation
+        launch_layernorm(src, l.norm, l.norm_bias, *l.eps, h, rstd, stream);
+      } else {
       if (o.need_grad) rstd = at::empty({rows}, x.options().dtype(at::kFloat).requires_grad(false));
       check(api.rmsnorm_fwd(dtype_code(p.dtype), rows, (int32_t)dim, src.data_ptr(), l.norm.data_ptr(), norm_eps(l), h.data_ptr(),
                             o.need_grad ? rstd.data_ptr<float>() : nullptr, stream.stream()), "castle_rmsnorm_fwd");
+      }
     }
     const Tensor packed = product(0, h, l.to_qkv, rows).view({B, N, 6, l.heads, l.dim_head});
     Inputs in;
@@ -802,9 +823,12 @@ Tensor layer_native(const Tensor& x, const Layer& l, Options o) {
   auto node = std::shared_ptr<LayerBackward>(new LayerBackward(), torch::autograd::deleteNode);
   std::vector<Tensor> vars{x, l.to_qkv, l.combine};
   if (has_norm) vars.push_back(l.norm);
+  if (l.norm_bias.defined()) vars.push_back(l.norm_bias);
   node->set_next_edges(torch::autograd::collect_next_edges(vars));
   node->dim = dim;
   node->has_norm = has_norm;
+  node->layer_norm = l.layer_norm;
+  node->has_bias = l.norm_bias.defined();
   node->dtype = p.dtype;
   node->x_sizes = x.sizes().vec();
   torch::autograd::set_history(out, node);
@@ -829,7 +853,7 @@ Tensor layer_native(const Tensor& x, const Layer& l, Options o) {
 }
 
 Tensor project(const Tensor& x, const Layer& l) {   // (B, N, 6, H, d)
-  Tensor h = l.norm.defined() ? at::rms_norm(x, {x.size(-1)}, l.norm, l.eps) : x;
+  Tensor h = !l.norm.defined() ? x : l.layer_norm ? at::layer_norm(x, {x.size(-1)}, l.norm, l.norm_bias, *l.eps) : at::rms_norm(x, {x.size(-1)}, l.norm, l.eps);
   return at::linear(h, l.to_qkv).view({x.size(0), x.size(1), 6, l.heads, l.dim_head});
 }
 
@@ -937,10 +961,25 @@ Tensor token_layer(const Tensor& x, const Layer& l, const Tensor* caches, int64_
   return at::mm(o, l.combine.t()).view({B, 1, l.combine.size(0)});
 }
 
+// A layer norm is a launch ahead of the others (the RMSNorm is part of the token's projection).
+Tensor token_layer_normed(const Tensor& x, const Layer& l, const Tensor* caches, int64_t t, double scale, const Rotary& rotary) {
+  Layer rest = l;
+  rest.norm = rest.norm_bias = Tensor();
+  rest.layer_norm = false;
+  Tensor h;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard guard(x.device());
+    h = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+    launch_layernorm(as_rows(x, x.size(0), x.size(2)), l.norm, l.norm_bias, *l.eps, h, Tensor(), c10::cuda::getCurrentCUDAStream(x.device().index()));
+  }
+  return token_layer(h, rest, caches, t, scale, rotary);
+}
+
 Tensor layer_decode(const Tensor& x, const Layer& l, const Tensor* caches, int64_t t, double scale, const Rotary& rotary) {
   // no gradient flows through the cached step, so only the last projection could need a graph
   if (plain_layer(x, l) && x.size(1) == 1 && !(at::GradMode::is_enabled() && l.combine.requires_grad()))
-    return token_layer(x, l, caches, t, scale, rotary);
+    return l.layer_norm ? token_layer_normed(x, l, caches, t, scale, rotary) : token_layer(x, l, caches, t, scale, rotary);
   return at::linear(decode_packed(project(x, l), caches, t, scale, rotary), l.combine);
 }
 
@@ -1088,7 +1127,8 @@ PyObject* py_decode_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-Layer arg_layer(PyObject* const* a) {   // norm weight or None, eps or None, to_all_qkv weight, combine_heads weight, heads, dim_head
+// norm weight or None, eps or None, to_all_qkv weight, combine_heads weight, heads, dim_head, whether the norm is a layer norm, its bias or None
+Layer arg_layer(PyObject* const* a) {
   Layer l;
   l.norm = arg_optional(a[0]);
   if (a[1] != Py_None) l.eps = arg_float(a[1]);
@@ -1096,34 +1136,38 @@ Layer arg_layer(PyObject* const* a) {   // norm weight or None, eps or None, to_
   l.combine = arg_tensor(a[3]);
   l.heads = arg_int(a[4]);
   l.dim_head = arg_int(a[5]);
+  l.layer_norm = PyObject_IsTrue(a[6]) == 1;
+  l.norm_bias = arg_optional(a[7]);
+  if (l.layer_norm && !(l.norm.defined() && l.eps)) throw std::runtime_error("castle: a layer norm needs its weight and eps");
+  if (!l.layer_norm && l.norm_bias.defined()) throw std::runtime_error("castle: only a layer norm has a bias");
   return l;
 }
 
 // Whether something records torch operations or may replace torch functions, so that the layer's have to be called from
 // Python: jit tracing, a tensor class of its own, or a torch function mode (but a default device).
 PyObject* device_context = nullptr;   // torch's class of the modes that set one
-bool watched(PyObject* const* a) {   // (x, <layer: 6>, ...)
+bool watched(PyObject* const* a) {   // (x, <layer: 8>, ...)
   if (torch::jit::tracer::isTracing()) return true;
-  for (int i : {0, 1, 3, 4})
+  for (int i : {0, 1, 3, 4, 8})
     if (a[i] != Py_None && !THPVariable_CheckExact(a[i])) return true;
   for (int64_t i = 0; i < at::impl::PythonTorchFunctionTLS::stack_len(); ++i)
     if (reinterpret_cast<PyObject*>(Py_TYPE(at::impl::PythonTorchFunctionTLS::get_stack_at(i)->ptr(getPyInterpreter()))) != device_context) return true;
   return false;
 }
 
-// layer_forward(x, <layer: 6>, scale, rotary freqs or None, caches or None, limit, long_seq); None where it is watched()
+// layer_forward(x, <layer: 8>, scale, rotary freqs or None, caches or None, limit, long_seq); None where it is watched()
 PyObject* py_layer_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    arg_count(n, 12);
+    arg_count(n, 14);
     if (watched(a)) Py_RETURN_NONE;
     const Tensor x = arg_tensor(a[0]);
     const Layer l = arg_layer(a + 1);
     Options o;
-    o.scale = arg_float(a[7]);
-    o.rotary.freqs = arg_optional(a[8]);
-    o.caches = arg_caches(a[9]);
-    o.limit = arg_int(a[10]);
-    o.long_seq = arg_int(a[11]);
+    o.scale = arg_float(a[9]);
+    o.rotary.freqs = arg_optional(a[10]);
+    o.caches = arg_caches(a[11]);
+    o.limit = arg_int(a[12]);
+    o.long_seq = arg_int(a[13]);
     Tensor out;
     {
       Unlocked u;
@@ -1133,19 +1177,19 @@ PyObject* py_layer_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// layer_decode(x, <layer: 6>, scale, rotary freqs or None, caches, cache_len); None where it is watched()
+// layer_decode(x, <layer: 8>, scale, rotary freqs or None, caches, cache_len); None where it is watched()
 PyObject* py_layer_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    arg_count(n, 11);
+    arg_count(n, 13);
     if (watched(a)) Py_RETURN_NONE;
     const Tensor x = arg_tensor(a[0]);
     const Layer l = arg_layer(a + 1);
-    const double scale = arg_float(a[7]);
+    const double scale = arg_float(a[9]);
     Rotary rotary;
-    rotary.freqs = arg_optional(a[8]);
-    const std::vector<Tensor> caches = arg_caches(a[9]);
+    rotary.freqs = arg_optional(a[10]);
+    const std::vector<Tensor> caches = arg_caches(a[11]);
     if (caches.size() != 4) throw std::runtime_error("castle: four cache tensors expected");
-    const int64_t t = rotary.position0 = arg_int(a[10]);
+    const int64_t t = rotary.position0 = arg_int(a[12]);
     Tensor out;
     {
       Unlocked u;
@@ -1170,6 +1214,37 @@ PyObject* py_decode_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
       Unlocked u;
       out = decode_packed(packed, caches.data(), t, scale, rotary);
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
+// embedding(tokens, weight, scale, padding row or -1)
+PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    arg_count(n, 4);
+    const Tensor tokens = arg_tensor(a[0]), weight = arg_tensor(a[1]);
+    const double scale = arg_float(a[2]);
+    const int64_t padding = arg_int(a[3]);
+    Tensor out;
+    {
+      Unlocked u;
+      out = embedding(tokens, weight, scale, padding);
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
+// layer_norm(x, weight or None, bias or None, eps)
+PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    arg_count(n, 4);
+    const Tensor x = arg_tensor(a[0]), weight = arg_optional(a[1]), bias = arg_optional(a[2]);
+    const double eps = arg_float(a[3]);
+    Tensor out;
+    {
+      Unlocked u;
+      out = layer_norm(x, weight, bias, eps);
     }
     return THPVariable_Wrap(out);
   });
@@ -1271,6 +1346,8 @@ PyObject* py_bind(PyObject*, PyObject* d) {
     CASTLE_BIND(rmsnorm_fwd); CASTLE_BIND(rmsnorm_bwd_workspace_bytes); CASTLE_BIND(rmsnorm_bwd); CASTLE_BIND(bwd_workspace_bytes); CASTLE_BIND(bwd); CASTLE_BIND(transform); CASTLE_BIND(amax_scale);
     CASTLE_BIND(decode_workspace_bytes); CASTLE_BIND(decode_step_fused); CASTLE_BIND(token_linear_fits); CASTLE_BIND(token_linear);
     CASTLE_BIND(linear); CASTLE_BIND(token_layer_fits); CASTLE_BIND(token_layer_workspace_bytes); CASTLE_BIND(token_layer);
+    CASTLE_BIND(layernorm_fwd); CASTLE_BIND(layernorm_bwd_workspace_bytes); CASTLE_BIND(layernorm_bwd);
+    CASTLE_BIND(embedding_fwd); CASTLE_BIND(embedding_bwd_workspace_bytes); CASTLE_BIND(embedding_bwd);
 #undef CASTLE_BIND
     PyObject* module = PyImport_ImportModule("torch.utils._device");
     Py_XDECREF(device_context);
@@ -1289,6 +1366,8 @@ PyMethodDef methods[] = {{"bind", py_bind, METH_O, nullptr},
                          {"layer_forward", FAST(py_layer_forward), nullptr},
                          {"layer_decode", FAST(py_layer_decode), nullptr},
                          {"decode_packed", FAST(py_decode_packed), nullptr},
+                         {"embedding", FAST(py_embedding), nullptr},
+                         {"layer_norm", FAST(py_layer_norm), nullptr},
                          {"forward_chunks", FAST(py_forward_chunks), nullptr},
                          {"first_rows", FAST(py_first_rows), nullptr},
                          {"new_caches", FAST(py_new_caches), nullptr},

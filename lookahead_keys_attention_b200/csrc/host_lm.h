@@ -1,0 +1,199 @@
+// Host side of the operators around a language model's layers: token lookup and layer norm, each with its autograd
+// node.  Part of host.cpp (inside its namespace, behind what it shares with the other operators).
+//
+// What the kernels take by address is checked here: device, type and shape; tensors whose last dimension is not contiguous, or
+// whose negation is still to be done, are copied first.  Nodes compute in the type of their inputs, under autocast too.
+
+// (..., dim) as rows that are `stride(0)` elements apart.
+Tensor as_rows(const Tensor& t, int64_t rows, int64_t dim) {
+  Tensor r = t.resolve_neg().reshape({rows, dim});
+  return dim > 1 && r.stride(1) != 1 ? r.contiguous() : r;
+}
+int64_t row_stride(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+// A tensor of its own memory: no wrapper of a batched gradient, of a transform or of a class with a dispatch of its own.
+bool own_memory(const Tensor& t) {
+  return t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.key_set().has(c10::DispatchKey::Batched) &&
+         !t.key_set().has(c10::DispatchKey::FuncTorchBatched) && !t.key_set().has(c10::DispatchKey::FuncTorchGradWrapper) &&
+         !t.key_set().has(c10::DispatchKey::Functionalize);
+}
+void need_plain(const Tensor& t, const char* who) {
+  if (!t.is_cuda()) throw std::runtime_error(std::string(who) + ": expected CUDA tensors; this package has no CPU path");
+  if (!own_memory(t)) throw std::runtime_error(std::string(who) + ": plain strided tensors expected (no tensor class of its own, no vmap or functional transform)");
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), who, ": forward-mode differentiation is not implemented");
+}
+void need_type(const Tensor& t, const char* who) {
+  if (dtype_code(t.scalar_type()) < 0) throw std::runtime_error(std::string(who) + ": bf16, fp16 or fp32 expected");
+}
+void need_gradient(const Tensor& g, at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev, const char* who) {
+  if (g.sizes() != sizes || g.scalar_type() != type || g.device() != dev || !own_memory(g))
+    throw std::runtime_error(std::string(who) + ": the gradient's shape, type or device is not the output's");
+}
+Tensor restored_rows(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev, int64_t rows, int64_t dim) {
+  return as_rows(restored(t, sizes, type, dev), rows, dim);
+}
+
+// ------------------------------------------------------------------------------------------------ token lookup
+struct EmbeddingBackward : public Node {
+  SavedVariable tokens;
+  std::vector<int64_t> token_sizes;
+  at::ScalarType token_type = at::kLong, dtype = at::kFloat;
+  int64_t vocab = 0, dim = 0, padding = -1;
+  double scale = 1;
+
+  std::string name() const override { return "CastleEmbeddingBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    tokens.reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (grads.empty() || !grads[0].defined()) return {Tensor()};
+    const Tensor saved = tokens.unpack();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Device dev = grads[0].device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
+    const Tensor t = restored(saved, token_sizes, token_type, dev).contiguous();
+    const int64_t n = t.numel();
+    std::vector<int64_t> out_sizes = token_sizes;
+    out_sizes.push_back(dim);
+    need_gradient(grads[0], out_sizes, dtype, dev, "castle_embedding");
+    const auto options = at::TensorOptions().dtype(dtype).device(dev);
+    if (n == 0) return {at::zeros({vocab, dim}, options)};
+    const Tensor g = as_rows(grads[0], n, dim);
+    const Tensor dw = at::empty({vocab, dim}, options), status = status_word(dev.index());
+    StreamUse use(stream);
+    const Tensor ws = use.scratch(api.embedding_bwd_workspace_bytes(n, vocab, (int32_t)dim));
+    check(api.embedding_bwd(dtype_code(dtype), (int32_t)t.element_size(), n, vocab, (int32_t)dim, t.data_ptr(), padding, g.data_ptr(), row_stride(g),
+                            (float)scale, dw.data_ptr(), ws.data_ptr(), ws.numel(), status.data_ptr<int32_t>(), stream.stream()),
+          "castle_embedding_bwd");
+    return {dw};
+  }
+};
+
+Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
+  const char* who = "castle_embedding";
+  need_plain(weight, who);
+  need_plain(tokens, who);
+  need_type(weight, who);
+  need(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, "castle_embedding: tokens must be int64 or int32");
+  need(weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) > 0, "castle_embedding: a (vocabulary, dim) weight expected");
+  need(weight.device() == tokens.device(), "castle_embedding: tokens and weight must be on one device");
+  const int64_t n = tokens.numel(), vocab = weight.size(0), dim = weight.size(1);
+  std::vector<int64_t> sizes = tokens.sizes().vec();
+  sizes.push_back(dim);
+  Tensor y;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Device dev = weight.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    y = at::empty(sizes, weight.options().requires_grad(false));
+    if (n > 0) {
+      const Tensor t = tokens.contiguous(), w = as_rows(weight, vocab, dim), status = status_word(dev.index());
+      check(api.embedding_fwd(dtype_code(weight.scalar_type()), (int32_t)t.element_size(), n, vocab, (int32_t)dim, t.data_ptr(), w.data_ptr(),
+                              row_stride(w), (float)scale, y.data_ptr(), status.data_ptr<int32_t>(),
+                              c10::cuda::getCurrentCUDAStream(dev.index()).stream()), "castle_embedding_fwd");
+    }
+  }
+  if (!(at::GradMode::is_enabled() && weight.requires_grad())) return y;
+  auto node = std::shared_ptr<EmbeddingBackward>(new EmbeddingBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(weight));
+  torch::autograd::set_history(y, node);
+  node->tokens = SavedVariable(tokens, false);
+  node->token_sizes = tokens.sizes().vec();
+  node->token_type = tokens.scalar_type();
+  node->dtype = weight.scalar_type();
+  node->vocab = vocab; node->dim = dim; node->padding = padding; node->scale = scale;
+  return y;
+}
+
+// ------------------------------------------------------------------------------------------------ layer norm
+// Launches on rows; y, dx contiguous.  Weight, bias and the results may be undefined.
+void launch_layernorm(const Tensor& rows, const Tensor& weight, const Tensor& bias, double eps, const Tensor& y, const Tensor& stats,
+                      const c10::cuda::CUDAStream& stream) {
+  check(api.layernorm_fwd(dtype_code(rows.scalar_type()), rows.size(0), (int32_t)rows.size(1), rows.data_ptr(), row_stride(rows),
+                          weight.defined() ? weight.data_ptr() : nullptr, bias.defined() ? bias.data_ptr() : nullptr, (float)eps, y.data_ptr(),
+                          stats.defined() ? stats.data_ptr<float>() : nullptr, stream.stream()), "castle_layernorm_fwd");
+}
+void launch_layernorm_bwd(const Tensor& dy, const Tensor& rows, const Tensor& weight, const Tensor& stats, const Tensor& dx, const Tensor& dw,
+                          const Tensor& db, const c10::cuda::CUDAStream& stream) {
+  StreamUse use(stream);
+  const Tensor ws = use.scratch(api.layernorm_bwd_workspace_bytes(rows.size(0), (int32_t)rows.size(1)));
+  auto address = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  check(api.layernorm_bwd(dtype_code(rows.scalar_type()), rows.size(0), (int32_t)rows.size(1), dy.data_ptr(), row_stride(dy), rows.data_ptr(),
+                          row_stride(rows), address(weight), stats.data_ptr<float>(), address(dx), address(dw), address(db), ws.data_ptr(),
+                          ws.numel(), stream.stream()), "castle_layernorm_bwd");
+}
+
+struct LayerNormBackward : public Node {   // of x, weight, bias
+  SavedVariable x, weight, stats;
+  std::vector<int64_t> sizes;
+  at::ScalarType dtype = at::kFloat;
+  bool has_weight = false;
+
+  std::string name() const override { return "CastleLayerNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    x.reset_data(); weight.reset_data(); stats.reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list result(3);
+    if (grads.empty() || !grads[0].defined()) return result;
+    const Tensor xs = x.unpack(), ws = has_weight ? weight.unpack() : Tensor(), ss = stats.unpack();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Device dev = grads[0].device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const int64_t dim = sizes.back();
+    need_gradient(grads[0], sizes, dtype, dev, "castle_layer_norm");
+    const int64_t rows = grads[0].numel() / dim;
+    const auto options = at::TensorOptions().dtype(dtype).device(dev);
+    for (int i = 0; i < 3; ++i)
+      if (task_should_compute_output(i)) result[i] = rows == 0 ? (i == 0 ? at::empty(sizes, options) : at::zeros({dim}, options))
+                                                              : i == 0 ? at::empty(sizes, options) : at::empty({dim}, options);
+    if (rows == 0 || !(result[0].defined() || result[1].defined() || result[2].defined())) return result;
+    const Tensor w = has_weight ? restored(ws, {dim}, dtype, dev).resolve_neg().contiguous() : Tensor();
+    launch_layernorm_bwd(as_rows(grads[0], rows, dim), restored_rows(xs, sizes, dtype, dev, rows, dim), w,
+                         restored_contiguous(ss, {rows, 2}, at::kFloat, dev), result[0], result[1], result[2], c10::cuda::getCurrentCUDAStream(dev.index()));
+    return result;
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
+  const char* who = "castle_layer_norm";
+  need_plain(x, who);
+  need_type(x, who);
+  need(x.dim() >= 1 && x.size(-1) > 0, "castle_layer_norm: (..., dim) rows expected");
+  const int64_t dim = x.size(-1), rows = x.numel() / dim;
+  for (const Tensor* t : {&weight, &bias}) {
+    if (!t->defined()) continue;
+    need_plain(*t, who);
+    need(t->dim() == 1 && t->size(0) == dim && t->scalar_type() == x.scalar_type() && t->device() == x.device(),
+         "castle_layer_norm: weight and bias must be (dim) tensors of the input's type and device");
+  }
+  const bool grad = at::GradMode::is_enabled() &&
+                    (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad()));
+  Tensor y, stats;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Device dev = x.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const auto options = x.options().requires_grad(false);
+    y = at::empty(x.sizes(), options.memory_format(at::MemoryFormat::Contiguous));
+    if (grad) stats = at::empty({rows, 2}, options.dtype(at::kFloat));
+    auto plain = [](const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; };
+    if (rows > 0) launch_layernorm(as_rows(x, rows, dim), plain(weight), plain(bias), eps, y, stats, c10::cuda::getCurrentCUDAStream(dev.index()));
+  }
+  if (!grad) return y;
+  auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x, weight, bias));
+  torch::autograd::set_history(y, node);
+  node->x = SavedVariable(x, false);
+  node->has_weight = weight.defined();
+  if (node->has_weight) node->weight = SavedVariable(weight, false);
+  node->stats = SavedVariable(stats, false);
+  node->sizes = x.sizes().vec();
+  node->dtype = x.scalar_type();
+  return y;
+}

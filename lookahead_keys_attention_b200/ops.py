@@ -36,7 +36,8 @@ def check_status(device=None):
         v = int(w.item())
         if v != 0:
             w.zero_()
-            raise RuntimeError(f"castle kernels reported status {v} on cuda:{d} (1 = a bounded wait ran out)")
+            raise RuntimeError(f"castle kernels reported status {v} on cuda:{d} (1 = a bounded wait ran out, "
+                               "4 = a token or target outside the vocabulary)")
 
 
 def release_workspaces():
@@ -101,6 +102,29 @@ class _Traced(torch.autograd.Function):
         return (None, None, None, *(next(grads) if t.requires_grad else None for t in leaves))
 
 
+class _TracedCall(torch.autograd.Function):
+    """The same for an operator with one result: `call(*inputs)`."""
+
+    @staticmethod
+    def forward(ctx, call, *inputs):
+        with torch.enable_grad():
+            leaves = [t.detach().requires_grad_(t.requires_grad) if isinstance(t, torch.Tensor) else t for t in inputs]
+            out = call(*leaves)
+        ctx.graph = leaves, out
+        return out.detach()
+
+    @staticmethod
+    def backward(ctx, grad):
+        leaves, out = ctx.graph
+        wanted = [t for t in leaves if isinstance(t, torch.Tensor) and t.requires_grad]
+        grads = iter(torch.autograd.grad(out, wanted, grad, retain_graph=True))
+        return (None, *(next(grads) if isinstance(t, torch.Tensor) and t.requires_grad else None for t in leaves))
+
+
+def _call(call, *inputs):
+    return _TracedCall.apply(call, *inputs) if torch._C._is_tracing() else call(*inputs)
+
+
 def castle_attention_packed(packed, scale, return_U_for_cache=False, cache_out=None):
     """Parallel CASTLE attention on the packed projection output (B, N, 6, H, d), order
     qu,ku,vu,qc,kc,vc (the layout `to_all_qkv` produces).  Returns out (B, H, N, d) [, U].
@@ -128,3 +152,25 @@ def castle_decode_step(qc, kc, vc, qu, ku, vu, U, qu_cache, kc_cache, vc_cache, 
     valid rows; they are updated IN PLACE (row `cache_len` appended, U[0:cache_len] rewritten).
     The six new-token tensors are (B, H, 1, d).  Returns out (B, H, 1, d)."""
     return _lib.host().decode_step(qc, kc, vc, qu, ku, vu, U, qu_cache, kc_cache, vc_cache, cache_len, scale)
+
+
+def castle_embedding(tokens, weight, scale: float = 1.0, padding_idx: int | None = None):
+    """Rows of `weight` (vocabulary, dim) at `tokens` (any shape, int64 or int32), times `scale` (rounded once): the input of a
+    language model around these layers (the reference's training script embeds its bytes, train_triton.py:73-175).
+    The gradient of `weight` is dense and the same from call to call: every row's gradients are summed in the order of
+    their positions, in fp32.  Tokens equal to `padding_idx` are looked up like others and contribute no gradient.  A token
+    outside the vocabulary gives a row of NaN and no gradient, and `check_status()` raises."""
+    if padding_idx is not None:
+        vocab = weight.shape[0]
+        if not -vocab <= padding_idx < vocab:
+            raise ValueError("castle_embedding: padding_idx out of range")
+        padding_idx %= vocab
+    host, padding = _lib.host(), -1 if padding_idx is None else padding_idx
+    return _call(lambda t, w: host.embedding(t, w, scale, padding), tokens, weight)
+
+
+def castle_layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
+    """Layer norm over the last dimension of `x` (any size), with an optional weight and bias of its type: mean, variance and
+    all sums in fp32, one rounding.  `Castle(..., prenorm="layer")` has it in front of the layer."""
+    host = _lib.host()
+    return _call(lambda *t: host.layer_norm(*t, eps), x, weight, bias)

@@ -1,0 +1,47 @@
+"""CPU: arguments that the entry points of the operators around the layers refuse on the host, before anything is launched."""
+import pytest
+import torch
+
+
+def _lib():
+    from lookahead_keys_attention_b200 import _lib
+    _lib.build()
+    return _lib, _lib.load()
+
+
+def test_layernorm_arguments():
+    L, lib = _lib()
+    def fwd(dtype=L.BF16, rows=4, dim=16, x=32, stride=16, w=32, b=32, y=32, stats=32):
+        return lib.castle_layernorm_fwd(dtype, rows, dim, x, stride, w, b, 1e-5, y, stats, None)
+    for bad in [dict(dtype=3), dict(rows=0), dict(rows=2 ** 31), dict(dim=0), dict(dim=2 ** 25), dict(x=None), dict(y=None), dict(stride=-1), dict(x=33),
+                dict(w=33), dict(b=1), dict(stats=4)]:
+        assert fwd(**bad) < 0 and "castle_layernorm_fwd" in L.last_error(), bad
+    size = lib.castle_layernorm_bwd_workspace_bytes(4, 16)
+    assert size == 1 * 2 * 16 * 4 and lib.castle_layernorm_bwd_workspace_bytes(0, 16) == 0
+    def bwd(dtype=L.F32, rows=4, dim=16, dy=32, x=32, w=32, stats=32, dx=32, dw=32, db=32, ws=32, n=size):
+        return lib.castle_layernorm_bwd(dtype, rows, dim, dy, 16, x, 16, w, stats, dx, dw, db, ws, n, None)
+    for bad in [dict(dtype=-1), dict(rows=-1), dict(dy=None), dict(x=None), dict(stats=None), dict(dx=2), dict(ws=None), dict(n=size - 1), dict(stats=36)]:
+        assert bwd(**bad) < 0 and "castle_layernorm_bwd" in L.last_error(), bad
+
+
+def test_embedding_arguments():
+    L, lib = _lib()
+    def fwd(dtype=L.BF16, ib=8, n=4, vocab=10, dim=16, t=32, w=32, stride=16, y=32, status=32):
+        return lib.castle_embedding_fwd(dtype, ib, n, vocab, dim, t, w, stride, 1.0, y, status, None)
+    for bad in [dict(dtype=7), dict(ib=2), dict(n=0), dict(n=2 ** 31), dict(vocab=0), dict(vocab=2 ** 31), dict(dim=0), dict(t=None), dict(t=36), dict(w=None),
+                dict(w=33), dict(stride=-2), dict(y=None), dict(status=None)]:
+        assert fwd(**bad) < 0 and "castle_embedding_fwd" in L.last_error(), bad
+    size = lib.castle_embedding_bwd_workspace_bytes(4, 10, 16)
+    assert size > 0 and lib.castle_embedding_bwd_workspace_bytes(4, 0, 16) == 0
+    def bwd(dtype=L.BF16, ib=4, n=4, vocab=10, dim=16, t=32, dy=32, stride=16, dw=32, ws=32, size=size, status=32):
+        return lib.castle_embedding_bwd(dtype, ib, n, vocab, dim, t, -1, dy, stride, 1.0, dw, ws, size, status, None)
+    for bad in [dict(dtype=-1), dict(ib=16), dict(n=-5), dict(dy=None), dict(dy=33), dict(dw=None), dict(ws=None), dict(ws=40), dict(size=size - 1), dict(status=None)]:
+        assert bwd(**bad) < 0 and "castle_embedding_bwd" in L.last_error(), bad
+
+
+def test_cpu_tensors_are_refused():
+    from lookahead_keys_attention_b200 import castle_embedding, castle_layer_norm
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        castle_layer_norm(torch.zeros(2, 8))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        castle_embedding(torch.zeros(2, dtype=torch.int64), torch.zeros(4, 8))
