@@ -173,6 +173,26 @@ int castle_embedding_bwd(int32_t dtype, int32_t index_bytes, int64_t tokens, int
                          int64_t padding_idx, const void* dy, int64_t dy_stride, float scale, void* dweight, void* workspace,
                          size_t workspace_bytes, int32_t* status, void* stream);
 
+/* ---- cross entropy of a linear head (logits and loss of the model that the reference trains, train_triton.py:73-175) ----
+ * loss_i = log sum_v exp(x_i . w_v) - x_i . w_target, without the logits in memory.  x: `rows` rows of `dim` elements, x_stride
+ * apart; weight: `vocab` rows, w_stride apart; targets: 64-bit; all sums in fp32.  Rows whose target is ignore_index take no part,
+ * whatever x holds there; a target outside the vocabulary gives NaN and sets CASTLE_STATUS_BAD_INDEX.  `loss` (fp32): the mean over
+ * the other rows (NaN if there are none), their sum, or with CASTLE_REDUCE_NONE each row's (0 where ignored); `lse` (fp32, rows):
+ * each row's log-sum-exp, for the backward.  Backward: `dloss` = the upstream gradient (one value, or one per row); dx (rows x dim,
+ * contiguous, 0 where ignored) and dweight (vocab x dim, contiguous), each NULL if not wanted.  Logits are formed again there, in
+ * pieces of the vocabulary that take about 1 GiB of the workspace; all results are the same from call to call.
+ */
+enum { CASTLE_REDUCE_MEAN = 0, CASTLE_REDUCE_SUM = 1, CASTLE_REDUCE_NONE = 2 };
+
+size_t castle_linear_ce_workspace_bytes(int32_t dtype, int64_t rows, int32_t dim, int64_t vocab, int32_t backward);
+int castle_linear_ce_fwd(int32_t dtype, int64_t rows, int32_t dim, int64_t vocab, const void* x, int64_t x_stride,
+                         const void* weight, int64_t w_stride, const int64_t* targets, int64_t ignore_index, int32_t reduction,
+                         float* loss, float* lse, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+int castle_linear_ce_bwd(int32_t dtype, int64_t rows, int32_t dim, int64_t vocab, const void* x, int64_t x_stride,
+                         const void* weight, int64_t w_stride, const int64_t* targets, int64_t ignore_index, int32_t reduction,
+                         const float* lse, const float* dloss, void* dx, void* dweight, void* workspace, size_t workspace_bytes,
+                         int32_t* status, void* stream);
+
 /* ---- parallel backward ---------------------------------------------------
  * Replaces CastleAttentionFunction.backward
  * (lookahead_keys_attention_triton.py:509-602) with its two kernels

@@ -15,7 +15,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libcastle_b200.so"
-SOURCES = ["api.cu", "decode.cu", "selftest.cu", "convert.cu", "transform.cu", "token_linear.cu", "token_layer.cu", "linear.cu", "norm.cu", "layernorm.cu", "embedding.cu", "fwd.cu", "bwd.cu", "bwd128.cu"]
+SOURCES = ["api.cu", "decode.cu", "selftest.cu", "convert.cu", "transform.cu", "token_linear.cu", "token_layer.cu", "linear.cu", "norm.cu", "layernorm.cu", "embedding.cu", "linear_ce.cu", "fwd.cu", "bwd.cu", "bwd128.cu"]
 
 BF16, F16, F32 = 0, 1, 2
 
@@ -192,6 +192,9 @@ _SIGNATURES = {
     "castle_embedding_bwd_workspace_bytes": (_sz, [ctypes.c_int64, ctypes.c_int64, _i32]),
     "castle_embedding_bwd": (ctypes.c_int, [_i32, _i32, ctypes.c_int64, ctypes.c_int64, _i32, _vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_float,
                                             _vp, _vp, _sz, _vp, _vp]),
+    "castle_linear_ce_workspace_bytes": (_sz, [_i32, ctypes.c_int64, _i32, ctypes.c_int64, _i32]),
+    "castle_linear_ce_fwd": (ctypes.c_int, [_i32, ctypes.c_int64, _i32, ctypes.c_int64] + [_vp, ctypes.c_int64] * 3 + [_i32, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "castle_linear_ce_bwd": (ctypes.c_int, [_i32, ctypes.c_int64, _i32, ctypes.c_int64] + [_vp, ctypes.c_int64] * 3 + [_i32] + [_vp] * 5 + [_sz, _vp, _vp]),
     "castle_bwd_workspace_bytes": (_sz, [_PR]),
     "castle_bwd": (ctypes.c_int, [_PR] + [_T] * 8 + [_vp, _vp] + [_T] * 6 + [_vp, _sz, _vp, _vp]),
     "castle_decode_workspace_bytes": (_sz, [_PR, _i32]),

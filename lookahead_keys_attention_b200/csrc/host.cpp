@@ -73,6 +73,9 @@ struct Api {
   decltype(&castle_embedding_fwd) embedding_fwd;
   decltype(&castle_embedding_bwd_workspace_bytes) embedding_bwd_workspace_bytes;
   decltype(&castle_embedding_bwd) embedding_bwd;
+  decltype(&castle_linear_ce_workspace_bytes) linear_ce_workspace_bytes;
+  decltype(&castle_linear_ce_fwd) linear_ce_fwd;
+  decltype(&castle_linear_ce_bwd) linear_ce_bwd;
 } api{};
 
 void check(int rc, const char* what) {
@@ -1250,6 +1253,21 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// linear_cross_entropy(x, weight, targets, target to ignore, reduction of the C ABI)
+PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    arg_count(n, 5);
+    const Tensor x = arg_tensor(a[0]), weight = arg_tensor(a[1]), targets = arg_tensor(a[2]);
+    const int64_t ignore = arg_int(a[3]), reduction = arg_int(a[4]);
+    Tensor out;
+    {
+      Unlocked u;
+      out = linear_cross_entropy(x, weight, targets, ignore, (int)reduction);
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
 // forward_chunks(B, H, bytes per pair, limit): the rectangles of a forward's launches as (b0, b1, h0, h1)
 PyObject* py_forward_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -1348,6 +1366,7 @@ PyObject* py_bind(PyObject*, PyObject* d) {
     CASTLE_BIND(linear); CASTLE_BIND(token_layer_fits); CASTLE_BIND(token_layer_workspace_bytes); CASTLE_BIND(token_layer);
     CASTLE_BIND(layernorm_fwd); CASTLE_BIND(layernorm_bwd_workspace_bytes); CASTLE_BIND(layernorm_bwd);
     CASTLE_BIND(embedding_fwd); CASTLE_BIND(embedding_bwd_workspace_bytes); CASTLE_BIND(embedding_bwd);
+    CASTLE_BIND(linear_ce_workspace_bytes); CASTLE_BIND(linear_ce_fwd); CASTLE_BIND(linear_ce_bwd);
 #undef CASTLE_BIND
     PyObject* module = PyImport_ImportModule("torch.utils._device");
     Py_XDECREF(device_context);
@@ -1368,6 +1387,7 @@ PyMethodDef methods[] = {{"bind", py_bind, METH_O, nullptr},
                          {"decode_packed", FAST(py_decode_packed), nullptr},
                          {"embedding", FAST(py_embedding), nullptr},
                          {"layer_norm", FAST(py_layer_norm), nullptr},
+                         {"linear_cross_entropy", FAST(py_linear_cross_entropy), nullptr},
                          {"forward_chunks", FAST(py_forward_chunks), nullptr},
                          {"first_rows", FAST(py_first_rows), nullptr},
                          {"new_caches", FAST(py_new_caches), nullptr},

@@ -1,5 +1,5 @@
-// Host side of the operators around a language model's layers: token lookup and layer norm, each with its autograd
-// node.  Part of host.cpp (inside its namespace, behind what it shares with the other operators).
+// Host side of the operators around a language model's layers: token lookup, layer norm and the head's cross entropy, each
+// with its autograd node.  Part of host.cpp (inside its namespace, behind what it shares with the other operators).
 //
 // What the kernels take by address is checked here: device, type and shape; tensors whose last dimension is not contiguous, or
 // whose negation is still to be done, are copied first.  Nodes compute in the type of their inputs, under autocast too.
@@ -196,4 +196,102 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, dou
   node->sizes = x.sizes().vec();
   node->dtype = x.scalar_type();
   return y;
+}
+
+// ------------------------------------------------------------------------------------------------ cross entropy of a linear head
+struct LinearCrossEntropyBackward : public Node {   // of x, weight
+  SavedVariable x, weight, targets, lse;
+  std::vector<int64_t> x_sizes, target_sizes;
+  at::ScalarType dtype = at::kFloat, target_type = at::kLong;
+  int64_t vocab = 0, ignore = -100;
+  int reduction = CASTLE_REDUCE_MEAN;
+
+  std::string name() const override { return "CastleLinearCrossEntropyBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&x, &weight, &targets, &lse}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    const char* who = "castle_linear_cross_entropy";
+    variable_list result(2);
+    if (grads.empty() || !grads[0].defined()) return result;
+    const Tensor xs = x.unpack(), ws = weight.unpack(), ts = targets.unpack(), ls = lse.unpack();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Device dev = grads[0].device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
+    const int64_t dim = x_sizes.back();
+    int64_t rows = 1;
+    for (size_t i = 0; i + 1 < x_sizes.size(); ++i) rows *= x_sizes[i];
+    const bool each = reduction == CASTLE_REDUCE_NONE;
+    need_gradient(grads[0], each ? at::IntArrayRef(target_sizes) : at::IntArrayRef(), at::kFloat, dev, who);
+    const auto options = at::TensorOptions().dtype(dtype).device(dev);
+    if (rows == 0) {
+      if (task_should_compute_output(0)) result[0] = at::empty(x_sizes, options);
+      if (task_should_compute_output(1)) result[1] = at::zeros({vocab, dim}, options);
+      return result;
+    }
+    if (task_should_compute_output(0)) result[0] = at::empty(x_sizes, options);
+    if (task_should_compute_output(1)) result[1] = at::empty({vocab, dim}, options);
+    const Tensor xr = restored_rows(xs, x_sizes, dtype, dev, rows, dim), w = restored_rows(ws, {vocab, dim}, dtype, dev, vocab, dim),
+                 t = restored(ts, target_sizes, target_type, dev).to(at::kLong).contiguous(), l = restored_contiguous(ls, {rows}, at::kFloat, dev),
+                 g = grads[0].resolve_neg().contiguous(), status = status_word(dev.index());
+    StreamUse use(stream);
+    const Tensor scratch = use.scratch(api.linear_ce_workspace_bytes(dtype_code(dtype), rows, (int32_t)dim, vocab, 1));
+    check(api.linear_ce_bwd(dtype_code(dtype), rows, (int32_t)dim, vocab, xr.data_ptr(), row_stride(xr), w.data_ptr(), row_stride(w), t.data_ptr<int64_t>(), ignore,
+                            reduction, l.data_ptr<float>(), g.data_ptr<float>(), result[0].defined() ? result[0].data_ptr() : nullptr,
+                            result[1].defined() ? result[1].data_ptr() : nullptr, scratch.data_ptr(), scratch.numel(), status.data_ptr<int32_t>(), stream.stream()),
+          "castle_linear_ce_bwd");
+    return result;
+  }
+};
+
+Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& targets, int64_t ignore, int reduction) {
+  const char* who = "castle_linear_cross_entropy";
+  for (const Tensor* t : {&x, &weight, &targets}) need_plain(*t, who);
+  need_type(x, who);
+  need(x.dim() >= 1 && x.size(-1) > 0 && weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) == x.size(-1),
+       "castle_linear_cross_entropy: (..., dim) inputs and a (vocabulary, dim) weight expected");
+  need(weight.scalar_type() == x.scalar_type() && weight.device() == x.device() && targets.device() == x.device(),
+       "castle_linear_cross_entropy: input and weight must have one type, and all tensors one device");
+  need(targets.scalar_type() == at::kLong || targets.scalar_type() == at::kInt, "castle_linear_cross_entropy: targets must be int64 or int32");
+  need(targets.sizes() == x.sizes().slice(0, x.dim() - 1), "castle_linear_cross_entropy: a target for each row of the input expected");
+  const int64_t dim = x.size(-1), rows = targets.numel(), vocab = weight.size(0);
+  const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()), each = reduction == CASTLE_REDUCE_NONE;
+  Tensor loss, lse;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Device dev = x.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
+    const auto options = at::TensorOptions().dtype(at::kFloat).device(dev);
+    if (rows == 0 && !each) loss = at::full({}, reduction == CASTLE_REDUCE_MEAN ? std::numeric_limits<double>::quiet_NaN() : 0.0, options);
+    else loss = each ? at::empty(targets.sizes(), options) : at::empty({}, options);
+    lse = at::empty({rows}, options);
+    if (rows > 0) {
+      const Tensor xr = as_rows(x, rows, dim), w = as_rows(weight, vocab, dim), t = targets.to(at::kLong).contiguous(), status = status_word(dev.index());
+      StreamUse use(stream);
+      const Tensor scratch = use.scratch(api.linear_ce_workspace_bytes(dtype_code(x.scalar_type()), rows, (int32_t)dim, vocab, 0));
+      check(api.linear_ce_fwd(dtype_code(x.scalar_type()), rows, (int32_t)dim, vocab, xr.data_ptr(), row_stride(xr), w.data_ptr(), row_stride(w),
+                              t.data_ptr<int64_t>(), ignore, reduction, loss.data_ptr<float>(), lse.data_ptr<float>(), scratch.data_ptr(), scratch.numel(),
+                              status.data_ptr<int32_t>(), stream.stream()), "castle_linear_ce_fwd");
+    }
+  }
+  if (!grad) return loss;
+  auto node = std::shared_ptr<LinearCrossEntropyBackward>(new LinearCrossEntropyBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x, weight));
+  torch::autograd::set_history(loss, node);
+  node->x = SavedVariable(x, false);
+  node->weight = SavedVariable(weight, false);
+  node->targets = SavedVariable(targets, false);
+  node->lse = SavedVariable(lse, false);
+  node->x_sizes = x.sizes().vec();
+  node->target_sizes = targets.sizes().vec();
+  node->dtype = x.scalar_type();
+  node->target_type = targets.scalar_type();
+  node->vocab = vocab;
+  node->ignore = ignore;
+  node->reduction = reduction;
+  return loss;
 }

@@ -174,3 +174,19 @@ def castle_layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     all sums in fp32, one rounding.  `Castle(..., prenorm="layer")` has it in front of the layer."""
     host = _lib.host()
     return _call(lambda *t: host.layer_norm(*t, eps), x, weight, bias)
+
+
+_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}   # CASTLE_REDUCE_* of the C ABI
+
+
+def castle_linear_cross_entropy(x, weight, targets, ignore_index: int = -100, reduction: str = "mean"):
+    """Cross entropy of the logits `x @ weight.T` against `targets`, without the logits in memory: the head and the loss of a
+    language model around these layers (the reference's training script, train_triton.py:73-175).  x (..., dim) and weight
+    (vocabulary, dim) of one type, targets (...) int64 or int32; the loss is fp32, logits and sums are, too.  Rows whose target is
+    `ignore_index` take no part, whatever x holds there, and cost nothing; `reduction`: the mean of the others (NaN if there are
+    none), their "sum", or "none" for each row's loss (0 where ignored).  The gradients of x and weight are formed in the backward
+    pass, from logits formed again, and are the same from call to call.  A target outside the vocabulary gives NaN, and `check_status()` raises."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"castle_linear_cross_entropy: reduction {reduction!r} is not one of {', '.join(_REDUCTIONS)}")
+    host, code = _lib.host(), _REDUCTIONS[reduction]
+    return _call(lambda x, w, t: host.linear_cross_entropy(x, w, t, ignore_index, code), x, weight, targets)

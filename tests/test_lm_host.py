@@ -45,3 +45,40 @@ def test_cpu_tensors_are_refused():
         castle_layer_norm(torch.zeros(2, 8))
     with pytest.raises(RuntimeError, match="no CPU path"):
         castle_embedding(torch.zeros(2, dtype=torch.int64), torch.zeros(4, 8))
+
+
+def test_linear_ce_arguments():
+    L, lib = _lib()
+    size = [lib.castle_linear_ce_workspace_bytes(L.BF16, 4, 16, 10, b) for b in (0, 1)]
+    assert min(size) > 0
+    for bad in [(5, 4, 16, 10), (0, 0, 16, 10), (0, 4, 0, 10), (0, 4, 16, 0), (0, 2 ** 31, 16, 10), (0, 4, 2 ** 21, 10), (0, 4, 16, 2 ** 31)]:
+        assert lib.castle_linear_ce_workspace_bytes(*bad, 1) == 0
+    def fwd(dtype=L.BF16, n=4, dim=16, vocab=10, x=256, xs=16, w=256, ws=16, t=256, red=0, loss=256, lse=256, work=256, size=size[0], status=256):
+        return lib.castle_linear_ce_fwd(dtype, n, dim, vocab, x, xs, w, ws, t, -100, red, loss, lse, work, size, status, None)
+    for bad in [dict(dtype=3), dict(n=0), dict(dim=0), dict(vocab=-1), dict(x=None), dict(x=257), dict(xs=-1), dict(w=None), dict(ws=-1), dict(t=None), dict(t=260),
+                dict(red=3), dict(red=-1), dict(loss=None), dict(lse=None), dict(lse=2), dict(work=None), dict(work=128), dict(size=size[0] - 1), dict(status=None)]:
+        assert fwd(**bad) < 0 and "castle_linear_ce_fwd" in L.last_error(), bad
+    def bwd(dtype=L.BF16, n=4, dim=16, vocab=10, lse=256, dloss=256, dx=256, dw=256, work=256, size=size[1]):
+        return lib.castle_linear_ce_bwd(dtype, n, dim, vocab, 256, 16, 256, 16, 256, -100, 0, lse, dloss, dx, dw, work, size, 256, None)
+    for bad in [dict(dtype=-1), dict(n=-1), dict(lse=None), dict(dloss=None), dict(dloss=6), dict(dx=1), dict(dw=3), dict(work=None), dict(size=size[1] - 1)]:
+        assert bwd(**bad) < 0 and "castle_linear_ce_bwd" in L.last_error(), bad
+    assert bwd(dx=None, dw=None) == 0          # nothing wanted, nothing launched
+
+
+def test_the_losses_scratch_is_bounded():
+    """About 1 GiB for a piece of the vocabulary beside what goes with the rows, whatever the vocabulary."""
+    L, lib = _lib()
+    for dtype, planes in ((L.BF16, 1), (L.F32, 3)):
+        for n, dim, vocab in [(8192, 4096, 1 << 20), (65536, 512, 300000), (16384, 8192, 200000)]:
+            for backward in (0, 1):
+                rows = planes * (n + 64) * dim * 2 + n * 64
+                slabs = n * dim * 4 * 32 * backward
+                assert lib.castle_linear_ce_workspace_bytes(dtype, n, dim, vocab, backward) <= (1 << 30) * 1.1 + rows + slabs
+
+
+def test_reduction_names():
+    from lookahead_keys_attention_b200 import castle_linear_cross_entropy
+    with pytest.raises(ValueError, match="reduction"):
+        castle_linear_cross_entropy(torch.zeros(2, 8), torch.zeros(3, 8), torch.zeros(2, dtype=torch.int64), reduction="avg")
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        castle_linear_cross_entropy(torch.zeros(2, 8), torch.zeros(3, 8), torch.zeros(2, dtype=torch.int64))
