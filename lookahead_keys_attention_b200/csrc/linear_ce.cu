@@ -18,11 +18,18 @@
 // half of tensor memory while the next one is summed in the other.  All sums, the logits and the statistics are fp32.
 //
 // fp32 tensors: every value is the sum of three bf16 ones (8 bits each: 24), and a product is the six largest of the nine products
-// of such parts (what is left out is 2^-24 of it).  So the same kernels serve, with six times the steps.
+// of such parts (what is left out is 2^-24 of it), the smallest first.  So the same kernels serve, with six times the steps.
+//
+// The tensor cores cut what they add to an accumulator, always towards zero, so a long sum is off by some 2^-24 per addition (197 rows
+// of 512, fp32: losses 3.3e-6 off, gradients of longer sums 1.7e-5, where fp32 arithmetic has 2e-7).  Where the result has 32 bits
+// (the logits' statistics, and everything of fp32 tensors), accumulators are therefore emptied every `flush` steps into sums that
+// the working warps keep in registers.
 //
 // G in 16 bits: c_i is taken in units of a power of two that leaves G below 2^15 (the unit is multiplied back in fp32 at the
 // end), so that fp16 keeps probabilities down to 2^-28 in full precision; rounding G is off by half a step of the type, as
 // rounding the logits' gradient is where logits are tensors of that type.
+#include <type_traits>
+
 #include "common.cuh"
 #include "vec.cuh"
 
@@ -35,6 +42,9 @@ constexpr uint32_t kCeA = kCeM * kCeK * 2, kCeB = kCeN * kCeK * 2, kCeStage = kC
 constexpr uint32_t kCeStaging = 8 * 4096;   // kGrad: 32 rows x 64 columns of each working warp
 constexpr size_t kCeSmem = kCeStages * kCeStage + kCeStaging + 1024;
 constexpr int64_t kCeScratch = (int64_t)1 << 30;   // bytes that a piece of the vocabulary may take
+// Steps between emptyings: of a 16-bit operand's logits (32 additions in the tensor cores), of fp32's parts (24).  197 x 512 in
+// fp32: TBD
+constexpr int kCeFlush = 8, kCeFlushF32 = 1, kCeNoFlush = 1 << 30;
 constexpr float kCeUnit = 16384.f;                 // of G: |c| < 2 units
 
 struct CeHead {          // at the start of the workspace, written by castle_ce_rows_kernel
@@ -46,7 +56,7 @@ struct CeHead {          // at the start of the workspace, written by castle_ce_
 };
 struct CeRow { int target; float lse, coef; int row; };   // of the rows that take part, in order; row: in the caller's tensors
 
-__constant__ const int8_t kTermA[6] = {0, 0, 1, 1, 0, 2}, kTermB[6] = {0, 1, 0, 1, 2, 0};
+__constant__ const int8_t kTermA[6] = {2, 0, 1, 1, 0, 0}, kTermB[6] = {0, 2, 1, 0, 1, 0};   // one term: the last
 
 // ------------------------------------------------------------------------------------------------ rows that take part
 struct CeRowsParams {
@@ -237,6 +247,7 @@ struct CeProduct {
   int b_row0;            // where the piece begins in B's rows (kLse, kGrad: along n, kDx: along k)
   int vocab0, vocab;     // the piece's first column of z, and how many there are (kLse, kGrad)
   int terms, splits, group;
+  int flush;             // steps after which an accumulator is emptied
   // kLse
   float2* parts;         // [2 per tile of n][parts_ld]
   float* target_logit;
@@ -279,6 +290,7 @@ template <typename T, typename OUT, CeMode MODE>
 __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_copy,
                                                                const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_g) {
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
+  constexpr bool REG = MODE == kLse || CePlanes<OUT>::count > 1;   // accumulators are emptied into registers on the way
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t bar_full[kCeStages], bar_free[kCeStages], bar_done[2], bar_read[2], bar_end;
@@ -314,11 +326,10 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         int m, n, split;
         tiles.at(t, m, n, split);
         const int m0 = m * kCeM, n0 = n * kCeN;
-        for (int term = 0; term < p.terms; ++term) {
-          const int pa = kTermA[term], pb = kTermB[term];
-          for (int ks = tiles.begin(split); ks < tiles.end(split); ++ks, ++it) {
-            const int s = it % kCeStages, k = ks * kCeK;
-            if (!mbar_wait_ok<true>(&bar_free[s], ((uint32_t)(it / kCeStages) & 1u) ^ 1u, abortp)) { ks = tiles.end(split); term = p.terms; break; }
+        for (int ks = tiles.begin(split); ks < tiles.end(split); ++ks) {
+          for (int term = 6 - p.terms; term < 6; ++term, ++it) {
+            const int s = it % kCeStages, k = ks * kCeK, pa = kTermA[term], pb = kTermB[term];
+            if (!mbar_wait_ok<true>(&bar_free[s], ((uint32_t)(it / kCeStages) & 1u) ^ 1u, abortp)) { ks = tiles.end(split); break; }
             uint8_t *a = smem + s * kCeStage, *b = a + kCeA;
             mbar_expect_tx(&bar_full[s], kCeStage);
             if (A_MN) {
@@ -346,26 +357,26 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
       for (int t = first; t < tiles.total && !*abortp; t += stride) {
         int m, n, split;
         tiles.at(t, m, n, split);
-        const int steps = (tiles.end(split) - tiles.begin(split)) * p.terms;
-        if (steps == 0) continue;
-        const int acc = turn & 1, cols = min(kCeN, (p.n - n * kCeN + 15) / 16 * 16);
+        const int cols = min(kCeN, (p.n - n * kCeN + 15) / 16 * 16);
         const uint32_t idesc = make_idesc(kCeM, 16, Elem<T>::fmt, A_MN, B_MN, false) + ((uint32_t)((cols - 16) >> 3) << 17);
-        const uint32_t d = tmem + acc * kCeN;
-        if (!mbar_wait_ok<true>(&bar_read[acc], ((uint32_t)(turn >> 1) & 1u) ^ 1u, abortp)) break;
-        tc_fence_after();
-        for (int j = 0; j < steps; ++j, ++it) {
-          const int s = it % kCeStages;
-          if (!mbar_wait_ok<true>(&bar_full[s], (uint32_t)(it / kCeStages) & 1u, abortp)) break;
+        for (int k0 = tiles.begin(split); k0 < tiles.end(split) && !*abortp; k0 += p.flush, ++turn) {
+          const int acc = turn & 1, steps = min(p.flush, tiles.end(split) - k0) * p.terms;
+          const uint32_t d = tmem + acc * kCeN;
+          if (!mbar_wait_ok<true>(&bar_read[acc], ((uint32_t)(turn >> 1) & 1u) ^ 1u, abortp)) break;
           tc_fence_after();
-          const uint32_t a = smem_u32(smem) + s * kCeStage, b = a + kCeA;
-          const uint64_t da = A_MN ? desc_mnmajor(a, kCeA / 2) : desc_kmajor(a), db = B_MN ? desc_mnmajor(b, kCeB / 4) : desc_kmajor(b);
+          for (int j = 0; j < steps; ++j, ++it) {
+            const int s = it % kCeStages;
+            if (!mbar_wait_ok<true>(&bar_full[s], (uint32_t)(it / kCeStages) & 1u, abortp)) break;
+            tc_fence_after();
+            const uint32_t a = smem_u32(smem) + s * kCeStage, b = a + kCeA;
+            const uint64_t da = A_MN ? desc_mnmajor(a, kCeA / 2) : desc_kmajor(a), db = B_MN ? desc_mnmajor(b, kCeB / 4) : desc_kmajor(b);
 #pragma unroll
-          for (int q = 0; q < kCeK / 16; ++q)
-            mma_ss(d, da + (uint64_t)(((A_MN ? 2048 : 32) * q) >> 4), db + (uint64_t)(((B_MN ? 2048 : 32) * q) >> 4), idesc, j > 0 || q > 0);
-          mma_commit(&bar_free[s]);
+            for (int q = 0; q < kCeK / 16; ++q)
+              mma_ss(d, da + (uint64_t)(((A_MN ? 2048 : 32) * q) >> 4), db + (uint64_t)(((B_MN ? 2048 : 32) * q) >> 4), idesc, j > 0 || q > 0);
+            mma_commit(&bar_free[s]);
+          }
+          mma_commit(&bar_done[acc]);
         }
-        mma_commit(&bar_done[acc]);
-        ++turn;
       }
       mma_commit(&bar_end);   // all products have read their operands
       mbar_drain(&bar_end, 0);
@@ -375,25 +386,71 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     uint8_t* staging = smem + kCeStages * kCeStage + (warp - 2) * 4096;
     int turn = 0;
-    for (int t = first; t < tiles.total; t += stride) {
+    bool over = false;
+    for (int t = first; t < tiles.total && !over; t += stride) {
       int m, n, split;
       tiles.at(t, m, n, split);
-      const bool empty = tiles.end(split) <= tiles.begin(split);
-      const int acc = turn & 1, row = m * kCeM + quarter * 32 + lane, c_base = n * kCeN + half * 128;
-      const uint32_t src = tmem + acc * kCeN + half * 128 + lanes;
+      const int row = m * kCeM + quarter * 32 + lane, c_base = n * kCeN + half * 128;
       const int cols = min(128, p.n - c_base);   // that there are; columns from `cols` rounded up to 16 on were not computed
-      if (!empty) {
-        if (mbar_wait_failed(&bar_done[acc], (uint32_t)(turn >> 1) & 1u, abortp)) break;
+      const uint32_t src = tmem + half * 128 + lanes;
+      const int k_end = tiles.end(split);
+      int k0 = tiles.begin(split);
+      const bool empty = k_end <= k0;
+      float sums[REG ? 128 : 1];
+      if constexpr (REG) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) sums[j] = 0.f;
+        for (; k0 < k_end; k0 += p.flush, ++turn) {
+          if (mbar_wait_failed(&bar_done[turn & 1], (uint32_t)(turn >> 1) & 1u, abortp)) { over = true; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int c0 = 0; c0 < 128; c0 += 16) {   // (32 at a time spill)
+            if (c0 >= cols) break;
+            float v[16];
+            tmem_ld16(src + (turn & 1) * kCeN + c0, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[c0 + j] += v[j];
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_read[turn & 1]);
+        }
+        if (over) break;
+      } else if (!empty) {
+        if (mbar_wait_failed(&bar_done[turn & 1], (uint32_t)(turn >> 1) & 1u, abortp)) break;
         tc_fence_after();
       }
+      // values [c0, c0 + COUNT) of the thread's half row
+      auto take = [&](auto count, int c0, float* v) {
+        constexpr int COUNT = decltype(count)::value;
+        if constexpr (REG) {
+#pragma unroll
+          for (int j = 0; j < COUNT; ++j) v[j] = sums[c0 + j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < COUNT; j += 32) tmem_ld32(src + (turn & 1) * kCeN + c0 + j, v + j);
+          tmem_ld_wait();
+        }
+      };
+      auto release = [&] {   // the accumulator has been read
+        if constexpr (!REG) {
+          if (empty) return;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_read[turn & 1]);
+        }
+      };
+      constexpr float kLog2e = 1.4426950408889634f;
       if constexpr (MODE == kLse) {
         const bool on = row < head.rows;
         const int target = on ? p.rows[row].target - p.vocab0 - c_base : -1;
         float best = -INFINITY, sum = 0.f;
-        for (int c0 = 0; c0 < 128 && c0 < cols; c0 += 32) {
+#pragma unroll
+        for (int c0 = 0; c0 < 128; c0 += 32) {
+          if (c0 >= cols) break;
           float v[32];
-          tmem_ld32(src + c0, v);
-          tmem_ld_wait();
+          take(std::integral_constant<int, 32>(), c0, v);
           if (c0 + 32 > cols) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = c0 + j < cols ? v[j] : -INFINITY;
@@ -409,7 +466,6 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           }
           __syncwarp();
           const float zero = top == -INFINITY ? 0.f : top;
-          constexpr float kLog2e = 1.4426950408889634f;
           float2 s2 = make_float2(0.f, 0.f);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
@@ -419,22 +475,19 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           sum = fmaf(sum, ex2_approx((best - zero) * kLog2e), s2.x + s2.y);
           best = top;
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_read[acc]);
         if (on) p.parts[(int64_t)(n * 2 + half) * p.parts_ld + row] = make_float2(best, sum);
       } else if constexpr (MODE == kGrad) {
         CeRow r;
         r.target = -1; r.lse = 0.f; r.coef = 0.f; r.row = 0;
         if (row < head.rows) r = p.rows[row];
         const int target = r.target - p.vocab0 - c_base;
-        constexpr float kLog2e = 1.4426950408889634f;
         constexpr int PLANES = CePlanes<OUT>::count;
-        for (int c0 = 0; c0 < 128 && c0 < cols; c0 += 64) {
+#pragma unroll
+        for (int c0 = 0; c0 < 128; c0 += 64) {
+          if (c0 >= cols) break;
           float v[64];
-          tmem_ld32(src + c0, v);
-          tmem_ld32(src + c0 + 32, v + 32);
-          tmem_ld_wait();
+          take(std::integral_constant<int, 64>(), c0, v);
+          if (c0 + 64 >= cols) release();
 #pragma unroll
           for (int j = 0; j < 64; j += 2) {
             const float2 d = mul2(add2(make_float2(v[j], v[j + 1]), splat(-r.lse)), splat(kLog2e));
@@ -448,11 +501,6 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = r.coef == 0.f ? 0.f : v[j] * r.coef;
-          if (c0 + 64 >= min(cols, 128)) {   // the accumulator has been read
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar_read[acc]);
-          }
 #pragma unroll
           for (int q = 0; q < PLANES; ++q) {
             if (lane == 0) bulk_wait_read0();   // what was stored from here before has left
@@ -476,22 +524,20 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
             }
           }
         }
-        if (cols <= 0) {   // a half without columns
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_read[acc]);
-        }
+        if (cols <= 0) release();   // a half without columns
       } else {
         const float unit = head.unit;
         const bool on = row < (MODE == kDw ? p.m : head.rows);
         const int64_t to = MODE == kDw ? p.out_row0 + row : on ? p.rows[row].row : 0;
-        for (int c0 = 0; c0 < 128 && c0 < cols; c0 += 32) {
+#pragma unroll
+        for (int c0 = 0; c0 < 128; c0 += 32) {
+          if (c0 >= cols) break;
           float v[32];
           if (empty) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = 0.f;
           } else {
-            tmem_ld32(src + c0, v);
-            tmem_ld_wait();
+            take(std::integral_constant<int, 32>(), c0, v);
           }
           const int col = c_base + c0, have = min(32, cols - c0);
           if (!on) {
@@ -523,13 +569,9 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           }
           __syncwarp();
         }
-        if (!empty) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_read[acc]);
-        }
+        release();
       }
-      if (!empty) ++turn;
+      if (!REG && !empty) ++turn;
     }
     if (MODE == kGrad && lane == 0) bulk_wait_read0();
   }
@@ -818,6 +860,7 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
     CeProduct p{};
     p.head = (const CeHead*)c.work; p.rows = (const CeRow*)(c.work + q.rows); p.n = (int)count; p.k = q.pitch; p.b_row0 = q.copy_w ? 0 : (int)v0;
     p.vocab0 = (int)v0; p.vocab = (int)c.vocab; p.terms = q.terms; p.splits = 1; p.group = 32;
+    p.flush = q.terms > 1 ? kCeFlushF32 : kCeFlush;
     p.parts = (float2*)(c.work + q.parts); p.parts_ld = q.copy_rows; p.target_logit = (float*)(c.work + q.logit); p.status = c.status;
     CE_CUDA((ce_launch<T, OUT, kLse>(p, tiles_m * tiles_n, x, copy, w, w, c.st)), "castle_linear_ce_fwd launch");
     CeJoin j{};
@@ -843,7 +886,7 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
   CE_TRY(ce_x_maps(c, q, op, kCeM, &x, &copy));
   CE_TRY(ce_x_maps(c, q, op, kCeK, &xk, &copyk));
   CeProduct base{};
-  base.head = (const CeHead*)c.work; base.rows = (const CeRow*)(c.work + q.rows); base.terms = q.terms; base.splits = 1; base.group = 32; base.status = c.status;
+  base.head = (const CeHead*)c.work; base.rows = (const CeRow*)(c.work + q.rows); base.terms = q.terms; base.flush = q.terms > 1 ? kCeFlushF32 : kCeNoFlush; base.splits = 1; base.group = 32; base.status = c.status;
   base.vocab = (int)c.vocab; base.ld = c.dim;
   auto sum = [&](int splits, int64_t rows, int64_t slab_rows, bool by_row, const float* slab, void* out) {
     CeSum s{};
