@@ -12,8 +12,8 @@
 // give every (row, warp) its place, and a second reading puts the positions there, lanes with the same token in the order of the
 // lanes.  CTAs need nothing of one another, and a row that takes all the tokens is no special case.
 //
-// Sums: a warp per row and slab of columns where a row has up to `piece` tokens (none: it writes the zeros); the sorted list of
-// longer ones is cut at multiples of `piece` entries, whose sums go to scratch and are added, in order, by a third launch.
+// Sums: a warp takes a slab of 256 columns of up to 16 neighbouring rows, whose tokens are one run of the sorted list, and writes a
+// row (or the zeros of one without tokens) when the run goes on to the next; the list's entries of rows with more than `piece` tokens are cut at multiples of `piece` entries, whose sums go to scratch and are added, in order, by a third launch.
 #include "common.cuh"
 #include "vec.cuh"
 
@@ -21,6 +21,7 @@ namespace castle {
 
 constexpr int kEmbThreads = 256, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kSortRows = 1536;   // most rows of a CTA: 32 counters of 4 bytes each
+constexpr int kSortBatch = 8;     // tokens that a lane has on their way
 
 template <typename I> __device__ __forceinline__ int64_t token_at(const void* t, int64_t i) { return (int64_t)static_cast<const I*>(t)[i]; }
 
@@ -66,14 +67,18 @@ __global__ void __launch_bounds__(kSortThreads) castle_token_sort_kernel(const v
   int32_t* mine = count + warp * rows;
   int below = 0;
   bool bad = false;
-#pragma unroll 4
-  for (int64_t i = i0 + lane; i < i1; i += 32) {
-    const int64_t t = token_at<I>(tokens, i);
-    const bool ok = t >= 0 && t < vocab;
-    bad |= !ok;
-    if (ok && t != padding) {
-      below += t < lo;
-      if (t >= lo && t < lo + own) atomicAdd(&mine[t - lo], 1);
+  for (int64_t i = i0; i < i1; i += 32 * kSortBatch) {
+    int64_t t[kSortBatch];
+#pragma unroll
+    for (int u = 0; u < kSortBatch; ++u) t[u] = i + u * 32 + lane < i1 ? token_at<I>(tokens, i + u * 32 + lane) : padding;
+#pragma unroll
+    for (int u = 0; u < kSortBatch; ++u) {
+      const bool in = i + u * 32 + lane < i1, ok = t[u] >= 0 && t[u] < vocab;
+      bad |= in && !ok;
+      if (in && ok && t[u] != padding) {
+        below += t[u] < lo;
+        if (t[u] >= lo && t[u] < lo + own) atomicAdd(&mine[t[u] - lo], 1);
+      }
     }
   }
   if (blockIdx.x == 0 && bad) atomicOr(status, CASTLE_STATUS_BAD_INDEX);
@@ -116,23 +121,28 @@ __global__ void __launch_bounds__(kSortThreads) castle_token_sort_kernel(const v
   }
   if (tid == 0 && lo + own == vocab) start[vocab] = base;
   __syncthreads();
-  for (int64_t i = i0; i < i1; i += 32) {
-    int64_t t = -1;
-    if (i + lane < i1) t = token_at<I>(tokens, i + lane);
-    const bool hit = t >= lo && t < lo + own && t != padding;
-    const unsigned hits = __ballot_sync(0xffffffffu, hit);
-    if (!hits) continue;
-    const unsigned peers = __match_any_sync(0xffffffffu, hit ? (int)(t - lo) : -1);
-    int at = 0;
-    if (hit) at = mine[t - lo];
-    __syncwarp();
-    if (hit) {
-      const int rank = __popc(peers & ((1u << lane) - 1));
-      if (rank == 0) mine[t - lo] = at + __popc(peers);
-      sorted[at + rank] = (int32_t)(i + lane);
-      row_of[at + rank] = (int32_t)t;
+  for (int64_t i = i0; i < i1; i += 32 * kSortBatch) {
+    int local[kSortBatch];
+#pragma unroll
+    for (int u = 0; u < kSortBatch; ++u) {
+      const int64_t k = i + u * 32 + lane, t = k < i1 ? token_at<I>(tokens, k) : -1;
+      local[u] = t >= lo && t < lo + own && t != padding ? (int)(t - lo) : -1;
     }
-    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < kSortBatch; ++u) {
+      const bool hit = local[u] >= 0;
+      if (!__any_sync(0xffffffffu, hit)) continue;
+      const unsigned peers = __match_any_sync(0xffffffffu, local[u]);
+      const int at = hit ? mine[local[u]] : 0;
+      __syncwarp();
+      if (hit) {
+        const int rank = __popc(peers & ((1u << lane) - 1));
+        if (rank == 0) mine[local[u]] = at + __popc(peers);
+        sorted[at + rank] = (int32_t)(i + u * 32 + lane);
+        row_of[at + rank] = (int32_t)(lo + local[u]);
+      }
+      __syncwarp();
+    }
   }
 }
 
@@ -140,36 +150,57 @@ struct EmbGrad {
   const int32_t *start, *sorted, *row_of;
   float* partial;   // [chunk][2][dim]: of the run that the chunk begins in, and of another one that it ends in
   int64_t vocab, dy_stride;
-  int dim, slabs, piece, chunks;
+  int dim, slabs, piece, chunks, group;
   float scale;
 };
 
-// The sum of dy over entries [a, b) of the sorted list, in order; eight rows on their way at a time.
-template <typename T, bool VEC>
-__device__ __forceinline__ void sum_entries(const EmbGrad& p, const T* __restrict__ dy, int a, int b, int slab, int lane, float* acc) {
+// Eight rows of dy, a lane's columns of each, as they lie until they are added.
+template <typename T, bool VEC> struct EmbBatch {
+  Raw8<T> raw[VEC ? 8 : 1];
+  float v[VEC ? 1 : 8][8];
+  __device__ __forceinline__ void load(int u, const T* row, int slab, int lane, int dim) {
+    if constexpr (VEC) {
+      const int c = column8<32, true>(slab, lane, 0);
+      raw[u] = c < dim ? *reinterpret_cast<const Raw8<T>*>(row + c) : Raw8<T>{};
+    } else {
+      load_columns8<T, 32, false>(row, slab, lane, dim, v[u]);
+    }
+  }
+  __device__ __forceinline__ void add(int u, float* acc) const {
+    float f[8];
+    if constexpr (VEC) load8<T>(reinterpret_cast<const T*>(&raw[u]), f);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    for (int j = 0; j < 8; ++j) acc[j] += VEC ? f[j] : v[VEC ? 0 : u][j];
+  }
+};
+
+// Entries [a, b) of the sorted list in order, eight rows of dy on their way at a time; next(k) is called (by the whole warp) before
+// entry k is added to acc.
+template <typename T, bool VEC, typename F>
+__device__ __forceinline__ void walk_entries(const EmbGrad& p, const T* __restrict__ dy, int a, int b, int slab, int lane, float* acc, F&& next) {
   for (int k0 = a; k0 < b; k0 += 32) {
     const int left = min(32, b - k0);
-    const int at = lane < left ? p.sorted[k0 + lane] : 0;
+    const int at = lane < left ? p.sorted[k0 + lane] : 0, row = lane < left ? p.row_of[k0 + lane] : 0;
     for (int k = 0; k < left; k += 8) {
-      float v[8][8];
+      EmbBatch<T, VEC> batch;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int64_t i = __shfl_sync(0xffffffffu, at, min(k + u, left - 1));
-        if (k + u < left) load_columns8<T, 32, VEC>(dy + i * p.dy_stride, slab, lane, p.dim, v[u]);
+        if (k + u < left) batch.load(u, dy + i * p.dy_stride, slab, lane, p.dim);
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < 8; ++u) {
+        const int r = __shfl_sync(0xffffffffu, row, min(k + u, left - 1));
         if (k + u < left) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) acc[j] += v[u][j];
+          next(r);
+          batch.add(u, acc);
         }
+      }
     }
   }
 }
 
-// Warps [0, chunks * slabs): pieces of long rows; the others: a row's slab each.
+// Warps [0, chunks * slabs): pieces of long rows; the others: a slab of `group` rows each.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kEmbThreads) castle_embedding_bwd_kernel(const EmbGrad p, const T* __restrict__ dy, T* __restrict__ dw) {
   const int lane = threadIdx.x & 31;
@@ -177,6 +208,10 @@ __global__ void __launch_bounds__(kEmbThreads) castle_embedding_bwd_kernel(const
   overlap_wait();
   const int64_t pieces = (int64_t)p.chunks * p.slabs;
   float acc[8];
+  auto clear = [&] {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  };
   if (item < pieces) {
     const int c = (int)(item / p.slabs), slab = (int)(item % p.slabs), total = p.start[p.vocab];
     const int a = c * p.piece, b = min(total, a + p.piece);
@@ -187,21 +222,38 @@ __global__ void __launch_bounds__(kEmbThreads) castle_embedding_bwd_kernel(const
       if (side == 1 && last == first) break;
       const int r0 = p.start[row], r1 = p.start[row + 1];
       if (r1 - r0 <= p.piece) continue;
-      sum_entries<T, VEC>(p, dy, max(a, r0), min(b, r1), slab, lane, acc);
+      clear();
+      walk_entries<T, VEC>(p, dy, max(a, r0), min(b, r1), slab, lane, acc, [](int) {});
       store_columns8<float, 32, VEC>(p.partial + ((int64_t)c * 2 + side) * p.dim, slab, lane, p.dim, acc);
     }
     return;
   }
   item -= pieces;
-  if (item >= p.vocab * p.slabs) return;
-  const int64_t row = item / p.slabs;
+  const int64_t first = item / p.slabs * p.group;
   const int slab = (int)(item % p.slabs);
-  const int r0 = p.start[row], r1 = p.start[row + 1];
-  if (r1 - r0 > p.piece) return;
-  sum_entries<T, VEC>(p, dy, r0, r1, slab, lane, acc);
+  if (first >= p.vocab) return;
+  const int rows = (int)min((int64_t)p.group, p.vocab - first);
+  const int begin = p.start[first + min(lane, rows)], count = __shfl_down_sync(0xffffffffu, begin, 1) - begin;   // of row first + lane
+  const unsigned longs = __ballot_sync(0xffffffffu, lane < rows && count > p.piece);
+  T* out = dw + first * p.dim;
+  int at = 0;   // the row that is being summed
+  clear();
+  auto store = [&] {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] *= p.scale;
-  store_columns8<T, 32, VEC>(dw + row * p.dim, slab, lane, p.dim, acc);
+    for (int j = 0; j < 8; ++j) acc[j] *= p.scale;
+    store_columns8<T, 32, VEC>(out + (int64_t)at * p.dim, slab, lane, p.dim, acc);
+    clear();
+    ++at;
+  };
+  while (at < rows) {   // the rows up to the next long one, as one run of entries
+    const unsigned ahead = longs >> at;
+    const int end = ahead ? at + __ffs(ahead) - 1 : rows;
+    walk_entries<T, VEC>(p, dy, __shfl_sync(0xffffffffu, begin, at), __shfl_sync(0xffffffffu, begin, end), slab, lane, acc, [&](int row) {
+      while (at < row - (int)first) store();
+    });
+    while (at < end) store();
+    at = end + 1;   // (the long row is not this warp's)
+  }
 }
 
 // A CTA per chunk and slab: if a long row begins in the chunk, the sums of its pieces, eight shares of them in order.
@@ -273,7 +325,7 @@ static int emb_check(const char* who, int32_t dtype, int32_t index_bytes, int64_
 
 template <typename T, bool VEC>
 static cudaError_t emb_bwd(const EmbGrad& p, const T* dy, T* dw, cudaStream_t st) {
-  const int64_t warps = ((int64_t)p.chunks + p.vocab) * p.slabs;
+  const int64_t warps = ((int64_t)p.chunks + (p.vocab + p.group - 1) / p.group) * p.slabs;
   const cudaError_t e = launch_kernel(castle_embedding_bwd_kernel<T, VEC>, dim3((unsigned)((warps + 7) / 8)), kEmbThreads, 0, st, true, p, dy, dw);
   return e != cudaSuccess ? e : launch_kernel(castle_embedding_join_kernel<T, VEC>, dim3(p.chunks, p.slabs), kEmbThreads, 0, st, true, p, dw);
 }
@@ -322,6 +374,8 @@ extern "C" int castle_embedding_bwd(int32_t dtype, int32_t index_bytes, int64_t 
   p.start = start; p.sorted = sorted; p.row_of = row_of; p.partial = (float*)(ws + s.partial);
   p.vocab = vocab; p.dy_stride = dy_stride; p.dim = dim; p.slabs = (dim + 255) / 256; p.piece = emb_piece(tokens, dim);
   p.chunks = (int)((tokens + p.piece - 1) / p.piece); p.scale = scale;
+  p.group = 1;   // rows of a warp: as many as leave some sixteen warps per SM, 16 at most (one load brings where all of them begin)
+  while (p.group < 16 && vocab * p.slabs / p.group > 148 * 16) p.group *= 2;
   if (p.slabs > 65535 || ((int64_t)p.chunks + vocab) * p.slabs / 8 > 2147483646) return reject("castle_embedding_bwd: too many rows");
   // a CTA per SM, of at most kSortRows rows
   int64_t ranges = vocab < 148 ? vocab : 148;

@@ -6,11 +6,14 @@
 // All sums are fp32; the variance is taken from the centred values (a second pass over registers, none over memory), since
 // mean x^2 - m^2 loses everything where a row's offset is large.
 //
-// Both directions are bound by memory: x in and y out; x and dy in and dx out.  A row is held in the registers of a group of
-// threads (16 elements each; 32 to 512 threads, up to 8192 columns), so it is read once.  In the backward the groups of a CTA
-// take rows in turn, the next one on its way meanwhile, and keep their share of dw and db in registers; a CTA leaves one fp32
-// row of each, and a last launch adds these in a fixed order.  Wider rows, and calls that want only some of the gradients, take
-// a pass per result that reads its rows from memory (or cache) as often as it needs them.
+// Both directions should be bound by memory (x in and y out; x and dy in and dx out), but 4096 columns of bf16 at 6.5 TB/s leave an SM
+// some seven instructions per element: one kernel per row with single arithmetic was bound by instruction issue (32768 rows: 135
+// and 174 us, where the bytes take 82 and 123).  So groups of threads (16 elements each; 32 to 512 threads) stay and take rows in
+// turn: the weight (and bias) is unpacked once, arithmetic is on packed pairs, and the rows ahead are on their way into shared memory,
+// each thread's columns into places of its own (asynchronous copies that it alone waits for, so nothing has to be synchronised).
+// The backward's groups keep their share of dw and db in registers; a CTA leaves one fp32 row of each, and a last launch adds
+// these in a fixed order.  Wider rows, and calls that want only some of the gradients, take a pass per result that reads its rows
+// from memory (or cache) as often as it needs them.
 #include <type_traits>
 
 #include "common.cuh"
@@ -43,44 +46,155 @@ __device__ __forceinline__ float2 group_sum2(float a, float b, float2* s, int tu
 
 template <int THREADS> constexpr int kLnBlock = THREADS > kLnThreads ? THREADS : kLnThreads;
 
+// The columns of one thread: NV stretches of eight, as pairs.
+template <int NV> struct LnRow { float2 v[NV][4]; };
+
+// Which of them there are: whole stretches (VEC), or single ones.
+template <int THREADS, bool VEC> __device__ __forceinline__ bool has_column(int q, int t, int j, int dim) {
+  return column8<THREADS, VEC>(q, t, VEC ? 0 : j) < dim;
+}
+
+// Rows of COUNT tensors (x, or x and dy) a few ahead of their use: VEC through shared memory, single elements at the time of use.
+constexpr int ln_ahead(size_t row_bytes) { return row_bytes * 4 <= 98304 ? 4 : row_bytes * 3 <= 98304 ? 3 : row_bytes * 2 <= 131072 ? 2 : 1; }
+template <typename T, bool VEC, int THREADS, int NV, int COUNT> struct LnRows {
+  static constexpr int BLOCK = kLnBlock<THREADS>, PARTS = sizeof(Raw8<T>) / 16;
+  static constexpr size_t kRow = VEC ? (size_t)COUNT * NV * BLOCK * sizeof(Raw8<T>) : 0;
+  static constexpr int AHEAD = VEC ? ln_ahead(kRow) : 1;
+  static constexpr size_t kBytes = kRow * AHEAD;
+  const T* base[COUNT];
+  int64_t stride[COUNT], rows, step;
+  uint4* ring;   // [row ahead][tensor][stretch][16-byte part][thread]
+  int dim, t, slot;
+
+  __device__ __forceinline__ uint4* place(int s, int which, int q, int part) const { return ring + (((s * COUNT + which) * NV + q) * PARTS + part) * BLOCK + threadIdx.x; }
+  __device__ __forceinline__ void fetch(int64_t r, int s) const {
+    if constexpr (VEC) {
+      if (r < rows) {
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+          const int c = column8<THREADS, true>(q, t, 0);
+          if (c < dim) {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+              for (int k = 0; k < PARTS; ++k)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(place(s, i, q, k))),
+                             "l"(base[i] + r * stride[i] + c + k * (16 / (int)sizeof(T))) : "memory");
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");   // also of nothing, so that groups can be counted
+    }
+  }
+  __device__ __forceinline__ void begin(int64_t r) {
+    slot = 0;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) fetch(r + k * step, k);
+  }
+  // Row r, and the row AHEAD further on is sent for.  Columns that are not there are zero.
+  __device__ __forceinline__ void take(int64_t r, LnRow<NV>* out) {
+    if constexpr (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        float f[8];
+        if constexpr (VEC) {
+          alignas(16) T raw[8];
+#pragma unroll
+          for (int k = 0; k < PARTS; ++k) reinterpret_cast<uint4*>(raw)[k] = *place(slot, i, q, k);
+          load8<T>(raw, f);
+          if (!has_column<THREADS, true>(q, t, 0, dim)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = 0.f;
+          }
+        } else {
+          load_columns8<T, THREADS, false>(base[i] + r * stride[i], q, t, dim, f);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[i].v[q][j] = make_float2(f[2 * j], f[2 * j + 1]);
+      }
+    fetch(r + AHEAD * step, slot);
+    slot = slot + 1 == AHEAD ? 0 : slot + 1;
+  }
+};
+
 template <typename T, bool VEC, int THREADS, int NV>
-__global__ void __launch_bounds__(kLnBlock<THREADS>) castle_layernorm_fwd_kernel(const T* __restrict__ x, int64_t stride, const T* __restrict__ w,
-                                                                                 const T* __restrict__ b, float eps, T* __restrict__ y,
-                                                                                 float2* __restrict__ stats, int64_t rows, int dim) {
-  constexpr int GROUPS = kLnBlock<THREADS> / THREADS;
-  __shared__ float2 s[GROUPS][2 * (THREADS / 32)];
-  const int group = threadIdx.x / THREADS, t = threadIdx.x % THREADS;
-  const int64_t r = (int64_t)blockIdx.x * GROUPS + group;
-  if (r >= rows) return;
-  float v[NV][8], sum = 0.f, sq = 0.f;
+__device__ __forceinline__ void ln_param(const T* p, float none, int t, int dim, LnRow<NV>& out) {
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
-    load_columns8<T, THREADS, VEC>(x + r * stride, q, t, dim, v[q]);
+    float f[8];
+    if (p) {
+      load_columns8<T, THREADS, VEC>(p, q, t, dim, f);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum += v[q][j];
+      for (int j = 0; j < 8; ++j) f[j] = none;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out.v[q][j] = make_float2(f[2 * j], f[2 * j + 1]);
   }
-  const float mean = group_sum2<THREADS>(sum, 0.f, s[group], 0, group).x / (float)dim;
+}
+
+template <typename T, bool VEC, int THREADS, int NV>
+__device__ __forceinline__ void ln_store(T* row, int t, int dim, const LnRow<NV>& v) {
+#pragma unroll
+  for (int q = 0; q < NV; ++q) store_columns8<T, THREADS, VEC>(row, q, t, dim, reinterpret_cast<const float*>(v.v[q]));
+}
+
+// Columns that are not there become zero again after something was added to them.
+template <int THREADS, bool VEC, int NV> __device__ __forceinline__ void ln_clear(int t, int dim, LnRow<NV>& v) {
 #pragma unroll
   for (int q = 0; q < NV; ++q)
+    if (VEC ? !has_column<THREADS, true>(q, t, 0, dim) : !has_column<THREADS, false>(q, t, 7, dim)) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool in = column8<THREADS, VEC>(q, t, j) < dim;
-      v[q][j] = in ? v[q][j] - mean : 0.f;
-      sq = fmaf(v[q][j], v[q][j], sq);
+      for (int j = 0; j < 4; ++j) {
+        if (!has_column<THREADS, VEC>(q, t, 2 * j, dim)) v.v[q][j].x = 0.f;
+        if (!has_column<THREADS, VEC>(q, t, 2 * j + 1, dim)) v.v[q][j].y = 0.f;
+      }
     }
-  const float rstd = rsqrtf(group_sum2<THREADS>(sq, 0.f, s[group], 1, group).x / (float)dim + eps);
+}
+
+template <typename T, bool VEC, int THREADS, int NV>
+__global__ void __launch_bounds__(kLnBlock<THREADS>, THREADS > kLnThreads ? 1 : 3) castle_layernorm_fwd_kernel(
+    const T* __restrict__ x, int64_t stride, const T* __restrict__ w, const T* __restrict__ b, float eps, T* __restrict__ y, float2* __restrict__ stats, int64_t rows,
+    int dim) {
+  constexpr int GROUPS = kLnBlock<THREADS> / THREADS;
+  __shared__ float2 s[GROUPS][2 * (THREADS / 32)];
+  extern __shared__ __align__(16) uint4 ring[];
+  const int group = threadIdx.x / THREADS, t = threadIdx.x % THREADS;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  int64_t r = (int64_t)blockIdx.x * GROUPS + group;
+  LnRows<T, VEC, THREADS, NV, 1> in{{x}, {stride}, rows, step, ring, dim, t, 0};
+  in.begin(r);
+  LnRow<NV> g, c, v;
+  ln_param<T, VEC, THREADS, NV>(w, 1.f, t, dim, g);
+  ln_param<T, VEC, THREADS, NV>(b, 0.f, t, dim, c);
+  const float over = 1.f / (float)dim;
+  for (; r < rows; r += step) {
+    in.take(r, &v);
+    float2 sum = make_float2(0.f, 0.f), sq = sum;
 #pragma unroll
-  for (int q = 0; q < NV; ++q) {
-    float g[8], c[8];
+    for (int q = 0; q < NV; ++q)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { g[j] = 1.f; c[j] = 0.f; }
-    if (w) load_columns8<T, THREADS, VEC>(w, q, t, dim, g);
-    if (b) load_columns8<T, THREADS, VEC>(b, q, t, dim, c);
+      for (int j = 0; j < 4; ++j) sum = add2(sum, v.v[q][j]);
+    const float mean = group_sum2<THREADS>(sum.x + sum.y, 0.f, s[group], 0, group).x * over;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[q][j] = fmaf(v[q][j] * rstd, g[j], c[j]);
-    store_columns8<T, THREADS, VEC>(y + r * dim, q, t, dim, v[q]);
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v.v[q][j] = add2(v.v[q][j], splat(-mean));
+    ln_clear<THREADS, VEC, NV>(t, dim, v);
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sq = fma2(v.v[q][j], v.v[q][j], sq);
+    const float rstd = rsqrtf(group_sum2<THREADS>(sq.x + sq.y, 0.f, s[group], 1, group).x * over + eps);
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v.v[q][j] = fma2(mul2(v.v[q][j], splat(rstd)), g.v[q][j], c.v[q][j]);
+    ln_store<T, VEC, THREADS, NV>(y + r * dim, t, dim, v);
+    if (stats && t == 0) stats[r] = make_float2(mean, rstd);
   }
-  if (stats && t == 0) stats[r] = make_float2(mean, rstd);
 }
 
 // Rows of any width: a CTA per row, read three times (the second and third time from the caches).
@@ -198,66 +312,46 @@ __global__ void __launch_bounds__(kLnBlock<THREADS>, THREADS > kLnThreads ? 1 : 
   constexpr int GROUPS = kLnBlock<THREADS> / THREADS, COLS = THREADS * NV * 8;
   __shared__ float2 s[GROUPS][2 * (THREADS / 32)];
   __shared__ float add[GROUPS > 1 ? GROUPS * COLS : 1];
+  extern __shared__ __align__(16) uint4 ring[];
   const int group = threadIdx.x / THREADS, t = threadIdx.x % THREADS;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
-  float dw[NV][8], db[NV][8];
-  alignas(16) T na[NV][8], nv[NV][8];   // the next row as it lies
-  float2 nst = make_float2(0.f, 0.f);
+  int64_t r = (int64_t)blockIdx.x * GROUPS + group;
+  LnRows<T, VEC, THREADS, NV, 2> in{{x, dy}, {stride, dy_stride}, rows, step, ring, dim, t, 0};
+  in.begin(r);
+  LnRow<NV> g, dw, db;
+  ln_param<T, VEC, THREADS, NV>(w, 1.f, t, dim, g);
 #pragma unroll
   for (int q = 0; q < NV; ++q)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dw[q][j] = db[q][j] = 0.f;
-  auto fetch = [&](int64_t r) {
-#pragma unroll
-    for (int q = 0; q < NV; ++q) {
-      if constexpr (VEC) {
-        const int c = column8<THREADS, true>(q, t, 0);
-        if (c < dim) {
-          *reinterpret_cast<Raw8<T>*>(na[q]) = *reinterpret_cast<const Raw8<T>*>(dy + r * dy_stride + c);
-          *reinterpret_cast<Raw8<T>*>(nv[q]) = *reinterpret_cast<const Raw8<T>*>(x + r * stride + c);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = column8<THREADS, false>(q, t, j);
-          if (c < dim) { na[q][j] = dy[r * dy_stride + c]; nv[q][j] = x[r * stride + c]; }
-        }
-      }
-    }
-    nst = stats[r];
-  };
-  int64_t r = (int64_t)blockIdx.x * GROUPS + group;
-  if (r < rows) fetch(r);
+    for (int j = 0; j < 4; ++j) dw.v[q][j] = db.v[q][j] = make_float2(0.f, 0.f);
+  float2 next = r < rows ? stats[r] : make_float2(0.f, 0.f);
+  const float over = 1.f / (float)dim;
   for (int turn = 0; r < rows; r += step, turn ^= 1) {
-    float a[NV][8], h[NV][8], sg = 0.f, sgh = 0.f;
-    const float2 st = nst;
+    LnRow<NV> v[2];   // x, then h; dy, then dy w
+    const float2 st = next;
+    if (r + step < rows) next = stats[r + step];
+    in.take(r, v);
+    float2 sg = make_float2(0.f, 0.f), sgh = sg;
 #pragma unroll
-    for (int q = 0; q < NV; ++q) {
-      float g[8];
+    for (int q = 0; q < NV; ++q)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = 1.f;
-      if (w) load_columns8<T, THREADS, VEC>(w, q, t, dim, g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = column8<THREADS, VEC>(q, t, j) < dim;
-        const float d = in ? load1<T>(&na[q][j]) : 0.f;
-        h[q][j] = in ? (load1<T>(&nv[q][j]) - st.x) * st.y : 0.f;
-        dw[q][j] = fmaf(d, h[q][j], dw[q][j]);
-        db[q][j] += d;
-        a[q][j] = d * g[j];
-        sg += a[q][j];
-        sgh = fmaf(a[q][j], h[q][j], sgh);
+      for (int j = 0; j < 4; ++j) {
+        const float2 h = mul2(add2(v[0].v[q][j], splat(-st.x)), splat(st.y)), d = v[1].v[q][j];   // (dy is zero where there is no column)
+        dw.v[q][j] = fma2(d, h, dw.v[q][j]);
+        db.v[q][j] = add2(db.v[q][j], d);
+        const float2 a = mul2(d, g.v[q][j]);
+        sg = add2(sg, a);
+        sgh = fma2(a, h, sgh);
+        v[0].v[q][j] = h;
+        v[1].v[q][j] = a;
       }
-    }
-    if (r + step < rows) fetch(r + step);
-    const float2 sums = group_sum2<THREADS>(sg, sgh, s[group], turn, group);
-    const float mg = sums.x / (float)dim, mgh = sums.y / (float)dim;
+    const float2 sums = group_sum2<THREADS>(sg.x + sg.y, sgh.x + sgh.y, s[group], turn, group);
+    const float2 mg = splat(-sums.x * over), mgh = splat(-sums.y * over);
 #pragma unroll
-    for (int q = 0; q < NV; ++q) {
+    for (int q = 0; q < NV; ++q)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a[q][j] = st.y * (a[q][j] - mg - h[q][j] * mgh);
-      store_columns8<T, THREADS, VEC>(dx + r * dim, q, t, dim, a[q]);
-    }
+      for (int j = 0; j < 4; ++j) v[1].v[q][j] = mul2(fma2(v[0].v[q][j], mgh, add2(v[1].v[q][j], mg)), splat(st.y));
+    ln_store<T, VEC, THREADS, NV>(dx + r * dim, t, dim, v[1]);
   }
   // the groups' sums, in order
   for (int side = 0; side < 2; ++side) {
@@ -266,7 +360,7 @@ __global__ void __launch_bounds__(kLnBlock<THREADS>, THREADS > kLnThreads ? 1 : 
 #pragma unroll
       for (int q = 0; q < NV; ++q)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) add[group * COLS + column8<THREADS, VEC>(q, t, j)] = side == 0 ? dw[q][j] : db[q][j];
+        for (int j = 0; j < 8; ++j) add[group * COLS + column8<THREADS, VEC>(q, t, j)] = reinterpret_cast<const float*>(side == 0 ? dw.v[q] : db.v[q])[j];
       __syncthreads();
       for (int col = threadIdx.x; col < COLS && col < dim; col += kLnBlock<THREADS>) {
         float sum = 0.f;
@@ -280,7 +374,7 @@ __global__ void __launch_bounds__(kLnBlock<THREADS>, THREADS > kLnThreads ? 1 : 
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int col = column8<THREADS, VEC>(q, t, j);
-          if (col < dim) partial[((int64_t)blockIdx.x * 2 + side) * dim + col] = side == 0 ? dw[q][j] : db[q][j];
+          if (col < dim) partial[((int64_t)blockIdx.x * 2 + side) * dim + col] = reinterpret_cast<const float*>(side == 0 ? dw.v[q] : db.v[q])[j];
         }
     }
   }
@@ -322,28 +416,37 @@ static int ln_parts(int64_t rows, int dim) {
   return (int)(have < most ? have : most);
 }
 
-// f<THREADS, NV>() with the group that holds a row of `dim` columns, 16 or (up to 256) 8 elements a thread
-template <typename F> static void ln_group(int dim, F&& f) {
+// f(THREADS, NV) with the group that holds a row of `dim` columns, 8 NV elements a thread.
+template <typename F> static cudaError_t ln_group(int dim, F&& f) {
   using std::integral_constant;
-  if (dim <= 256) f(integral_constant<int, 32>(), integral_constant<int, 1>());
-  else if (dim <= 512) f(integral_constant<int, 32>(), integral_constant<int, 2>());
-  else if (dim <= 1024) f(integral_constant<int, 64>(), integral_constant<int, 2>());
-  else if (dim <= 2048) f(integral_constant<int, 128>(), integral_constant<int, 2>());
-  else if (dim <= 4096) f(integral_constant<int, 256>(), integral_constant<int, 2>());
-  else f(integral_constant<int, 512>(), integral_constant<int, 2>());
+  if (dim <= 256) return f(integral_constant<int, 32>(), integral_constant<int, 1>());
+  if (dim <= 512) return f(integral_constant<int, 32>(), integral_constant<int, 2>());
+  if (dim <= 1024) return f(integral_constant<int, 64>(), integral_constant<int, 2>());
+  if (dim <= 2048) return f(integral_constant<int, 128>(), integral_constant<int, 2>());
+  if (dim <= 4096) return f(integral_constant<int, 256>(), integral_constant<int, 2>());
+  return f(integral_constant<int, 512>(), integral_constant<int, 2>());
+}
+template <typename K, typename... A> static cudaError_t ln_launch(K kernel, int64_t grid, int threads, size_t ring, cudaStream_t st, A... args) {
+  if (ring > 16384) {   // (beside up to 17 KB of the kernel's own)
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
+    if (e != cudaSuccess) return e;
+  }
+  kernel<<<(unsigned)grid, threads, ring, st>>>(args...);
+  return cudaGetLastError();
 }
 
 template <typename T, bool VEC>
 static cudaError_t ln_fwd(int64_t rows, int dim, const T* x, int64_t stride, const T* w, const T* b, float eps, T* y, float2* stats, cudaStream_t st) {
   if (dim > kLnWhole) {
     castle_layernorm_fwd_wide_kernel<T, VEC><<<(unsigned)rows, kLnThreads, 0, st>>>(x, stride, w, b, eps, y, stats, dim);
-  } else {
-    ln_group(dim, [&](auto threads, auto nv) {
-      constexpr int TH = decltype(threads)::value, G = kLnBlock<TH> / TH;
-      castle_layernorm_fwd_kernel<T, VEC, TH, decltype(nv)::value><<<(unsigned)((rows + G - 1) / G), kLnBlock<TH>, 0, st>>>(x, stride, w, b, eps, y, stats, rows, dim);
-    });
+    return cudaGetLastError();
   }
-  return cudaGetLastError();
+  return ln_group(dim, [&](auto threads, auto nv) {
+    constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value, G = kLnBlock<TH> / TH;
+    const int64_t have = (rows + G - 1) / G, most = 148 * (TH > kLnThreads ? 1 : 3);
+    return ln_launch(castle_layernorm_fwd_kernel<T, VEC, TH, NV>, have < most ? have : most, kLnBlock<TH>, LnRows<T, VEC, TH, NV, 1>::kBytes, st, x, stride, w, b, eps, y,
+                     stats, rows, dim);
+  });
 }
 
 template <typename T, bool VEC>
@@ -352,10 +455,12 @@ static cudaError_t ln_bwd(int64_t rows, int dim, const T* dy, int64_t dy_stride,
   const int parts = ln_parts(rows, dim);
   const bool params = dw || db;
   if (dx && params && dim <= kLnWhole) {
-    ln_group(dim, [&](auto threads, auto nv) {
-      constexpr int TH = decltype(threads)::value;
-      castle_layernorm_bwd_kernel<T, VEC, TH, decltype(nv)::value><<<parts, kLnBlock<TH>, 0, st>>>(dy, dy_stride, x, stride, w, stats, dx, ws, rows, dim);
+    const cudaError_t e = ln_group(dim, [&](auto threads, auto nv) {
+      constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value;
+      return ln_launch(castle_layernorm_bwd_kernel<T, VEC, TH, NV>, parts, kLnBlock<TH>, LnRows<T, VEC, TH, NV, 2>::kBytes, st, dy, dy_stride, x, stride, w, stats, dx, ws,
+                       rows, dim);
     });
+    if (e != cudaSuccess) return e;
   } else {
     if (dx) castle_layernorm_dx_kernel<T, VEC><<<(unsigned)rows, kLnThreads, 0, st>>>(dy, dy_stride, x, stride, w, stats, dx, dim);
     if (params)
