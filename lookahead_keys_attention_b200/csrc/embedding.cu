@@ -12,8 +12,10 @@
 // give every (row, warp) its place, and a second reading puts the positions there, lanes with the same token in the order of the
 // lanes.  CTAs need nothing of one another, and a row that takes all the tokens is no special case.
 //
-// Sums: a warp takes a slab of 256 columns of up to 16 neighbouring rows, whose tokens are one run of the sorted list, and writes a
-// row (or the zeros of one without tokens) when the run goes on to the next; the list's entries of rows with more than `piece` tokens are cut at multiples of `piece` entries, whose sums go to scratch and are added, in order, by a third launch.
+// Sums: the sorted list is cut into chunks of `piece` entries; a warp takes a chunk's sums in a slab of 256 columns and writes a row when
+// its entries end.  (A warp per row instead took 600 us for 65536 tokens with the frequencies of text in 131072 rows of 2048; one per
+// sixteen rows 383: the frequent rows are neighbours.)  A row of more entries than a chunk leaves its parts' sums in scratch, which a
+// third launch adds in order.
 #include "common.cuh"
 #include "vec.cuh"
 
@@ -22,6 +24,7 @@ namespace castle {
 constexpr int kEmbThreads = 256, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kSortRows = 1536;   // most rows of a CTA: 32 counters of 4 bytes each
 constexpr int kSortBatch = 8;     // tokens that a lane has on their way
+constexpr int kSortSeen = 8;      // words of 32 x 32 tokens each per warp: the second reading of up to 262144 tokens skips what the first knows
 
 template <typename I> __device__ __forceinline__ int64_t token_at(const void* t, int64_t i) { return (int64_t)static_cast<const I*>(t)[i]; }
 
@@ -57,18 +60,22 @@ __global__ void __launch_bounds__(kSortThreads) castle_token_sort_kernel(const v
                                                                          int32_t* __restrict__ start, int32_t* __restrict__ sorted,
                                                                          int32_t* __restrict__ row_of, int32_t* status) {
   extern __shared__ int32_t count[];   // [warp][row]
+  __shared__ uint32_t seen[kSortWarps][kSortSeen];   // bit k: of the warp's share, 32 tokens from 32 k on, one is in the range
   __shared__ int32_t warp_sums[kSortWarps + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t lo = (int64_t)blockIdx.x * rows;
   const int own = (int)min((int64_t)rows, vocab - lo);
   const int64_t share = ((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32, i0 = warp * share, i1 = min(n, i0 + share);
   for (int k = tid; k < kSortWarps * rows; k += kSortThreads) count[k] = 0;
+  const bool skip = share <= 1024 * kSortSeen;
+  if (lane < kSortSeen) seen[warp][lane] = 0;
   __syncthreads();
   int32_t* mine = count + warp * rows;
   int below = 0;
   bool bad = false;
   for (int64_t i = i0; i < i1; i += 32 * kSortBatch) {
     int64_t t[kSortBatch];
+    unsigned hits = 0;
 #pragma unroll
     for (int u = 0; u < kSortBatch; ++u) t[u] = i + u * 32 + lane < i1 ? token_at<I>(tokens, i + u * 32 + lane) : padding;
 #pragma unroll
@@ -77,8 +84,16 @@ __global__ void __launch_bounds__(kSortThreads) castle_token_sort_kernel(const v
       bad |= in && !ok;
       if (in && ok && t[u] != padding) {
         below += t[u] < lo;
-        if (t[u] >= lo && t[u] < lo + own) atomicAdd(&mine[t[u] - lo], 1);
+        if (t[u] >= lo && t[u] < lo + own) {
+          atomicAdd(&mine[t[u] - lo], 1);
+          hits |= 1u << u;
+        }
       }
+    }
+    hits = __reduce_or_sync(0xffffffffu, hits);
+    if (skip && hits && lane == 0) {
+      const int k = (int)((i - i0) / 32);   // a multiple of the batch, which divides 32
+      seen[warp][k / 32] |= hits << (k % 32);
     }
   }
   if (blockIdx.x == 0 && bad) atomicOr(status, CASTLE_STATUS_BAD_INDEX);
@@ -123,9 +138,12 @@ __global__ void __launch_bounds__(kSortThreads) castle_token_sort_kernel(const v
   __syncthreads();
   for (int64_t i = i0; i < i1; i += 32 * kSortBatch) {
     int local[kSortBatch];
+    unsigned look = ~0u;
+    if (skip) look = seen[warp][(i - i0) / 1024] >> ((i - i0) / 32 % 32);
+    if (!(look & ((1u << kSortBatch) - 1))) continue;
 #pragma unroll
     for (int u = 0; u < kSortBatch; ++u) {
-      const int64_t k = i + u * 32 + lane, t = k < i1 ? token_at<I>(tokens, k) : -1;
+      const int64_t k = i + u * 32 + lane, t = k < i1 && (look >> u & 1) ? token_at<I>(tokens, k) : -1;
       local[u] = t >= lo && t < lo + own && t != padding ? (int)(t - lo) : -1;
     }
 #pragma unroll
@@ -174,8 +192,8 @@ template <typename T, bool VEC> struct EmbBatch {
   }
 };
 
-// Entries [a, b) of the sorted list in order, eight rows of dy on their way at a time; next(k) is called (by the whole warp) before
-// entry k is added to acc.
+// Entries [a, b) of the sorted list in order, eight rows of dy on their way at a time; next(row) is called (by the whole warp) before
+// an entry is added to acc.
 template <typename T, bool VEC, typename F>
 __device__ __forceinline__ void walk_entries(const EmbGrad& p, const T* __restrict__ dy, int a, int b, int slab, int lane, float* acc, F&& next) {
   for (int k0 = a; k0 < b; k0 += 32) {
@@ -200,7 +218,8 @@ __device__ __forceinline__ void walk_entries(const EmbGrad& p, const T* __restri
   }
 }
 
-// Warps [0, chunks * slabs): pieces of long rows; the others: a slab of `group` rows each.
+// Warps [0, chunks * slabs): the sums of a chunk's entries in a slab of columns.  A short row (up to `piece` entries, the length of
+// a chunk) belongs to the chunk in which it begins, of a longer one each chunk sums its part.  The others: zeros for rows without entries.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kEmbThreads) castle_embedding_bwd_kernel(const EmbGrad p, const T* __restrict__ dy, T* __restrict__ dw) {
   const int lane = threadIdx.x & 31;
@@ -212,47 +231,55 @@ __global__ void __launch_bounds__(kEmbThreads) castle_embedding_bwd_kernel(const
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.f;
   };
+  clear();
   if (item < pieces) {
     const int c = (int)(item / p.slabs), slab = (int)(item % p.slabs), total = p.start[p.vocab];
     const int a = c * p.piece, b = min(total, a + p.piece);
     if (a >= b) return;
-    const int first = p.row_of[a], last = p.row_of[b - 1];
-    for (int side = 0; side < 2; ++side) {
-      const int row = side == 0 ? first : last;
-      if (side == 1 && last == first) break;
-      const int r0 = p.start[row], r1 = p.start[row + 1];
-      if (r1 - r0 <= p.piece) continue;
-      clear();
-      walk_entries<T, VEC>(p, dy, max(a, r0), min(b, r1), slab, lane, acc, [](int) {});
+    auto part = [&](int from, int to, int side) {   // of a long row
+      walk_entries<T, VEC>(p, dy, from, to, slab, lane, acc, [](int) {});
       store_columns8<float, 32, VEC>(p.partial + ((int64_t)c * 2 + side) * p.dim, slab, lane, p.dim, acc);
+      clear();
+    };
+    const int first = p.row_of[a], last = p.row_of[b - 1];
+    const int f0 = p.start[first], f1 = p.start[first + 1], l0 = p.start[last], l1 = p.start[last + 1];
+    int from = a, to = l1;
+    if (f1 - f0 > p.piece) {
+      from = min(b, f1);
+      part(a, from, 0);
+    } else if (f0 < a) {
+      from = f1;
     }
+    if (l1 - l0 > p.piece) {
+      to = l0;
+      if (l0 >= from) part(l0, b, 1);
+    }
+    if (from >= to) return;
+    int row = p.row_of[from];
+    auto store = [&](int next) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] *= p.scale;
+      store_columns8<T, 32, VEC>(dw + (int64_t)row * p.dim, slab, lane, p.dim, acc);
+      clear();
+      row = next;
+    };
+    walk_entries<T, VEC>(p, dy, from, to, slab, lane, acc, [&](int next) {
+      if (next != row) store(next);
+    });
+    store(0);
     return;
   }
   item -= pieces;
-  const int64_t first = item / p.slabs * p.group;
-  const int slab = (int)(item % p.slabs);
-  if (first >= p.vocab) return;
-  const int rows = (int)min((int64_t)p.group, p.vocab - first);
-  const int begin = p.start[first + min(lane, rows)], count = __shfl_down_sync(0xffffffffu, begin, 1) - begin;   // of row first + lane
-  const unsigned longs = __ballot_sync(0xffffffffu, lane < rows && count > p.piece);
-  T* out = dw + first * p.dim;
-  int at = 0;   // the row that is being summed
-  clear();
-  auto store = [&] {
+  const int wide = (p.slabs + 3) / 4;   // four slabs at a time
+  const int64_t row0 = item / wide * p.group;
+  const int slab = (int)(item % wide) * 4;
+  if (row0 >= p.vocab) return;
+  const int rows = (int)min((int64_t)p.group, p.vocab - row0);
+  const int begin = p.start[row0 + min(lane, rows)], count = __shfl_down_sync(0xffffffffu, begin, 1) - begin;   // of row row0 + lane
+  for (unsigned none = __ballot_sync(0xffffffffu, lane < rows && count == 0); none; none &= none - 1) {
+    T* out = dw + (row0 + __ffs(none) - 1) * p.dim;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] *= p.scale;
-    store_columns8<T, 32, VEC>(out + (int64_t)at * p.dim, slab, lane, p.dim, acc);
-    clear();
-    ++at;
-  };
-  while (at < rows) {   // the rows up to the next long one, as one run of entries
-    const unsigned ahead = longs >> at;
-    const int end = ahead ? at + __ffs(ahead) - 1 : rows;
-    walk_entries<T, VEC>(p, dy, __shfl_sync(0xffffffffu, begin, at), __shfl_sync(0xffffffffu, begin, end), slab, lane, acc, [&](int row) {
-      while (at < row - (int)first) store();
-    });
-    while (at < end) store();
-    at = end + 1;   // (the long row is not this warp's)
+    for (int q = 0; q < 4; ++q) store_columns8<T, 32, VEC>(out, slab + q, lane, p.dim, acc);
   }
 }
 
@@ -291,11 +318,11 @@ __global__ void __launch_bounds__(kEmbThreads) castle_embedding_join_kernel(cons
   store_columns8<T, 32, VEC>(dw + (int64_t)row * p.dim, slab, lane, p.dim, acc);
 }
 
-// Entries per piece: as many as leave some sixteen warps per SM with a piece, 16 to 128.
+// Entries of a chunk: as many as leave some sixteen warps per SM with one, 16 to 64.
 static int emb_piece(int64_t n, int dim) {
   const int64_t slabs = (dim + 255) / 256;
   int piece = 16;
-  while (piece < 128 && n * slabs / piece > 148 * 16) piece *= 2;
+  while (piece < 64 && n * slabs / piece > 148 * 16) piece *= 2;
   return piece;
 }
 
@@ -325,7 +352,7 @@ static int emb_check(const char* who, int32_t dtype, int32_t index_bytes, int64_
 
 template <typename T, bool VEC>
 static cudaError_t emb_bwd(const EmbGrad& p, const T* dy, T* dw, cudaStream_t st) {
-  const int64_t warps = ((int64_t)p.chunks + (p.vocab + p.group - 1) / p.group) * p.slabs;
+  const int64_t warps = (int64_t)p.chunks * p.slabs + (p.vocab + p.group - 1) / p.group * ((p.slabs + 3) / 4);
   const cudaError_t e = launch_kernel(castle_embedding_bwd_kernel<T, VEC>, dim3((unsigned)((warps + 7) / 8)), kEmbThreads, 0, st, true, p, dy, dw);
   return e != cudaSuccess ? e : launch_kernel(castle_embedding_join_kernel<T, VEC>, dim3(p.chunks, p.slabs), kEmbThreads, 0, st, true, p, dw);
 }
@@ -374,8 +401,8 @@ extern "C" int castle_embedding_bwd(int32_t dtype, int32_t index_bytes, int64_t 
   p.start = start; p.sorted = sorted; p.row_of = row_of; p.partial = (float*)(ws + s.partial);
   p.vocab = vocab; p.dy_stride = dy_stride; p.dim = dim; p.slabs = (dim + 255) / 256; p.piece = emb_piece(tokens, dim);
   p.chunks = (int)((tokens + p.piece - 1) / p.piece); p.scale = scale;
-  p.group = 1;   // rows of a warp: as many as leave some sixteen warps per SM, 16 at most (one load brings where all of them begin)
-  while (p.group < 16 && vocab * p.slabs / p.group > 148 * 16) p.group *= 2;
+  p.group = 1;   // rows that a warp looks through for empty ones: as many as leave some sixteen warps per SM, 16 at most
+  while (p.group < 16 && vocab * ((p.slabs + 3) / 4) / p.group > 148 * 16) p.group *= 2;
   if (p.slabs > 65535 || ((int64_t)p.chunks + vocab) * p.slabs / 8 > 2147483646) return reject("castle_embedding_bwd: too many rows");
   // a CTA per SM, of at most kSortRows rows
   int64_t ranges = vocab < 148 ? vocab : 148;
