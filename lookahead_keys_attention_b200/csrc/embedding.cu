@@ -7,10 +7,14 @@
 // so a row's gradients are added in the order of their positions, in fp32, and the result is the same from call to call
 // (atomic additions into the rows would be in arrival order, would need an fp32 table and a pass to round it).
 //
-// Sort, one launch: a CTA owns a range of rows and reads all tokens, in as many contiguous shares as it has warps.  It counts the
-// tokens of smaller rows (where its part of the sorted list begins) and, per warp, those of each of its own; sums of these
-// give every (row, warp) its place, and a second reading puts the positions there, lanes with the same token in the order of the
-// lanes.  CTAs need nothing of one another, and a row that takes all the tokens is no special case.
+// Sort, two launches.  A row has one of 128 owners (or 256 and so on: as many as one's counters need), its number modulo theirs.  First,
+// 128 CTAs take a slice of the tokens each and put it in the order of the owners; then a CTA per owner takes its part of every slice and puts
+// these in the order of its rows.  Where an owner begins in the whole list is the sum of where it begins in the slices, so CTAs of a launch
+// need nothing of one another, and a row that takes all the tokens is no special case.  Both count per warp and key, tokens shared out among
+// the warps in contiguous parts, and sums of these give every (key, warp) its place; a second reading puts the tokens there, lanes
+// with the same key in the order of the lanes.  The list is in the order (owner, row): tokenisers give frequent tokens low
+// numbers, and owners of neighbouring rows would be as unequal as the tokens are.  (One launch, in which each owner read all tokens: 38 us
+// for 65536 of them, 108 for 200000.)
 //
 // Sums: the sorted list is cut into chunks of `piece` entries; a warp takes a chunk's sums in a slab of 256 columns and writes a row when
 // its entries end.  (A warp per row instead took 600 us for 65536 tokens with the frequencies of text in 131072 rows of 2048; one per
@@ -21,10 +25,10 @@
 
 namespace castle {
 
-constexpr int kEmbThreads = 256, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kSortRows = 1536;   // most rows of a CTA: 32 counters of 4 bytes each
-constexpr int kSortBatch = 8;     // tokens that a lane has on their way
-constexpr int kSortSeen = 8;      // words of 32 x 32 tokens each per warp: the second reading of up to 262144 tokens skips what the first knows
+constexpr int kEmbThreads = 256, kBinThreads = 512, kBinWarps = kBinThreads / 32, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kSlices = 128, kWarpSlices = kSlices / kSortWarps;
+constexpr int kSortRows = 1536;    // most rows of an owner: 32 counters of 4 bytes each
+constexpr int kMaxOwners = 2048;   // 16 counters each
 
 template <typename I> __device__ __forceinline__ int64_t token_at(const void* t, int64_t i) { return (int64_t)static_cast<const I*>(t)[i]; }
 
@@ -53,62 +57,40 @@ __global__ void __launch_bounds__(kEmbThreads) castle_embedding_fwd_kernel(const
   }
 }
 
-// start[v] = number of tokens (with a row of their own) below v; sorted[start[v] .. start[v + 1]) the positions of v's, in order;
-// row_of[k] the token of entry k.
-template <typename I>
-__global__ void __launch_bounds__(kSortThreads) castle_token_sort_kernel(const void* __restrict__ tokens, int64_t n, int64_t vocab, int64_t padding, int rows,
-                                                                         int32_t* __restrict__ start, int32_t* __restrict__ sorted,
-                                                                         int32_t* __restrict__ row_of, int32_t* status) {
-  extern __shared__ int32_t count[];   // [warp][row]
-  __shared__ uint32_t seen[kSortWarps][kSortSeen];   // bit k: of the warp's share, 32 tokens from 32 k on, one is in the range
-  __shared__ int32_t warp_sums[kSortWarps + 1];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t lo = (int64_t)blockIdx.x * rows;
-  const int own = (int)min((int64_t)rows, vocab - lo);
-  const int64_t share = ((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32, i0 = warp * share, i1 = min(n, i0 + share);
-  for (int k = tid; k < kSortWarps * rows; k += kSortThreads) count[k] = 0;
-  const bool skip = share <= 1024 * kSortSeen;
-  if (lane < kSortSeen) seen[warp][lane] = 0;
-  __syncthreads();
-  int32_t* mine = count + warp * rows;
-  int below = 0;
-  bool bad = false;
-  for (int64_t i = i0; i < i1; i += 32 * kSortBatch) {
-    int64_t t[kSortBatch];
-    unsigned hits = 0;
-#pragma unroll
-    for (int u = 0; u < kSortBatch; ++u) t[u] = i + u * 32 + lane < i1 ? token_at<I>(tokens, i + u * 32 + lane) : padding;
-#pragma unroll
-    for (int u = 0; u < kSortBatch; ++u) {
-      const bool in = i + u * 32 + lane < i1, ok = t[u] >= 0 && t[u] < vocab;
-      bad |= in && !ok;
-      if (in && ok && t[u] != padding) {
-        below += t[u] < lo;
-        if (t[u] >= lo && t[u] < lo + own) {
-          atomicAdd(&mine[t[u] - lo], 1);
-          hits |= 1u << u;
-        }
-      }
-    }
-    hits = __reduce_or_sync(0xffffffffu, hits);
-    if (skip && hits && lane == 0) {
-      const int k = (int)((i - i0) / 32);   // a multiple of the batch, which divides 32
-      seen[warp][k / 32] |= hits << (k % 32);
-    }
+// The sorted list's order of rows: row v is number (v mod owners) * per + v / owners, owners = 2^shift, per = rows of an owner.
+struct EmbOrder {
+  int shift, per;
+  __host__ __device__ __forceinline__ int owners() const { return 1 << shift; }
+  __device__ __forceinline__ int number(int row) const { return (row & (owners() - 1)) * per + (row >> shift); }
+  __device__ __forceinline__ int64_t row(int number) const { return ((int64_t)(number % per) << shift) + number / per; }
+};
+
+constexpr uint32_t kNoRow = 0xffffffffu;
+// A token as a row's number in the table; kNoRow: outside of it (`bad`), or the padding's.
+template <typename I> __device__ __forceinline__ uint32_t token_row(const void* tokens, int64_t i, uint32_t vocab, uint32_t padding, bool& bad) {
+  uint32_t t;
+  bool in;
+  if constexpr (sizeof(I) == 8) {
+    const uint2 w = static_cast<const uint2*>(tokens)[i];
+    t = w.x;
+    in = w.y == 0 && t < vocab;
+  } else {
+    t = static_cast<const uint32_t*>(tokens)[i];
+    in = t < vocab;
   }
-  if (blockIdx.x == 0 && bad) atomicOr(status, CASTLE_STATUS_BAD_INDEX);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
-  if (lane == 0) warp_sums[warp] = below;
-  __syncthreads();
-  int base = 0;
-  for (int k = 0; k < kSortWarps; ++k) base += warp_sums[k];
-  // where each row of the range begins, 1024 rows at a time
-  for (int r0 = 0; r0 < own; r0 += kSortThreads) {
-    const int r = r0 + tid;
+  bad |= !in;
+  return in && t != padding ? t : kNoRow;
+}
+
+// Counters [warp][key] of a CTA of WARPS warps become the places where each (key, warp) begins, from `base` on; begin(key, place) is called for
+// every key.  Returns the end.
+template <int WARPS, typename F> __device__ __forceinline__ int places(int32_t* count, int keys, int base, int32_t* warp_sums, F&& begin) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int k0 = 0; k0 < keys; k0 += WARPS * 32) {
+    const int key = k0 + tid;
     int total = 0;
-    if (r < own)
-      for (int k = 0; k < kSortWarps; ++k) total += count[k * rows + r];
+    if (key < keys)
+      for (int w = 0; w < WARPS; ++w) total += count[w * keys + key];
     int scan = total;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -118,48 +100,120 @@ __global__ void __launch_bounds__(kSortThreads) castle_token_sort_kernel(const v
     __syncthreads();
     if (lane == 31) warp_sums[warp] = scan;
     __syncthreads();
-    int before = base + scan - total, all = 0;
-    for (int k = 0; k < kSortWarps; ++k) {
-      if (k < warp) before += warp_sums[k];
-      all += warp_sums[k];
+    int at = base + scan - total, all = 0;
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) at += warp_sums[w];
+      all += warp_sums[w];
     }
-    if (r < own) {
-      start[lo + r] = before;
-      int at = before;
-      for (int k = 0; k < kSortWarps; ++k) {
-        const int c = count[k * rows + r];
-        count[k * rows + r] = at;
+    if (key < keys) {
+      begin(key, at);
+      for (int w = 0; w < WARPS; ++w) {
+        const int c = count[w * keys + key];
+        count[w * keys + key] = at;
         at += c;
       }
     }
     base += all;
   }
-  if (tid == 0 && lo + own == vocab) start[vocab] = base;
   __syncthreads();
-  for (int64_t i = i0; i < i1; i += 32 * kSortBatch) {
-    int local[kSortBatch];
-    unsigned look = ~0u;
-    if (skip) look = seen[warp][(i - i0) / 1024] >> ((i - i0) / 32 % 32);
-    if (!(look & ((1u << kSortBatch) - 1))) continue;
+  return base;
+}
+// The place of a lane's entry with `key` (-1: none) behind those of its warp before it; by a whole warp.
+__device__ __forceinline__ int next_place(int32_t* mine, int key, int lane) {
+  const unsigned peers = __match_any_sync(0xffffffffu, key);
+  const int at = key >= 0 ? mine[key] : 0, rank = __popc(peers & ((1u << lane) - 1));
+  __syncwarp();
+  if (key >= 0 && rank == 0) mine[key] = at + __popc(peers);
+  __syncwarp();
+  return at + rank;
+}
+
+// A slice in the order of the owners: bins[slice * length ..] as (row of the owner, position); begins[slice][owner] where each begins in it.
+template <typename I>
+__global__ void __launch_bounds__(kBinThreads) castle_token_bin_kernel(const void* __restrict__ tokens, int64_t n, int length, uint32_t vocab, uint32_t padding,
+                                                                       EmbOrder order, int2* __restrict__ bins, int32_t* __restrict__ begins, int32_t* long_count,
+                                                                       int32_t* status) {
+  extern __shared__ int32_t count[];   // [warp][owner]
+  __shared__ int32_t warp_sums[kBinWarps];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *long_count = 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, owners = order.owners();
+  const int64_t s0 = (int64_t)blockIdx.x * length, s1 = min(n, s0 + length);
+  const int share = (length + kBinThreads - 1) / kBinThreads * 32;
+  const int64_t i0 = min(s1, s0 + warp * share), i1 = min(s1, i0 + share);
+  for (int k = tid; k < kBinWarps * owners; k += kBinThreads) count[k] = 0;
+  __syncthreads();
+  int32_t* mine = count + warp * owners;
+  bool bad = false;
+#pragma unroll 4
+  for (int64_t i = i0 + lane; i < i1; i += 32) {
+    const uint32_t t = token_row<I>(tokens, i, vocab, padding, bad);
+    if (t != kNoRow) atomicAdd(&mine[t & (owners - 1)], 1);
+  }
+  if (bad) atomicOr(status, CASTLE_STATUS_BAD_INDEX);
+  __syncthreads();
+  int32_t* out = begins + (int64_t)blockIdx.x * (owners + 1);
+  const int end = places<kBinWarps>(count, owners, 0, warp_sums, [&](int owner, int at) { out[owner] = at; });
+  if (tid == 0) out[owners] = end;
+#pragma unroll 4
+  for (int64_t i = i0; i < i1; i += 32) {
+    const uint32_t t = i + lane < i1 ? token_row<I>(tokens, i + lane, vocab, padding, bad) : kNoRow;
+    const int at = next_place(mine, t != kNoRow ? (int)(t & (owners - 1)) : -1, lane);
+    if (t != kNoRow) bins[s0 + at] = make_int2((int)(t >> order.shift), (int)(i + lane));
+  }
+}
+
+// An owner's entries of all slices in the order of its rows.  start[k] = number of tokens (with a row of their own) in rows before number
+// k; sorted[start[k] .. start[k + 1]) the positions of row k's, in order; row_of[e] the number of entry e's row.
+__global__ void __launch_bounds__(kSortThreads) castle_token_sort_kernel(const int2* __restrict__ bins, const int32_t* __restrict__ begins, int length, EmbOrder order,
+                                                                         int32_t* __restrict__ start, int32_t* __restrict__ sorted, int32_t* __restrict__ row_of) {
+  extern __shared__ int32_t count[];   // [warp][row]
+  __shared__ int32_t warp_sums[kSortWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = order.per, me = blockIdx.x, owners = order.owners();
+  for (int k = tid; k < kSortWarps * rows; k += kSortThreads) count[k] = 0;
+  overlap_wait();
+  // lane j < kWarpSlices: where the owner's entries of the warp's slice j lie, and how many there are up to its end
+  int first = 0, upto = 0;
+  if (lane < kWarpSlices) {
+    const int32_t* b = begins + (int64_t)(warp * kWarpSlices + lane) * (owners + 1) + me;
+    first = b[0];
+    upto = b[1] - b[0];
+  }
+  int below = lane < kWarpSlices ? first : 0;
 #pragma unroll
-    for (int u = 0; u < kSortBatch; ++u) {
-      const int64_t k = i + u * 32 + lane, t = k < i1 && (look >> u & 1) ? token_at<I>(tokens, k) : -1;
-      local[u] = t >= lo && t < lo + own && t != padding ? (int)(t - lo) : -1;
+  for (int o = 1; o < kWarpSlices; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += up;
+    below += __shfl_xor_sync(0xffffffffu, below, o);
+  }
+  const int all = __shfl_sync(0xffffffffu, upto, kWarpSlices - 1);
+  auto entry = [&](int e) {   // of the warp's, by a whole warp; any beyond the last is not used
+    int slice = 0, before = 0;
+#pragma unroll
+    for (int j = 0; j + 1 < kWarpSlices; ++j) {
+      const int end = __shfl_sync(0xffffffffu, upto, j);
+      if (e >= end) { slice = j + 1; before = end; }
     }
-#pragma unroll
-    for (int u = 0; u < kSortBatch; ++u) {
-      const bool hit = local[u] >= 0;
-      if (!__any_sync(0xffffffffu, hit)) continue;
-      const unsigned peers = __match_any_sync(0xffffffffu, local[u]);
-      const int at = hit ? mine[local[u]] : 0;
-      __syncwarp();
-      if (hit) {
-        const int rank = __popc(peers & ((1u << lane) - 1));
-        if (rank == 0) mine[local[u]] = at + __popc(peers);
-        sorted[at + rank] = (int32_t)(i + u * 32 + lane);
-        row_of[at + rank] = (int32_t)(lo + local[u]);
-      }
-      __syncwarp();
+    const int at = __shfl_sync(0xffffffffu, first, slice) + e - before;
+    return e < all ? bins[(int64_t)(warp * kWarpSlices + slice) * length + at] : make_int2(-1, 0);
+  };
+  if (lane == 0) warp_sums[warp] = below;
+  __syncthreads();
+  int base = 0;
+  for (int k = 0; k < kSortWarps; ++k) base += warp_sums[k];
+  int32_t* mine = count + warp * rows;
+  for (int e0 = 0; e0 < all; e0 += 32) {
+    const int2 v = entry(e0 + lane);
+    if (v.x >= 0) atomicAdd(&mine[v.x], 1);
+  }
+  __syncthreads();
+  const int end = places<kSortWarps>(count, rows, base, warp_sums, [&](int row, int at) { start[(int64_t)me * rows + row] = at; });
+  if (tid == 0 && me == owners - 1) start[(int64_t)owners * rows] = end;
+  for (int e0 = 0; e0 < all; e0 += 32) {
+    const int2 v = entry(e0 + lane);
+    const int at = next_place(mine, v.x, lane);
+    if (v.x >= 0) {
+      sorted[at] = v.y;
+      row_of[at] = me * rows + v.x;
     }
   }
 }
@@ -167,9 +221,12 @@ __global__ void __launch_bounds__(kSortThreads) castle_token_sort_kernel(const v
 struct EmbGrad {
   const int32_t *start, *sorted, *row_of;
   float* partial;   // [chunk][2][dim]: of the run that the chunk begins in, and of another one that it ends in
+  EmbOrder order;
+  int numbers;      // of rows in the sorted list's order: owners * per
   int64_t vocab, dy_stride;
-  int dim, slabs, piece, chunks, group;
+  int dim, slabs, piece, chunks, sum_blocks;
   float scale;
+  int32_t *longs, *long_count;   // chunks in which a row of more than a chunk begins, in any order
 };
 
 // Eight rows of dy, a lane's columns of each, as they lie until they are added.
@@ -218,24 +275,27 @@ __device__ __forceinline__ void walk_entries(const EmbGrad& p, const T* __restri
   }
 }
 
-// Warps [0, chunks * slabs): the sums of a chunk's entries in a slab of columns.  A short row (up to `piece` entries, the length of
-// a chunk) belongs to the chunk in which it begins, of a longer one each chunk sums its part.  The others: zeros for rows without entries.
+// Blocks [0, sum_blocks), a warp each: the sums of a chunk's entries in a slab of columns.  A short row (up to `piece` entries, the length
+// of a chunk) belongs to the chunk in which it begins, of a longer one each chunk sums its part.  The other blocks: zeros for rows without
+// entries, four threads a row: bulk copies of a buffer of zeros (VEC; stores of the warps took 67 us for 200 MB beside 25 MB of sums).
+constexpr int kZeros = 1024, kZeroRows = kEmbThreads / 4;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kEmbThreads) castle_embedding_bwd_kernel(const EmbGrad p, const T* __restrict__ dy, T* __restrict__ dw) {
-  const int lane = threadIdx.x & 31;
-  int64_t item = (int64_t)blockIdx.x * (kEmbThreads / 32) + (threadIdx.x >> 5);
-  overlap_wait();
-  const int64_t pieces = (int64_t)p.chunks * p.slabs;
-  float acc[8];
-  auto clear = [&] {
+  __shared__ __align__(128) uint4 zeros[VEC ? kZeros / 16 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if ((int)blockIdx.x < p.sum_blocks) {
+    const int64_t item = (int64_t)blockIdx.x * (kEmbThreads / 32) + warp;
+    overlap_wait();
+    const int c = (int)(item / p.slabs), slab = (int)(item % p.slabs), total = p.start[p.numbers];
+    const int64_t a64 = (int64_t)c * p.piece;
+    if (a64 >= total) return;
+    const int a = (int)a64, b = min(total, a + p.piece);
+    float acc[8];
+    auto clear = [&] {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-  };
-  clear();
-  if (item < pieces) {
-    const int c = (int)(item / p.slabs), slab = (int)(item % p.slabs), total = p.start[p.vocab];
-    const int a = c * p.piece, b = min(total, a + p.piece);
-    if (a >= b) return;
+      for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    };
+    clear();
     auto part = [&](int from, int to, int side) {   // of a long row
       walk_entries<T, VEC>(p, dy, from, to, slab, lane, acc, [](int) {});
       store_columns8<float, 32, VEC>(p.partial + ((int64_t)c * 2 + side) * p.dim, slab, lane, p.dim, acc);
@@ -253,13 +313,14 @@ __global__ void __launch_bounds__(kEmbThreads) castle_embedding_bwd_kernel(const
     if (l1 - l0 > p.piece) {
       to = l0;
       if (l0 >= from) part(l0, b, 1);
+      if (l0 >= a && slab == 0 && lane == 0) p.longs[atomicAdd(p.long_count, 1)] = c;
     }
     if (from >= to) return;
     int row = p.row_of[from];
     auto store = [&](int next) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] *= p.scale;
-      store_columns8<T, 32, VEC>(dw + (int64_t)row * p.dim, slab, lane, p.dim, acc);
+      store_columns8<T, 32, VEC>(dw + p.order.row(row) * p.dim, slab, lane, p.dim, acc);
       clear();
       row = next;
     };
@@ -269,53 +330,71 @@ __global__ void __launch_bounds__(kEmbThreads) castle_embedding_bwd_kernel(const
     store(0);
     return;
   }
-  item -= pieces;
-  const int wide = (p.slabs + 3) / 4;   // four slabs at a time
-  const int64_t row0 = item / wide * p.group;
-  const int slab = (int)(item % wide) * 4;
-  if (row0 >= p.vocab) return;
-  const int rows = (int)min((int64_t)p.group, p.vocab - row0);
-  const int begin = p.start[row0 + min(lane, rows)], count = __shfl_down_sync(0xffffffffu, begin, 1) - begin;   // of row row0 + lane
-  for (unsigned none = __ballot_sync(0xffffffffu, lane < rows && count == 0); none; none &= none - 1) {
-    T* out = dw + (row0 + __ffs(none) - 1) * p.dim;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) store_columns8<T, 32, VEC>(out, slab + q, lane, p.dim, acc);
+  const int64_t row = (int64_t)(blockIdx.x - p.sum_blocks) * kZeroRows + threadIdx.x / 4;
+  if constexpr (VEC) {
+    if (threadIdx.x < kZeros / 16) zeros[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+    fence_async_smem();
+    __syncthreads();
+  }
+  overlap_wait();
+  bool none = false;
+  if (row < p.vocab) {
+    const int number = p.order.number((int)row);
+    none = p.start[number] == p.start[number + 1];
+  }
+  if constexpr (VEC) {
+    if (none) {
+      char* out = reinterpret_cast<char*>(dw + row * p.dim);
+      const int bytes = p.dim * (int)sizeof(T);
+      for (int o = (threadIdx.x & 3) * kZeros; o < bytes; o += 4 * kZeros) bulk_s2g(out + o, zeros, min(kZeros, bytes - o));
+      bulk_commit();
+      bulk_wait_read0();
+    }
+  } else {
+    const float zero[8] = {};
+    for (unsigned left = __ballot_sync(0xffffffffu, none) & 0x11111111u; left; left &= left - 1) {
+      T* out = dw + (row - lane / 4 + __ffs(left) / 4) * p.dim;
+      for (int q = 0; q < p.slabs; ++q) store_columns8<T, 32, false>(out, q, lane, p.dim, zero);
+    }
   }
 }
 
-// A CTA per chunk and slab: if a long row begins in the chunk, the sums of its pieces, eight shares of them in order.
+// A CTA per slab of a long row: the sums of its pieces, eight shares of them in order.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kEmbThreads) castle_embedding_join_kernel(const EmbGrad p, T* __restrict__ dw) {
   __shared__ float s[kEmbThreads / 32][256];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x, slab = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   overlap_wait();
-  const int total = p.start[p.vocab], a = c * p.piece, b = min(total, a + p.piece);
-  if (a >= b) return;
-  const int row = p.row_of[b - 1], r0 = p.start[row], r1 = p.start[row + 1];
-  if (r0 < a || r1 - r0 <= p.piece) return;
-  const int parts = (r1 - 1) / p.piece - c + 1, share = (parts + 7) / 8, k1 = min(parts, (warp + 1) * share);
-  float acc[8];
+  const int64_t items = (int64_t)*p.long_count * p.slabs;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int c = p.longs[item / p.slabs], slab = (int)(item % p.slabs), a = c * p.piece, b = min(p.start[p.numbers], a + p.piece);
+    const int row = p.row_of[b - 1], r0 = p.start[row], r1 = p.start[row + 1];
+    const int parts = (r1 - 1) / p.piece - c + 1, share = (parts + 7) / 8, k1 = min(parts, (warp + 1) * share);
+    float acc[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
 #pragma unroll 4
-  for (int k = warp * share; k < k1; ++k) {
-    float v[8];
-    const int side = k == 0 && r0 > a;   // in its first chunk the row is the one that the chunk ends in, unless it is the first, too
-    load_columns8<float, 32, VEC>(p.partial + ((int64_t)(c + k) * 2 + side) * p.dim, slab, lane, p.dim, v);
+    for (int k = warp * share; k < k1; ++k) {
+      float v[8];
+      const int side = k == 0 && r0 > a;   // in its first chunk the row is the one that the chunk ends in, unless it is the first, too
+      load_columns8<float, 32, VEC>(p.partial + ((int64_t)(c + k) * 2 + side) * p.dim, slab, lane, p.dim, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += v[j];
+      for (int j = 0; j < 8; ++j) acc[j] += v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[warp][j * 32 + lane] = acc[j];
+    __syncthreads();
+    if (warp == 0) {
+      for (int k = 1; k < kEmbThreads / 32; ++k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += s[k][j * 32 + lane];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] *= p.scale;
+      store_columns8<T, 32, VEC>(dw + p.order.row(row) * p.dim, slab, lane, p.dim, acc);
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) s[warp][j * 32 + lane] = acc[j];
-  __syncthreads();
-  if (warp > 0) return;
-  for (int k = 1; k < kEmbThreads / 32; ++k) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += s[k][j * 32 + lane];
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] *= p.scale;
-  store_columns8<T, 32, VEC>(dw + (int64_t)row * p.dim, slab, lane, p.dim, acc);
 }
 
 // Entries of a chunk: as many as leave some sixteen warps per SM with one, 16 to 64.
@@ -326,15 +405,28 @@ static int emb_piece(int64_t n, int dim) {
   return piece;
 }
 
-struct EmbScratch { size_t start, sorted, row_of, partial, bytes; };
+static EmbOrder emb_order(int64_t vocab) {
+  EmbOrder o{7, 0};
+  while (((vocab - 1) >> o.shift) + 1 > kSortRows) ++o.shift;
+  o.per = (int)((vocab - 1) >> o.shift) + 1;
+  return o;
+}
+
+static int emb_slice(int64_t n) { return (int)((n + kSlices - 1) / kSlices); }
+
+struct EmbScratch { size_t start, sorted, row_of, bins, begins, longs, partial, bytes; };
 static EmbScratch emb_scratch(int64_t n, int64_t vocab, int dim) {
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   const int piece = emb_piece(n, dim);
   EmbScratch s;
   s.start = 0;
-  s.sorted = up((size_t)(vocab + 1) * 4);
+  const EmbOrder order = emb_order(vocab);
+  s.sorted = up(((size_t)order.owners() * order.per + 1) * 4);
   s.row_of = s.sorted + up((size_t)n * 4);
-  s.partial = s.row_of + up((size_t)n * 4);
+  s.bins = s.row_of + up((size_t)n * 4);
+  s.begins = s.bins + up((size_t)emb_slice(n) * kSlices * sizeof(int2));
+  s.longs = s.begins + up((size_t)kSlices * (order.owners() + 1) * 4);
+  s.partial = s.longs + up(((size_t)((n + piece - 1) / piece) + 1) * 4);
   s.bytes = s.partial + (size_t)((n + piece - 1) / piece) * 2 * dim * 4;
   return s;
 }
@@ -343,7 +435,7 @@ static int emb_check(const char* who, int32_t dtype, int32_t index_bytes, int64_
                      const int32_t* status) {
   if (dtype < CASTLE_BF16 || dtype > CASTLE_F32) return reject("%s: unknown dtype", who);
   if (index_bytes != 4 && index_bytes != 8) return reject("%s: tokens must be 32- or 64-bit integers", who);
-  if (tokens <= 0 || tokens > 2147483647 || vocab <= 0 || vocab > 2147483646 || dim <= 0 || dim > (1 << 24))
+  if (tokens <= 0 || tokens > 2147483647 || vocab <= 0 || vocab > kSortRows * kMaxOwners || dim <= 0 || dim > (1 << 24))
     return reject("%s: %lld tokens, vocabulary %lld, dim %d not supported", who, (long long)tokens, (long long)vocab, dim);
   if (!index || (uintptr_t)index % index_bytes || !status) return reject("%s: tokens (aligned to their size) and a status word are needed", who);
   if (stride < 0) return reject("%s: negative strides are not supported", who);
@@ -352,9 +444,11 @@ static int emb_check(const char* who, int32_t dtype, int32_t index_bytes, int64_
 
 template <typename T, bool VEC>
 static cudaError_t emb_bwd(const EmbGrad& p, const T* dy, T* dw, cudaStream_t st) {
-  const int64_t warps = (int64_t)p.chunks * p.slabs + (p.vocab + p.group - 1) / p.group * ((p.slabs + 3) / 4);
-  const cudaError_t e = launch_kernel(castle_embedding_bwd_kernel<T, VEC>, dim3((unsigned)((warps + 7) / 8)), kEmbThreads, 0, st, true, p, dy, dw);
-  return e != cudaSuccess ? e : launch_kernel(castle_embedding_join_kernel<T, VEC>, dim3(p.chunks, p.slabs), kEmbThreads, 0, st, true, p, dw);
+  const int64_t blocks = p.sum_blocks + (p.vocab + kZeroRows - 1) / kZeroRows;
+  const cudaError_t e = launch_kernel(castle_embedding_bwd_kernel<T, VEC>, dim3((unsigned)blocks), kEmbThreads, 0, st, true, p, dy, dw);
+  if (e != cudaSuccess) return e;
+  const int64_t most = (int64_t)p.chunks * p.slabs;
+  return launch_kernel(castle_embedding_join_kernel<T, VEC>, dim3((unsigned)(most < 148 * 4 ? most : 148 * 4)), kEmbThreads, 0, st, true, p, dw);
 }
 
 }  // namespace castle
@@ -399,25 +493,27 @@ extern "C" int castle_embedding_bwd(int32_t dtype, int32_t index_bytes, int64_t 
   char* ws = static_cast<char*>(workspace);
   int32_t *start = (int32_t*)(ws + s.start), *sorted = (int32_t*)(ws + s.sorted), *row_of = (int32_t*)(ws + s.row_of);
   p.start = start; p.sorted = sorted; p.row_of = row_of; p.partial = (float*)(ws + s.partial);
+  p.order = emb_order(vocab); p.numbers = p.order.owners() * p.order.per;
   p.vocab = vocab; p.dy_stride = dy_stride; p.dim = dim; p.slabs = (dim + 255) / 256; p.piece = emb_piece(tokens, dim);
   p.chunks = (int)((tokens + p.piece - 1) / p.piece); p.scale = scale;
-  p.group = 1;   // rows that a warp looks through for empty ones: as many as leave some sixteen warps per SM, 16 at most
-  while (p.group < 16 && vocab * ((p.slabs + 3) / 4) / p.group > 148 * 16) p.group *= 2;
-  if (p.slabs > 65535 || ((int64_t)p.chunks + vocab) * p.slabs / 8 > 2147483646) return reject("castle_embedding_bwd: too many rows");
-  // a CTA per SM, of at most kSortRows rows
-  int64_t ranges = vocab < 148 ? vocab : 148;
-  if ((vocab + ranges - 1) / ranges > kSortRows) ranges = (vocab + kSortRows - 1) / kSortRows;
-  const int rows = (int)((vocab + ranges - 1) / ranges);
-  const unsigned grid = (unsigned)((vocab + rows - 1) / rows);
-  const int smem = rows * kSortWarps * 4;
+  p.longs = (int32_t*)(ws + s.longs); p.long_count = p.longs + p.chunks;
+  p.sum_blocks = (int)(((int64_t)p.chunks * p.slabs + 7) / 8);
+  if ((int64_t)p.chunks * p.slabs > 2000000000) return reject("castle_embedding_bwd: too many tokens for the width");
   const cudaStream_t st = (cudaStream_t)stream;
-  auto sort = [&](auto kernel) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortRows * kSortWarps * 4);
+  const int slice = emb_slice(tokens), bin_smem = p.order.owners() * kBinWarps * 4, sort_smem = p.order.per * kSortWarps * 4;
+  int2* bins = (int2*)(ws + s.bins);
+  int32_t* begins = (int32_t*)(ws + s.begins);
+  auto bin = [&](auto kernel) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxOwners * kBinWarps * 4);
     if (e != cudaSuccess) return e;
-    kernel<<<grid, kSortThreads, smem, st>>>(index, tokens, vocab, padding_idx, rows, start, sorted, row_of, status);
+    kernel<<<kSlices, kBinThreads, bin_smem, st>>>(index, tokens, slice, (uint32_t)vocab, padding_idx < 0 ? kNoRow : (uint32_t)padding_idx, p.order, bins, begins, p.long_count, status);
     return cudaGetLastError();
   };
-  cudaError_t e = index_bytes == 8 ? sort(castle_token_sort_kernel<int64_t>) : sort(castle_token_sort_kernel<int32_t>);
+  cudaError_t e = index_bytes == 8 ? bin(castle_token_bin_kernel<int64_t>) : bin(castle_token_bin_kernel<int32_t>);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(castle_token_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortRows * kSortWarps * 4);
+  if (e == cudaSuccess)
+    e = launch_kernel(castle_token_sort_kernel, dim3(p.order.owners()), kSortThreads, sort_smem, st, true, (const int2*)bins, (const int32_t*)begins, slice, p.order, start,
+                      sorted, row_of);
   if (e == cudaSuccess)
     by_type(dtype, [&](auto t) {
       using T = decltype(t);
