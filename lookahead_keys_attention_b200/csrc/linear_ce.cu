@@ -10,12 +10,17 @@
 //   castle_ce_kernel<kLse>   tiles of z; each leaves (max, sum of exponentials) of its part of every row
 //   castle_ce_join_kernel    these parts together: lse, the losses and their sum
 //   castle_ce_kernel<kGrad>  tiles of z again, and from them G in the operands' type, for a piece of the vocabulary
-//   castle_ce_kernel<kDx>    dx += G W of the piece (fp32 sums in scratch if there are several pieces, or shares of a long sum)
+//   castle_ce_kernel<kDx>    dx += G W of the piece (fp32 sums in scratch if there are several pieces)
 //   castle_ce_kernel<kDw>    dW of the piece
 //
-// The four products are one kernel: CTAs that stay, one per SM, with a warp that loads tiles by TMA, a warp that issues the tensor
-// cores' products (128 x 256 of the result, 64 of the contraction at a time), and eight warps that work on a finished tile in one
-// half of tensor memory while the next one is summed in the other.  All sums, the logits and the statistics are fp32.
+// The four products are one kernel: CTAs that stay, one per SM, in pairs (256 x 256 of the result, 64 of the contraction at a time) or, where
+// there is less to do, alone (128 x 256, 128 or 64), each with a warp that loads tiles by TMA, a warp that issues the tensor cores'
+// products, and eight warps that work on a finished tile in one half of tensor memory while the next one is summed in the other.
+// Alone, an SM's shared memory brings in and reads 24 KB in the 128 cycles of a product of 16, more than it can (78 % of the tensor cores' cycles at
+// a contraction of 50021); a pair shares B's tile.  All sums, the logits and the statistics are fp32.
+//
+// dx and dW have few tiles and long contractions.  As many tiles as go evenly to the workers are theirs whole; the steps of the others
+// are dealt out in equal parts, whose sums go to scratch and are added, in order, by castle_ce_sum_kernel.
 //
 // fp32 tensors: every value is the sum of three bf16 ones (8 bits each: 24), and a product is the six largest of the nine products
 // of such parts (what is left out is 2^-24 of it), the smallest first.  So the same kernels serve, with six times the steps.
@@ -37,10 +42,14 @@ namespace castle {
 
 enum CeMode { kLse, kGrad, kDx, kDw };
 
-constexpr int kCeM = 128, kCeN = 256, kCeK = 64, kCeStages = 4, kCeThreads = 320;
-constexpr uint32_t kCeA = kCeM * kCeK * 2, kCeB = kCeN * kCeK * 2, kCeStage = kCeA + kCeB;
-constexpr uint32_t kCeStaging = 8 * 4096;   // kGrad: 32 rows x 64 columns of each working warp
-constexpr size_t kCeSmem = kCeStages * kCeStage + kCeStaging + 1024;
+constexpr int kCeM = 128, kCeN = 256, kCeK = 64, kCeThreads = 320;
+constexpr uint32_t kCeA = kCeM * kCeK * 2;
+template <int PAIR> constexpr uint32_t kCeB = kCeN / PAIR * kCeK * 2;   // PAIR: CTAs that work on a tile
+template <int PAIR> constexpr uint32_t kCeStage = kCeA + kCeB<PAIR>;
+template <int PAIR> constexpr int kCeStages = PAIR == 2 ? 6 : 4;
+constexpr uint32_t kCeStaging = 8 * 4096;   // a buffer of each working warp, for results on their way out
+constexpr size_t kCeSmem = 4 * kCeStage<1> + kCeStaging + 1024;
+static_assert(kCeStages<2> * kCeStage<2> == 4 * kCeStage<1>, "");
 constexpr int64_t kCeScratch = (int64_t)1 << 30;   // bytes that a piece of the vocabulary may take
 // Steps between emptyings: of a 16-bit operand's logits (32 additions in the tensor cores), of fp32's parts (24).  197 x 512 in
 // fp32: TBD
@@ -240,167 +249,254 @@ __global__ void __launch_bounds__(256) castle_ce_split_kernel(const T* __restric
 }
 
 // ------------------------------------------------------------------------------------------------ the products
+constexpr int kCeWorkers = 148;   // CTAs of a launch
+constexpr int kCeLeast = 16;      // steps that sharing tiles out has to save a worker: a step takes 0.3 us, adding the parts some 5
 struct CeProduct {
   const CeHead* head;
   const CeRow* rows;
   int m, n, k;           // of the result and the contraction; m (kDw: k) is the number of rows that take part instead
+  int bn;                // columns of a tile
   int b_row0;            // where the piece begins in B's rows (kLse, kGrad: along n, kDx: along k)
-  int vocab0, vocab;     // the piece's first column of z, and how many there are (kLse, kGrad)
-  int terms, splits, group;
+  int vocab0;            // the piece's first column of z (kLse, kGrad)
+  int terms, group;
   int flush;             // steps after which an accumulator is emptied
+  bool share;            // tiles may be shared out among workers (kDx, kDw)
+  bool vec;              // out can be stored 16 bytes at a time
   // kLse
   float2* parts;         // [2 per tile of n][parts_ld]
   float* target_logit;
   int64_t parts_ld;
   // kDx, kDw
   void* out;             // (rows, ld)
-  float* slab;           // [split][slab_rows][slab_ld] instead of out, if not NULL
-  int64_t ld, slab_rows, slab_ld, out_row0;
-  bool vec, add;         // out can be stored 16 bytes at a time; the slab's values are added to
+  int64_t ld, out_row0;
+  float4* slab;          // parts of shared tiles: [worker][2][column / 4][row of the tile]
+  float* acc;            // kDx, several pieces of the vocabulary: sums so far, (rows that take part, acc_ld); else NULL
+  int64_t acc_ld;
+  bool acc_add, acc_out; // not the first piece; the last one
   int32_t* status;
 };
 
-template <CeMode MODE> struct CeTiles {
-  int tiles_m, tiles_n, steps, total, group;   // steps: of 64 of the contraction, all shares and terms
-  int per;                                      // steps of a share
-  __device__ __forceinline__ CeTiles(const CeProduct& p, int rows) {
-    tiles_m = ((MODE == kDw ? p.m : rows) + kCeM - 1) / kCeM;
-    tiles_n = (p.n + kCeN - 1) / kCeN;
+// What a worker (a CTA, or a pair) does: tiles, and parts of the contraction (steps of 64) of shared ones.
+template <CeMode MODE, int PAIR> struct CeWork {
+  int tiles_m, tiles_n, steps, whole, workers, group;
+  int64_t shared;   // steps of all shared tiles, the last `tiles - whole` ones
+  __device__ __forceinline__ CeWork(const CeProduct& p, int rows, int count) : workers(count) {
+    tiles_m = ((MODE == kDw ? p.m : rows) + kCeM * PAIR - 1) / (kCeM * PAIR);
+    tiles_n = (p.n + p.bn - 1) / p.bn;
     steps = ((MODE == kDw ? rows : p.k) + kCeK - 1) / kCeK;
-    per = (steps + p.splits - 1) / p.splits;
-    total = tiles_m * tiles_n * p.splits;
-    group = min(p.group, max(tiles_m, 1));
+    group = max(1, min(p.group, tiles_m));
+    whole = tiles_m * tiles_n;
+    shared = 0;
+    if (MODE == kDx || MODE == kDw) {
+      const int left = whole % workers;
+      if (p.share && left > 0 && (int64_t)steps * (workers - left) >= (int64_t)kCeLeast * workers) {
+        whole -= left;
+        shared = (int64_t)left * steps;
+      }
+    }
   }
-  // Tiles in bands of `group` tiles of rows, down the rows first: CTAs that run together share rows of both operands.
-  __device__ __forceinline__ void at(int t, int& m, int& n, int& split) const {
-    const int plane = tiles_m * tiles_n;
-    split = t / plane;
-    t -= split * plane;
+  // The i-th piece of a worker's work: tile, steps [k0, k1), slot of its part in the slab (-1: the whole tile).  False: there is none.
+  __device__ __forceinline__ bool at(int worker, int i, int& m, int& n, int& k0, int& k1, int& slot) const {
+    int t = worker + i * workers;
+    slot = -1;
+    k0 = 0;
+    k1 = steps;
+    if (t >= whole) {
+      if (shared == 0) return false;
+      const int j = i - whole / workers;   // (`whole` is a multiple of the workers then)
+      const int64_t lo = shared * worker / workers, hi = shared * (worker + 1) / workers;
+      const int tile = (int)(lo / steps) + j;
+      const int64_t begin = (int64_t)tile * steps;
+      if (j > 1 || begin >= hi) return false;
+      k0 = (int)(max(lo, begin) - begin);
+      k1 = (int)(min(hi, begin + steps) - begin);
+      if (k0 > 0 || k1 < steps) slot = j;
+      t = whole + tile;
+    }
+    place(t, m, n);
+    return true;
+  }
+  // Tiles in bands of `group` tiles of rows, down the rows first: workers that run together share rows of both operands.
+  __device__ __forceinline__ void place(int t, int& m, int& n) const {
     const int band = t / (group * tiles_n), first = band * group, high = min(group, tiles_m - first);
     t -= band * group * tiles_n;
     n = t / high;
     m = first + t - n * high;
   }
-  __device__ __forceinline__ int begin(int split) const { return min(steps, split * per); }
-  __device__ __forceinline__ int end(int split) const { return min(steps, (split + 1) * per); }
 };
 
-// T: the operands' type, OUT: the result's (kDx, kDw) or the caller's (kGrad: float means three planes of G).
-template <typename T, typename OUT, CeMode MODE>
+// Four or more values of a row of dx or dW go out: to the sums over the pieces of the vocabulary, or scaled to the result (`to`: its row).
+template <typename OUT, int COUNT>
+__device__ __forceinline__ void ce_emit(const CeProduct& p, float unit, int64_t row, int64_t to, int col, int have, float* v) {
+  if (p.acc) {
+    float* acc = p.acc + row * p.acc_ld + col;
+#pragma unroll
+    for (int j = 0; j < COUNT; j += 4)
+      if (j < have) {   // (acc_ld is a multiple of 8)
+        if (p.acc_add) {
+          const float4 old = *reinterpret_cast<const float4*>(acc + j);
+          v[j] += old.x; v[j + 1] += old.y; v[j + 2] += old.z; v[j + 3] += old.w;
+        }
+        if (!p.acc_out) *reinterpret_cast<float4*>(acc + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      }
+    if (!p.acc_out) return;
+  }
+#pragma unroll
+  for (int j = 0; j < COUNT; ++j) v[j] *= unit;
+  OUT* out = static_cast<OUT*>(p.out) + to * p.ld + col;
+  if constexpr (COUNT % 8 == 0) {
+    if (p.vec) {
+#pragma unroll
+      for (int j = 0; j < COUNT; j += 8)
+        if (j < have) store8<OUT>(out + j, v + j);
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < COUNT; ++j)
+    if (j < have) store1<OUT>(out + j, v[j]);
+}
+
+// T: the operands' type, OUT: the result's (kDx, kDw) or the caller's (kGrad: float means three planes of G).  REG: accumulators are emptied into
+// registers on the way.
+template <typename T, typename OUT, CeMode MODE, bool REG, int PAIR>
 __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_copy,
                                                                const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_g) {
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
-  constexpr bool REG = MODE == kLse || CePlanes<OUT>::count > 1;   // accumulators are emptied into registers on the way
+  constexpr int STAGES = kCeStages<PAIR>;
+  constexpr uint32_t STAGE = kCeStage<PAIR>;
+  constexpr int GRAIN = 16 * PAIR;   // columns come in multiples of it
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t bar_full[kCeStages], bar_free[kCeStages], bar_done[2], bar_read[2], bar_end;
+  __shared__ uint64_t bar_full[STAGES], bar_free[STAGES], bar_done[2], bar_read[2], bar_end;   // of a pair, full and read are the first CTA's
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = PAIR == 2 ? cluster_rank() : 0;
   if (tid == 0) {
-    for (int s = 0; s < kCeStages; ++s) { mbar_init(&bar_full[s], 1); mbar_init(&bar_free[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&bar_done[s], 1); mbar_init(&bar_read[s], 8); }
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&bar_full[s], 1); mbar_init(&bar_free[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&bar_done[s], 1); mbar_init(&bar_read[s], 8 * PAIR); }
     mbar_init(&bar_end, 1);
     mbar_fence_init();
     abort_flag = 0;
     tma_prefetch_desc(&map_a); tma_prefetch_desc(&map_b);
   }
-  if (warp == 1) { tmem_alloc(&tmem_base_s, 512); tmem_relinquish(); }
+  if (warp == 1) {
+    if constexpr (PAIR == 2) tmem_alloc_pair(&tmem_base_s, 512);
+    else { tmem_alloc(&tmem_base_s, 512); tmem_relinquish(); }
+  }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR == 2) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
   volatile int* abortp = &abort_flag;
   overlap_wait();
   const CeHead head = *p.head;
-  const CeTiles<MODE> tiles(p, head.rows);
-  const int first = blockIdx.x, stride = gridDim.x;
+  const CeWork<MODE, PAIR> work(p, head.rows, gridDim.x / PAIR);
+  const int worker = blockIdx.x / PAIR;
+  int m, n, k0, k1, slot;
+  // columns of a tile that are computed
+  auto columns = [&](int n) { return min(p.bn, (p.n - n * p.bn + GRAIN - 1) / GRAIN * GRAIN); };
 
   if (warp == 0) {
     if (elect_one()) {
       const bool copy = head.gathered;
       const CUtensorMap* ma = MODE != kDx && MODE != kDw && copy ? &map_copy : &map_a;
       const CUtensorMap* mb = MODE == kDw && copy ? &map_copy : &map_b;
+      const int b_rows = p.bn / PAIR;
+      const uint32_t bytes = (kCeA + b_rows * kCeK * 2) * PAIR;   // of the pair
       int it = 0;
-      for (int t = first; t < tiles.total && !*abortp; t += stride) {
-        int m, n, split;
-        tiles.at(t, m, n, split);
-        const int m0 = m * kCeM, n0 = n * kCeN;
-        for (int ks = tiles.begin(split); ks < tiles.end(split); ++ks) {
+      for (int i = 0; work.at(worker, i, m, n, k0, k1, slot) && !*abortp; ++i) {
+        const int m0 = (m * PAIR + rank) * kCeM, n0 = n * p.bn + (PAIR == 2 ? rank * (columns(n) / 2) : 0);
+        for (int ks = k0; ks < k1; ++ks) {
           for (int term = 6 - p.terms; term < 6; ++term, ++it) {
-            const int s = it % kCeStages, k = ks * kCeK, pa = kTermA[term], pb = kTermB[term];
-            if (!mbar_wait_ok<true>(&bar_free[s], ((uint32_t)(it / kCeStages) & 1u) ^ 1u, abortp)) { ks = tiles.end(split); break; }
-            uint8_t *a = smem + s * kCeStage, *b = a + kCeA;
-            mbar_expect_tx(&bar_full[s], kCeStage);
+            const int s = it % STAGES, k = ks * kCeK, pa = kTermA[term], pb = kTermB[term];
+            if (!mbar_wait_ok<true>(&bar_free[s], ((uint32_t)(it / STAGES) & 1u) ^ 1u, abortp)) { ks = k1; break; }
+            uint8_t *a = smem + s * STAGE, *b = a + kCeA;
+            if (rank == 0) mbar_expect_tx(&bar_full[s], bytes);
+            auto load = [&](void* dst, const CUtensorMap* map, int c0, int c1, int plane) {
+              if constexpr (PAIR == 2) tma_load_4d_pair(dst, map, of_cta(&bar_full[s], 0), c0, c1, plane, 0);
+              else tma_load_4d(dst, map, &bar_full[s], c0, c1, plane, 0);
+            };
             if (A_MN) {
-              tma_load_4d(a, ma, &bar_full[s], m0, k, pa, 0);
-              tma_load_4d(a + kCeA / 2, ma, &bar_full[s], m0 + 64, k, pa, 0);
+              load(a, ma, m0, k, pa);
+              load(a + kCeA / 2, ma, m0 + 64, k, pa);
             } else {
-              tma_load_4d(a, ma, &bar_full[s], k, m0, pa, 0);
+              load(a, ma, k, m0, pa);
             }
             if (B_MN) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) tma_load_4d(b + j * (kCeB / 4), mb, &bar_full[s], n0 + j * 64, k + (MODE == kDx ? p.b_row0 : 0), pb, 0);
+              for (int j = 0; j < kCeN / PAIR / 64; ++j) load(b + j * 8192, mb, n0 + j * 64, k + (MODE == kDx ? p.b_row0 : 0), pb);
             } else {
-              tma_load_4d(b, mb, &bar_full[s], k, p.b_row0 + n0, pb, 0);
+              load(b, mb, k, p.b_row0 + n0, pb);
             }
           }
         }
       }
       // a copy that nobody waited for (after an abort) must not arrive in another CTA's shared memory
-      if (*abortp)
-        for (int j = max(0, it - kCeStages); j < it; ++j) mbar_drain(&bar_full[j % kCeStages], (uint32_t)(j / kCeStages) & 1u);
+      if (*abortp && rank == 0)
+        for (int j = max(0, it - STAGES); j < it; ++j) mbar_drain(&bar_full[j % STAGES], (uint32_t)(j / STAGES) & 1u);
     }
   } else if (warp == 1) {
-    if (elect_one()) {
+    if (rank == 0 && elect_one()) {
+      auto commit = [&](uint64_t* bar) {
+        if constexpr (PAIR == 2) mma_commit_pair(bar);
+        else mma_commit(bar);
+      };
       int it = 0, turn = 0;
-      for (int t = first; t < tiles.total && !*abortp; t += stride) {
-        int m, n, split;
-        tiles.at(t, m, n, split);
-        const int cols = min(kCeN, (p.n - n * kCeN + 15) / 16 * 16);
-        const uint32_t idesc = make_idesc(kCeM, 16, Elem<T>::fmt, A_MN, B_MN, false) + ((uint32_t)((cols - 16) >> 3) << 17);
-        for (int k0 = tiles.begin(split); k0 < tiles.end(split) && !*abortp; k0 += p.flush, ++turn) {
-          const int acc = turn & 1, steps = min(p.flush, tiles.end(split) - k0) * p.terms;
+      for (int i = 0; work.at(worker, i, m, n, k0, k1, slot) && !*abortp; ++i) {
+        const uint32_t idesc = make_idesc(kCeM * PAIR, 16, Elem<T>::fmt, A_MN, B_MN, false) + ((uint32_t)((columns(n) - 16) >> 3) << 17);
+        for (; k0 < k1 && !*abortp; k0 += p.flush, ++turn) {
+          const int acc = turn & 1, steps = min(p.flush, k1 - k0) * p.terms;
           const uint32_t d = tmem + acc * kCeN;
           if (!mbar_wait_ok<true>(&bar_read[acc], ((uint32_t)(turn >> 1) & 1u) ^ 1u, abortp)) break;
           tc_fence_after();
           for (int j = 0; j < steps; ++j, ++it) {
-            const int s = it % kCeStages;
-            if (!mbar_wait_ok<true>(&bar_full[s], (uint32_t)(it / kCeStages) & 1u, abortp)) break;
+            const int s = it % STAGES;
+            if (!mbar_wait_ok<true>(&bar_full[s], (uint32_t)(it / STAGES) & 1u, abortp)) break;
             tc_fence_after();
-            const uint32_t a = smem_u32(smem) + s * kCeStage, b = a + kCeA;
-            const uint64_t da = A_MN ? desc_mnmajor(a, kCeA / 2) : desc_kmajor(a), db = B_MN ? desc_mnmajor(b, kCeB / 4) : desc_kmajor(b);
+            const uint32_t a = smem_u32(smem) + s * STAGE, b = a + kCeA;
+            const uint64_t da = A_MN ? desc_mnmajor(a, 8192) : desc_kmajor(a), db = B_MN ? desc_mnmajor(b, 8192) : desc_kmajor(b);
 #pragma unroll
-            for (int q = 0; q < kCeK / 16; ++q)
-              mma_ss(d, da + (uint64_t)(((A_MN ? 2048 : 32) * q) >> 4), db + (uint64_t)(((B_MN ? 2048 : 32) * q) >> 4), idesc, j > 0 || q > 0);
-            mma_commit(&bar_free[s]);
+            for (int q = 0; q < kCeK / 16; ++q) {
+              const uint64_t ao = da + (uint64_t)(((A_MN ? 2048 : 32) * q) >> 4), bo = db + (uint64_t)(((B_MN ? 2048 : 32) * q) >> 4);
+              if constexpr (PAIR == 2) mma_ss_pair(d, ao, bo, idesc, j > 0 || q > 0);
+              else mma_ss(d, ao, bo, idesc, j > 0 || q > 0);
+            }
+            commit(&bar_free[s]);
           }
-          mma_commit(&bar_done[acc]);
+          commit(&bar_done[acc]);
         }
       }
-      mma_commit(&bar_end);   // all products have read their operands
+      commit(&bar_end);   // all products have read their operands
       mbar_drain(&bar_end, 0);
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    uint8_t* staging = smem + kCeStages * kCeStage + (warp - 2) * 4096;
+    const int quarter = warp & 3, half = (warp - 2) >> 2, width = p.bn / 2;   // a warp has 32 rows and half the columns
+    const uint32_t src = tmem + half * width + ((uint32_t)(quarter * 32) << 16);
+    uint8_t* staging = smem + STAGES * STAGE + (warp - 2) * 4096;
+    const uint32_t read_at = PAIR == 2 ? of_cta(&bar_read[0], 0) : 0;
     int turn = 0;
     bool over = false;
-    for (int t = first; t < tiles.total && !over; t += stride) {
-      int m, n, split;
-      tiles.at(t, m, n, split);
-      const int row = m * kCeM + quarter * 32 + lane, c_base = n * kCeN + half * 128;
-      const int cols = min(128, p.n - c_base);   // that there are; columns from `cols` rounded up to 16 on were not computed
-      const uint32_t src = tmem + half * 128 + lanes;
-      const int k_end = tiles.end(split);
-      int k0 = tiles.begin(split);
-      const bool empty = k_end <= k0;
+    auto release = [&] {   // the accumulator has been read
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR == 2) mbar_arrive_at(read_at + (turn & 1) * 8);
+        else mbar_arrive(&bar_read[turn & 1]);
+      }
+      ++turn;
+    };
+    for (int i = 0; !over && work.at(worker, i, m, n, k0, k1, slot); ++i) {
+      const int local = rank * kCeM + quarter * 32 + lane, row = m * PAIR * kCeM + local, c_base = n * p.bn + half * width;
+      const int cols = min(width, p.n - c_base);   // that there are; of the others up to the next grain are computed
+      const bool empty = k1 <= k0;
       float sums[REG ? 128 : 1];
       if constexpr (REG) {
 #pragma unroll
         for (int j = 0; j < 128; ++j) sums[j] = 0.f;
-        for (; k0 < k_end; k0 += p.flush, ++turn) {
+        for (; k0 < k1; k0 += p.flush) {
           if (mbar_wait_failed(&bar_done[turn & 1], (uint32_t)(turn >> 1) & 1u, abortp)) { over = true; break; }
           tc_fence_after();
 #pragma unroll
@@ -412,33 +508,26 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
 #pragma unroll
             for (int j = 0; j < 16; ++j) sums[c0 + j] += v[j];
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_read[turn & 1]);
+          release();
         }
         if (over) break;
       } else if (!empty) {
         if (mbar_wait_failed(&bar_done[turn & 1], (uint32_t)(turn >> 1) & 1u, abortp)) break;
         tc_fence_after();
       }
-      // values [c0, c0 + COUNT) of the thread's half row
+      // values [c0, c0 + COUNT) of the thread's part of a row
       auto take = [&](auto count, int c0, float* v) {
         constexpr int COUNT = decltype(count)::value;
         if constexpr (REG) {
 #pragma unroll
           for (int j = 0; j < COUNT; ++j) v[j] = sums[c0 + j];
+        } else if (MODE == kDw && empty) {   // no rows take part
+#pragma unroll
+          for (int j = 0; j < COUNT; ++j) v[j] = 0.f;
         } else {
 #pragma unroll
           for (int j = 0; j < COUNT; j += 32) tmem_ld32(src + (turn & 1) * kCeN + c0 + j, v + j);
           tmem_ld_wait();
-        }
-      };
-      auto release = [&] {   // the accumulator has been read
-        if constexpr (!REG) {
-          if (empty) return;
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_read[turn & 1]);
         }
       };
       constexpr float kLog2e = 1.4426950408889634f;
@@ -487,7 +576,6 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           if (c0 >= cols) break;
           float v[64];
           take(std::integral_constant<int, 64>(), c0, v);
-          if (c0 + 64 >= cols) release();
 #pragma unroll
           for (int j = 0; j < 64; j += 2) {
             const float2 d = mul2(add2(make_float2(v[j], v[j + 1]), splat(-r.lse)), splat(kLog2e));
@@ -518,13 +606,12 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
             }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) {
-              tma_store_4d(&map_g, staging, c_base + c0, m * kCeM + quarter * 32, q, 0);
+            if (lane == 0) {   // (a tile is 128 columns wide at least: 64 for either half)
+              tma_store_4d(&map_g, staging, c_base + c0, row - lane, q, 0);
               bulk_commit();
             }
           }
         }
-        if (cols <= 0) release();   // a half without columns
       } else {
         const float unit = head.unit;
         const bool on = row < (MODE == kDw ? p.m : head.rows);
@@ -533,89 +620,60 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         for (int c0 = 0; c0 < 128; c0 += 32) {
           if (c0 >= cols) break;
           float v[32];
-          if (empty) {
+          take(std::integral_constant<int, 32>(), c0, v);
+          if (slot >= 0) {
+            float4* out = p.slab + ((int64_t)(worker * 2 + slot) * (kCeN / 4) + (half * width + c0) / 4) * (kCeM * PAIR) + local;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0.f;
-          } else {
-            take(std::integral_constant<int, 32>(), c0, v);
-          }
-          const int col = c_base + c0, have = min(32, cols - c0);
-          if (!on) {
-          } else if (p.slab) {
-            float* out = p.slab + ((int64_t)split * p.slab_rows + row) * p.slab_ld + col;
-#pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              if (j < have) {
-                float4 o = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                if (p.add) {
-                  const float4 old = *reinterpret_cast<const float4*>(out + j);
-                  o.x += old.x; o.y += old.y; o.z += old.z; o.w += old.w;
-                }
-                *reinterpret_cast<float4*>(out + j) = o;
-              }
-          } else {
-            OUT* out = static_cast<OUT*>(p.out) + to * p.ld + col;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= unit;
-            if (p.vec) {
-#pragma unroll
-              for (int j = 0; j < 32; j += 8)
-                if (j < have) store8<OUT>(out + j, v + j);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < have) store1<OUT>(out + j, v[j]);
-            }
+            for (int j = 0; j < 32; j += 4) out[(j / 4) * (kCeM * PAIR)] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          } else if (on) {
+            ce_emit<OUT, 32>(p, unit, row, to, c_base + c0, min(32, cols - c0), v);
           }
           __syncwarp();
         }
-        release();
       }
-      if (!REG && !empty) ++turn;
+      if (!REG && !empty) release();
     }
     if (MODE == kGrad && lane == 0) bulk_wait_read0();
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if constexpr (PAIR == 2) cluster_sync();   // the other's products read this CTA's tiles, its warps arrive at this CTA's barriers
+  if (warp == 1) {
+    if constexpr (PAIR == 2) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
+  }
   if (tid == 0 && abort_flag) atomicOr(p.status, CASTLE_STATUS_WAIT_TIMEOUT);
 }
 
-// The shares of a long sum, or the sums over the pieces of the vocabulary, added in order and rounded.
-struct CeSum {
-  const CeHead* head;
-  const CeRow* rows;      // dx: where each row goes; NULL: rows [0, m) of out
-  const float* slab;
-  int64_t slab_rows, slab_ld, ld, m;
-  void* out;
-  int n, splits;
-};
-template <typename OUT>
-__global__ void __launch_bounds__(256) castle_ce_sum_kernel(const CeSum p) {
+// The parts of shared tiles, added in the order of the workers: a thread per four values of a row, blockIdx.y the tile.
+template <typename OUT, CeMode MODE, int PAIR>
+__global__ void __launch_bounds__(256) castle_ce_sum_kernel(const CeProduct p) {
+  constexpr int ROWS = kCeM * PAIR;
   overlap_wait();
-  const int64_t m = p.rows ? p.head->rows : p.m;
-  const float unit = p.head->unit;
-  const int quads = (p.n + 3) / 4;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < m * quads; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / quads;
-    const int col = (int)(i - row * quads) * 4;
-    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < p.splits; ++s) {
-      const float4 v = *reinterpret_cast<const float4*>(p.slab + (s * p.slab_rows + row) * p.slab_ld + col);
-      t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
-    }
-    const float v[4] = {t.x, t.y, t.z, t.w};
-    OUT* out = static_cast<OUT*>(p.out) + (p.rows ? (int64_t)p.rows[row].row : row) * p.ld + col;
-    if (p.ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0) {
-      if constexpr (sizeof(OUT) == 4) *reinterpret_cast<float4*>(out) = make_float4(v[0] * unit, v[1] * unit, v[2] * unit, v[3] * unit);
-      else *reinterpret_cast<uint2*>(out) = make_uint2(Elem<OUT>::pack2(v[0] * unit, v[1] * unit), Elem<OUT>::pack2(v[2] * unit, v[3] * unit));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col + j < p.n) store1<OUT>(out + j, v[j] * unit);
-    }
+  const CeHead head = *p.head;
+  const int workers = kCeWorkers / PAIR;
+  const CeWork<MODE, PAIR> work(p, head.rows, workers);
+  const int tile = blockIdx.y;
+  if (work.shared == 0 || (int64_t)tile * work.steps >= work.shared) return;
+  const int64_t begin = (int64_t)tile * work.steps, end = begin + work.steps;
+  int m, n;
+  work.place(work.whole + tile, m, n);
+  const int at = blockIdx.x * 256 + threadIdx.x, local = at % ROWS, quad = at / ROWS;   // neighbouring threads: neighbouring rows
+  const int row = m * ROWS + local, col = n * p.bn + quad * 4;
+  if (row >= (MODE == kDw ? p.m : head.rows) || col >= p.n) return;
+  int w = (int)(begin * workers / work.shared);   // the first worker whose share goes beyond `begin`
+  while (work.shared * (w + 1) / workers <= begin) ++w;
+  if (work.shared * w / workers <= begin && work.shared * (w + 1) / workers >= end) return;   // one worker had all of it
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (; w < workers && work.shared * w / workers < end; ++w) {
+    const int slot = work.shared * w / workers < begin;   // its second tile
+    const float4 v = p.slab[((int64_t)(w * 2 + slot) * (kCeN / 4) + quad) * ROWS + local];
+    t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
   }
+  float v[4] = {t.x, t.y, t.z, t.w};
+  ce_emit<OUT, 4>(p, head.unit, row, MODE == kDw ? p.out_row0 + row : p.rows[row].row, col, min(4, p.n - col), v);
 }
 
 // ------------------------------------------------------------------------------------------------ the losses
@@ -699,19 +757,11 @@ __global__ void __launch_bounds__(256) castle_ce_join_kernel(const CeJoin p) {
 
 // ------------------------------------------------------------------------------------------------ host
 struct CePlan {
-  int planes, terms, pitch, piece_fwd, piece_bwd, parts_per_piece;
+  int planes, terms, pitch, piece_fwd, piece_bwd, parts_per_piece, pieces;
   bool copy_x, copy_w;        // operands are laid out anew: fp32, or rows that TMA cannot read
   int64_t copy_rows, g_rows;
-  int dx_splits, dw_splits, pieces;
-  size_t rows, copy, wcopy, parts, running, logit, sums, g, slab_dx, slab_dw, bytes;   // offsets
+  size_t rows, copy, wcopy, parts, running, logit, sums, g, slab, acc, bytes;   // offsets
 };
-
-static int ce_splits(int64_t tiles, int64_t steps) {   // shares of a long sum where the tiles alone leave SMs idle, of 16 steps at least
-  if (tiles >= 148) return 1;
-  const int64_t want = 148 / tiles, most = steps / 16;
-  const int64_t s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
-}
 
 static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, bool w_ok, bool backward) {
   CePlan q{};
@@ -723,7 +773,7 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
   q.copy_x = f32 || !x_ok;
   q.copy_w = f32 || !w_ok;
   q.copy_rows = up(n, kCeK);
-  q.g_rows = up(n, kCeM);
+  q.g_rows = up(n, 2 * kCeM);
   const int64_t w_row = q.copy_w ? (int64_t)q.planes * q.pitch * 2 : 0;
   auto piece = [&](int64_t per_column) {
     int64_t v = kCeScratch / (per_column > 0 ? per_column : 1) / kCeN * kCeN;
@@ -740,20 +790,17 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
   const int64_t most = backward ? q.piece_bwd : q.piece_fwd;
   q.wcopy = take(q.copy_w ? (size_t)most * w_row : 0);
   if (!backward) {
-    q.parts_per_piece = 2 * (int)((q.piece_fwd + kCeN - 1) / kCeN);
+    // two for each tile of a row: 256 columns, or less where 128 rows by twice as many would make fewer than 148 tiles (ce_cut)
+    const int64_t wide = (q.piece_fwd + kCeN - 1) / kCeN, few = 296 / ((n + kCeM - 1) / kCeM) + 1, most_tiles = wide > few ? wide : few;
+    q.parts_per_piece = 2 * (int)(most_tiles < (q.piece_fwd + 63) / 64 ? most_tiles : (q.piece_fwd + 63) / 64);
     q.parts = take((size_t)q.parts_per_piece * q.copy_rows * sizeof(float2));
     q.running = take((size_t)n * sizeof(float2));
     q.logit = take((size_t)n * sizeof(float));
     q.sums = take((size_t)((n + 7) / 8) * sizeof(double));
   } else {
-    const int64_t g_pitch = up(q.piece_bwd, 8);
-    q.g = take((size_t)q.planes * q.g_rows * g_pitch * 2);
-    const int64_t tiles_d = (dim + kCeN - 1) / kCeN;
-    q.dx_splits = ce_splits((n + kCeM - 1) / kCeM * tiles_d, (int64_t)q.piece_bwd / kCeK * q.terms);
-    q.dw_splits = ce_splits(((int64_t)q.piece_bwd + kCeM - 1) / kCeM * tiles_d, n / kCeK * q.terms);
-    const int64_t slab_ld = up(dim, 4);
-    q.slab_dx = take(q.dx_splits > 1 || q.pieces > 1 ? (size_t)q.dx_splits * n * slab_ld * 4 : 0);
-    q.slab_dw = take(q.dw_splits > 1 ? (size_t)q.dw_splits * q.piece_bwd * slab_ld * 4 : 0);
+    q.g = take((size_t)q.planes * q.g_rows * up(q.piece_bwd, 8) * 2);
+    q.slab = take((size_t)kCeWorkers * 2 * kCeM * kCeN * sizeof(float));
+    q.acc = take(q.pieces > 1 ? (size_t)n * up(dim, 8) * sizeof(float) : 0);
   }
   q.bytes = at;
   return q;
@@ -782,13 +829,48 @@ static int ce_map(CUtensorMap* m, const void* p, int op, int64_t rows, int cols,
   return make_tmap_16bit(m, &t, op, 1, planes, (int)rows, cols, box_rows, what);
 }
 
-template <typename T, typename OUT, CeMode MODE>
-static cudaError_t ce_launch(const CeProduct& p, int64_t most_tiles, const CUtensorMap& a, const CUtensorMap& copy, const CUtensorMap& b, const CUtensorMap& g,
-                             cudaStream_t st) {
-  auto kernel = castle_ce_kernel<T, OUT, MODE>;
+// How a result of m x n is cut: pairs of CTAs where there are tiles for half of them (or a long contraction to share out), else single
+// ones, with narrower tiles while there are SMs without one.  us, pairs / single: TBD
+struct CeCut { int pair, bn; };
+static CeCut ce_cut(int64_t m, int64_t n, bool shared, int least) {
+  const int64_t tiles = (m + 255) / 256 * ((n + 255) / 256);
+  if (m > kCeM && (tiles >= 37 || shared)) return {2, 256};
+  int bn = 256;
+  while (!shared && bn > least && (m + 127) / 128 * ((n + bn - 1) / bn) < 148) bn /= 2;
+  return {1, bn};
+}
+
+template <typename T, typename OUT, CeMode MODE, bool REG, int PAIR>
+static cudaError_t ce_launch_as(const CeProduct& p, int64_t tiles, const CUtensorMap& a, const CUtensorMap& copy, const CUtensorMap& b, const CUtensorMap& g,
+                                cudaStream_t st) {
+  auto kernel = castle_ce_kernel<T, OUT, MODE, REG, PAIR>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kCeSmem);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3((unsigned)(most_tiles < 148 ? most_tiles : 148)), kCeThreads, kCeSmem, st, true, p, a, copy, b, g);
+  const int64_t most = p.share ? kCeWorkers : tiles * PAIR;
+  cudaLaunchConfig_t c = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = PAIR;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  c.gridDim = dim3((unsigned)(most < kCeWorkers ? most : kCeWorkers));
+  c.blockDim = dim3(kCeThreads);
+  c.dynamicSmemBytes = kCeSmem;
+  c.stream = st;
+  c.attrs = attr;
+  c.numAttrs = PAIR == 2 ? 2 : 1;
+  return cudaLaunchKernelEx(&c, kernel, p, a, copy, b, g);
+}
+template <typename T, typename OUT, CeMode MODE>
+static cudaError_t ce_launch(const CeProduct& p, int pair, int64_t tiles, const CUtensorMap& a, const CUtensorMap& copy, const CUtensorMap& b, const CUtensorMap& g,
+                             cudaStream_t st) {
+  constexpr bool F32 = CePlanes<OUT>::count > 1;
+  if constexpr (MODE == kLse && !F32) {   // one emptying of an accumulator is none: it is read where it is
+    if (p.k > p.flush * kCeK)
+      return pair == 2 ? ce_launch_as<T, OUT, MODE, true, 2>(p, tiles, a, copy, b, g, st) : ce_launch_as<T, OUT, MODE, true, 1>(p, tiles, a, copy, b, g, st);
+  }
+  return pair == 2 ? ce_launch_as<T, OUT, MODE, F32, 2>(p, tiles, a, copy, b, g, st) : ce_launch_as<T, OUT, MODE, F32, 1>(p, tiles, a, copy, b, g, st);
 }
 
 static int ce_rows_per_cta(int64_t n) {   // a CTA per SM, at least 32 rows each
@@ -851,18 +933,19 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
   CE_CUDA(ce_rows<OUT>(c, q, nullptr, nullptr, nullptr, each ? loss : nullptr, lse), "castle_linear_ce_fwd launch");
   CUtensorMap x, copy, w;
   CE_TRY(ce_x_maps(c, q, op, kCeM, &x, &copy));
-  const int64_t tiles_m = (c.n + kCeM - 1) / kCeM;
   for (int64_t v0 = 0; v0 < c.vocab; v0 += q.piece_fwd) {
     const int64_t count = c.vocab - v0 < q.piece_fwd ? c.vocab - v0 : q.piece_fwd;
-    const int tiles_n = (int)((count + kCeN - 1) / kCeN);
+    const CeCut cut = ce_cut(c.n, count, false, 64);
+    const int tiles_n = (int)((count + cut.bn - 1) / cut.bn);
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), "castle_linear_ce_fwd launch");
-    CE_TRY(ce_w_map(c, q, op, count, kCeN, &w));
+    CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
     CeProduct p{};
-    p.head = (const CeHead*)c.work; p.rows = (const CeRow*)(c.work + q.rows); p.n = (int)count; p.k = q.pitch; p.b_row0 = q.copy_w ? 0 : (int)v0;
-    p.vocab0 = (int)v0; p.vocab = (int)c.vocab; p.terms = q.terms; p.splits = 1; p.group = 32;
+    p.head = (const CeHead*)c.work; p.rows = (const CeRow*)(c.work + q.rows); p.n = (int)count; p.k = q.pitch; p.bn = cut.bn; p.b_row0 = q.copy_w ? 0 : (int)v0;
+    p.vocab0 = (int)v0; p.terms = q.terms; p.group = 32 / cut.pair;
     p.flush = q.terms > 1 ? kCeFlushF32 : kCeFlush;
     p.parts = (float2*)(c.work + q.parts); p.parts_ld = q.copy_rows; p.target_logit = (float*)(c.work + q.logit); p.status = c.status;
-    CE_CUDA((ce_launch<T, OUT, kLse>(p, tiles_m * tiles_n, x, copy, w, w, c.st)), "castle_linear_ce_fwd launch");
+    const int64_t tiles_m = (c.n + kCeM * cut.pair - 1) / (kCeM * cut.pair);
+    CE_CUDA((ce_launch<T, OUT, kLse>(p, cut.pair, tiles_m * tiles_n, x, copy, w, w, c.st)), "castle_linear_ce_fwd launch");
     CeJoin j{};
     j.head = (CeHead*)c.work; j.rows = p.rows; j.parts = p.parts; j.running = (float2*)(c.work + q.running); j.target_logit = p.target_logit;
     j.sums = (double*)(c.work + q.sums); j.lse = lse; j.loss = loss; j.parts_ld = q.copy_rows; j.parts_n = 2 * tiles_n;
@@ -879,49 +962,51 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
   using T = typename CePlanes<OUT>::Op;
   const char* what = "castle_linear_ce_bwd launch";
   const int op = c.dtype == CASTLE_F16 ? CASTLE_F16 : CASTLE_BF16;
-  const int64_t tiles_m = (c.n + kCeM - 1) / kCeM, slab_ld = (c.dim + 3) / 4 * 4;
-  const int tiles_d = (c.dim + kCeN - 1) / kCeN, es = elem_size(c.dtype);
   CE_CUDA(ce_rows<OUT>(c, q, lse, dloss, dx, nullptr, nullptr), what);
   CUtensorMap x, copy, xk, copyk, w, wk, g, ga, gt;
   CE_TRY(ce_x_maps(c, q, op, kCeM, &x, &copy));
   CE_TRY(ce_x_maps(c, q, op, kCeK, &xk, &copyk));
   CeProduct base{};
-  base.head = (const CeHead*)c.work; base.rows = (const CeRow*)(c.work + q.rows); base.terms = q.terms; base.flush = q.terms > 1 ? kCeFlushF32 : kCeNoFlush; base.splits = 1; base.group = 32; base.status = c.status;
-  base.vocab = (int)c.vocab; base.ld = c.dim;
-  auto sum = [&](int splits, int64_t rows, int64_t slab_rows, bool by_row, const float* slab, void* out) {
-    CeSum s{};
-    s.head = base.head; s.rows = by_row ? base.rows : nullptr; s.slab = slab; s.slab_rows = slab_rows; s.slab_ld = slab_ld; s.ld = c.dim; s.m = rows; s.out = out;
-    s.n = c.dim; s.splits = splits;
-    const int64_t blocks = (rows * (slab_ld / 4) + 255) / 256;
-    return launch_kernel(castle_ce_sum_kernel<OUT>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), 256, 0, c.st, true, s);
+  base.head = (const CeHead*)c.work; base.rows = (const CeRow*)(c.work + q.rows); base.terms = q.terms; base.flush = q.terms > 1 ? kCeFlushF32 : kCeNoFlush;
+  base.status = c.status; base.ld = c.dim; base.bn = kCeN; base.slab = (float4*)(c.work + q.slab);
+  // What the workers share out: launched with the product whenever there could be something.
+  auto product = [&](auto mode, const CeProduct& p, const CeCut& cut, int64_t m, const CUtensorMap& a, const CUtensorMap& acopy, const CUtensorMap& b) -> cudaError_t {
+    constexpr CeMode MODE = decltype(mode)::value;
+    const int64_t tiles = (m + kCeM * cut.pair - 1) / (kCeM * cut.pair) * ((p.n + kCeN - 1) / kCeN);
+    const cudaError_t e = ce_launch<T, OUT, MODE>(p, cut.pair, tiles, a, acopy, b, b, c.st);
+    if (e != cudaSuccess || !p.share) return e;
+    const int64_t shared = tiles < kCeWorkers / cut.pair ? tiles : kCeWorkers / cut.pair;
+    const dim3 grid(kCeM * cut.pair * kCeN / 4 / 256, (unsigned)shared);
+    return cut.pair == 2 ? launch_kernel(castle_ce_sum_kernel<OUT, MODE, 2>, grid, 256, 0, c.st, true, p) : launch_kernel(castle_ce_sum_kernel<OUT, MODE, 1>, grid, 256, 0, c.st, true, p);
   };
   for (int64_t v0 = 0; v0 < c.vocab; v0 += q.piece_bwd) {
     const int64_t count = c.vocab - v0 < q.piece_bwd ? c.vocab - v0 : q.piece_bwd, pitch = (count + 7) / 8 * 8;
     uint16_t* gp = (uint16_t*)(c.work + q.g);
+    const CeCut cut = ce_cut(c.n, count, false, 128), cut_dx = ce_cut(c.n, c.dim, true, kCeN), cut_dw = ce_cut(count, c.dim, true, kCeN);
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), what);
-    CE_TRY(ce_w_map(c, q, op, count, kCeN, &w));
+    CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
     CE_TRY(ce_w_map(c, q, op, count, kCeK, &wk));
     CE_TRY(ce_map(&g, gp, op, q.g_rows, (int)count, pitch, q.g_rows * pitch, q.planes, 32, "castle_linear_ce: logits' gradient"));
     CE_TRY(ce_map(&ga, gp, op, q.g_rows, (int)count, pitch, q.g_rows * pitch, q.planes, kCeM, "castle_linear_ce: logits' gradient"));
     CE_TRY(ce_map(&gt, gp, op, q.g_rows, (int)count, pitch, q.g_rows * pitch, q.planes, kCeK, "castle_linear_ce: logits' gradient"));
     CeProduct p = base;
-    p.n = (int)count; p.k = q.pitch; p.b_row0 = q.copy_w ? 0 : (int)v0; p.vocab0 = (int)v0;
-    CE_CUDA((ce_launch<T, OUT, kGrad>(p, tiles_m * ((count + kCeN - 1) / kCeN), x, copy, w, g, c.st)), what);
+    p.n = (int)count; p.k = q.pitch; p.bn = cut.bn; p.b_row0 = q.copy_w ? 0 : (int)v0; p.vocab0 = (int)v0; p.group = 32 / cut.pair;
+    const int64_t tiles_m = (c.n + kCeM * cut.pair - 1) / (kCeM * cut.pair);
+    CE_CUDA((ce_launch<T, OUT, kGrad>(p, cut.pair, tiles_m * ((count + cut.bn - 1) / cut.bn), x, copy, w, g, c.st)), what);
     if (dx) {
       p = base;
-      p.n = c.dim; p.k = (int)count; p.b_row0 = q.copy_w ? 0 : (int)v0; p.out = dx; p.splits = q.dx_splits; p.group = 16;
+      p.n = c.dim; p.k = (int)count; p.b_row0 = q.copy_w ? 0 : (int)v0; p.out = dx; p.group = 16 / cut_dx.pair;
       p.vec = c.dim % 8 == 0 && (uintptr_t)dx % 16 == 0;
-      if (q.dx_splits > 1 || q.pieces > 1) { p.slab = (float*)(c.work + q.slab_dx); p.slab_rows = c.n; p.slab_ld = slab_ld; p.add = v0 > 0; }
-      CE_CUDA((ce_launch<T, OUT, kDx>(p, tiles_m * tiles_d * p.splits, ga, ga, wk, wk, c.st)), what);
-      if (p.slab && v0 + count == c.vocab) CE_CUDA(sum(p.splits, c.n, c.n, true, p.slab, dx), what);
+      p.share = (p.k + kCeK - 1) / kCeK >= kCeLeast;
+      if (q.pieces > 1) { p.acc = (float*)(c.work + q.acc); p.acc_ld = (c.dim + 7) / 8 * 8; p.acc_add = v0 > 0; p.acc_out = v0 + count == c.vocab; }
+      CE_CUDA(product(std::integral_constant<CeMode, kDx>(), p, cut_dx, c.n, ga, ga, wk), what);
     }
     if (dw) {
       p = base;
-      p.m = (int)count; p.n = c.dim; p.out = dw; p.out_row0 = v0; p.splits = q.dw_splits; p.group = 16;
+      p.m = (int)count; p.n = c.dim; p.out = dw; p.out_row0 = v0; p.group = 16 / cut_dw.pair;
       p.vec = c.dim % 8 == 0 && (uintptr_t)dw % 16 == 0;
-      if (q.dw_splits > 1) { p.slab = (float*)(c.work + q.slab_dw); p.slab_rows = q.piece_bwd; p.slab_ld = slab_ld; }
-      CE_CUDA((ce_launch<T, OUT, kDw>(p, (count + kCeM - 1) / kCeM * tiles_d * p.splits, gt, copyk, xk, xk, c.st)), what);
-      if (p.slab) CE_CUDA(sum(p.splits, count, p.slab_rows, false, p.slab, static_cast<char*>(dw) + v0 * c.dim * es), what);
+      p.share = (c.n + kCeK - 1) / kCeK >= kCeLeast;
+      CE_CUDA(product(std::integral_constant<CeMode, kDw>(), p, cut_dw, count, gt, copyk, xk), what);
     }
   }
   return 0;
