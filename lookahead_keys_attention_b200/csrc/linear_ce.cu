@@ -19,8 +19,8 @@
 // Alone, an SM's shared memory brings in and reads 24 KB in the 128 cycles of a product of 16, more than it can (78 % of the tensor cores' cycles at
 // a contraction of 50021); a pair shares B's tile.  All sums, the logits and the statistics are fp32.
 //
-// dx and dW have few tiles and long contractions.  As many tiles as go evenly to the workers are theirs whole; the steps of the others
-// are dealt out in equal parts, whose sums go to scratch and are added, in order, by castle_ce_sum_kernel.
+// dx and dW can have few tiles and long contractions.  As many tiles as go evenly to the workers are theirs whole; of the others the
+// contraction is cut into slices, whose sums go to scratch and are added, in order, by castle_ce_sum_kernel.
 //
 // fp32 tensors: every value is the sum of three bf16 ones (8 bits each: 24), and a product is the six largest of the nine products
 // of such parts (what is left out is 2^-24 of it), the smallest first.  So the same kernels serve, with six times the steps.
@@ -250,7 +250,8 @@ __global__ void __launch_bounds__(256) castle_ce_split_kernel(const T* __restric
 
 // ------------------------------------------------------------------------------------------------ the products
 constexpr int kCeWorkers = 148;   // CTAs of a launch
-constexpr int kCeLeast = 16;      // steps that sharing tiles out has to save a worker: a step takes 0.3 us, adding the parts some 5
+constexpr int kCeShare = 24;   // steps from which on it can pay to share tiles out
+constexpr int kCeParts = 4 * kCeWorkers;   // tiles of one CTA that the slab holds
 struct CeProduct {
   const CeHead* head;
   const CeRow* rows;
@@ -269,49 +270,61 @@ struct CeProduct {
   // kDx, kDw
   void* out;             // (rows, ld)
   int64_t ld, out_row0;
-  float4* slab;          // parts of shared tiles: [worker][2][column / 4][row of the tile]
+  float4* slab;          // parts of shared tiles: [part][column / 4][row of the tile]
   float* acc;            // kDx, several pieces of the vocabulary: sums so far, (rows that take part, acc_ld); else NULL
   int64_t acc_ld;
   bool acc_add, acc_out; // not the first piece; the last one
   int32_t* status;
 };
 
-// What a worker (a CTA, or a pair) does: tiles, and parts of the contraction (steps of 64) of shared ones.
+// What a worker (a CTA, or a pair) does: tiles, and slices of the contraction (steps of 64) of those that do not go evenly to the workers.
+// Slices are dealt out one after the other, each with all its tiles, so that workers that run together read the same part of the operands
+// (one worker's equal share of all steps in a row instead read them from memory again and again: 243 us where this takes TBD).
 template <CeMode MODE, int PAIR> struct CeWork {
-  int tiles_m, tiles_n, steps, whole, workers, group;
-  int64_t shared;   // steps of all shared tiles, the last `tiles - whole` ones
+  int tiles_m, tiles_n, steps, whole, left, slices, per, workers, group;
   __device__ __forceinline__ CeWork(const CeProduct& p, int rows, int count) : workers(count) {
     tiles_m = ((MODE == kDw ? p.m : rows) + kCeM * PAIR - 1) / (kCeM * PAIR);
     tiles_n = (p.n + p.bn - 1) / p.bn;
     steps = ((MODE == kDw ? rows : p.k) + kCeK - 1) / kCeK;
     group = max(1, min(p.group, tiles_m));
     whole = tiles_m * tiles_n;
-    shared = 0;
-    if (MODE == kDx || MODE == kDw) {
-      const int left = whole % workers;
-      if (p.share && left > 0 && (int64_t)steps * (workers - left) >= (int64_t)kCeLeast * workers) {
-        whole -= left;
-        shared = (int64_t)left * steps;
+    left = 0;
+    slices = 1;
+    per = steps;
+    if ((MODE == kDx || MODE == kDw) && p.share) {
+      // The least time in steps (0.3 us): rounds times a slice's steps, and for several slices the launch that adds them (5 us) and its
+      // 256 or 128 KB a part, written and read.
+      const int rest = whole % workers;
+      float best = (float)steps;
+#pragma unroll
+      for (int k = 0; k < 11; ++k) {
+        const int s = k < 5 ? k + 2 : k == 5 ? 8 : k == 6 ? 12 : k == 7 ? 16 : k == 8 ? 24 : k == 9 ? 32 : 37;
+        if (rest == 0 || s > steps || rest * s * PAIR > kCeParts) continue;
+        const float time = (float)((rest * s + workers - 1) / workers) * (float)((steps + s - 1) / s) + 16.f + 0.18f * PAIR * (float)(rest * s);
+        if (time < best) { best = time; slices = s; }
+      }
+      if (slices > 1) {
+        per = (steps + slices - 1) / slices;
+        slices = (steps + per - 1) / per;
+        left = rest;
+        whole -= rest;
       }
     }
   }
-  // The i-th piece of a worker's work: tile, steps [k0, k1), slot of its part in the slab (-1: the whole tile).  False: there is none.
+  // The i-th piece of a worker's work: tile, steps [k0, k1), its part's place in the slab (-1: the whole tile).  False: there is none.
   __device__ __forceinline__ bool at(int worker, int i, int& m, int& n, int& k0, int& k1, int& slot) const {
     int t = worker + i * workers;
     slot = -1;
     k0 = 0;
     k1 = steps;
     if (t >= whole) {
-      if (shared == 0) return false;
-      const int j = i - whole / workers;   // (`whole` is a multiple of the workers then)
-      const int64_t lo = shared * worker / workers, hi = shared * (worker + 1) / workers;
-      const int tile = (int)(lo / steps) + j;
-      const int64_t begin = (int64_t)tile * steps;
-      if (j > 1 || begin >= hi) return false;
-      k0 = (int)(max(lo, begin) - begin);
-      k1 = (int)(min(hi, begin + steps) - begin);
-      if (k0 > 0 || k1 < steps) slot = j;
-      t = whole + tile;
+      const int part = t - whole;
+      if (part >= left * slices) return false;
+      const int slice = part / left;
+      k0 = slice * per;
+      k1 = min(steps, k0 + per);
+      slot = part;
+      t = whole + part - slice * left;
     }
     place(t, m, n);
     return true;
@@ -622,7 +635,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           float v[32];
           take(std::integral_constant<int, 32>(), c0, v);
           if (slot >= 0) {
-            float4* out = p.slab + ((int64_t)(worker * 2 + slot) * (kCeN / 4) + (half * width + c0) / 4) * (kCeM * PAIR) + local;
+            float4* out = p.slab + ((int64_t)slot * (kCeN / 4) + (half * width + c0) / 4) * (kCeM * PAIR) + local;
 #pragma unroll
             for (int j = 0; j < 32; j += 4) out[(j / 4) * (kCeM * PAIR)] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
           } else if (on) {
@@ -646,30 +659,24 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
   if (tid == 0 && abort_flag) atomicOr(p.status, CASTLE_STATUS_WAIT_TIMEOUT);
 }
 
-// The parts of shared tiles, added in the order of the workers: a thread per four values of a row, blockIdx.y the tile.
+// The parts of shared tiles, added in order: a thread per four values of a row, blockIdx.y the tile.
 template <typename OUT, CeMode MODE, int PAIR>
 __global__ void __launch_bounds__(256) castle_ce_sum_kernel(const CeProduct p) {
   constexpr int ROWS = kCeM * PAIR;
   overlap_wait();
   const CeHead head = *p.head;
-  const int workers = kCeWorkers / PAIR;
-  const CeWork<MODE, PAIR> work(p, head.rows, workers);
+  const CeWork<MODE, PAIR> work(p, head.rows, kCeWorkers / PAIR);
   const int tile = blockIdx.y;
-  if (work.shared == 0 || (int64_t)tile * work.steps >= work.shared) return;
-  const int64_t begin = (int64_t)tile * work.steps, end = begin + work.steps;
+  if (tile >= work.left) return;
   int m, n;
   work.place(work.whole + tile, m, n);
   const int at = blockIdx.x * 256 + threadIdx.x, local = at % ROWS, quad = at / ROWS;   // neighbouring threads: neighbouring rows
   const int row = m * ROWS + local, col = n * p.bn + quad * 4;
   if (row >= (MODE == kDw ? p.m : head.rows) || col >= p.n) return;
-  int w = (int)(begin * workers / work.shared);   // the first worker whose share goes beyond `begin`
-  while (work.shared * (w + 1) / workers <= begin) ++w;
-  if (work.shared * w / workers <= begin && work.shared * (w + 1) / workers >= end) return;   // one worker had all of it
   float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (; w < workers && work.shared * w / workers < end; ++w) {
-    const int slot = work.shared * w / workers < begin;   // its second tile
-    const float4 v = p.slab[((int64_t)(w * 2 + slot) * (kCeN / 4) + quad) * ROWS + local];
+#pragma unroll 8
+  for (int s = 0; s < work.slices; ++s) {
+    const float4 v = p.slab[((int64_t)(s * work.left + tile) * (kCeN / 4) + quad) * ROWS + local];
     t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
   }
   float v[4] = {t.x, t.y, t.z, t.w};
@@ -799,7 +806,7 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
     q.sums = take((size_t)((n + 7) / 8) * sizeof(double));
   } else {
     q.g = take((size_t)q.planes * q.g_rows * up(q.piece_bwd, 8) * 2);
-    q.slab = take((size_t)kCeWorkers * 2 * kCeM * kCeN * sizeof(float));
+    q.slab = take((size_t)kCeParts * kCeM * kCeN * sizeof(float));
     q.acc = take(q.pieces > 1 ? (size_t)n * up(dim, 8) * sizeof(float) : 0);
   }
   q.bytes = at;
@@ -997,7 +1004,7 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
       p = base;
       p.n = c.dim; p.k = (int)count; p.b_row0 = q.copy_w ? 0 : (int)v0; p.out = dx; p.group = 16 / cut_dx.pair;
       p.vec = c.dim % 8 == 0 && (uintptr_t)dx % 16 == 0;
-      p.share = (p.k + kCeK - 1) / kCeK >= kCeLeast;
+      p.share = (p.k + kCeK - 1) / kCeK >= kCeShare;
       if (q.pieces > 1) { p.acc = (float*)(c.work + q.acc); p.acc_ld = (c.dim + 7) / 8 * 8; p.acc_add = v0 > 0; p.acc_out = v0 + count == c.vocab; }
       CE_CUDA(product(std::integral_constant<CeMode, kDx>(), p, cut_dx, c.n, ga, ga, wk), what);
     }
@@ -1005,7 +1012,7 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
       p = base;
       p.m = (int)count; p.n = c.dim; p.out = dw; p.out_row0 = v0; p.group = 16 / cut_dw.pair;
       p.vec = c.dim % 8 == 0 && (uintptr_t)dw % 16 == 0;
-      p.share = (c.n + kCeK - 1) / kCeK >= kCeLeast;
+      p.share = (c.n + kCeK - 1) / kCeK >= kCeShare;
       CE_CUDA(product(std::integral_constant<CeMode, kDw>(), p, cut_dw, count, gt, copyk, xk), what);
     }
   }
