@@ -42,12 +42,14 @@ namespace castle {
 
 enum CeMode { kLse, kGrad, kDx, kDw };
 
-constexpr int kCeM = 128, kCeN = 256, kCeK = 64, kCeThreads = 320;
+constexpr int kCeM = 128, kCeN = 256, kCeK = 64;
+// The warps that work on tiles.  (Sixteen instead of eight: no faster; the logits' gradient of 4095 x 1024 against 50021 188 us instead of 172.)
+constexpr int kCeWarps = 8, kCeShares = kCeWarps / 4, kCeThreads = (kCeWarps + 2) * 32, kCeWidth = kCeN / kCeShares;
 constexpr uint32_t kCeA = kCeM * kCeK * 2;
 template <int PAIR> constexpr uint32_t kCeB = kCeN / PAIR * kCeK * 2;   // PAIR: CTAs that work on a tile
 template <int PAIR> constexpr uint32_t kCeStage = kCeA + kCeB<PAIR>;
 template <int PAIR> constexpr int kCeStages = PAIR == 2 ? 6 : 4;
-constexpr uint32_t kCeStaging = 8 * 4096;   // a buffer of each working warp, for results on their way out
+constexpr uint32_t kCeStaging = kCeWarps * 4096;   // kGrad: 32 rows x 64 columns of each working warp
 constexpr size_t kCeSmem = 4 * kCeStage<1> + kCeStaging + 1024;
 static_assert(kCeStages<2> * kCeStage<2> == 4 * kCeStage<1>, "");
 constexpr int64_t kCeScratch = (int64_t)1 << 30;   // bytes that a piece of the vocabulary may take
@@ -264,7 +266,7 @@ struct CeProduct {
   bool share;            // tiles may be shared out among workers (kDx, kDw)
   bool vec;              // out can be stored 16 bytes at a time
   // kLse
-  float2* parts;         // [2 per tile of n][parts_ld]
+  float2* parts;         // [kCeShares per tile of n][parts_ld]
   float* target_logit;
   int64_t parts_ld;
   // kDx, kDw
@@ -292,7 +294,7 @@ template <CeMode MODE, int PAIR> struct CeWork {
     slices = 1;
     per = steps;
     if ((MODE == kDx || MODE == kDw) && p.share) {
-      // The least time in steps (0.3 us): rounds times a slice's steps, and for several slices the launch that adds them (5 us) and its
+      // The least time in steps (0.3 us): rounds times a slice's steps, and for several slices the launch that adds them (7 us) and its
       // 256 or 128 KB a part, written and read.
       const int rest = whole % workers;
       float best = (float)steps;
@@ -300,7 +302,7 @@ template <CeMode MODE, int PAIR> struct CeWork {
       for (int k = 0; k < 11; ++k) {
         const int s = k < 5 ? k + 2 : k == 5 ? 8 : k == 6 ? 12 : k == 7 ? 16 : k == 8 ? 24 : k == 9 ? 32 : 37;
         if (rest == 0 || s > steps || rest * s * PAIR > kCeParts) continue;
-        const float time = (float)((rest * s + workers - 1) / workers) * (float)((steps + s - 1) / s) + 16.f + 0.18f * PAIR * (float)(rest * s);
+        const float time = (float)((rest * s + workers - 1) / workers) * (float)((steps + s - 1) / s) + 24.f + 0.18f * PAIR * (float)(rest * s);
         if (time < best) { best = time; slices = s; }
       }
       if (slices > 1) {
@@ -376,7 +378,7 @@ template <typename T, typename OUT, CeMode MODE, bool REG, int PAIR>
 __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_copy,
                                                                const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_g) {
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
-  constexpr int STAGES = kCeStages<PAIR>;
+  constexpr int STAGES = kCeStages<PAIR>, WIDTH = kCeWidth;
   constexpr uint32_t STAGE = kCeStage<PAIR>;
   constexpr int GRAIN = 16 * PAIR;   // columns come in multiples of it
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
   const uint32_t rank = PAIR == 2 ? cluster_rank() : 0;
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&bar_full[s], 1); mbar_init(&bar_free[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&bar_done[s], 1); mbar_init(&bar_read[s], 8 * PAIR); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&bar_done[s], 1); mbar_init(&bar_read[s], kCeWarps * PAIR); }
     mbar_init(&bar_end, 1);
     mbar_fence_init();
     abort_flag = 0;
@@ -486,8 +488,8 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
       mbar_drain(&bar_end, 0);
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2, width = p.bn / 2;   // a warp has 32 rows and half the columns
-    const uint32_t src = tmem + half * width + ((uint32_t)(quarter * 32) << 16);
+    const int quarter = warp & 3, share = (warp - 2) >> 2, width = p.bn / kCeShares;   // a warp has 32 rows and a share of the columns
+    const uint32_t src = tmem + share * width + ((uint32_t)(quarter * 32) << 16);
     uint8_t* staging = smem + STAGES * STAGE + (warp - 2) * 4096;
     const uint32_t read_at = PAIR == 2 ? of_cta(&bar_read[0], 0) : 0;
     int turn = 0;
@@ -502,18 +504,18 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
       ++turn;
     };
     for (int i = 0; !over && work.at(worker, i, m, n, k0, k1, slot); ++i) {
-      const int local = rank * kCeM + quarter * 32 + lane, row = m * PAIR * kCeM + local, c_base = n * p.bn + half * width;
+      const int local = rank * kCeM + quarter * 32 + lane, row = m * PAIR * kCeM + local, c_base = n * p.bn + share * width;
       const int cols = min(width, p.n - c_base);   // that there are; of the others up to the next grain are computed
       const bool empty = k1 <= k0;
-      float sums[REG ? 128 : 1];
+      float sums[REG ? WIDTH : 1];
       if constexpr (REG) {
 #pragma unroll
-        for (int j = 0; j < 128; ++j) sums[j] = 0.f;
+        for (int j = 0; j < WIDTH; ++j) sums[j] = 0.f;
         for (; k0 < k1; k0 += p.flush) {
           if (mbar_wait_failed(&bar_done[turn & 1], (uint32_t)(turn >> 1) & 1u, abortp)) { over = true; break; }
           tc_fence_after();
 #pragma unroll
-          for (int c0 = 0; c0 < 128; c0 += 16) {   // (32 at a time spill)
+          for (int c0 = 0; c0 < WIDTH; c0 += 16) {
             if (c0 >= cols) break;
             float v[16];
             tmem_ld16(src + (turn & 1) * kCeN + c0, v);
@@ -549,7 +551,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         const int target = on ? p.rows[row].target - p.vocab0 - c_base : -1;
         float best = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += 32) {
+        for (int c0 = 0; c0 < WIDTH; c0 += 32) {
           if (c0 >= cols) break;
           float v[32];
           take(std::integral_constant<int, 32>(), c0, v);
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           float top = best;
 #pragma unroll
           for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
-          if (target >= c0 && target < c0 + 32) {
+          if (target >= c0 && target < min(c0 + 32, cols)) {
             float z = 0.f;
 #pragma unroll
             for (int j = 0; j < 32; ++j) z = c0 + j == target ? v[j] : z;
@@ -577,7 +579,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           sum = fmaf(sum, ex2_approx((best - zero) * kLog2e), s2.x + s2.y);
           best = top;
         }
-        if (on) p.parts[(int64_t)(n * 2 + half) * p.parts_ld + row] = make_float2(best, sum);
+        if (on) p.parts[(int64_t)(n * kCeShares + share) * p.parts_ld + row] = make_float2(best, sum);
       } else if constexpr (MODE == kGrad) {
         CeRow r;
         r.target = -1; r.lse = 0.f; r.coef = 0.f; r.row = 0;
@@ -585,7 +587,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         const int target = r.target - p.vocab0 - c_base;
         constexpr int PLANES = CePlanes<OUT>::count;
 #pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += 64) {
+        for (int c0 = 0; c0 < WIDTH; c0 += 64) {
           if (c0 >= cols) break;
           float v[64];
           take(std::integral_constant<int, 64>(), c0, v);
@@ -619,7 +621,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
             }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) {   // (a tile is 128 columns wide at least: 64 for either half)
+            if (lane == 0) {   // (a tile is 128 columns wide at least: 64 for each share)
               tma_store_4d(&map_g, staging, c_base + c0, row - lane, q, 0);
               bulk_commit();
             }
@@ -630,12 +632,12 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         const bool on = row < (MODE == kDw ? p.m : head.rows);
         const int64_t to = MODE == kDw ? p.out_row0 + row : on ? p.rows[row].row : 0;
 #pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += 32) {
+        for (int c0 = 0; c0 < WIDTH; c0 += 32) {
           if (c0 >= cols) break;
           float v[32];
           take(std::integral_constant<int, 32>(), c0, v);
           if (slot >= 0) {
-            float4* out = p.slab + ((int64_t)slot * (kCeN / 4) + (half * width + c0) / 4) * (kCeM * PAIR) + local;
+            float4* out = p.slab + ((int64_t)slot * (kCeN / 4) + (share * width + c0) / 4) * (kCeM * PAIR) + local;
 #pragma unroll
             for (int j = 0; j < 32; j += 4) out[(j / 4) * (kCeM * PAIR)] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
           } else if (on) {
@@ -659,8 +661,8 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
   if (tid == 0 && abort_flag) atomicOr(p.status, CASTLE_STATUS_WAIT_TIMEOUT);
 }
 
-// The parts of shared tiles, added in order: a thread per four values of a row, blockIdx.y the tile.
-template <typename OUT, CeMode MODE, int PAIR>
+// The parts of shared tiles, added in order: a thread per COLS values of a row, blockIdx.y the tile.
+template <typename OUT, CeMode MODE, int PAIR, int COLS>
 __global__ void __launch_bounds__(256) castle_ce_sum_kernel(const CeProduct p) {
   constexpr int ROWS = kCeM * PAIR;
   overlap_wait();
@@ -670,17 +672,21 @@ __global__ void __launch_bounds__(256) castle_ce_sum_kernel(const CeProduct p) {
   if (tile >= work.left) return;
   int m, n;
   work.place(work.whole + tile, m, n);
-  const int at = blockIdx.x * 256 + threadIdx.x, local = at % ROWS, quad = at / ROWS;   // neighbouring threads: neighbouring rows
-  const int row = m * ROWS + local, col = n * p.bn + quad * 4;
+  const int at = blockIdx.x * 256 + threadIdx.x, local = at % ROWS, first = at / ROWS * COLS;   // neighbouring threads: neighbouring rows
+  const int row = m * ROWS + local, col = n * p.bn + first;
   if (row >= (MODE == kDw ? p.m : head.rows) || col >= p.n) return;
-  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+  float t[COLS];
+#pragma unroll
+  for (int j = 0; j < COLS; ++j) t[j] = 0.f;
+#pragma unroll(COLS == 4 ? 8 : 2)
   for (int s = 0; s < work.slices; ++s) {
-    const float4 v = p.slab[((int64_t)(s * work.left + tile) * (kCeN / 4) + quad) * ROWS + local];
-    t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+#pragma unroll
+    for (int j = 0; j < COLS; j += 4) {
+      const float4 v = p.slab[((int64_t)(s * work.left + tile) * (kCeN / 4) + (first + j) / 4) * ROWS + local];
+      t[j] += v.x; t[j + 1] += v.y; t[j + 2] += v.z; t[j + 3] += v.w;
+    }
   }
-  float v[4] = {t.x, t.y, t.z, t.w};
-  ce_emit<OUT, 4>(p, head.unit, row, MODE == kDw ? p.out_row0 + row : p.rows[row].row, col, min(4, p.n - col), v);
+  ce_emit<OUT, COLS>(p, head.unit, row, MODE == kDw ? p.out_row0 + row : p.rows[row].row, col, min(COLS, p.n - col), t);
 }
 
 // ------------------------------------------------------------------------------------------------ the losses
@@ -787,7 +793,7 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
     if (v < kCeN) v = kCeN;
     return (int)(v < vocab ? v : vocab);
   };
-  q.piece_fwd = piece(w_row + q.copy_rows / 16);
+  q.piece_fwd = piece(w_row + q.copy_rows * kCeShares * (int64_t)sizeof(float2) / kCeN);
   q.piece_bwd = piece(w_row + q.planes * q.g_rows * 2);
   q.pieces = (int)((vocab + q.piece_bwd - 1) / q.piece_bwd);
   size_t at = 1024;   // behind the CeHead
@@ -797,9 +803,9 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
   const int64_t most = backward ? q.piece_bwd : q.piece_fwd;
   q.wcopy = take(q.copy_w ? (size_t)most * w_row : 0);
   if (!backward) {
-    // two for each tile of a row: 256 columns, or less where 128 rows by twice as many would make fewer than 148 tiles (ce_cut)
+    // kCeShares for each tile of a row: 256 columns, or less where 128 rows by twice as many would make fewer than 148 tiles (ce_cut)
     const int64_t wide = (q.piece_fwd + kCeN - 1) / kCeN, few = 296 / ((n + kCeM - 1) / kCeM) + 1, most_tiles = wide > few ? wide : few;
-    q.parts_per_piece = 2 * (int)(most_tiles < (q.piece_fwd + 63) / 64 ? most_tiles : (q.piece_fwd + 63) / 64);
+    q.parts_per_piece = kCeShares * (int)(most_tiles < (q.piece_fwd + 63) / 64 ? most_tiles : (q.piece_fwd + 63) / 64);
     q.parts = take((size_t)q.parts_per_piece * q.copy_rows * sizeof(float2));
     q.running = take((size_t)n * sizeof(float2));
     q.logit = take((size_t)n * sizeof(float));
@@ -942,7 +948,7 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
   CE_TRY(ce_x_maps(c, q, op, kCeM, &x, &copy));
   for (int64_t v0 = 0; v0 < c.vocab; v0 += q.piece_fwd) {
     const int64_t count = c.vocab - v0 < q.piece_fwd ? c.vocab - v0 : q.piece_fwd;
-    const CeCut cut = ce_cut(c.n, count, false, 64);
+    const CeCut cut = ce_cut(c.n, count, false, 32 * kCeShares);
     const int tiles_n = (int)((count + cut.bn - 1) / cut.bn);
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), "castle_linear_ce_fwd launch");
     CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
@@ -955,7 +961,7 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
     CE_CUDA((ce_launch<T, OUT, kLse>(p, cut.pair, tiles_m * tiles_n, x, copy, w, w, c.st)), "castle_linear_ce_fwd launch");
     CeJoin j{};
     j.head = (CeHead*)c.work; j.rows = p.rows; j.parts = p.parts; j.running = (float2*)(c.work + q.running); j.target_logit = p.target_logit;
-    j.sums = (double*)(c.work + q.sums); j.lse = lse; j.loss = loss; j.parts_ld = q.copy_rows; j.parts_n = 2 * tiles_n;
+    j.sums = (double*)(c.work + q.sums); j.lse = lse; j.loss = loss; j.parts_ld = q.copy_rows; j.parts_n = kCeShares * tiles_n;
     j.begin = v0 == 0; j.end = v0 + count == c.vocab; j.each = each; j.mean = c.reduction == CASTLE_REDUCE_MEAN;
     // few rows: a warp each; many: neighbouring threads on neighbouring rows
     if (c.n >= 4096) CE_CUDA(launch_kernel(castle_ce_join_kernel<32>, dim3((unsigned)((c.n + 31) / 32)), 256, 0, c.st, true, j), "castle_linear_ce_fwd launch");
@@ -983,13 +989,19 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
     const cudaError_t e = ce_launch<T, OUT, MODE>(p, cut.pair, tiles, a, acopy, b, b, c.st);
     if (e != cudaSuccess || !p.share) return e;
     const int64_t shared = tiles < kCeWorkers / cut.pair ? tiles : kCeWorkers / cut.pair;
-    const dim3 grid(kCeM * cut.pair * kCeN / 4 / 256, (unsigned)shared);
-    return cut.pair == 2 ? launch_kernel(castle_ce_sum_kernel<OUT, MODE, 2>, grid, 256, 0, c.st, true, p) : launch_kernel(castle_ce_sum_kernel<OUT, MODE, 1>, grid, 256, 0, c.st, true, p);
+    auto sum = [&](auto pair, auto cols) {
+      constexpr int PAIR = decltype(pair)::value, COLS = decltype(cols)::value;
+      return launch_kernel(castle_ce_sum_kernel<OUT, MODE, PAIR, COLS>, dim3(kCeM * PAIR * kCeN / COLS / 256, (unsigned)shared), 256, 0, c.st, true, p);
+    };
+    using std::integral_constant;
+    // few tiles: many parts of each, added by many threads; else whole sectors of the result by each thread
+    if (cut.pair == 1) return sum(integral_constant<int, 1>(), integral_constant<int, 4>());
+    return shared < 16 ? sum(integral_constant<int, 2>(), integral_constant<int, 4>()) : sum(integral_constant<int, 2>(), integral_constant<int, 16>());
   };
   for (int64_t v0 = 0; v0 < c.vocab; v0 += q.piece_bwd) {
     const int64_t count = c.vocab - v0 < q.piece_bwd ? c.vocab - v0 : q.piece_bwd, pitch = (count + 7) / 8 * 8;
     uint16_t* gp = (uint16_t*)(c.work + q.g);
-    const CeCut cut = ce_cut(c.n, count, false, 128), cut_dx = ce_cut(c.n, c.dim, true, kCeN), cut_dw = ce_cut(count, c.dim, true, kCeN);
+    const CeCut cut = ce_cut(c.n, count, false, 64 * kCeShares), cut_dx = ce_cut(c.n, c.dim, true, kCeN), cut_dw = ce_cut(count, c.dim, true, kCeN);
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), what);
     CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
     CE_TRY(ce_w_map(c, q, op, count, kCeK, &wk));
