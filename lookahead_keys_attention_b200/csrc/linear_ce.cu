@@ -46,12 +46,19 @@ constexpr int kCeM = 128, kCeN = 256, kCeK = 64;
 // The warps that work on tiles.  (Sixteen instead of eight: no faster; the logits' gradient of 4095 x 1024 against 50021 188 us instead of 172.)
 constexpr int kCeWarps = 8, kCeShares = kCeWarps / 4, kCeThreads = (kCeWarps + 2) * 32, kCeWidth = kCeN / kCeShares;
 constexpr uint32_t kCeA = kCeM * kCeK * 2;
-template <int PAIR> constexpr uint32_t kCeB = kCeN / PAIR * kCeK * 2;   // PAIR: CTAs that work on a tile
-template <int PAIR> constexpr uint32_t kCeStage = kCeA + kCeB<PAIR>;
-template <int PAIR> constexpr int kCeStages = PAIR == 2 ? 6 : 4;
-constexpr uint32_t kCeStaging = kCeWarps * 4096;   // kGrad: 32 rows x 64 columns of each working warp
-constexpr size_t kCeSmem = 4 * kCeStage<1> + kCeStaging + 1024;
-static_assert(kCeStages<2> * kCeStage<2> == 4 * kCeStage<1>, "");
+constexpr uint32_t kCeRing = 4 * (kCeA + kCeN * kCeK * 2);   // stages: 4 of a CTA alone with a tile of 256 columns, 6 of 128 or of a pair, 8 of 64
+constexpr int kCeStages = 8;
+constexpr uint32_t kCeStaging = kCeWarps * 4096;   // results on their way out: 32 rows x 128 bytes of each working warp
+constexpr size_t kCeSmem = kCeRing + kCeStaging + 1024;
+// The stages in turn: which, and in which of its barriers' two phases.
+struct CeTurn {
+  int stages, s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ explicit CeTurn(int n) : stages(n) {}
+  __device__ __forceinline__ void next() {
+    if (++s == stages) { s = 0; phase ^= 1u; }
+  }
+};
 constexpr int64_t kCeScratch = (int64_t)1 << 30;   // bytes that a piece of the vocabulary may take
 // Steps between emptyings: of a 16-bit operand's logits (32 additions in the tensor cores), of fp32's parts (24).  197 x 512 in
 // fp32: TBD
@@ -85,17 +92,6 @@ struct CeRowsParams {
   int32_t* status;
 };
 
-__device__ __forceinline__ int block_sum(int v, int* s) {   // of 1024 threads
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int t = 0;
-  for (int k = 0; k < 32; ++k) t += s[k];
-  return t;
-}
-
 // One value as one 16-bit number, or as three whose sum it is.
 template <typename T> struct CePlanes {
   static constexpr int count = 1;
@@ -117,56 +113,88 @@ template <typename T>
 __device__ __forceinline__ void copy_row(const T* src, uint16_t* dst, int64_t plane, int dim, int pitch, int lane) {
   using Op = typename CePlanes<T>::Op;
   constexpr int P = CePlanes<T>::count;
-  const bool vec = P == 1 && dim % 8 == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0;
-  if (vec) {
+  if (dim % 8 == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0) {
 #pragma unroll 4
-    for (int c = lane * 8; c < dim; c += 256) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+    for (int c = lane * 8; c < dim; c += 256) {
+      if constexpr (P == 1) {
+        *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+      } else {
+        float v[8], w[P][8];
+        load8<T>(src + c, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float a[P];
+          CePlanes<T>::split(v[j], a);
+#pragma unroll
+          for (int q = 0; q < P; ++q) w[q][j] = a[q];
+        }
+#pragma unroll
+        for (int q = 0; q < P; ++q) store8<Op>(reinterpret_cast<Op*>(dst + q * plane + c), w[q]);
+      }
+    }
     return;
   }
+#pragma unroll 4
   for (int c = lane * 2; c < pitch; c += 64) {
     float a[P], b[P];
     CePlanes<T>::split(c < dim ? load1<T>(src + c) : 0.f, a);
     CePlanes<T>::split(c + 1 < dim ? load1<T>(src + c + 1) : 0.f, b);
 #pragma unroll
-    for (int p = 0; p < P; ++p) *reinterpret_cast<uint32_t*>(dst + p * plane + c) = Elem<Op>::pack2(a[p], b[p]);
+    for (int q = 0; q < P; ++q) *reinterpret_cast<uint32_t*>(dst + q * plane + c) = Elem<Op>::pack2(a[q], b[q]);
   }
 }
 
 // Every CTA reads all targets (and, in a backward with a gradient per row, these), so it needs nothing of the others.
 template <typename T>
 __global__ void __launch_bounds__(1024, 1) castle_ce_rows_kernel(const CeRowsParams p) {
-  __shared__ int s[32];
+  __shared__ int s[3][32];
   __shared__ float sf[32];
   __shared__ int place[1024];   // of a row in the gathered order, -1: it takes no part
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t r0 = (int64_t)blockIdx.x * p.rows_per_cta, r1 = min(p.n, r0 + p.rows_per_cta);
   overlap_wait();
-  int before = 0, all = 0, ignored = 0;
+  int sums[3] = {0, 0, 0};   // rows that take part before the CTA's own, all of them, ignored ones
   float most = 0.f;
-#pragma unroll 4
-  for (int64_t i = tid; i < p.n; i += 1024) {
-    const int64_t t = p.targets[i];
-    const bool on = t != p.ignore && t >= 0 && t < p.vocab;
-    ignored += t == p.ignore;
-    all += on;
-    before += on && i < r0;
-    if (p.each && on) {
-      const float g = fabsf(p.dloss[i]);
-      if (g < INFINITY) most = fmaxf(most, g);
+  for (int64_t i0 = tid; i0 < p.n; i0 += 1024 * 8) {
+    int64_t t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t[u] = i0 + u * 1024 < p.n ? p.targets[i0 + u * 1024] : -1;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t i = i0 + u * 1024;
+      const bool in = i < p.n, skip = t[u] == p.ignore, on = in && !skip && t[u] >= 0 && t[u] < p.vocab;
+      sums[0] += on && i < r0;
+      sums[1] += on;
+      sums[2] += in && skip;
+      if (p.each && on) {
+        const float g = fabsf(p.dloss[i]);
+        if (g < INFINITY) most = fmaxf(most, g);
+      }
     }
   }
-  before = block_sum(before, s);
-  all = block_sum(all, s);
-  ignored = block_sum(ignored, s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) sums[k] += __shfl_xor_sync(0xffffffffu, sums[k], o);
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  }
+  if (lane < 3) s[lane][warp] = lane == 0 ? sums[0] : lane == 1 ? sums[1] : sums[2];
+  if (lane == 0) sf[warp] = most;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) sums[k] = s[k][lane];
+  most = sf[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) sums[k] += __shfl_xor_sync(0xffffffffu, sums[k], o);
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  }
+  int before = sums[0];
+  const int all = sums[1], ignored = sums[2];
   float g_one = 0.f, unit = 1.f;
   if (p.dloss) {
-    if (p.each) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (lane == 0) sf[warp] = most;
-      __syncthreads();
-      for (int k = 0; k < 32; ++k) most = fmaxf(most, sf[k]);
-    } else {
+    if (!p.each) {
       g_one = p.dloss[0];
       if (p.mean) g_one /= (float)(p.n - ignored);
       if (fabsf(g_one) < INFINITY) most = fabsf(g_one);
@@ -195,12 +223,12 @@ __global__ void __launch_bounds__(1024, 1) castle_ce_rows_kernel(const CeRowsPar
     }
     const unsigned vote = __ballot_sync(0xffffffffu, on);
     __syncthreads();
-    if (lane == 0) s[warp] = __popc(vote);
+    if (lane == 0) s[0][warp] = __popc(vote);
     __syncthreads();
     int at = before, total = 0;
     for (int k = 0; k < 32; ++k) {
-      if (k < warp) at += s[k];
-      total += s[k];
+      if (k < warp) at += s[0][k];
+      total += s[0][k];
     }
     at += __popc(vote & ((1u << lane) - 1));
     before += total;
@@ -378,18 +406,17 @@ template <typename T, typename OUT, CeMode MODE, bool REG, int PAIR>
 __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_copy,
                                                                const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_g) {
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
-  constexpr int STAGES = kCeStages<PAIR>, WIDTH = kCeWidth;
-  constexpr uint32_t STAGE = kCeStage<PAIR>;
+  constexpr int WIDTH = kCeWidth;
   constexpr int GRAIN = 16 * PAIR;   // columns come in multiples of it
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t bar_full[STAGES], bar_free[STAGES], bar_done[2], bar_read[2], bar_end;   // of a pair, full and read are the first CTA's
+  __shared__ uint64_t bar_full[kCeStages], bar_free[kCeStages], bar_done[2], bar_read[2], bar_end;   // of a pair, full and read are the first CTA's
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = PAIR == 2 ? cluster_rank() : 0;
   if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&bar_full[s], 1); mbar_init(&bar_free[s], 1); }
+    for (int s = 0; s < kCeStages; ++s) { mbar_init(&bar_full[s], 1); mbar_init(&bar_free[s], 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(&bar_done[s], 1); mbar_init(&bar_read[s], kCeWarps * PAIR); }
     mbar_init(&bar_end, 1);
     mbar_fence_init();
@@ -411,6 +438,8 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
   const CeWork<MODE, PAIR> work(p, head.rows, gridDim.x / PAIR);
   const int worker = blockIdx.x / PAIR;
   int m, n, k0, k1, slot;
+  const uint32_t stage = kCeA + p.bn / PAIR * kCeK * 2;   // bytes
+  CeTurn ring(min(kCeStages, (int)(kCeRing / stage)));
   // columns of a tile that are computed
   auto columns = [&](int n) { return min(p.bn, (p.n - n * p.bn + GRAIN - 1) / GRAIN * GRAIN); };
 
@@ -419,17 +448,16 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
       const bool copy = head.gathered;
       const CUtensorMap* ma = MODE != kDx && MODE != kDw && copy ? &map_copy : &map_a;
       const CUtensorMap* mb = MODE == kDw && copy ? &map_copy : &map_b;
-      const int b_rows = p.bn / PAIR;
-      const uint32_t bytes = (kCeA + b_rows * kCeK * 2) * PAIR;   // of the pair
-      int it = 0;
+      bool sent = false;
       for (int i = 0; work.at(worker, i, m, n, k0, k1, slot) && !*abortp; ++i) {
         const int m0 = (m * PAIR + rank) * kCeM, n0 = n * p.bn + (PAIR == 2 ? rank * (columns(n) / 2) : 0);
         for (int ks = k0; ks < k1; ++ks) {
-          for (int term = 6 - p.terms; term < 6; ++term, ++it) {
-            const int s = it % STAGES, k = ks * kCeK, pa = kTermA[term], pb = kTermB[term];
-            if (!mbar_wait_ok<true>(&bar_free[s], ((uint32_t)(it / STAGES) & 1u) ^ 1u, abortp)) { ks = k1; break; }
-            uint8_t *a = smem + s * STAGE, *b = a + kCeA;
-            if (rank == 0) mbar_expect_tx(&bar_full[s], bytes);
+          for (int term = 6 - p.terms; term < 6; ++term, ring.next()) {
+            const int s = ring.s, k = ks * kCeK, pa = kTermA[term], pb = kTermB[term];
+            if (!mbar_wait_ok<true>(&bar_free[s], ring.phase ^ 1u, abortp)) { ks = k1; break; }
+            uint8_t *a = smem + s * stage, *b = a + kCeA;
+            if (rank == 0) mbar_expect_tx(&bar_full[s], stage * PAIR);
+            sent = true;
             auto load = [&](void* dst, const CUtensorMap* map, int c0, int c1, int plane) {
               if constexpr (PAIR == 2) tma_load_4d_pair(dst, map, of_cta(&bar_full[s], 0), c0, c1, plane, 0);
               else tma_load_4d(dst, map, &bar_full[s], c0, c1, plane, 0);
@@ -450,8 +478,8 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         }
       }
       // a copy that nobody waited for (after an abort) must not arrive in another CTA's shared memory
-      if (*abortp && rank == 0)
-        for (int j = max(0, it - STAGES); j < it; ++j) mbar_drain(&bar_full[j % STAGES], (uint32_t)(j / STAGES) & 1u);
+      if (*abortp && rank == 0 && sent)
+        for (int j = 0; j < ring.stages; ++j, ring.next()) mbar_drain(&bar_full[ring.s], ring.phase ^ 1u);   // the last round of each
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
@@ -459,7 +487,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         if constexpr (PAIR == 2) mma_commit_pair(bar);
         else mma_commit(bar);
       };
-      int it = 0, turn = 0;
+      int turn = 0;
       for (int i = 0; work.at(worker, i, m, n, k0, k1, slot) && !*abortp; ++i) {
         const uint32_t idesc = make_idesc(kCeM * PAIR, 16, Elem<T>::fmt, A_MN, B_MN, false) + ((uint32_t)((columns(n) - 16) >> 3) << 17);
         for (; k0 < k1 && !*abortp; k0 += p.flush, ++turn) {
@@ -467,11 +495,11 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           const uint32_t d = tmem + acc * kCeN;
           if (!mbar_wait_ok<true>(&bar_read[acc], ((uint32_t)(turn >> 1) & 1u) ^ 1u, abortp)) break;
           tc_fence_after();
-          for (int j = 0; j < steps; ++j, ++it) {
-            const int s = it % STAGES;
-            if (!mbar_wait_ok<true>(&bar_full[s], (uint32_t)(it / STAGES) & 1u, abortp)) break;
+          for (int j = 0; j < steps; ++j, ring.next()) {
+            const int s = ring.s;
+            if (!mbar_wait_ok<true>(&bar_full[s], ring.phase, abortp)) break;
             tc_fence_after();
-            const uint32_t a = smem_u32(smem) + s * STAGE, b = a + kCeA;
+            const uint32_t a = smem_u32(smem) + s * stage, b = a + kCeA;
             const uint64_t da = A_MN ? desc_mnmajor(a, 8192) : desc_kmajor(a), db = B_MN ? desc_mnmajor(b, 8192) : desc_kmajor(b);
 #pragma unroll
             for (int q = 0; q < kCeK / 16; ++q) {
@@ -490,7 +518,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
   } else {
     const int quarter = warp & 3, share = (warp - 2) >> 2, width = p.bn / kCeShares;   // a warp has 32 rows and a share of the columns
     const uint32_t src = tmem + share * width + ((uint32_t)(quarter * 32) << 16);
-    uint8_t* staging = smem + STAGES * STAGE + (warp - 2) * 4096;
+    uint8_t* staging = smem + kCeRing + (warp - 2) * 4096;
     const uint32_t read_at = PAIR == 2 ? of_cta(&bar_read[0], 0) : 0;
     int turn = 0;
     bool over = false;
@@ -631,6 +659,8 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         const float unit = head.unit;
         const bool on = row < (MODE == kDw ? p.m : head.rows);
         const int64_t to = MODE == kDw ? p.out_row0 + row : on ? p.rows[row].row : 0;
+        constexpr int PANEL = 128 / (int)sizeof(OUT);   // columns of 128 bytes of a row
+        const bool direct = slot < 0 && !p.acc && p.vec;
 #pragma unroll
         for (int c0 = 0; c0 < WIDTH; c0 += 32) {
           if (c0 >= cols) break;
@@ -640,6 +670,24 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
             float4* out = p.slab + ((int64_t)slot * (kCeN / 4) + (share * width + c0) / 4) * (kCeM * PAIR) + local;
 #pragma unroll
             for (int j = 0; j < 32; j += 4) out[(j / 4) * (kCeM * PAIR)] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          } else if (direct) {
+            // through shared memory, so that eight lanes store a row's 128 bytes
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= unit;
+            if constexpr (sizeof(OUT) == 4) store_row32_f32(staging, lane, v);
+            else store_row32<OUT>(staging, 4096, lane, c0 % 64, v);
+            if (c0 % PANEL + 32 == PANEL || c0 + 32 >= cols) {
+              __syncwarp();
+              const int first = c0 / PANEL * PANEL, col = first + (lane & 7) * (PANEL / 8);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int r = j * 4 + (lane >> 3);
+                const int64_t row_to = __shfl_sync(0xffffffffu, to, r);
+                if (__shfl_sync(0xffffffffu, on, r) && col < min(cols, c0 + 32))
+                  *reinterpret_cast<uint4*>(static_cast<OUT*>(p.out) + row_to * p.ld + c_base + col) = *reinterpret_cast<const uint4*>(staging + swz_off(r, lane & 7));
+              }
+              __syncwarp();
+            }
           } else if (on) {
             ce_emit<OUT, 32>(p, unit, row, to, c_base + c0, min(32, cols - c0), v);
           }
@@ -707,7 +755,6 @@ template <int ROWS>
 __global__ void __launch_bounds__(256) castle_ce_join_kernel(const CeJoin p) {
   constexpr int LANES = 256 / ROWS;
   __shared__ float2 s[LANES][ROWS];
-  __shared__ double total;
   __shared__ bool last;
   const int r = threadIdx.x % ROWS, l = threadIdx.x / ROWS;
   const int64_t row = (int64_t)blockIdx.x * ROWS + r;
@@ -742,27 +789,28 @@ __global__ void __launch_bounds__(256) castle_ce_join_kernel(const CeJoin p) {
   }
   if (!p.end || p.each) return;
   // the CTA's sum, and by the last CTA all CTAs', in a fixed order
-  __shared__ double ds[ROWS];
-  if (l == 0) ds[r] = loss;
-  __syncthreads();
+  __shared__ double ds[8];
+  auto cta_sum = [&](double v) {   // of all threads; thread 0 has it
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) ds[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return threadIdx.x == 0 ? ((ds[0] + ds[1]) + (ds[2] + ds[3])) + ((ds[4] + ds[5]) + (ds[6] + ds[7])) : 0.0;
+  };
+  const double mine = cta_sum(loss);
   if (threadIdx.x == 0) {
-    double t = 0.0;
-    for (int k = 0; k < ROWS; ++k) t += ds[k];
-    p.sums[blockIdx.x] = t;
+    p.sums[blockIdx.x] = mine;
     __threadfence();
     last = atomicAdd(&p.head->done, 1u) + 1 == gridDim.x;
     __threadfence();
   }
   __syncthreads();
   if (!last) return;
-  __shared__ double all[256];
   double t = 0.0;
   for (int k = threadIdx.x; k < (int)gridDim.x; k += 256) t += __ldcg(p.sums + k);
-  all[threadIdx.x] = t;
-  __syncthreads();
+  double total = cta_sum(t);
   if (threadIdx.x == 0) {
-    total = 0.0;
-    for (int k = 0; k < 256; ++k) total += all[k];
     if (p.mean) total /= (double)rows;
     p.loss[0] = p.head->bad ? __int_as_float(0x7fffffff) : (float)total;
   }
