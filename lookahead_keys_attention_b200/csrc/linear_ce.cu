@@ -30,9 +30,11 @@
 // (the logits' statistics, and everything of fp32 tensors), accumulators are therefore emptied every `flush` steps into sums that
 // the working warps keep in registers.
 //
-// G in 16 bits: c_i is taken in units of a power of two that leaves G below 2^15 (the unit is multiplied back in fp32 at the
-// end), so that fp16 keeps probabilities down to 2^-28 in full precision; rounding G is off by half a step of the type, as
-// rounding the logits' gradient is where logits are tensors of that type.
+// G in 16 bits is taken in units of a power of two (the largest c_i's) with 2^14 on top, so that fp16 keeps probabilities down to 2^-28 in full
+// precision; the unit is multiplied back in fp32 at the end.  Where all rows have one coefficient (mean, sum) that is the unit and none
+// of it is in G: -1 for a target that has no probability is exact, where c would be off by the same half step in every row (1789 rows
+// against 132536, bf16: gradients 3.2e-3 off in their norm, 1.7e-3 by rounding the result).  A row's largest entry by far is
+// mostly its target's.  What rounding took from it is kept in fp32, and dx gets its product with the target's row of W.
 #include <type_traits>
 
 #include "common.cuh"
@@ -63,7 +65,7 @@ constexpr int64_t kCeScratch = (int64_t)1 << 30;   // bytes that a piece of the 
 // Steps between emptyings: of a 16-bit operand's logits (32 additions in the tensor cores), of fp32's parts (24).  197 x 512 in
 // fp32: TBD
 constexpr int kCeFlush = 8, kCeFlushF32 = 1, kCeNoFlush = 1 << 30;
-constexpr float kCeUnit = 16384.f;                 // of G: |c| < 2 units
+constexpr float kCeUnit = 16384.f;                 // of G: below 2 units
 
 struct CeHead {          // at the start of the workspace, written by castle_ce_rows_kernel
   int rows;              // that take part
@@ -72,7 +74,7 @@ struct CeHead {          // at the start of the workspace, written by castle_ce_
   unsigned done;         // CTAs of the join that have ended
   float unit;            // of G, multiplied back into dx and dW
 };
-struct CeRow { int target; float lse, coef; int row; };   // of the rows that take part, in order; row: in the caller's tensors
+struct CeRow { int target; float lse, coef; int row; };   // of the rows that take part, in order; coef: G's, row: in the caller's tensors
 
 __constant__ const int8_t kTermA[6] = {2, 0, 1, 1, 0, 0}, kTermB[6] = {0, 2, 1, 0, 1, 0};   // one term: the last
 
@@ -193,14 +195,8 @@ __global__ void __launch_bounds__(1024, 1) castle_ce_rows_kernel(const CeRowsPar
   int before = sums[0];
   const int all = sums[1], ignored = sums[2];
   float g_one = 0.f, unit = 1.f;
-  if (p.dloss) {
-    if (!p.each) {
-      g_one = p.dloss[0];
-      if (p.mean) g_one /= (float)(p.n - ignored);
-      if (fabsf(g_one) < INFINITY) most = fabsf(g_one);
-    }
-    if (most > 0.f) unit = __uint_as_float(max(__float_as_uint(most) & 0x7f800000u, 0x00800000u));   // its power of two
-  }
+  if (p.dloss && !p.each) g_one = p.mean ? p.dloss[0] / (float)(p.n - ignored) : p.dloss[0];
+  if (most > 0.f) unit = __uint_as_float(max(__float_as_uint(most) & 0x7f800000u, 0x00800000u));   // the largest coefficient's power of two
   const bool gather = all < p.n;
   if (blockIdx.x == 0 && tid == 0) {
     CeHead h;
@@ -208,7 +204,7 @@ __global__ void __launch_bounds__(1024, 1) castle_ce_rows_kernel(const CeRowsPar
     h.gathered = gather || p.copy_always;
     h.bad = (int)(p.n - ignored) - all;
     h.done = 0;
-    h.unit = unit * (1.f / kCeUnit);
+    h.unit = (p.each ? unit : g_one) * (1.f / kCeUnit);
     *p.head = h;
     if (h.bad) atomicOr(p.status, CASTLE_STATUS_BAD_INDEX);
   }
@@ -238,7 +234,7 @@ __global__ void __launch_bounds__(1024, 1) castle_ce_rows_kernel(const CeRowsPar
       r.target = (int)t;
       r.row = (int)i;
       r.lse = p.lse ? p.lse[i] : 0.f;
-      r.coef = p.dloss ? (p.each ? p.dloss[i] : g_one) / unit * kCeUnit : 0.f;
+      r.coef = p.each ? p.dloss[i] / unit * kCeUnit : kCeUnit;
       p.rows[at] = r;
     } else if (i < r1 && p.lse_out) {
       const float none = skip ? 0.f : __int_as_float(0x7fffffff);
@@ -292,12 +288,15 @@ struct CeProduct {
   int terms, group;
   int flush;             // steps after which an accumulator is emptied
   bool share;            // tiles may be shared out among workers (kDx, kDw)
-  bool vec;              // out can be stored 16 bytes at a time
+  bool vec, w_vec;       // out can be stored, the weight read 16 bytes at a time
   // kLse
   float2* parts;         // [kCeShares per tile of n][parts_ld]
   float* target_logit;
   int64_t parts_ld;
   // kDx, kDw
+  float* lost;           // kGrad, kDx (16 bits): what rounding took from the target's entry of G, of each row that takes part
+  const void* w;         // kDx: the weight, w_stride apart, of which the piece has rows [vocab0, vocab0 + k)
+  int64_t w_stride;
   void* out;             // (rows, ld)
   int64_t ld, out_row0;
   float4* slab;          // parts of shared tiles: [part][column / 4][row of the tile]
@@ -367,6 +366,37 @@ template <CeMode MODE, int PAIR> struct CeWork {
     m = first + t - n * high;
   }
 };
+
+// Where a row of the result goes, and for dx the row of W that its sums get a multiple of (NULL: none, or the target is of another piece).
+template <typename OUT> struct CeOut { int64_t to; const OUT* w; float lost; };
+template <CeMode MODE, typename OUT> __device__ __forceinline__ CeOut<OUT> ce_out(const CeProduct& p, int row, bool on) {
+  CeOut<OUT> o{MODE == kDw ? p.out_row0 + row : 0, nullptr, 0.f};
+  if (MODE == kDw || !on) return o;
+  const CeRow r = p.rows[row];
+  o.to = r.row;
+  if (CePlanes<OUT>::count == 1 && r.target >= p.vocab0 && r.target < p.vocab0 + p.k) {
+    o.w = static_cast<const OUT*>(p.w) + r.target * p.w_stride;
+    o.lost = p.lost[row];
+  }
+  return o;
+}
+template <typename OUT, int COUNT> __device__ __forceinline__ void ce_add_lost(const CeProduct& p, const CeOut<OUT>& o, int col, int have, float* v) {
+  if (CePlanes<OUT>::count > 1 || !o.w || o.lost == 0.f) return;
+  if (p.w_vec && COUNT % 8 == 0) {
+#pragma unroll
+    for (int j = 0; j < COUNT; j += 8)
+      if (j < have) {
+        float f[8];
+        load8<OUT>(o.w + col + j, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j + i] = fmaf(o.lost, f[i], v[j + i]);
+      }
+  } else {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j)
+      if (j < have) v[j] = fmaf(o.lost, load1<OUT>(o.w + col + j), v[j]);
+  }
+}
 
 // Four or more values of a row of dx or dW go out: to the sums over the pieces of the vocabulary, or scaled to the result (`to`: its row).
 template <typename OUT, int COUNT>
@@ -632,6 +662,14 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = r.coef == 0.f ? 0.f : v[j] * r.coef;
+          if (PLANES == 1 && target >= c0 && target < min(c0 + 64, cols)) {
+            float g = 0.f;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) g = c0 + j == target ? v[j] : g;
+            const float lost = g - Elem<T>::to_f(Elem<T>::from_f(g));
+            p.lost[row] = isfinite(lost) ? lost : 0.f;
+          }
+          __syncwarp();
 #pragma unroll
           for (int q = 0; q < PLANES; ++q) {
             if (lane == 0) bulk_wait_read0();   // what was stored from here before has left
@@ -656,9 +694,10 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           }
         }
       } else {
-        const float unit = head.unit;
         const bool on = row < (MODE == kDw ? p.m : head.rows);
-        const int64_t to = MODE == kDw ? p.out_row0 + row : on ? p.rows[row].row : 0;
+        const float unit = head.unit;
+        const CeOut<OUT> dst = ce_out<MODE, OUT>(p, row, on);
+        const int64_t to = dst.to;
         constexpr int PANEL = 128 / (int)sizeof(OUT);   // columns of 128 bytes of a row
         const bool direct = slot < 0 && !p.acc && p.vec;
 #pragma unroll
@@ -672,6 +711,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
             for (int j = 0; j < 32; j += 4) out[(j / 4) * (kCeM * PAIR)] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
           } else if (direct) {
             // through shared memory, so that eight lanes store a row's 128 bytes
+            if constexpr (MODE == kDx) ce_add_lost<OUT, 32>(p, dst, c_base + c0, min(32, cols - c0), v);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= unit;
             if constexpr (sizeof(OUT) == 4) store_row32_f32(staging, lane, v);
@@ -689,6 +729,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
               __syncwarp();
             }
           } else if (on) {
+            if constexpr (MODE == kDx) ce_add_lost<OUT, 32>(p, dst, c_base + c0, min(32, cols - c0), v);
             ce_emit<OUT, 32>(p, unit, row, to, c_base + c0, min(32, cols - c0), v);
           }
           __syncwarp();
@@ -734,7 +775,9 @@ __global__ void __launch_bounds__(256) castle_ce_sum_kernel(const CeProduct p) {
       t[j] += v.x; t[j + 1] += v.y; t[j + 2] += v.z; t[j + 3] += v.w;
     }
   }
-  ce_emit<OUT, COLS>(p, head.unit, row, MODE == kDw ? p.out_row0 + row : p.rows[row].row, col, min(COLS, p.n - col), t);
+  const CeOut<OUT> dst = ce_out<MODE, OUT>(p, row, true);
+  if constexpr (MODE == kDx) ce_add_lost<OUT, COLS>(p, dst, col, min(COLS, p.n - col), t);
+  ce_emit<OUT, COLS>(p, head.unit, row, dst.to, col, min(COLS, p.n - col), t);
 }
 
 // ------------------------------------------------------------------------------------------------ the losses
@@ -821,7 +864,7 @@ struct CePlan {
   int planes, terms, pitch, piece_fwd, piece_bwd, parts_per_piece, pieces;
   bool copy_x, copy_w;        // operands are laid out anew: fp32, or rows that TMA cannot read
   int64_t copy_rows, g_rows;
-  size_t rows, copy, wcopy, parts, running, logit, sums, g, slab, acc, bytes;   // offsets
+  size_t rows, copy, wcopy, parts, running, logit, sums, g, lost, slab, acc, bytes;   // offsets
 };
 
 static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, bool w_ok, bool backward) {
@@ -860,6 +903,7 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
     q.sums = take((size_t)((n + 7) / 8) * sizeof(double));
   } else {
     q.g = take((size_t)q.planes * q.g_rows * up(q.piece_bwd, 8) * 2);
+    q.lost = take((size_t)n * sizeof(float));
     q.slab = take((size_t)kCeParts * kCeM * kCeN * sizeof(float));
     q.acc = take(q.pieces > 1 ? (size_t)n * up(dim, 8) * sizeof(float) : 0);
   }
@@ -1030,6 +1074,7 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
   CeProduct base{};
   base.head = (const CeHead*)c.work; base.rows = (const CeRow*)(c.work + q.rows); base.terms = q.terms; base.flush = q.terms > 1 ? kCeFlushF32 : kCeNoFlush;
   base.status = c.status; base.ld = c.dim; base.bn = kCeN; base.slab = (float4*)(c.work + q.slab);
+  base.lost = (float*)(c.work + q.lost);
   // What the workers share out: launched with the product whenever there could be something.
   auto product = [&](auto mode, const CeProduct& p, const CeCut& cut, int64_t m, const CUtensorMap& a, const CUtensorMap& acopy, const CUtensorMap& b) -> cudaError_t {
     constexpr CeMode MODE = decltype(mode)::value;
@@ -1062,6 +1107,7 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
     CE_CUDA((ce_launch<T, OUT, kGrad>(p, cut.pair, tiles_m * ((count + cut.bn - 1) / cut.bn), x, copy, w, g, c.st)), what);
     if (dx) {
       p = base;
+      p.vocab0 = (int)v0; p.w = c.w; p.w_stride = c.ws; p.w_vec = c.dim % 8 == 0 && (uintptr_t)c.w % 16 == 0 && c.ws % 8 == 0;
       p.n = c.dim; p.k = (int)count; p.b_row0 = q.copy_w ? 0 : (int)v0; p.out = dx; p.group = 16 / cut_dx.pair;
       p.vec = c.dim % 8 == 0 && (uintptr_t)dx % 16 == 0;
       p.share = (p.k + kCeK - 1) / kCeK >= kCeShare;
