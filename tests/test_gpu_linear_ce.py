@@ -249,6 +249,22 @@ def test_only_one_gradient():
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("reduction,up", [("mean", 3.0), ("sum", 1.7), ("none", None)])
+def test_dx_of_rows_that_have_not_learnt(reduction, up, dtype):
+    """A row's gradient is the target's row of the weight but for little; its coefficient and that entry of G are exact or made up for, so
+    what is left is the result's rounding: a mean square of at most h^2 / 3, here with a tenth on top for the other entries of G."""
+    n, dim, vocab = 300, 256, 20000
+    x, w, t = case(n, dim, vocab, dtype, spread=0.5)
+    up = torch.linspace(0.3, 2.9, n, device="cuda") if up is None else torch.full((), up * (n if reduction == "mean" else 1), device="cuda")
+    xl = x.requires_grad_()
+    (dx,) = torch.autograd.grad(castle_linear_cross_entropy(xl, w, t, reduction=reduction), [xl], up)
+    G = torch.softmax(x.double() @ w.double().t(), 1)
+    G[torch.arange(n, device="cuda"), t] -= 1
+    want = (up.double().expand(n)[:, None] / (n if reduction == "mean" else 1) * G) @ w.double()
+    assert ((dx.double() - want).norm() <= 1.1 * half_step(dtype) / 3 ** 0.5 * want.norm()).item()
+
+
 def test_the_same_from_call_to_call():
     x, w, t = case(3000, 256, 5001, torch.bfloat16, 0.2)
     first = check_values(x, w, t)
