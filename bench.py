@@ -479,12 +479,13 @@ class ByteLM(torch.nn.Module):
         self.logits = nn.Linear(dim, 256, bias=False)
 
     def forward(self, ids):
+        from lookahead_keys_attention_b200 import castle_embedding, castle_linear_cross_entropy
         x, y = ids[:, :-1], ids[:, 1:]
-        h = self.emb(x)
+        h = castle_embedding(x, self.emb.weight)
         for a, f in zip(self.attn, self.ff):
             h = a(h) + h
             h = f(h) + h
-        return torch.nn.functional.cross_entropy(self.logits(self.norm(h)).float().flatten(0, 1), y.flatten())
+        return castle_linear_cross_entropy(self.norm(h), self.logits.weight, y)
 
 
 def cfg3_graph_step(lm, ids, c):
