@@ -294,6 +294,8 @@ struct CeProduct {
   float* target_logit;
   int64_t parts_ld;
   // kDx, kDw
+  uint16_t* g;           // kGrad: [plane][row, up to the tiles' end][g_ld]
+  int64_t g_ld, g_plane;
   float* lost;           // kGrad, kDx (16 bits): what rounding took from the target's entry of G, of each row that takes part
   const void* w;         // kDx: the weight, w_stride apart, of which the piece has rows [vocab0, vocab0 + k)
   int64_t w_stride;
@@ -374,9 +376,12 @@ template <CeMode MODE, typename OUT> __device__ __forceinline__ CeOut<OUT> ce_ou
   if (MODE == kDw || !on) return o;
   const CeRow r = p.rows[row];
   o.to = r.row;
-  if (CePlanes<OUT>::count == 1 && r.target >= p.vocab0 && r.target < p.vocab0 + p.k) {
-    o.w = static_cast<const OUT*>(p.w) + r.target * p.w_stride;
-    o.lost = p.lost[row];
+  if constexpr (CePlanes<OUT>::count == 1) {
+    const float lost = p.lost[row];
+    if (r.target >= p.vocab0 && r.target < p.vocab0 + p.k) {
+      o.w = static_cast<const OUT*>(p.w) + r.target * p.w_stride;
+      o.lost = lost;
+    }
   }
   return o;
 }
@@ -434,7 +439,7 @@ __device__ __forceinline__ void ce_emit(const CeProduct& p, float unit, int64_t 
 // registers on the way.
 template <typename T, typename OUT, CeMode MODE, bool REG, int PAIR>
 __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_copy,
-                                                               const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_g) {
+                                                               const __grid_constant__ CUtensorMap map_b) {
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
   constexpr int WIDTH = kCeWidth;
   constexpr int GRAIN = 16 * PAIR;   // columns come in multiples of it
@@ -565,6 +570,9 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
       const int local = rank * kCeM + quarter * 32 + lane, row = m * PAIR * kCeM + local, c_base = n * p.bn + share * width;
       const int cols = min(width, p.n - c_base);   // that there are; of the others up to the next grain are computed
       const bool empty = k1 <= k0;
+      const bool on = row < (MODE == kDw ? p.m : head.rows), direct = slot < 0 && !p.acc && p.vec;
+      CeOut<OUT> dst{0, nullptr, 0.f};
+      if constexpr (MODE == kDx || MODE == kDw) dst = ce_out<MODE, OUT>(p, row, on);
       float sums[REG ? WIDTH : 1];
       if constexpr (REG) {
 #pragma unroll
@@ -579,7 +587,11 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
             tmem_ld16(src + (turn & 1) * kCeN + c0, v);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sums[c0 + j] += v[j];
+            for (int j = 0; j < 16; j += 2) {
+              const float2 t = add2(make_float2(sums[c0 + j], sums[c0 + j + 1]), make_float2(v[j], v[j + 1]));
+              sums[c0 + j] = t.x;
+              sums[c0 + j + 1] = t.y;
+            }
           }
           release();
         }
@@ -605,7 +617,6 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
       };
       constexpr float kLog2e = 1.4426950408889634f;
       if constexpr (MODE == kLse) {
-        const bool on = row < head.rows;
         const int target = on ? p.rows[row].target - p.vocab0 - c_base : -1;
         float best = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -672,8 +683,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           __syncwarp();
 #pragma unroll
           for (int q = 0; q < PLANES; ++q) {
-            if (lane == 0) bulk_wait_read0();   // what was stored from here before has left
-            __syncwarp();
+            __syncwarp();   // what was here before has been read
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float w[32];
@@ -685,21 +695,23 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
               }
               store_row32<T>(staging, 4096, lane, h * 32, w);
             }
-            fence_async_smem();
             __syncwarp();
-            if (lane == 0) {   // (a tile is 128 columns wide at least: 64 for each share)
-              tma_store_4d(&map_g, staging, c_base + c0, row - lane, q, 0);
-              bulk_commit();
+            // Eight lanes store a row's 128 bytes; also the zeros of rows behind the last one.
+            uint16_t* out = p.g + q * p.g_plane + (int64_t)(row - lane) * p.g_ld + c_base + c0;
+            const int col = (lane & 7) * 8;
+            if (c0 + col < cols) {   // (g_ld is a multiple of 8)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int r = j * 4 + (lane >> 3);
+                *reinterpret_cast<uint4*>(out + r * p.g_ld + col) = *reinterpret_cast<const uint4*>(staging + swz_off(r, lane & 7));
+              }
             }
           }
         }
       } else {
-        const bool on = row < (MODE == kDw ? p.m : head.rows);
         const float unit = head.unit;
-        const CeOut<OUT> dst = ce_out<MODE, OUT>(p, row, on);
         const int64_t to = dst.to;
         constexpr int PANEL = 128 / (int)sizeof(OUT);   // columns of 128 bytes of a row
-        const bool direct = slot < 0 && !p.acc && p.vec;
 #pragma unroll
         for (int c0 = 0; c0 < WIDTH; c0 += 32) {
           if (c0 >= cols) break;
@@ -737,7 +749,6 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
       }
       if (!REG && !empty) release();
     }
-    if (MODE == kGrad && lane == 0) bulk_wait_read0();
   }
   __syncwarp();
   tc_fence_before();
@@ -946,8 +957,7 @@ static CeCut ce_cut(int64_t m, int64_t n, bool shared, int least) {
 }
 
 template <typename T, typename OUT, CeMode MODE, bool REG, int PAIR>
-static cudaError_t ce_launch_as(const CeProduct& p, int64_t tiles, const CUtensorMap& a, const CUtensorMap& copy, const CUtensorMap& b, const CUtensorMap& g,
-                                cudaStream_t st) {
+static cudaError_t ce_launch_as(const CeProduct& p, int64_t tiles, const CUtensorMap& a, const CUtensorMap& copy, const CUtensorMap& b, cudaStream_t st) {
   auto kernel = castle_ce_kernel<T, OUT, MODE, REG, PAIR>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kCeSmem);
   if (e != cudaSuccess) return e;
@@ -965,17 +975,16 @@ static cudaError_t ce_launch_as(const CeProduct& p, int64_t tiles, const CUtenso
   c.stream = st;
   c.attrs = attr;
   c.numAttrs = PAIR == 2 ? 2 : 1;
-  return cudaLaunchKernelEx(&c, kernel, p, a, copy, b, g);
+  return cudaLaunchKernelEx(&c, kernel, p, a, copy, b);
 }
 template <typename T, typename OUT, CeMode MODE>
-static cudaError_t ce_launch(const CeProduct& p, int pair, int64_t tiles, const CUtensorMap& a, const CUtensorMap& copy, const CUtensorMap& b, const CUtensorMap& g,
-                             cudaStream_t st) {
+static cudaError_t ce_launch(const CeProduct& p, int pair, int64_t tiles, const CUtensorMap& a, const CUtensorMap& copy, const CUtensorMap& b, cudaStream_t st) {
   constexpr bool F32 = CePlanes<OUT>::count > 1;
   if constexpr (MODE == kLse && !F32) {   // one emptying of an accumulator is none: it is read where it is
     if (p.k > p.flush * kCeK)
-      return pair == 2 ? ce_launch_as<T, OUT, MODE, true, 2>(p, tiles, a, copy, b, g, st) : ce_launch_as<T, OUT, MODE, true, 1>(p, tiles, a, copy, b, g, st);
+      return pair == 2 ? ce_launch_as<T, OUT, MODE, true, 2>(p, tiles, a, copy, b, st) : ce_launch_as<T, OUT, MODE, true, 1>(p, tiles, a, copy, b, st);
   }
-  return pair == 2 ? ce_launch_as<T, OUT, MODE, F32, 2>(p, tiles, a, copy, b, g, st) : ce_launch_as<T, OUT, MODE, F32, 1>(p, tiles, a, copy, b, g, st);
+  return pair == 2 ? ce_launch_as<T, OUT, MODE, F32, 2>(p, tiles, a, copy, b, st) : ce_launch_as<T, OUT, MODE, F32, 1>(p, tiles, a, copy, b, st);
 }
 
 static int ce_rows_per_cta(int64_t n) {   // a CTA per SM, at least 32 rows each
@@ -1050,7 +1059,7 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
     p.flush = q.terms > 1 ? kCeFlushF32 : kCeFlush;
     p.parts = (float2*)(c.work + q.parts); p.parts_ld = q.copy_rows; p.target_logit = (float*)(c.work + q.logit); p.status = c.status;
     const int64_t tiles_m = (c.n + kCeM * cut.pair - 1) / (kCeM * cut.pair);
-    CE_CUDA((ce_launch<T, OUT, kLse>(p, cut.pair, tiles_m * tiles_n, x, copy, w, w, c.st)), "castle_linear_ce_fwd launch");
+    CE_CUDA((ce_launch<T, OUT, kLse>(p, cut.pair, tiles_m * tiles_n, x, copy, w, c.st)), "castle_linear_ce_fwd launch");
     CeJoin j{};
     j.head = (CeHead*)c.work; j.rows = p.rows; j.parts = p.parts; j.running = (float2*)(c.work + q.running); j.target_logit = p.target_logit;
     j.sums = (double*)(c.work + q.sums); j.lse = lse; j.loss = loss; j.parts_ld = q.copy_rows; j.parts_n = kCeShares * tiles_n;
@@ -1068,7 +1077,7 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
   const char* what = "castle_linear_ce_bwd launch";
   const int op = c.dtype == CASTLE_F16 ? CASTLE_F16 : CASTLE_BF16;
   CE_CUDA(ce_rows<OUT>(c, q, lse, dloss, dx, nullptr, nullptr), what);
-  CUtensorMap x, copy, xk, copyk, w, wk, g, ga, gt;
+  CUtensorMap x, copy, xk, copyk, w, wk, ga, gt;
   CE_TRY(ce_x_maps(c, q, op, kCeM, &x, &copy));
   CE_TRY(ce_x_maps(c, q, op, kCeK, &xk, &copyk));
   CeProduct base{};
@@ -1079,7 +1088,7 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
   auto product = [&](auto mode, const CeProduct& p, const CeCut& cut, int64_t m, const CUtensorMap& a, const CUtensorMap& acopy, const CUtensorMap& b) -> cudaError_t {
     constexpr CeMode MODE = decltype(mode)::value;
     const int64_t tiles = (m + kCeM * cut.pair - 1) / (kCeM * cut.pair) * ((p.n + kCeN - 1) / kCeN);
-    const cudaError_t e = ce_launch<T, OUT, MODE>(p, cut.pair, tiles, a, acopy, b, b, c.st);
+    const cudaError_t e = ce_launch<T, OUT, MODE>(p, cut.pair, tiles, a, acopy, b, c.st);
     if (e != cudaSuccess || !p.share) return e;
     const int64_t shared = tiles < kCeWorkers / cut.pair ? tiles : kCeWorkers / cut.pair;
     auto sum = [&](auto pair, auto cols) {
@@ -1098,13 +1107,13 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), what);
     CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
     CE_TRY(ce_w_map(c, q, op, count, kCeK, &wk));
-    CE_TRY(ce_map(&g, gp, op, q.g_rows, (int)count, pitch, q.g_rows * pitch, q.planes, 32, "castle_linear_ce: logits' gradient"));
     CE_TRY(ce_map(&ga, gp, op, q.g_rows, (int)count, pitch, q.g_rows * pitch, q.planes, kCeM, "castle_linear_ce: logits' gradient"));
     CE_TRY(ce_map(&gt, gp, op, q.g_rows, (int)count, pitch, q.g_rows * pitch, q.planes, kCeK, "castle_linear_ce: logits' gradient"));
     CeProduct p = base;
     p.n = (int)count; p.k = q.pitch; p.bn = cut.bn; p.b_row0 = q.copy_w ? 0 : (int)v0; p.vocab0 = (int)v0; p.group = 32 / cut.pair;
+    p.g = gp; p.g_ld = pitch; p.g_plane = q.g_rows * pitch;
     const int64_t tiles_m = (c.n + kCeM * cut.pair - 1) / (kCeM * cut.pair);
-    CE_CUDA((ce_launch<T, OUT, kGrad>(p, cut.pair, tiles_m * ((count + cut.bn - 1) / cut.bn), x, copy, w, g, c.st)), what);
+    CE_CUDA((ce_launch<T, OUT, kGrad>(p, cut.pair, tiles_m * ((count + cut.bn - 1) / cut.bn), x, copy, w, c.st)), what);
     if (dx) {
       p = base;
       p.vocab0 = (int)v0; p.w = c.w; p.w_stride = c.ws; p.w_vec = c.dim % 8 == 0 && (uintptr_t)c.w % 16 == 0 && c.ws % 8 == 0;
