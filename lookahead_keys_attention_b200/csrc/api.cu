@@ -1,4 +1,8 @@
 // Version and error-text entry points of the C ABI.
+#include <map>
+#include <mutex>
+#include <utility>
+
 #include "common.cuh"
 
 namespace castle {
@@ -9,6 +13,23 @@ char* last_error_buf() {
 KernelEvents& kernel_events(int which) {
   static KernelEvents ev[3];  // process-wide: torch runs backward passes on its own worker thread
   return ev[which];
+}
+cudaError_t allow_smem(const void* kernel, int bytes) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  try {
+    static std::mutex mutex;
+    static auto& known = *new std::map<std::pair<const void*, int>, int>();   // never destroyed: other threads may still call at exit
+    std::lock_guard<std::mutex> lock(mutex);
+    int& have = known[{kernel, device}];
+    if (have >= bytes) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) have = bytes;
+    return e;
+  } catch (...) {   // no memory for the record: ask each time
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  }
 }
 }  // namespace castle
 

@@ -47,6 +47,10 @@ inline cudaError_t launch_kernel(void (*kernel)(P...), dim3 grid, int threads, s
   return cudaLaunchKernelEx(&c, kernel, P(args)...);
 }
 
+// Dynamic shared memory beyond 48 KB for a kernel on the current device, asked for once (a call costs the host half a microsecond).
+cudaError_t allow_smem(const void* kernel, int bytes);   // defined in api.cu
+template <typename K> inline cudaError_t allow_smem(K* kernel, int bytes) { return allow_smem(reinterpret_cast<const void*>(kernel), bytes); }
+
 inline int elem_size(int dtype) { return dtype == CASTLE_F32 ? 4 : 2; }
 
 inline bool tensor_ok(const castle_tensor_t* t, int dtype, const char* name, int* rc) {

@@ -504,13 +504,13 @@ extern "C" int castle_embedding_bwd(int32_t dtype, int32_t index_bytes, int64_t 
   int2* bins = (int2*)(ws + s.bins);
   int32_t* begins = (int32_t*)(ws + s.begins);
   auto bin = [&](auto kernel) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxOwners * kBinWarps * 4);
+    const cudaError_t e = allow_smem(kernel, kMaxOwners * kBinWarps * 4);
     if (e != cudaSuccess) return e;
     kernel<<<kSlices, kBinThreads, bin_smem, st>>>(index, tokens, slice, (uint32_t)vocab, padding_idx < 0 ? kNoRow : (uint32_t)padding_idx, p.order, bins, begins, p.long_count, status);
     return cudaGetLastError();
   };
   cudaError_t e = index_bytes == 8 ? bin(castle_token_bin_kernel<int64_t>) : bin(castle_token_bin_kernel<int32_t>);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(castle_token_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortRows * kSortWarps * 4);
+  if (e == cudaSuccess) e = allow_smem(castle_token_sort_kernel, kSortRows * kSortWarps * 4);
   if (e == cudaSuccess)
     e = launch_kernel(castle_token_sort_kernel, dim3(p.order.owners()), kSortThreads, sort_smem, st, true, (const int2*)bins, (const int32_t*)begins, slice, p.order, start,
                       sorted, row_of);

@@ -428,7 +428,7 @@ template <typename F> static cudaError_t ln_group(int dim, F&& f) {
 }
 template <typename K, typename... A> static cudaError_t ln_launch(K kernel, int64_t grid, int threads, size_t ring, cudaStream_t st, A... args) {
   if (ring > 16384) {   // (beside up to 17 KB of the kernel's own)
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
+    const cudaError_t e = allow_smem(kernel, (int)ring);
     if (e != cudaSuccess) return e;
   }
   kernel<<<(unsigned)grid, threads, ring, st>>>(args...);

@@ -62,8 +62,8 @@ struct CeTurn {
   }
 };
 constexpr int64_t kCeScratch = (int64_t)1 << 30;   // bytes that a piece of the vocabulary may take
-// Steps between emptyings: of a 16-bit operand's logits (32 additions in the tensor cores), of fp32's parts (24).  197 x 512 in
-// fp32: TBD
+// Steps between emptyings: of a 16-bit operand's logits (32 additions in the tensor cores), of fp32's parts (24).  With these the losses of
+// 197 x 512 in fp32 are 6.7e-8 of their norm off; not emptied 3.3e-6 and, of logits over 1024 in 16 bits, 8 % faster (166 us, 152).
 constexpr int kCeFlush = 8, kCeFlushF32 = 1, kCeNoFlush = 1 << 30;
 constexpr float kCeUnit = 16384.f;                 // of G: below 2 units
 
@@ -310,7 +310,7 @@ struct CeProduct {
 
 // What a worker (a CTA, or a pair) does: tiles, and slices of the contraction (steps of 64) of those that do not go evenly to the workers.
 // Slices are dealt out one after the other, each with all its tiles, so that workers that run together read the same part of the operands
-// (one worker's equal share of all steps in a row instead read them from memory again and again: 243 us where this takes TBD).
+// (one worker's equal share of all steps in a row instead read them from memory again and again: 243 us where this takes 160).
 template <CeMode MODE, int PAIR> struct CeWork {
   int tiles_m, tiles_n, steps, whole, left, slices, per, workers, group;
   __device__ __forceinline__ CeWork(const CeProduct& p, int rows, int count) : workers(count) {
@@ -685,15 +685,20 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           for (int q = 0; q < PLANES; ++q) {
             __syncwarp();   // what was here before has been read
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float w[32];
+            for (int c = 0; c < 8; ++c) {   // a plane's part of each value, and what it leaves to the next
+              uint4 o;
+              uint32_t* u = &o.x;
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                float parts[PLANES];
-                CePlanes<OUT>::split(v[h * 32 + j], parts);
-                w[j] = parts[q];
+              for (int j = 0; j < 4; ++j) {
+                float* pair = v + c * 8 + 2 * j;
+                u[j] = Elem<T>::pack2(pair[0], pair[1]);
+                if (q + 1 < PLANES) {
+                  const float2 f = Elem<T>::unpack2(u[j]);
+                  pair[0] -= f.x;
+                  pair[1] -= f.y;
+                }
               }
-              store_row32<T>(staging, 4096, lane, h * 32, w);
+              *reinterpret_cast<uint4*>(staging + swz_off(lane, c)) = o;
             }
             __syncwarp();
             // Eight lanes store a row's 128 bytes; also the zeros of rows behind the last one.
@@ -825,11 +830,17 @@ __global__ void __launch_bounds__(256) castle_ce_join_kernel(const CeJoin p) {
 #pragma unroll 4
     for (int k = l; k < p.parts_n; k += LANES) join(p.parts[(int64_t)k * p.parts_ld + row]);
   }
-  s[l][r] = make_float2(best, sum);
+  if constexpr (ROWS == 1) {   // trees: 256 parts one after the other would take as long as the rest
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) join(make_float2(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, sum, o)));
+    if ((l & 31) == 0) s[l >> 5][0] = make_float2(best, sum);
+  } else {
+    s[l][r] = make_float2(best, sum);
+  }
   __syncthreads();
   double loss = 0.0;
   if (l == 0 && row < rows) {
-    for (int k = 1; k < LANES; ++k) join(s[k][r]);
+    for (int k = 1; k < (ROWS == 1 ? 8 : LANES); ++k) join(s[k][r]);
     if (!p.end) {
       p.running[row] = make_float2(best, sum);
     } else {
@@ -905,13 +916,13 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
   const int64_t most = backward ? q.piece_bwd : q.piece_fwd;
   q.wcopy = take(q.copy_w ? (size_t)most * w_row : 0);
   if (!backward) {
-    // kCeShares for each tile of a row: 256 columns, or less where 128 rows by twice as many would make fewer than 148 tiles (ce_cut)
-    const int64_t wide = (q.piece_fwd + kCeN - 1) / kCeN, few = 296 / ((n + kCeM - 1) / kCeM) + 1, most_tiles = wide > few ? wide : few;
-    q.parts_per_piece = kCeShares * (int)(most_tiles < (q.piece_fwd + 63) / 64 ? most_tiles : (q.piece_fwd + 63) / 64);
+    // kCeShares for each tile of a row: of 256 columns, or fewer where all tiles run at once (ce_cut)
+    const int64_t wide = (q.piece_fwd + kCeN - 1) / kCeN;
+    q.parts_per_piece = kCeShares * (int)(wide > kCeWorkers ? wide : kCeWorkers);
     q.parts = take((size_t)q.parts_per_piece * q.copy_rows * sizeof(float2));
     q.running = take((size_t)n * sizeof(float2));
     q.logit = take((size_t)n * sizeof(float));
-    q.sums = take((size_t)((n + 7) / 8) * sizeof(double));
+    q.sums = take((size_t)((n + 7) / 8 + 256) * sizeof(double));
   } else {
     q.g = take((size_t)q.planes * q.g_rows * up(q.piece_bwd, 8) * 2);
     q.lost = take((size_t)n * sizeof(float));
@@ -945,21 +956,29 @@ static int ce_map(CUtensorMap* m, const void* p, int op, int64_t rows, int cols,
   return make_tmap_16bit(m, &t, op, 1, planes, (int)rows, cols, box_rows, what);
 }
 
-// How a result of m x n is cut: pairs of CTAs where there are tiles for half of them (or a long contraction to share out), else single
-// ones, with narrower tiles while there are SMs without one.  us, pairs / single: TBD
+// How a result of m x n over a contraction of k is cut.  Pairs of CTAs are some 15 % faster per row where the contraction is long and 8 %
+// slower where it is short (the second CTA waits for the first's products at a tile's start and end), and pad the rows to 256
+// instead of 128.  us, pairs / single: logits 197 x 4096 against 131072 213 / 228, 300 x 1024 against 50021 49 / 41, 600 x 1024 59 / 57, 2000 x 512
+// against 8000 20.6 / 18.6; dx of 600 x 1024 72 / 80, of 300 x 1024 55 / 51; dW, whose rows are the vocabulary, at 300 rows 53 / 44, at 600 63 / 67, at
+// 1000 32 / 36.  Narrower tiles (of single ones that do not share a contraction out) as long as all of them run at once: 130 x 512 against
+// 256 5.9 / 8.0 with 256 columns, but two rounds of half tiles are slower than one of whole ones (50 x 768 against 32000 in fp32 55 / 43).
 struct CeCut { int pair, bn; };
-static CeCut ce_cut(int64_t m, int64_t n, bool shared, int least) {
-  const int64_t tiles = (m + 255) / 256 * ((n + 255) / 256);
-  if (m > kCeM && (tiles >= 37 || shared)) return {2, 256};
+static CeCut ce_cut(CeMode mode, int64_t m, int64_t n, int64_t k) {
+  const int64_t single = (m + 127) / 128 * 128, pairs = (m + 255) / 256 * 256;
+  const bool logits = mode == kLse || mode == kGrad;
+  if (mode == kDw ? m > kCeM && k > 512 : k >= 1024 ? pairs * 85 < single * 100 : pairs * 108 < single * 100) {
+    if (!logits || pairs / 256 * ((n + 255) / 256) >= 37) return {2, 256};   // (half of the pairs have a tile)
+  }
+  const int least = mode == kLse ? 32 * kCeShares : mode == kGrad ? 64 * kCeShares : 256;   // what a warp works on at a time
   int bn = 256;
-  while (!shared && bn > least && (m + 127) / 128 * ((n + bn - 1) / bn) < 148) bn /= 2;
+  while (bn > least && single / 128 * ((2 * n + bn - 1) / bn) <= kCeWorkers) bn /= 2;
   return {1, bn};
 }
 
 template <typename T, typename OUT, CeMode MODE, bool REG, int PAIR>
 static cudaError_t ce_launch_as(const CeProduct& p, int64_t tiles, const CUtensorMap& a, const CUtensorMap& copy, const CUtensorMap& b, cudaStream_t st) {
   auto kernel = castle_ce_kernel<T, OUT, MODE, REG, PAIR>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kCeSmem);
+  const cudaError_t e = allow_smem(kernel, (int)kCeSmem);
   if (e != cudaSuccess) return e;
   const int64_t most = p.share ? kCeWorkers : tiles * PAIR;
   cudaLaunchConfig_t c = {};
@@ -1049,7 +1068,7 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
   CE_TRY(ce_x_maps(c, q, op, kCeM, &x, &copy));
   for (int64_t v0 = 0; v0 < c.vocab; v0 += q.piece_fwd) {
     const int64_t count = c.vocab - v0 < q.piece_fwd ? c.vocab - v0 : q.piece_fwd;
-    const CeCut cut = ce_cut(c.n, count, false, 32 * kCeShares);
+    const CeCut cut = ce_cut(kLse, c.n, count, q.pitch);
     const int tiles_n = (int)((count + cut.bn - 1) / cut.bn);
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), "castle_linear_ce_fwd launch");
     CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
@@ -1064,8 +1083,9 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
     j.head = (CeHead*)c.work; j.rows = p.rows; j.parts = p.parts; j.running = (float2*)(c.work + q.running); j.target_logit = p.target_logit;
     j.sums = (double*)(c.work + q.sums); j.lse = lse; j.loss = loss; j.parts_ld = q.copy_rows; j.parts_n = kCeShares * tiles_n;
     j.begin = v0 == 0; j.end = v0 + count == c.vocab; j.each = each; j.mean = c.reduction == CASTLE_REDUCE_MEAN;
-    // few rows: a warp each; many: neighbouring threads on neighbouring rows
-    if (c.n >= 4096) CE_CUDA(launch_kernel(castle_ce_join_kernel<32>, dim3((unsigned)((c.n + 31) / 32)), 256, 0, c.st, true, j), "castle_linear_ce_fwd launch");
+    // few rows: a CTA or a warp each; many: neighbouring threads on neighbouring rows
+    if (c.n < 256) CE_CUDA(launch_kernel(castle_ce_join_kernel<1>, dim3((unsigned)c.n), 256, 0, c.st, true, j), "castle_linear_ce_fwd launch");
+    else if (c.n >= 4096) CE_CUDA(launch_kernel(castle_ce_join_kernel<32>, dim3((unsigned)((c.n + 31) / 32)), 256, 0, c.st, true, j), "castle_linear_ce_fwd launch");
     else CE_CUDA(launch_kernel(castle_ce_join_kernel<8>, dim3((unsigned)((c.n + 7) / 8)), 256, 0, c.st, true, j), "castle_linear_ce_fwd launch");
   }
   return 0;
@@ -1097,13 +1117,13 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
     };
     using std::integral_constant;
     // few tiles: many parts of each, added by many threads; else whole sectors of the result by each thread
-    if (cut.pair == 1) return sum(integral_constant<int, 1>(), integral_constant<int, 4>());
+    if (cut.pair == 1) return shared < 32 ? sum(integral_constant<int, 1>(), integral_constant<int, 4>()) : sum(integral_constant<int, 1>(), integral_constant<int, 16>());
     return shared < 16 ? sum(integral_constant<int, 2>(), integral_constant<int, 4>()) : sum(integral_constant<int, 2>(), integral_constant<int, 16>());
   };
   for (int64_t v0 = 0; v0 < c.vocab; v0 += q.piece_bwd) {
     const int64_t count = c.vocab - v0 < q.piece_bwd ? c.vocab - v0 : q.piece_bwd, pitch = (count + 7) / 8 * 8;
     uint16_t* gp = (uint16_t*)(c.work + q.g);
-    const CeCut cut = ce_cut(c.n, count, false, 64 * kCeShares), cut_dx = ce_cut(c.n, c.dim, true, kCeN), cut_dw = ce_cut(count, c.dim, true, kCeN);
+    const CeCut cut = ce_cut(kGrad, c.n, count, q.pitch), cut_dx = ce_cut(kDx, c.n, c.dim, count), cut_dw = ce_cut(kDw, count, c.dim, c.n);
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), what);
     CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
     CE_TRY(ce_w_map(c, q, op, count, kCeK, &wk));
