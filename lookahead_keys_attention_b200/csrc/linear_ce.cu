@@ -615,6 +615,13 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           tmem_ld_wait();
         }
       };
+      bool held = !REG && !empty;
+      auto last_taken = [&](bool last) {   // the next product into the accumulator runs under the rest
+        if (held && last) {
+          release();
+          held = false;
+        }
+      };
       constexpr float kLog2e = 1.4426950408889634f;
       if constexpr (MODE == kLse) {
         const int target = on ? p.rows[row].target - p.vocab0 - c_base : -1;
@@ -624,6 +631,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           if (c0 >= cols) break;
           float v[32];
           take(std::integral_constant<int, 32>(), c0, v);
+          last_taken(c0 + 32 >= cols);
           if (c0 + 32 > cols) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = c0 + j < cols ? v[j] : -INFINITY;
@@ -660,6 +668,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           if (c0 >= cols) break;
           float v[64];
           take(std::integral_constant<int, 64>(), c0, v);
+          last_taken(c0 + 64 >= cols);
 #pragma unroll
           for (int j = 0; j < 64; j += 2) {
             const float2 d = mul2(add2(make_float2(v[j], v[j + 1]), splat(-r.lse)), splat(kLog2e));
@@ -722,6 +731,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           if (c0 >= cols) break;
           float v[32];
           take(std::integral_constant<int, 32>(), c0, v);
+          last_taken(c0 + 32 >= cols);
           if (slot >= 0) {
             float4* out = p.slab + ((int64_t)slot * (kCeN / 4) + (share * width + c0) / 4) * (kCeM * PAIR) + local;
 #pragma unroll
@@ -739,8 +749,17 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 const int r = j * 4 + (lane >> 3);
-                const int64_t row_to = __shfl_sync(0xffffffffu, to, r);
-                if (__shfl_sync(0xffffffffu, on, r) && col < min(cols, c0 + 32))
+                int64_t row_to;
+                bool there;
+                if constexpr (MODE == kDw) {
+                  there = row - lane + r < p.m;
+                  row_to = to - lane + r;
+                } else {
+                  const int target = __shfl_sync(0xffffffffu, on ? (int)to : -1, r);
+                  there = target >= 0;
+                  row_to = target;
+                }
+                if (there && col < min(cols, c0 + 32))
                   *reinterpret_cast<uint4*>(static_cast<OUT*>(p.out) + row_to * p.ld + c_base + col) = *reinterpret_cast<const uint4*>(staging + swz_off(r, lane & 7));
               }
               __syncwarp();
@@ -752,7 +771,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           __syncwarp();
         }
       }
-      if (!REG && !empty) release();
+      last_taken(true);
     }
   }
   __syncwarp();
@@ -956,7 +975,7 @@ static int ce_map(CUtensorMap* m, const void* p, int op, int64_t rows, int cols,
   return make_tmap_16bit(m, &t, op, 1, planes, (int)rows, cols, box_rows, what);
 }
 
-// How a result of m x n over a contraction of k is cut.  Pairs of CTAs are some 15 % faster per row where the contraction is long and 8 %
+// How a result of m x n over a contraction of k (all terms of it) is cut.  Pairs of CTAs are some 15 % faster per row where the contraction is long and 8 %
 // slower where it is short (the second CTA waits for the first's products at a tile's start and end), and pad the rows to 256
 // instead of 128.  us, pairs / single: logits 197 x 4096 against 131072 213 / 228, 300 x 1024 against 50021 49 / 41, 600 x 1024 59 / 57, 2000 x 512
 // against 8000 20.6 / 18.6; dx of 600 x 1024 72 / 80, of 300 x 1024 55 / 51; dW, whose rows are the vocabulary, at 300 rows 53 / 44, at 600 63 / 67, at
@@ -1068,7 +1087,7 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
   CE_TRY(ce_x_maps(c, q, op, kCeM, &x, &copy));
   for (int64_t v0 = 0; v0 < c.vocab; v0 += q.piece_fwd) {
     const int64_t count = c.vocab - v0 < q.piece_fwd ? c.vocab - v0 : q.piece_fwd;
-    const CeCut cut = ce_cut(kLse, c.n, count, q.pitch);
+    const CeCut cut = ce_cut(kLse, c.n, count, (int64_t)q.pitch * q.terms);
     const int tiles_n = (int)((count + cut.bn - 1) / cut.bn);
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), "castle_linear_ce_fwd launch");
     CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
@@ -1123,7 +1142,8 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
   for (int64_t v0 = 0; v0 < c.vocab; v0 += q.piece_bwd) {
     const int64_t count = c.vocab - v0 < q.piece_bwd ? c.vocab - v0 : q.piece_bwd, pitch = (count + 7) / 8 * 8;
     uint16_t* gp = (uint16_t*)(c.work + q.g);
-    const CeCut cut = ce_cut(kGrad, c.n, count, q.pitch), cut_dx = ce_cut(kDx, c.n, c.dim, count), cut_dw = ce_cut(kDw, count, c.dim, c.n);
+    const CeCut cut = ce_cut(kGrad, c.n, count, (int64_t)q.pitch * q.terms), cut_dx = ce_cut(kDx, c.n, c.dim, count * q.terms),
+                cut_dw = ce_cut(kDw, count, c.dim, c.n * q.terms);
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), what);
     CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
     CE_TRY(ce_w_map(c, q, op, count, kCeK, &wk));
