@@ -15,7 +15,7 @@
 //
 // The four products are one kernel: CTAs that stay, one per SM, in pairs (256 x 256 of the result, 64 of the contraction at a time) or, where
 // there is less to do, alone (128 x 256, 128 or 64), each with a warp that loads tiles by TMA, a warp that issues the tensor cores'
-// products, and eight warps that work on a finished tile in one half of tensor memory while the next one is summed in the other.
+// products, and eight or sixteen warps that work on a finished tile in one half of tensor memory while the next one is summed in the other.
 // Alone, an SM's shared memory brings in and reads 24 KB in the 128 cycles of a product of 16, more than it can (78 % of the tensor cores' cycles at
 // a contraction of 50021); a pair shares B's tile.  All sums, the logits and the statistics are fp32.
 //
@@ -45,12 +45,16 @@ namespace castle {
 enum CeMode { kLse, kGrad, kDx, kDw };
 
 constexpr int kCeM = 128, kCeN = 256, kCeK = 64;
-// The warps that work on tiles.  (Sixteen instead of eight: no faster; the logits' gradient of 4095 x 1024 against 50021 188 us instead of 172.)
-constexpr int kCeWarps = 8, kCeShares = kCeWarps / 4, kCeThreads = (kCeWarps + 2) * 32, kCeWidth = kCeN / kCeShares;
+// The warps that work on tiles.  Sixteen hide what each waits for better where results are written (131072 x 4096 of dW over 8 rows: TBD);
+// with eight a row's statistics have fewer parts.
+template <CeMode MODE> constexpr int kCeWarps = MODE == kLse ? 8 : 16;
+template <CeMode MODE> constexpr int kCeShares = kCeWarps<MODE> / 4;      // of a tile's columns
+template <CeMode MODE> constexpr int kCeThreads = (kCeWarps<MODE> + 2) * 32;
 constexpr uint32_t kCeA = kCeM * kCeK * 2;
 constexpr uint32_t kCeRing = 4 * (kCeA + kCeN * kCeK * 2);   // stages: 4 of a CTA alone with a tile of 256 columns, 6 of 128 or of a pair, 8 of 64
 constexpr int kCeStages = 8;
-constexpr uint32_t kCeStaging = kCeWarps * 4096;   // results on their way out: 32 rows x 128 bytes of each working warp
+constexpr uint32_t kCeStaging = 16 * 2048;   // results on their way out: 32 rows x 64 bytes of each working warp
+__device__ __forceinline__ uint32_t staging_off(int row, int chunk16) { return row * 64 + ((chunk16 ^ ((row >> 1) & 3)) << 4); }   // without bank conflicts
 constexpr size_t kCeSmem = kCeRing + kCeStaging + 1024;
 // The stages in turn: which, and in which of its barriers' two phases.
 struct CeTurn {
@@ -290,7 +294,7 @@ struct CeProduct {
   bool share;            // tiles may be shared out among workers (kDx, kDw)
   bool vec, w_vec;       // out can be stored, the weight read 16 bytes at a time
   // kLse
-  float2* parts;         // [kCeShares per tile of n][parts_ld]
+  float2* parts;         // [kCeShares<kLse> per tile of n][parts_ld]
   float* target_logit;
   int64_t parts_ld;
   // kDx, kDw
@@ -438,10 +442,10 @@ __device__ __forceinline__ void ce_emit(const CeProduct& p, float unit, int64_t 
 // T: the operands' type, OUT: the result's (kDx, kDw) or the caller's (kGrad: float means three planes of G).  REG: accumulators are emptied into
 // registers on the way.
 template <typename T, typename OUT, CeMode MODE, bool REG, int PAIR>
-__global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_copy,
+__global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const CeProduct p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_copy,
                                                                const __grid_constant__ CUtensorMap map_b) {
   constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDx || MODE == kDw;
-  constexpr int WIDTH = kCeWidth;
+  constexpr int SHARES = kCeShares<MODE>, WIDTH = kCeN / SHARES;
   constexpr int GRAIN = 16 * PAIR;   // columns come in multiples of it
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -452,7 +456,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
   const uint32_t rank = PAIR == 2 ? cluster_rank() : 0;
   if (tid == 0) {
     for (int s = 0; s < kCeStages; ++s) { mbar_init(&bar_full[s], 1); mbar_init(&bar_free[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&bar_done[s], 1); mbar_init(&bar_read[s], kCeWarps * PAIR); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&bar_done[s], 1); mbar_init(&bar_read[s], kCeWarps<MODE> * PAIR); }
     mbar_init(&bar_end, 1);
     mbar_fence_init();
     abort_flag = 0;
@@ -551,9 +555,9 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
       mbar_drain(&bar_end, 0);
     }
   } else {
-    const int quarter = warp & 3, share = (warp - 2) >> 2, width = p.bn / kCeShares;   // a warp has 32 rows and a share of the columns
+    const int quarter = warp & 3, share = (warp - 2) >> 2, width = p.bn / SHARES;   // a warp has 32 rows and a share of the columns
     const uint32_t src = tmem + share * width + ((uint32_t)(quarter * 32) << 16);
-    uint8_t* staging = smem + kCeRing + (warp - 2) * 4096;
+    uint8_t* staging = smem + kCeRing + (warp - 2) * 2048;
     const uint32_t read_at = PAIR == 2 ? of_cta(&bar_read[0], 0) : 0;
     int turn = 0;
     bool over = false;
@@ -600,18 +604,15 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         if (mbar_wait_failed(&bar_done[turn & 1], (uint32_t)(turn >> 1) & 1u, abortp)) break;
         tc_fence_after();
       }
-      // values [c0, c0 + COUNT) of the thread's part of a row
-      auto take = [&](auto count, int c0, float* v) {
-        constexpr int COUNT = decltype(count)::value;
+      auto take = [&](int c0, float* v) {   // values [c0, c0 + 32) of the thread's part of a row
         if constexpr (REG) {
 #pragma unroll
-          for (int j = 0; j < COUNT; ++j) v[j] = sums[c0 + j];
+          for (int j = 0; j < 32; ++j) v[j] = sums[c0 + j];
         } else if (MODE == kDw && empty) {   // no rows take part
 #pragma unroll
-          for (int j = 0; j < COUNT; ++j) v[j] = 0.f;
+          for (int j = 0; j < 32; ++j) v[j] = 0.f;
         } else {
-#pragma unroll
-          for (int j = 0; j < COUNT; j += 32) tmem_ld32(src + (turn & 1) * kCeN + c0 + j, v + j);
+          tmem_ld32(src + (turn & 1) * kCeN + c0, v);
           tmem_ld_wait();
         }
       };
@@ -630,7 +631,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         for (int c0 = 0; c0 < WIDTH; c0 += 32) {
           if (c0 >= cols) break;
           float v[32];
-          take(std::integral_constant<int, 32>(), c0, v);
+          take(c0, v);
           last_taken(c0 + 32 >= cols);
           if (c0 + 32 > cols) {
 #pragma unroll
@@ -656,7 +657,7 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
           sum = fmaf(sum, ex2_approx((best - zero) * kLog2e), s2.x + s2.y);
           best = top;
         }
-        if (on) p.parts[(int64_t)(n * kCeShares + share) * p.parts_ld + row] = make_float2(best, sum);
+        if (on) p.parts[(int64_t)(n * SHARES + share) * p.parts_ld + row] = make_float2(best, sum);
       } else if constexpr (MODE == kGrad) {
         CeRow r;
         r.target = -1; r.lse = 0.f; r.coef = 0.f; r.row = 0;
@@ -664,37 +665,38 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
         const int target = r.target - p.vocab0 - c_base;
         constexpr int PLANES = CePlanes<OUT>::count;
 #pragma unroll
-        for (int c0 = 0; c0 < WIDTH; c0 += 64) {
+        for (int c0 = 0; c0 < WIDTH; c0 += 32) {
           if (c0 >= cols) break;
-          float v[64];
-          take(std::integral_constant<int, 64>(), c0, v);
-          last_taken(c0 + 64 >= cols);
+          float v[32];
+          take(c0, v);
+          last_taken(c0 + 32 >= cols);
 #pragma unroll
-          for (int j = 0; j < 64; j += 2) {
+          for (int j = 0; j < 32; j += 2) {
             const float2 d = mul2(add2(make_float2(v[j], v[j + 1]), splat(-r.lse)), splat(kLog2e));
             v[j] = ex2_approx(d.x);
             v[j + 1] = ex2_approx(d.y);
           }
-          if (target >= c0 && target < c0 + 64) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = c0 + j == target ? v[j] - 1.f : v[j];
-          }
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] = r.coef == 0.f ? 0.f : v[j] * r.coef;
-          if (PLANES == 1 && target >= c0 && target < min(c0 + 64, cols)) {
+          if (target >= c0 && target < min(c0 + 32, cols)) {
             float g = 0.f;
 #pragma unroll
-            for (int j = 0; j < 64; ++j) g = c0 + j == target ? v[j] : g;
-            const float lost = g - Elem<T>::to_f(Elem<T>::from_f(g));
-            p.lost[row] = isfinite(lost) ? lost : 0.f;
+            for (int j = 0; j < 32; ++j) {
+              v[j] = c0 + j == target ? v[j] - 1.f : v[j];
+              g = c0 + j == target ? v[j] : g;
+            }
+            if (PLANES == 1) {
+              g *= r.coef;
+              const float lost = g - Elem<T>::to_f(Elem<T>::from_f(g));
+              p.lost[row] = isfinite(lost) ? lost : 0.f;
+            }
           }
           __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = r.coef == 0.f ? 0.f : v[j] * r.coef;
 #pragma unroll
           for (int q = 0; q < PLANES; ++q) {
             __syncwarp();   // what was here before has been read
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {   // a plane's part of each value, and what it leaves to the next
+            for (int c = 0; c < 4; ++c) {   // a plane's part of each value, and what it leaves to the next
               uint4 o;
               uint32_t* u = &o.x;
 #pragma unroll
@@ -707,17 +709,17 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
                   pair[1] -= f.y;
                 }
               }
-              *reinterpret_cast<uint4*>(staging + swz_off(lane, c)) = o;
+              *reinterpret_cast<uint4*>(staging + staging_off(lane, c)) = o;
             }
             __syncwarp();
-            // Eight lanes store a row's 128 bytes; also the zeros of rows behind the last one.
+            // Four lanes store a row's 64 bytes; also the zeros of rows behind the last one.
             uint16_t* out = p.g + q * p.g_plane + (int64_t)(row - lane) * p.g_ld + c_base + c0;
-            const int col = (lane & 7) * 8;
+            const int col = (lane & 3) * 8;
             if (c0 + col < cols) {   // (g_ld is a multiple of 8)
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int r = j * 4 + (lane >> 3);
-                *reinterpret_cast<uint4*>(out + r * p.g_ld + col) = *reinterpret_cast<const uint4*>(staging + swz_off(r, lane & 7));
+              for (int j = 0; j < 4; ++j) {
+                const int at = j * 8 + (lane >> 2);
+                *reinterpret_cast<uint4*>(out + at * p.g_ld + col) = *reinterpret_cast<const uint4*>(staging + staging_off(at, lane & 3));
               }
             }
           }
@@ -725,42 +727,47 @@ __global__ void __launch_bounds__(kCeThreads) castle_ce_kernel(const CeProduct p
       } else {
         const float unit = head.unit;
         const int64_t to = dst.to;
-        constexpr int PANEL = 128 / (int)sizeof(OUT);   // columns of 128 bytes of a row
 #pragma unroll
         for (int c0 = 0; c0 < WIDTH; c0 += 32) {
           if (c0 >= cols) break;
           float v[32];
-          take(std::integral_constant<int, 32>(), c0, v);
+          take(c0, v);
           last_taken(c0 + 32 >= cols);
           if (slot >= 0) {
             float4* out = p.slab + ((int64_t)slot * (kCeN / 4) + (share * width + c0) / 4) * (kCeM * PAIR) + local;
 #pragma unroll
             for (int j = 0; j < 32; j += 4) out[(j / 4) * (kCeM * PAIR)] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
           } else if (direct) {
-            // through shared memory, so that eight lanes store a row's 128 bytes
+            // through shared memory, so that four lanes store 64 bytes of a row
             if constexpr (MODE == kDx) ce_add_lost<OUT, 32>(p, dst, c_base + c0, min(32, cols - c0), v);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= unit;
-            if constexpr (sizeof(OUT) == 4) store_row32_f32(staging, lane, v);
-            else store_row32<OUT>(staging, 4096, lane, c0 % 64, v);
-            if (c0 % PANEL + 32 == PANEL || c0 + 32 >= cols) {
-              __syncwarp();
-              const int first = c0 / PANEL * PANEL, col = first + (lane & 7) * (PANEL / 8);
+            constexpr int PIECE = 16 / (int)sizeof(OUT), PANEL = 4 * PIECE;   // columns of 16 bytes, and of 64
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int r = j * 4 + (lane >> 3);
+            for (int h = 0; h < 32; h += PANEL) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const float* f = v + h + c * PIECE;
+                if constexpr (sizeof(OUT) == 4) *reinterpret_cast<float4*>(staging + staging_off(lane, c)) = make_float4(f[0], f[1], f[2], f[3]);
+                else store8<OUT>(reinterpret_cast<OUT*>(staging + staging_off(lane, c)), f);
+              }
+              __syncwarp();
+              const int col = c0 + h + (lane & 3) * PIECE;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int at = j * 8 + (lane >> 2);
                 int64_t row_to;
                 bool there;
                 if constexpr (MODE == kDw) {
-                  there = row - lane + r < p.m;
-                  row_to = to - lane + r;
+                  there = row - lane + at < p.m;
+                  row_to = to - lane + at;
                 } else {
-                  const int target = __shfl_sync(0xffffffffu, on ? (int)to : -1, r);
+                  const int target = __shfl_sync(0xffffffffu, on ? (int)to : -1, at);
                   there = target >= 0;
                   row_to = target;
                 }
-                if (there && col < min(cols, c0 + 32))
-                  *reinterpret_cast<uint4*>(static_cast<OUT*>(p.out) + row_to * p.ld + c_base + col) = *reinterpret_cast<const uint4*>(staging + swz_off(r, lane & 7));
+                if (there && col < cols)
+                  *reinterpret_cast<uint4*>(static_cast<OUT*>(p.out) + row_to * p.ld + c_base + col) = *reinterpret_cast<const uint4*>(staging + staging_off(at, lane & 3));
               }
               __syncwarp();
             }
@@ -925,7 +932,7 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
     if (v < kCeN) v = kCeN;
     return (int)(v < vocab ? v : vocab);
   };
-  q.piece_fwd = piece(w_row + q.copy_rows * kCeShares * (int64_t)sizeof(float2) / kCeN);
+  q.piece_fwd = piece(w_row + q.copy_rows * kCeShares<kLse> * (int64_t)sizeof(float2) / kCeN);
   q.piece_bwd = piece(w_row + q.planes * q.g_rows * 2);
   q.pieces = (int)((vocab + q.piece_bwd - 1) / q.piece_bwd);
   size_t at = 1024;   // behind the CeHead
@@ -935,9 +942,9 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
   const int64_t most = backward ? q.piece_bwd : q.piece_fwd;
   q.wcopy = take(q.copy_w ? (size_t)most * w_row : 0);
   if (!backward) {
-    // kCeShares for each tile of a row: of 256 columns, or fewer where all tiles run at once (ce_cut)
+    // so many for each tile of a row: of 256 columns, or fewer where all tiles run at once (ce_cut)
     const int64_t wide = (q.piece_fwd + kCeN - 1) / kCeN;
-    q.parts_per_piece = kCeShares * (int)(wide > kCeWorkers ? wide : kCeWorkers);
+    q.parts_per_piece = kCeShares<kLse> * (int)(wide > kCeWorkers ? wide : kCeWorkers);
     q.parts = take((size_t)q.parts_per_piece * q.copy_rows * sizeof(float2));
     q.running = take((size_t)n * sizeof(float2));
     q.logit = take((size_t)n * sizeof(float));
@@ -988,7 +995,7 @@ static CeCut ce_cut(CeMode mode, int64_t m, int64_t n, int64_t k) {
   if (mode == kDw ? m > kCeM && k > 512 : k >= 1024 ? pairs * 85 < single * 100 : pairs * 108 < single * 100) {
     if (!logits || pairs / 256 * ((n + 255) / 256) >= 37) return {2, 256};   // (half of the pairs have a tile)
   }
-  const int least = mode == kLse ? 32 * kCeShares : mode == kGrad ? 64 * kCeShares : 256;   // what a warp works on at a time
+  const int least = mode == kLse ? 32 * kCeShares<kLse> : mode == kGrad ? 32 * kCeShares<kGrad> : 256;   // 32 columns of each share
   int bn = 256;
   while (bn > least && single / 128 * ((2 * n + bn - 1) / bn) <= kCeWorkers) bn /= 2;
   return {1, bn};
@@ -1008,7 +1015,7 @@ static cudaError_t ce_launch_as(const CeProduct& p, int64_t tiles, const CUtenso
   attr[1].val.clusterDim.x = PAIR;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   c.gridDim = dim3((unsigned)(most < kCeWorkers ? most : kCeWorkers));
-  c.blockDim = dim3(kCeThreads);
+  c.blockDim = dim3(kCeThreads<MODE>);
   c.dynamicSmemBytes = kCeSmem;
   c.stream = st;
   c.attrs = attr;
@@ -1100,7 +1107,7 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
     CE_CUDA((ce_launch<T, OUT, kLse>(p, cut.pair, tiles_m * tiles_n, x, copy, w, c.st)), "castle_linear_ce_fwd launch");
     CeJoin j{};
     j.head = (CeHead*)c.work; j.rows = p.rows; j.parts = p.parts; j.running = (float2*)(c.work + q.running); j.target_logit = p.target_logit;
-    j.sums = (double*)(c.work + q.sums); j.lse = lse; j.loss = loss; j.parts_ld = q.copy_rows; j.parts_n = kCeShares * tiles_n;
+    j.sums = (double*)(c.work + q.sums); j.lse = lse; j.loss = loss; j.parts_ld = q.copy_rows; j.parts_n = kCeShares<kLse> * tiles_n;
     j.begin = v0 == 0; j.end = v0 + count == c.vocab; j.each = each; j.mean = c.reduction == CASTLE_REDUCE_MEAN;
     // few rows: a CTA or a warp each; many: neighbouring threads on neighbouring rows
     if (c.n < 256) CE_CUDA(launch_kernel(castle_ce_join_kernel<1>, dim3((unsigned)c.n), 256, 0, c.st, true, j), "castle_linear_ce_fwd launch");
