@@ -773,7 +773,7 @@ struct LayerBackward : public Node {
     if (need_weight) result[3] = at::empty({dim}, dh.options());
     if (layer_norm) {
       if (need_bias) result[4] = at::empty({dim}, dh.options());
-      launch_layernorm_bwd(as_rows(dh, rows, dim), xc.view({rows, dim}), wn, rs, result[0], result[3], has_bias ? result[4] : Tensor(), stream);
+      launch_layernorm_bwd(as_rows(dh, rows, dim), as_rows(xc, rows, dim), dtype, wn, rs, result[0], result[3], has_bias ? result[4] : Tensor(), stream);
       return result;
     }
     const size_t bytes = api.rmsnorm_bwd_workspace_bytes(rows, (int32_t)dim);
@@ -807,11 +807,11 @@ Tensor layer_native(const Tensor& x, const Layer& l, Options o) {
       h = at::empty({rows, dim}, x.options().requires_grad(false));
       if (l.layer_norm) {
         if (o.need_grad) rstd = at::empty({rows, 2}, x.options().dtype(at::kFloat).requires_grad(false));   // mean and 1 / deviation
-        launch_layernorm(src, l.norm, l.norm_bias, *l.eps, h, rstd, stream);
+        launch_layernorm(as_rows(src, rows, dim), p.dtype, l.norm, l.norm_bias, *l.eps, h, rstd, stream);
       } else {
-      if (o.need_grad) rstd = at::empty({rows}, x.options().dtype(at::kFloat).requires_grad(false));
-      check(api.rmsnorm_fwd(dtype_code(p.dtype), rows, (int32_t)dim, src.data_ptr(), l.norm.data_ptr(), norm_eps(l), h.data_ptr(),
-                            o.need_grad ? rstd.data_ptr<float>() : nullptr, stream.stream()), "castle_rmsnorm_fwd");
+        if (o.need_grad) rstd = at::empty({rows}, x.options().dtype(at::kFloat).requires_grad(false));
+        check(api.rmsnorm_fwd(dtype_code(p.dtype), rows, (int32_t)dim, src.data_ptr(), l.norm.data_ptr(), norm_eps(l), h.data_ptr(),
+                              o.need_grad ? rstd.data_ptr<float>() : nullptr, stream.stream()), "castle_rmsnorm_fwd");
       }
     }
     const Tensor packed = product(0, h, l.to_qkv, rows).view({B, N, 6, l.heads, l.dim_head});
@@ -974,7 +974,7 @@ Tensor token_layer_normed(const Tensor& x, const Layer& l, const Tensor* caches,
     at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(x.device());
     h = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
-    launch_layernorm(as_rows(x, x.size(0), x.size(2)), l.norm, l.norm_bias, *l.eps, h, Tensor(), c10::cuda::getCurrentCUDAStream(x.device().index()));
+    launch_layernorm(as_rows(x, x.size(0), x.size(2)), x.scalar_type(), l.norm, l.norm_bias, *l.eps, h, Tensor(), c10::cuda::getCurrentCUDAStream(x.device().index()));
   }
   return token_layer(h, rest, caches, t, scale, rotary);
 }

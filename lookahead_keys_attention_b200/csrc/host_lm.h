@@ -4,12 +4,23 @@
 // What the kernels take by address is checked here: device, type and shape; tensors whose last dimension is not contiguous, or
 // whose negation is still to be done, are copied first.  Nodes compute in the type of their inputs, under autocast too.
 
-// (..., dim) as rows that are `stride(0)` elements apart.
-Tensor as_rows(const Tensor& t, int64_t rows, int64_t dim) {
+// (..., dim) as rows that are `stride` elements apart.  A contiguous tensor is taken as it is: views made by the dispatcher cost as much as
+// a launch's half, and a token's norm or lookup is little more than its launch.
+struct Rows {
+  Tensor keep;
+  void* data;
+  int64_t count, dim, stride;
+};
+Rows as_rows(const Tensor& t, int64_t rows, int64_t dim) {
+  if (!t.is_neg() && t.is_contiguous()) return {t, t.data_ptr(), rows, dim, dim};
   Tensor r = t.resolve_neg().reshape({rows, dim});
-  return dim > 1 && r.stride(1) != 1 ? r.contiguous() : r;
+  if (dim > 1 && r.stride(1) != 1) r = r.contiguous();
+  void* data = r.data_ptr();
+  const int64_t stride = rows > 1 ? r.stride(0) : dim;
+  return {std::move(r), data, rows, dim, stride};
 }
-int64_t row_stride(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+Tensor as_plain(const Tensor& t) { return !t.defined() || (!t.is_neg() && t.is_contiguous()) ? t : t.resolve_neg().contiguous(); }
+Tensor as_long(const Tensor& t) { return t.scalar_type() == at::kLong && t.is_contiguous() ? t : t.to(at::kLong).contiguous(); }
 
 // A tensor of its own memory: no wrapper of a batched gradient, of a transform or of a class with a dispatch of its own.
 bool own_memory(const Tensor& t) {
@@ -29,7 +40,7 @@ void need_gradient(const Tensor& g, at::IntArrayRef sizes, at::ScalarType type, 
   if (g.sizes() != sizes || g.scalar_type() != type || g.device() != dev || !own_memory(g))
     throw std::runtime_error(std::string(who) + ": the gradient's shape, type or device is not the output's");
 }
-Tensor restored_rows(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev, int64_t rows, int64_t dim) {
+Rows restored_rows(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev, int64_t rows, int64_t dim) {
   return as_rows(restored(t, sizes, type, dev), rows, dim);
 }
 
@@ -61,11 +72,11 @@ struct EmbeddingBackward : public Node {
     need_gradient(grads[0], out_sizes, dtype, dev, "castle_embedding");
     const auto options = at::TensorOptions().dtype(dtype).device(dev);
     if (n == 0) return {at::zeros({vocab, dim}, options)};
-    const Tensor g = as_rows(grads[0], n, dim);
+    const Rows g = as_rows(grads[0], n, dim);
     const Tensor dw = at::empty({vocab, dim}, options), status = status_word(dev.index());
     StreamUse use(stream);
     const Tensor ws = use.scratch(api.embedding_bwd_workspace_bytes(n, vocab, (int32_t)dim));
-    check(api.embedding_bwd(dtype_code(dtype), (int32_t)t.element_size(), n, vocab, (int32_t)dim, t.data_ptr(), padding, g.data_ptr(), row_stride(g),
+    check(api.embedding_bwd(dtype_code(dtype), (int32_t)t.element_size(), n, vocab, (int32_t)dim, t.data_ptr(), padding, g.data, g.stride,
                             (float)scale, dw.data_ptr(), ws.data_ptr(), ws.numel(), status.data_ptr<int32_t>(), stream.stream()),
           "castle_embedding_bwd");
     return {dw};
@@ -90,9 +101,10 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64
     const c10::cuda::CUDAGuard guard(dev);
     y = at::empty(sizes, weight.options().requires_grad(false));
     if (n > 0) {
-      const Tensor t = tokens.contiguous(), w = as_rows(weight, vocab, dim), status = status_word(dev.index());
-      check(api.embedding_fwd(dtype_code(weight.scalar_type()), (int32_t)t.element_size(), n, vocab, (int32_t)dim, t.data_ptr(), w.data_ptr(),
-                              row_stride(w), (float)scale, y.data_ptr(), status.data_ptr<int32_t>(),
+      const Tensor t = tokens.contiguous(), status = status_word(dev.index());
+      const Rows w = as_rows(weight, vocab, dim);
+      check(api.embedding_fwd(dtype_code(weight.scalar_type()), (int32_t)t.element_size(), n, vocab, (int32_t)dim, t.data_ptr(), w.data,
+                              w.stride, (float)scale, y.data_ptr(), status.data_ptr<int32_t>(),
                               c10::cuda::getCurrentCUDAStream(dev.index()).stream()), "castle_embedding_fwd");
     }
   }
@@ -110,20 +122,19 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64
 
 // ------------------------------------------------------------------------------------------------ layer norm
 // Launches on rows; y, dx contiguous.  Weight, bias and the results may be undefined.
-void launch_layernorm(const Tensor& rows, const Tensor& weight, const Tensor& bias, double eps, const Tensor& y, const Tensor& stats,
+void launch_layernorm(const Rows& x, at::ScalarType type, const Tensor& weight, const Tensor& bias, double eps, const Tensor& y, const Tensor& stats,
                       const c10::cuda::CUDAStream& stream) {
-  check(api.layernorm_fwd(dtype_code(rows.scalar_type()), rows.size(0), (int32_t)rows.size(1), rows.data_ptr(), row_stride(rows),
-                          weight.defined() ? weight.data_ptr() : nullptr, bias.defined() ? bias.data_ptr() : nullptr, (float)eps, y.data_ptr(),
-                          stats.defined() ? stats.data_ptr<float>() : nullptr, stream.stream()), "castle_layernorm_fwd");
+  check(api.layernorm_fwd(dtype_code(type), x.count, (int32_t)x.dim, x.data, x.stride, weight.defined() ? weight.data_ptr() : nullptr,
+                          bias.defined() ? bias.data_ptr() : nullptr, (float)eps, y.data_ptr(), stats.defined() ? stats.data_ptr<float>() : nullptr,
+                          stream.stream()), "castle_layernorm_fwd");
 }
-void launch_layernorm_bwd(const Tensor& dy, const Tensor& rows, const Tensor& weight, const Tensor& stats, const Tensor& dx, const Tensor& dw,
+void launch_layernorm_bwd(const Rows& dy, const Rows& x, at::ScalarType type, const Tensor& weight, const Tensor& stats, const Tensor& dx, const Tensor& dw,
                           const Tensor& db, const c10::cuda::CUDAStream& stream) {
   StreamUse use(stream);
-  const Tensor ws = use.scratch(api.layernorm_bwd_workspace_bytes(rows.size(0), (int32_t)rows.size(1)));
+  const Tensor ws = use.scratch(api.layernorm_bwd_workspace_bytes(x.count, (int32_t)x.dim));
   auto address = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
-  check(api.layernorm_bwd(dtype_code(rows.scalar_type()), rows.size(0), (int32_t)rows.size(1), dy.data_ptr(), row_stride(dy), rows.data_ptr(),
-                          row_stride(rows), address(weight), stats.data_ptr<float>(), address(dx), address(dw), address(db), ws.data_ptr(),
-                          ws.numel(), stream.stream()), "castle_layernorm_bwd");
+  check(api.layernorm_bwd(dtype_code(type), x.count, (int32_t)x.dim, dy.data, dy.stride, x.data, x.stride, address(weight), stats.data_ptr<float>(),
+                          address(dx), address(dw), address(db), ws.data_ptr(), ws.numel(), stream.stream()), "castle_layernorm_bwd");
 }
 
 struct LayerNormBackward : public Node {   // of x, weight, bias
@@ -153,8 +164,8 @@ struct LayerNormBackward : public Node {   // of x, weight, bias
       if (task_should_compute_output(i)) result[i] = rows == 0 ? (i == 0 ? at::empty(sizes, options) : at::zeros({dim}, options))
                                                               : i == 0 ? at::empty(sizes, options) : at::empty({dim}, options);
     if (rows == 0 || !(result[0].defined() || result[1].defined() || result[2].defined())) return result;
-    const Tensor w = has_weight ? restored(ws, {dim}, dtype, dev).resolve_neg().contiguous() : Tensor();
-    launch_layernorm_bwd(as_rows(grads[0], rows, dim), restored_rows(xs, sizes, dtype, dev, rows, dim), w,
+    const Tensor w = has_weight ? as_plain(restored(ws, {dim}, dtype, dev)) : Tensor();
+    launch_layernorm_bwd(as_rows(grads[0], rows, dim), restored_rows(xs, sizes, dtype, dev, rows, dim), dtype, w,
                          restored_contiguous(ss, {rows, 2}, at::kFloat, dev), result[0], result[1], result[2], c10::cuda::getCurrentCUDAStream(dev.index()));
     return result;
   }
@@ -182,8 +193,8 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, dou
     const auto options = x.options().requires_grad(false);
     y = at::empty(x.sizes(), options.memory_format(at::MemoryFormat::Contiguous));
     if (grad) stats = at::empty({rows, 2}, options.dtype(at::kFloat));
-    auto plain = [](const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; };
-    if (rows > 0) launch_layernorm(as_rows(x, rows, dim), plain(weight), plain(bias), eps, y, stats, c10::cuda::getCurrentCUDAStream(dev.index()));
+    if (rows > 0)
+      launch_layernorm(as_rows(x, rows, dim), x.scalar_type(), as_plain(weight), as_plain(bias), eps, y, stats, c10::cuda::getCurrentCUDAStream(dev.index()));
   }
   if (!grad) return y;
   auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(), torch::autograd::deleteNode);
@@ -234,12 +245,12 @@ struct LinearCrossEntropyBackward : public Node {   // of x, weight
     }
     if (task_should_compute_output(0)) result[0] = at::empty(x_sizes, options);
     if (task_should_compute_output(1)) result[1] = at::empty({vocab, dim}, options);
-    const Tensor xr = restored_rows(xs, x_sizes, dtype, dev, rows, dim), w = restored_rows(ws, {vocab, dim}, dtype, dev, vocab, dim),
-                 t = restored(ts, target_sizes, target_type, dev).to(at::kLong).contiguous(), l = restored_contiguous(ls, {rows}, at::kFloat, dev),
-                 g = grads[0].resolve_neg().contiguous(), status = status_word(dev.index());
+    const Rows xr = restored_rows(xs, x_sizes, dtype, dev, rows, dim), w = restored_rows(ws, {vocab, dim}, dtype, dev, vocab, dim);
+    const Tensor t = as_long(restored(ts, target_sizes, target_type, dev)), l = restored_contiguous(ls, {rows}, at::kFloat, dev), g = as_plain(grads[0]),
+                 status = status_word(dev.index());
     StreamUse use(stream);
     const Tensor scratch = use.scratch(api.linear_ce_workspace_bytes(dtype_code(dtype), rows, (int32_t)dim, vocab, 1));
-    check(api.linear_ce_bwd(dtype_code(dtype), rows, (int32_t)dim, vocab, xr.data_ptr(), row_stride(xr), w.data_ptr(), row_stride(w), t.data_ptr<int64_t>(), ignore,
+    check(api.linear_ce_bwd(dtype_code(dtype), rows, (int32_t)dim, vocab, xr.data, xr.stride, w.data, w.stride, t.data_ptr<int64_t>(), ignore,
                             reduction, l.data_ptr<float>(), g.data_ptr<float>(), result[0].defined() ? result[0].data_ptr() : nullptr,
                             result[1].defined() ? result[1].data_ptr() : nullptr, scratch.data_ptr(), scratch.numel(), status.data_ptr<int32_t>(), stream.stream()),
           "castle_linear_ce_bwd");
@@ -270,10 +281,11 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
     else loss = each ? at::empty(targets.sizes(), options) : at::empty({}, options);
     lse = at::empty({rows}, options);
     if (rows > 0) {
-      const Tensor xr = as_rows(x, rows, dim), w = as_rows(weight, vocab, dim), t = targets.to(at::kLong).contiguous(), status = status_word(dev.index());
+      const Rows xr = as_rows(x, rows, dim), w = as_rows(weight, vocab, dim);
+      const Tensor t = as_long(targets), status = status_word(dev.index());
       StreamUse use(stream);
       const Tensor scratch = use.scratch(api.linear_ce_workspace_bytes(dtype_code(x.scalar_type()), rows, (int32_t)dim, vocab, 0));
-      check(api.linear_ce_fwd(dtype_code(x.scalar_type()), rows, (int32_t)dim, vocab, xr.data_ptr(), row_stride(xr), w.data_ptr(), row_stride(w),
+      check(api.linear_ce_fwd(dtype_code(x.scalar_type()), rows, (int32_t)dim, vocab, xr.data, xr.stride, w.data, w.stride,
                               t.data_ptr<int64_t>(), ignore, reduction, loss.data_ptr<float>(), lse.data_ptr<float>(), scratch.data_ptr(), scratch.numel(),
                               status.data_ptr<int32_t>(), stream.stream()), "castle_linear_ce_fwd");
     }

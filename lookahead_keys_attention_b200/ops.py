@@ -121,10 +121,6 @@ class _TracedCall(torch.autograd.Function):
         return (None, *(next(grads) if isinstance(t, torch.Tensor) and t.requires_grad else None for t in leaves))
 
 
-def _call(call, *inputs):
-    return _TracedCall.apply(call, *inputs) if torch._C._is_tracing() else call(*inputs)
-
-
 def castle_attention_packed(packed, scale, return_U_for_cache=False, cache_out=None):
     """Parallel CASTLE attention on the packed projection output (B, N, 6, H, d), order
     qu,ku,vu,qc,kc,vc (the layout `to_all_qkv` produces).  Returns out (B, H, N, d) [, U].
@@ -165,15 +161,18 @@ def castle_embedding(tokens, weight, scale: float = 1.0, padding_idx: int | None
         if not -vocab <= padding_idx < vocab:
             raise ValueError("castle_embedding: padding_idx out of range")
         padding_idx %= vocab
-    host, padding = _lib.host(), -1 if padding_idx is None else padding_idx
-    return _call(lambda t, w: host.embedding(t, w, scale, padding), tokens, weight)
+    padding = -1 if padding_idx is None else padding_idx
+    if torch._C._is_tracing():
+        return _TracedCall.apply(lambda t, w: _lib.host().embedding(t, w, scale, padding), tokens, weight)
+    return _lib.host().embedding(tokens, weight, scale, padding)
 
 
 def castle_layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """Layer norm over the last dimension of `x` (any size), with an optional weight and bias of its type: mean, variance and
     all sums in fp32, one rounding.  `Castle(..., prenorm="layer")` has it in front of the layer."""
-    host = _lib.host()
-    return _call(lambda *t: host.layer_norm(*t, eps), x, weight, bias)
+    if torch._C._is_tracing():
+        return _TracedCall.apply(lambda *t: _lib.host().layer_norm(*t, eps), x, weight, bias)
+    return _lib.host().layer_norm(x, weight, bias, eps)
 
 
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}   # CASTLE_REDUCE_* of the C ABI
@@ -188,5 +187,7 @@ def castle_linear_cross_entropy(x, weight, targets, ignore_index: int = -100, re
     pass, from logits formed again, and are the same from call to call.  A target outside the vocabulary gives NaN, and `check_status()` raises."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"castle_linear_cross_entropy: reduction {reduction!r} is not one of {', '.join(_REDUCTIONS)}")
-    host, code = _lib.host(), _REDUCTIONS[reduction]
-    return _call(lambda x, w, t: host.linear_cross_entropy(x, w, t, ignore_index, code), x, weight, targets)
+    code = _REDUCTIONS[reduction]
+    if torch._C._is_tracing():
+        return _TracedCall.apply(lambda x, w, t: _lib.host().linear_cross_entropy(x, w, t, ignore_index, code), x, weight, targets)
+    return _lib.host().linear_cross_entropy(x, weight, targets, ignore_index, code)
