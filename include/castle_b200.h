@@ -9,7 +9,7 @@
  * Return value: 0 = launched; < 0 = argument rejected (see castle_last_error());
  * > 0 = a cudaError_t raised by a launch or by tensor-map encoding.
  *
- * Device-side failures (a bounded wait that ran out) are reported through the
+ * Device-side failures (a bounded wait that ran out, an index outside a table) are reported through the
  * caller's `status` word: the kernels OR a non-zero code into it and return.
  *
  * Tensors are described by a base pointer and element strides over

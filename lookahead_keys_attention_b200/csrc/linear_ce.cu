@@ -16,8 +16,12 @@
 // The four products are one kernel: CTAs that stay, one per SM, in pairs (256 x 256 of the result, 64 of the contraction at a time) or, where
 // there is less to do, alone (128 x 256, 128 or 64), each with a warp that loads tiles by TMA, a warp that issues the tensor cores'
 // products, and eight or sixteen warps that work on a finished tile in one half of tensor memory while the next one is summed in the other.
-// Alone, an SM's shared memory brings in and reads 24 KB in the 128 cycles of a product of 16, more than it can (78 % of the tensor cores' cycles at
-// a contraction of 50021); a pair shares B's tile.  All sums, the logits and the statistics are fp32.
+// Alone, an SM's shared memory brings in and reads 24 KB in the 128 cycles of a product of 16, more than it can (78 % of the tensor cores' cycles
+// at a contraction of 50021); a pair shares B's tile (92 %).  All sums, the logits and the statistics are fp32.
+//
+// What bounds it: at 8192 x 4096 against 131072 forward and backward take 25.2 to 26.5 ms by the box for 35.2 TFLOP, 1330 to 1400 TFLOP/s: the
+// power limit (the library's product, back to back, 1406 of measured), at clocks of 1.3 to 1.5 GHz.  8.8 of the 35.2 are the logits formed again.  Few
+// rows: the weight is read three times and dW written, 8 x 4096 against 131072 851 us of kernels for 4.3 GB.
 //
 // dx and dW can have few tiles and long contractions.  As many tiles as go evenly to the workers are theirs whole; of the others the
 // contraction is cut into slices, whose sums go to scratch and are added, in order, by castle_ce_sum_kernel.
@@ -25,8 +29,8 @@
 // fp32 tensors: every value is the sum of three bf16 ones (8 bits each: 24), and a product is the six largest of the nine products
 // of such parts (what is left out is 2^-24 of it), the smallest first.  So the same kernels serve, with six times the steps.
 //
-// The tensor cores cut what they add to an accumulator, always towards zero, so a long sum is off by some 2^-24 per addition (197 rows
-// of 512, fp32: losses 3.3e-6 off, gradients of longer sums 1.7e-5, where fp32 arithmetic has 2e-7).  Where the result has 32 bits
+// What the tensor cores add to an accumulator loses more than rounding to nearest would, and the losses of a long sum add up (197 rows of 512,
+// fp32: losses 3.3e-6 off, gradients of longer sums 1.7e-5, where fp32 arithmetic has 2e-7).  Where the result has 32 bits
 // (the logits' statistics, and everything of fp32 tensors), accumulators are therefore emptied every `flush` steps into sums that
 // the working warps keep in registers.
 //
@@ -45,8 +49,8 @@ namespace castle {
 enum CeMode { kLse, kGrad, kDx, kDw };
 
 constexpr int kCeM = 128, kCeN = 256, kCeK = 64;
-// The warps that work on tiles.  Sixteen hide what each waits for better where results are written (131072 x 4096 of dW over 8 rows: TBD);
-// with eight a row's statistics have fewer parts.
+// The warps that work on tiles.  Sixteen hide what each waits for better where results are written (dW of 131072 x 4096 over 8 rows: 257 us,
+// with eight 319); with eight a row's statistics have fewer parts.
 template <CeMode MODE> constexpr int kCeWarps = MODE == kLse ? 8 : 16;
 template <CeMode MODE> constexpr int kCeShares = kCeWarps<MODE> / 4;      // of a tile's columns
 template <CeMode MODE> constexpr int kCeThreads = (kCeWarps<MODE> + 2) * 32;
@@ -982,17 +986,19 @@ static int ce_map(CUtensorMap* m, const void* p, int op, int64_t rows, int cols,
   return make_tmap_16bit(m, &t, op, 1, planes, (int)rows, cols, box_rows, what);
 }
 
-// How a result of m x n over a contraction of k (all terms of it) is cut.  Pairs of CTAs are some 15 % faster per row where the contraction is long and 8 %
-// slower where it is short (the second CTA waits for the first's products at a tile's start and end), and pad the rows to 256
-// instead of 128.  us, pairs / single: logits 197 x 4096 against 131072 213 / 228, 300 x 1024 against 50021 49 / 41, 600 x 1024 59 / 57, 2000 x 512
-// against 8000 20.6 / 18.6; dx of 600 x 1024 72 / 80, of 300 x 1024 55 / 51; dW, whose rows are the vocabulary, at 300 rows 53 / 44, at 600 63 / 67, at
-// 1000 32 / 36.  Narrower tiles (of single ones that do not share a contraction out) as long as all of them run at once: 130 x 512 against
-// 256 5.9 / 8.0 with 256 columns, but two rounds of half tiles are slower than one of whole ones (50 x 768 against 32000 in fp32 55 / 43).
+// How a result of m x n over a contraction of k (all terms of it) is cut.  Pairs of CTAs are faster per row where the contraction is long and
+// slower where it is short (the second CTA waits for the first's products at a tile's start and end), and pad the rows to 256 instead of
+// 128.  us, pairs / single: logits and their gradient of 4096 x 1024 against 50021 282, 289 / 296, 363; 197 x 4096 against 131072 214, 208 / 236, 240;
+// 300 x 1024 against 50021 48, 48 / 40, 40; 2000 x 512 against 8000 21, 26 / 19, 23.  dx of 4096 x 1024 312 / 340, of 600 x 1024 73 / 81, of 300 x 1024 56 / 51.
+// dW, whose rows are the vocabulary: over 300 tokens 48 / 44, 600 61 / 66, 1000 33 / 36.  Narrower tiles (of single ones with one product's
+// contraction each) as long as all of them run at once: logits of 130 x 512 against 256 6.0, with 256 columns 8.3; but two rounds of half
+// tiles are slower than one of whole ones (50 x 768 against 32000 in fp32 55 / 43).
 struct CeCut { int pair, bn; };
 static CeCut ce_cut(CeMode mode, int64_t m, int64_t n, int64_t k) {
   const int64_t single = (m + 127) / 128 * 128, pairs = (m + 255) / 256 * 256;
   const bool logits = mode == kLse || mode == kGrad;
-  if (mode == kDw ? m > kCeM && k > 512 : k >= 1024 ? pairs * 85 < single * 100 : pairs * 108 < single * 100) {
+  const int64_t cost = mode == kDx ? 80 : k >= 1024 ? 85 : 108;   // of a pair's row, in hundredths of a single CTA's
+  if (mode == kDw ? m > kCeM && k > 512 : pairs * cost < single * 100) {
     if (!logits || pairs / 256 * ((n + 255) / 256) >= 37) return {2, 256};   // (half of the pairs have a tile)
   }
   const int least = mode == kLse ? 32 * kCeShares<kLse> : mode == kGrad ? 32 * kCeShares<kGrad> : 256;   // 32 columns of each share
