@@ -21,7 +21,7 @@
 //
 // What bounds it: at 8192 x 4096 against 131072 forward and backward take 25.2 to 26.5 ms by the box for 35.2 TFLOP, 1330 to 1400 TFLOP/s: the
 // power limit (the library's product, back to back, 1406 of measured), at clocks of 1.3 to 1.5 GHz.  8.8 of the 35.2 are the logits formed again.  Few
-// rows: the weight is read three times and dW written, 8 x 4096 against 131072 851 us of kernels for 4.3 GB.
+// rows: the weight is read three times and dW written, 8 x 4096 against 131072 790 us of kernels for 4.3 GB.
 //
 // dx and dW can have few tiles and long contractions.  As many tiles as go evenly to the workers are theirs whole; of the others the
 // contraction is cut into slices, whose sums go to scratch and are added, in order, by castle_ce_sum_kernel.
@@ -71,7 +71,7 @@ struct CeTurn {
 };
 constexpr int64_t kCeScratch = (int64_t)1 << 30;   // bytes that a piece of the vocabulary may take
 // Steps between emptyings: of a 16-bit operand's logits (32 additions in the tensor cores), of fp32's parts (24).  With these the losses of
-// 197 x 512 in fp32 are 6.7e-8 of their norm off; not emptied 3.3e-6 and, of logits over 1024 in 16 bits, 8 % faster (166 us, 152).
+// 197 x 512 in fp32 are 6.7e-8 of their norm off (emptied every second step 3.0e-7, and 8 % faster); not emptied 3.3e-6 and, of logits over 1024 in 16 bits, 8 % faster (166 us, 152).
 constexpr int kCeFlush = 8, kCeFlushF32 = 1, kCeNoFlush = 1 << 30;
 constexpr float kCeUnit = 16384.f;                 // of G: below 2 units
 
@@ -291,6 +291,7 @@ struct CeProduct {
   const CeRow* rows;
   int m, n, k;           // of the result and the contraction; m (kDw: k) is the number of rows that take part instead
   int bn;                // columns of a tile
+  int a_rows, k_rows;    // rows that a load of A's tile brings (not kDw), and of the contraction that a step has (kDw): fewer where there are fewer
   int b_row0;            // where the piece begins in B's rows (kLse, kGrad: along n, kDx: along k)
   int vocab0;            // the piece's first column of z (kLse, kGrad)
   int terms, group;
@@ -491,6 +492,8 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
       const bool copy = head.gathered;
       const CUtensorMap* ma = MODE != kDx && MODE != kDw && copy ? &map_copy : &map_a;
       const CUtensorMap* mb = MODE == kDw && copy ? &map_copy : &map_b;
+      // what a step brings, of the pair
+      const uint32_t bytes = PAIR * ((A_MN ? 2 * p.k_rows : p.a_rows) * 128 + (MODE == kDw ? kCeN / PAIR / 64 * p.k_rows * 128 : p.bn / PAIR * kCeK * 2));
       bool sent = false;
       for (int i = 0; work.at(worker, i, m, n, k0, k1, slot) && !*abortp; ++i) {
         const int m0 = (m * PAIR + rank) * kCeM, n0 = n * p.bn + (PAIR == 2 ? rank * (columns(n) / 2) : 0);
@@ -499,7 +502,7 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
             const int s = ring.s, k = ks * kCeK, pa = kTermA[term], pb = kTermB[term];
             if (!mbar_wait_ok<true>(&bar_free[s], ring.phase ^ 1u, abortp)) { ks = k1; break; }
             uint8_t *a = smem + s * stage, *b = a + kCeA;
-            if (rank == 0) mbar_expect_tx(&bar_full[s], stage * PAIR);
+            if (rank == 0) mbar_expect_tx(&bar_full[s], bytes);
             sent = true;
             auto load = [&](void* dst, const CUtensorMap* map, int c0, int c1, int plane) {
               if constexpr (PAIR == 2) tma_load_4d_pair(dst, map, of_cta(&bar_full[s], 0), c0, c1, plane, 0);
@@ -546,6 +549,7 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
             const uint64_t da = A_MN ? desc_mnmajor(a, 8192) : desc_kmajor(a), db = B_MN ? desc_mnmajor(b, 8192) : desc_kmajor(b);
 #pragma unroll
             for (int q = 0; q < kCeK / 16; ++q) {
+              if (MODE == kDw && q * 16 >= p.k_rows) break;
               const uint64_t ao = da + (uint64_t)(((A_MN ? 2048 : 32) * q) >> 4), bo = db + (uint64_t)(((B_MN ? 2048 : 32) * q) >> 4);
               if constexpr (PAIR == 2) mma_ss_pair(d, ao, bo, idesc, j > 0 || q > 0);
               else mma_ss(d, ao, bo, idesc, j > 0 || q > 0);
@@ -913,6 +917,7 @@ __global__ void __launch_bounds__(256) castle_ce_join_kernel(const CeJoin p) {
 
 // ------------------------------------------------------------------------------------------------ host
 struct CePlan {
+  int a_rows, k_rows;         // of a load, see CeProduct
   int planes, terms, pitch, piece_fwd, piece_bwd, parts_per_piece, pieces;
   bool copy_x, copy_w;        // operands are laid out anew: fp32, or rows that TMA cannot read
   int64_t copy_rows, g_rows;
@@ -928,6 +933,10 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
   q.pitch = (int)up(dim, 8);
   q.copy_x = f32 || !x_ok;
   q.copy_w = f32 || !w_ok;
+  // A tile's rows behind the last one need not be loaded (their results go nowhere); of the contraction they have to be zero, 16 at a time.  Rows that
+  // TMA has to fill take it longer than rows that it reads (8 x 4096 against 131072: logits 241 -> 187 us, their gradient 243 -> 180, dW 257 -> 239).
+  q.a_rows = (int)(n < kCeM ? up(n, 8) : kCeM);
+  q.k_rows = (int)(n < kCeK ? up(n, 16) : kCeK);
   q.copy_rows = up(n, kCeK);
   q.g_rows = up(n, 2 * kCeM);
   const int64_t w_row = q.copy_w ? (int64_t)q.planes * q.pitch * 2 : 0;
@@ -946,8 +955,8 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
   const int64_t most = backward ? q.piece_bwd : q.piece_fwd;
   q.wcopy = take(q.copy_w ? (size_t)most * w_row : 0);
   if (!backward) {
-    // so many for each tile of a row: of 256 columns, or fewer where all tiles run at once (ce_cut)
-    const int64_t wide = (q.piece_fwd + kCeN - 1) / kCeN;
+    // so many for each tile of a row: of 256 columns, or 128 if the rows are one tile, or fewer where all tiles run at once (ce_cut)
+    const int64_t width = n <= kCeM ? 128 : kCeN, wide = (q.piece_fwd + width - 1) / width;
     q.parts_per_piece = kCeShares<kLse> * (int)(wide > kCeWorkers ? wide : kCeWorkers);
     q.parts = take((size_t)q.parts_per_piece * q.copy_rows * sizeof(float2));
     q.running = take((size_t)n * sizeof(float2));
@@ -992,7 +1001,8 @@ static int ce_map(CUtensorMap* m, const void* p, int op, int64_t rows, int cols,
 // 300 x 1024 against 50021 48, 48 / 40, 40; 2000 x 512 against 8000 21, 26 / 19, 23.  dx of 4096 x 1024 312 / 340, of 600 x 1024 73 / 81, of 300 x 1024 56 / 51.
 // dW, whose rows are the vocabulary: over 300 tokens 48 / 44, 600 61 / 66, 1000 33 / 36.  Narrower tiles (of single ones with one product's
 // contraction each) as long as all of them run at once: logits of 130 x 512 against 256 6.0, with 256 columns 8.3; but two rounds of half
-// tiles are slower than one of whole ones (50 x 768 against 32000 in fp32 55 / 43).
+// tiles are slower than one of whole ones (50 x 768 against 32000 in fp32 55 / 43).  With one tile of rows, half as wide ones also where their
+// rounds come out shorter (128 x 4096 against 131072, 7 of 128 columns for 4 of 256: logits 192 -> 189 us, their gradient 190 -> 184).
 struct CeCut { int pair, bn; };
 static CeCut ce_cut(CeMode mode, int64_t m, int64_t n, int64_t k) {
   const int64_t single = (m + 127) / 128 * 128, pairs = (m + 255) / 256 * 256;
@@ -1004,6 +1014,10 @@ static CeCut ce_cut(CeMode mode, int64_t m, int64_t n, int64_t k) {
   const int least = mode == kLse ? 32 * kCeShares<kLse> : mode == kGrad ? 32 * kCeShares<kGrad> : 256;   // 32 columns of each share
   int bn = 256;
   while (bn > least && single / 128 * ((2 * n + bn - 1) / bn) <= kCeWorkers) bn /= 2;
+  if (logits && m <= kCeM && bn == 256) {   // one tile of rows: the weight's bytes are the time
+    auto rounds = [&](int64_t width) { return ((n + width - 1) / width + kCeWorkers - 1) / kCeWorkers; };
+    if (rounds(128) * 133 < rounds(256) * 256) bn = 128;
+  }
   return {1, bn};
 }
 
@@ -1097,7 +1111,7 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
   const bool each = c.reduction == CASTLE_REDUCE_NONE;
   CE_CUDA(ce_rows<OUT>(c, q, nullptr, nullptr, nullptr, each ? loss : nullptr, lse), "castle_linear_ce_fwd launch");
   CUtensorMap x, copy, w;
-  CE_TRY(ce_x_maps(c, q, op, kCeM, &x, &copy));
+  CE_TRY(ce_x_maps(c, q, op, q.a_rows, &x, &copy));
   for (int64_t v0 = 0; v0 < c.vocab; v0 += q.piece_fwd) {
     const int64_t count = c.vocab - v0 < q.piece_fwd ? c.vocab - v0 : q.piece_fwd;
     const CeCut cut = ce_cut(kLse, c.n, count, (int64_t)q.pitch * q.terms);
@@ -1105,7 +1119,7 @@ static int ce_forward(const CeCall& c, const CePlan& q, float* loss, float* lse)
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), "castle_linear_ce_fwd launch");
     CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
     CeProduct p{};
-    p.head = (const CeHead*)c.work; p.rows = (const CeRow*)(c.work + q.rows); p.n = (int)count; p.k = q.pitch; p.bn = cut.bn; p.b_row0 = q.copy_w ? 0 : (int)v0;
+    p.head = (const CeHead*)c.work; p.rows = (const CeRow*)(c.work + q.rows); p.n = (int)count; p.k = q.pitch; p.bn = cut.bn; p.a_rows = q.a_rows; p.k_rows = kCeK; p.b_row0 = q.copy_w ? 0 : (int)v0;
     p.vocab0 = (int)v0; p.terms = q.terms; p.group = 32 / cut.pair;
     p.flush = q.terms > 1 ? kCeFlushF32 : kCeFlush;
     p.parts = (float2*)(c.work + q.parts); p.parts_ld = q.copy_rows; p.target_logit = (float*)(c.work + q.logit); p.status = c.status;
@@ -1130,11 +1144,11 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
   const int op = c.dtype == CASTLE_F16 ? CASTLE_F16 : CASTLE_BF16;
   CE_CUDA(ce_rows<OUT>(c, q, lse, dloss, dx, nullptr, nullptr), what);
   CUtensorMap x, copy, xk, copyk, w, wk, ga, gt;
-  CE_TRY(ce_x_maps(c, q, op, kCeM, &x, &copy));
-  CE_TRY(ce_x_maps(c, q, op, kCeK, &xk, &copyk));
+  CE_TRY(ce_x_maps(c, q, op, q.a_rows, &x, &copy));
+  CE_TRY(ce_x_maps(c, q, op, q.k_rows, &xk, &copyk));
   CeProduct base{};
   base.head = (const CeHead*)c.work; base.rows = (const CeRow*)(c.work + q.rows); base.terms = q.terms; base.flush = q.terms > 1 ? kCeFlushF32 : kCeNoFlush;
-  base.status = c.status; base.ld = c.dim; base.bn = kCeN; base.slab = (float4*)(c.work + q.slab);
+  base.status = c.status; base.ld = c.dim; base.bn = kCeN; base.a_rows = q.a_rows; base.k_rows = q.k_rows; base.slab = (float4*)(c.work + q.slab);
   base.lost = (float*)(c.work + q.lost);
   // What the workers share out: launched with the product whenever there could be something.
   auto product = [&](auto mode, const CeProduct& p, const CeCut& cut, int64_t m, const CUtensorMap& a, const CUtensorMap& acopy, const CUtensorMap& b) -> cudaError_t {
@@ -1160,8 +1174,8 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
     CE_CUDA(ce_weight<OUT>(c, q, v0, count), what);
     CE_TRY(ce_w_map(c, q, op, count, cut.bn / cut.pair, &w));
     CE_TRY(ce_w_map(c, q, op, count, kCeK, &wk));
-    CE_TRY(ce_map(&ga, gp, op, q.g_rows, (int)count, pitch, q.g_rows * pitch, q.planes, kCeM, "castle_linear_ce: logits' gradient"));
-    CE_TRY(ce_map(&gt, gp, op, q.g_rows, (int)count, pitch, q.g_rows * pitch, q.planes, kCeK, "castle_linear_ce: logits' gradient"));
+    CE_TRY(ce_map(&ga, gp, op, q.g_rows, (int)count, pitch, q.g_rows * pitch, q.planes, q.a_rows, "castle_linear_ce: logits' gradient"));
+    CE_TRY(ce_map(&gt, gp, op, q.g_rows, (int)count, pitch, q.g_rows * pitch, q.planes, q.k_rows, "castle_linear_ce: logits' gradient"));
     CeProduct p = base;
     p.n = (int)count; p.k = q.pitch; p.bn = cut.bn; p.b_row0 = q.copy_w ? 0 : (int)v0; p.vocab0 = (int)v0; p.group = 32 / cut.pair;
     p.g = gp; p.g_ld = pitch; p.g_plane = q.g_rows * pitch;
