@@ -177,7 +177,7 @@ int castle_embedding_bwd(int32_t dtype, int32_t index_bytes, int64_t tokens, int
  * loss_i = log sum_v exp(x_i . w_v) - x_i . w_target, without the logits in memory.  x: `rows` rows of `dim` elements, x_stride
  * apart; weight: `vocab` rows, w_stride apart; targets: 64-bit; all sums in fp32.  Rows whose target is ignore_index take no part,
  * whatever x holds there; a target outside the vocabulary gives NaN and sets CASTLE_STATUS_BAD_INDEX.  `loss` (fp32): the mean over
- * the other rows (NaN if there are none), their sum, or with CASTLE_REDUCE_NONE each row's (0 where ignored); `lse` (fp32, rows):
+ * the other rows (NaN if there are none; its gradients are zero), their sum, or with CASTLE_REDUCE_NONE each row's (0 where ignored); `lse` (fp32, rows):
  * each row's log-sum-exp, for the backward.  Backward: `dloss` = the upstream gradient (one value, or one per row); dx (rows x dim,
  * contiguous, 0 where ignored) and dweight (vocab x dim, contiguous), each NULL if not wanted.  Logits are formed again there, in
  * pieces of the vocabulary that take about 1 GiB of the workspace; all results are the same from call to call.

@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(1024, 1) castle_ce_rows_kernel(const CeRowsPar
     h.gathered = gather || p.copy_always;
     h.bad = (int)(p.n - ignored) - all;
     h.done = 0;
-    h.unit = (p.each ? unit : g_one) * (1.f / kCeUnit);
+    h.unit = all > 0 ? (p.each ? unit : g_one) * (1.f / kCeUnit) : 0.f;   // (the mean over no rows is not a number, its gradients are zero)
     *p.head = h;
     if (h.bad) atomicOr(p.status, CASTLE_STATUS_BAD_INDEX);
   }

@@ -183,7 +183,7 @@ def castle_linear_cross_entropy(x, weight, targets, ignore_index: int = -100, re
     language model around these layers (the reference's training script, train_triton.py:73-175).  x (..., dim) and weight
     (vocabulary, dim) of one type, targets (...) int64 or int32; the loss is fp32, logits and sums are, too.  Rows whose target is
     `ignore_index` take no part, whatever x holds there, and cost nothing; `reduction`: the mean of the others (NaN if there are
-    none), their "sum", or "none" for each row's loss (0 where ignored).  The gradients of x and weight are formed in the backward
+    none, with gradients of zero), their "sum", or "none" for each row's loss (0 where ignored).  The gradients of x and weight are formed in the backward
     pass, from logits formed again, and are the same from call to call.  A target outside the vocabulary gives NaN, and `check_status()` raises."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"castle_linear_cross_entropy: reduction {reduction!r} is not one of {', '.join(_REDUCTIONS)}")
