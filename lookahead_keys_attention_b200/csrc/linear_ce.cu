@@ -285,7 +285,8 @@ __global__ void __launch_bounds__(256) castle_ce_split_kernel(const T* __restric
 // ------------------------------------------------------------------------------------------------ the products
 constexpr int kCeWorkers = 148;   // CTAs of a launch
 constexpr int kCeShare = 24;   // steps from which on it can pay to share tiles out
-constexpr int kCeParts = 4 * kCeWorkers;   // tiles of one CTA that the slab holds
+constexpr int kCeParts = 4 * kCeWorkers;   // tiles of one CTA that the slab holds at most
+constexpr int kCeSlices = 37;     // most slices of a contraction
 struct CeProduct {
   const CeHead* head;
   const CeRow* rows;
@@ -338,7 +339,7 @@ template <CeMode MODE, int PAIR> struct CeWork {
       float best = (float)steps;
 #pragma unroll
       for (int k = 0; k < 11; ++k) {
-        const int s = k < 5 ? k + 2 : k == 5 ? 8 : k == 6 ? 12 : k == 7 ? 16 : k == 8 ? 24 : k == 9 ? 32 : 37;
+        const int s = k < 5 ? k + 2 : k == 5 ? 8 : k == 6 ? 12 : k == 7 ? 16 : k == 8 ? 24 : k == 9 ? 32 : kCeSlices;
         if (rest == 0 || s > steps || rest * s * PAIR > kCeParts) continue;
         const float time = (float)((rest * s + workers - 1) / workers) * (float)((steps + s - 1) / s) + 24.f + 0.18f * PAIR * (float)(rest * s);
         if (time < best) { best = time; slices = s; }
@@ -539,7 +540,8 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
         for (; k0 < k1 && !*abortp; k0 += p.flush, ++turn) {
           const int acc = turn & 1, steps = min(p.flush, k1 - k0) * p.terms;
           const uint32_t d = tmem + acc * kCeN;
-          if (!mbar_wait_ok<true>(&bar_read[acc], ((uint32_t)(turn >> 1) & 1u) ^ 1u, abortp)) break;
+          const uint32_t phase = ((uint32_t)(turn >> 1) & 1u) ^ 1u;
+          if (!(PAIR == 2 ? mbar_wait_ok_cluster(&bar_read[acc], phase, abortp) : mbar_wait_ok<true>(&bar_read[acc], phase, abortp))) break;
           tc_fence_after();
           for (int j = 0; j < steps; ++j, ring.next()) {
             const int s = ring.s;
@@ -916,6 +918,32 @@ __global__ void __launch_bounds__(256) castle_ce_join_kernel(const CeJoin p) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
+// How a result of m x n over a contraction of k (all terms of it) is cut.  Pairs of CTAs are faster per row where the contraction is long and
+// slower where it is short (the second CTA waits for the first's products at a tile's start and end), and pad the rows to 256 instead of
+// 128.  us, pairs / single: logits and their gradient of 4096 x 1024 against 50021 282, 289 / 296, 363; 197 x 4096 against 131072 214, 208 / 236, 240;
+// 300 x 1024 against 50021 48, 48 / 40, 40; 2000 x 512 against 8000 21, 26 / 19, 23.  dx of 4096 x 1024 312 / 340, of 600 x 1024 73 / 81, of 300 x 1024 56 / 51.
+// dW, whose rows are the vocabulary: over 300 tokens 48 / 44, 600 61 / 66, 1000 33 / 36.  Narrower tiles (of single ones with one product's
+// contraction each) as long as all of them run at once: logits of 130 x 512 against 256 6.0, with 256 columns 8.3; but two rounds of half
+// tiles are slower than one of whole ones (50 x 768 against 32000 in fp32 55 / 43).  With one tile of rows, half as wide ones also where their
+// rounds come out shorter (128 x 4096 against 131072, 7 of 128 columns for 4 of 256: logits 192 -> 189 us, their gradient 190 -> 184).
+struct CeCut { int pair, bn; };
+static CeCut ce_cut(CeMode mode, int64_t m, int64_t n, int64_t k) {
+  const int64_t single = (m + 127) / 128 * 128, pairs = (m + 255) / 256 * 256;
+  const bool logits = mode == kLse || mode == kGrad;
+  const int64_t cost = mode == kDx ? 80 : k >= 1024 ? 85 : 108;   // of a pair's row, in hundredths of a single CTA's
+  if (mode == kDw ? m > kCeM && k > 512 : pairs * cost < single * 100) {
+    if (!logits || pairs / 256 * ((n + 255) / 256) >= 37) return {2, 256};   // (half of the pairs have a tile)
+  }
+  const int least = mode == kLse ? 32 * kCeShares<kLse> : mode == kGrad ? 32 * kCeShares<kGrad> : 256;   // 32 columns of each share
+  int bn = 256;
+  while (bn > least && single / 128 * ((2 * n + bn - 1) / bn) <= kCeWorkers) bn /= 2;
+  if (logits && m <= kCeM && bn == 256) {   // one tile of rows: the weight's bytes are the time
+    auto rounds = [&](int64_t width) { return ((n + width - 1) / width + kCeWorkers - 1) / kCeWorkers; };
+    if (rounds(128) * 133 < rounds(256) * 256) bn = 128;
+  }
+  return {1, bn};
+}
+
 struct CePlan {
   int a_rows, k_rows;         // of a load, see CeProduct
   int planes, terms, pitch, piece_fwd, piece_bwd, parts_per_piece, pieces;
@@ -957,7 +985,8 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
   if (!backward) {
     // so many for each tile of a row: of 256 columns, or 128 if the rows are one tile, or fewer where all tiles run at once (ce_cut)
     const int64_t width = n <= kCeM ? 128 : kCeN, wide = (q.piece_fwd + width - 1) / width;
-    q.parts_per_piece = kCeShares<kLse> * (int)(wide > kCeWorkers ? wide : kCeWorkers);
+    const int64_t few = kCeWorkers / ((n + kCeM - 1) / kCeM);
+    q.parts_per_piece = kCeShares<kLse> * (int)(wide > few ? wide : few);
     q.parts = take((size_t)q.parts_per_piece * q.copy_rows * sizeof(float2));
     q.running = take((size_t)n * sizeof(float2));
     q.logit = take((size_t)n * sizeof(float));
@@ -965,7 +994,14 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
   } else {
     q.g = take((size_t)q.planes * q.g_rows * up(q.piece_bwd, 8) * 2);
     q.lost = take((size_t)n * sizeof(float));
-    q.slab = take((size_t)kCeParts * kCeM * kCeN * sizeof(float));
+    // the slab: as many parts as CeWork can choose
+    auto parts = [&](const CeCut& cut, int64_t m, int64_t k) {
+      const int64_t tiles = (m + kCeM * cut.pair - 1) / (kCeM * cut.pair) * ((dim + kCeN - 1) / kCeN), most = tiles * kCeSlices * cut.pair;
+      return k < kCeShare * kCeK - kCeK + 1 ? 0 : most < kCeParts ? most : kCeParts;
+    };
+    const int64_t for_dx = parts(ce_cut(kDx, n, dim, (int64_t)q.piece_bwd * q.terms), n, q.piece_bwd);
+    const int64_t for_dw = parts(ce_cut(kDw, q.piece_bwd, dim, n * q.terms), q.piece_bwd, n);
+    q.slab = take((size_t)(for_dx > for_dw ? for_dx : for_dw) * kCeM * kCeN * sizeof(float));
     q.acc = take(q.pieces > 1 ? (size_t)n * up(dim, 8) * sizeof(float) : 0);
   }
   q.bytes = at;
@@ -993,32 +1029,6 @@ static bool ce_tma_rows(int dtype, int64_t rows, int dim, const void* p, int64_t
 static int ce_map(CUtensorMap* m, const void* p, int op, int64_t rows, int cols, int64_t pitch, int64_t plane, int planes, int box_rows, const char* what) {
   const castle_tensor_t t{const_cast<void*>(p), 0, plane, pitch};
   return make_tmap_16bit(m, &t, op, 1, planes, (int)rows, cols, box_rows, what);
-}
-
-// How a result of m x n over a contraction of k (all terms of it) is cut.  Pairs of CTAs are faster per row where the contraction is long and
-// slower where it is short (the second CTA waits for the first's products at a tile's start and end), and pad the rows to 256 instead of
-// 128.  us, pairs / single: logits and their gradient of 4096 x 1024 against 50021 282, 289 / 296, 363; 197 x 4096 against 131072 214, 208 / 236, 240;
-// 300 x 1024 against 50021 48, 48 / 40, 40; 2000 x 512 against 8000 21, 26 / 19, 23.  dx of 4096 x 1024 312 / 340, of 600 x 1024 73 / 81, of 300 x 1024 56 / 51.
-// dW, whose rows are the vocabulary: over 300 tokens 48 / 44, 600 61 / 66, 1000 33 / 36.  Narrower tiles (of single ones with one product's
-// contraction each) as long as all of them run at once: logits of 130 x 512 against 256 6.0, with 256 columns 8.3; but two rounds of half
-// tiles are slower than one of whole ones (50 x 768 against 32000 in fp32 55 / 43).  With one tile of rows, half as wide ones also where their
-// rounds come out shorter (128 x 4096 against 131072, 7 of 128 columns for 4 of 256: logits 192 -> 189 us, their gradient 190 -> 184).
-struct CeCut { int pair, bn; };
-static CeCut ce_cut(CeMode mode, int64_t m, int64_t n, int64_t k) {
-  const int64_t single = (m + 127) / 128 * 128, pairs = (m + 255) / 256 * 256;
-  const bool logits = mode == kLse || mode == kGrad;
-  const int64_t cost = mode == kDx ? 80 : k >= 1024 ? 85 : 108;   // of a pair's row, in hundredths of a single CTA's
-  if (mode == kDw ? m > kCeM && k > 512 : pairs * cost < single * 100) {
-    if (!logits || pairs / 256 * ((n + 255) / 256) >= 37) return {2, 256};   // (half of the pairs have a tile)
-  }
-  const int least = mode == kLse ? 32 * kCeShares<kLse> : mode == kGrad ? 32 * kCeShares<kGrad> : 256;   // 32 columns of each share
-  int bn = 256;
-  while (bn > least && single / 128 * ((2 * n + bn - 1) / bn) <= kCeWorkers) bn /= 2;
-  if (logits && m <= kCeM && bn == 256) {   // one tile of rows: the weight's bytes are the time
-    auto rounds = [&](int64_t width) { return ((n + width - 1) / width + kCeWorkers - 1) / kCeWorkers; };
-    if (rounds(128) * 133 < rounds(256) * 256) bn = 128;
-  }
-  return {1, bn};
 }
 
 template <typename T, typename OUT, CeMode MODE, bool REG, int PAIR>

@@ -279,6 +279,23 @@ __device__ __forceinline__ uint32_t of_cta(const void* p, uint32_t rank) {   // 
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {   // of another CTA's barrier, see of_cta
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// A wait for arrivals of either CTA (see mbar_wait_ok).
+__device__ __forceinline__ bool mbar_wait_ok_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 0; i < kWaitPollLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((i & 63u) == 63u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
 // A tile for this CTA whose arrival is counted at a barrier of the pair's.
 __device__ __forceinline__ void tma_load_4d_pair(void* dst, const void* tmap, uint32_t bar, int c0, int c1, int c2, int c3) {
   asm volatile(
