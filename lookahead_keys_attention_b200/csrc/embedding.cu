@@ -29,6 +29,7 @@ constexpr int kEmbThreads = 256, kBinThreads = 512, kBinWarps = kBinThreads / 32
 constexpr int kSlices = 128, kWarpSlices = kSlices / kSortWarps;
 constexpr int kSortRows = 1536;    // most rows of an owner: 32 counters of 4 bytes each
 constexpr int kMaxOwners = 2048;   // 16 counters each
+constexpr int64_t kMostTokens = 1 << 30, kMostRows = (int64_t)kSortRows * kMaxOwners;   // places in the list, and a chunk behind the last, are 32 bits
 
 template <typename I> __device__ __forceinline__ int64_t token_at(const void* t, int64_t i) { return (int64_t)static_cast<const I*>(t)[i]; }
 
@@ -435,7 +436,7 @@ static int emb_check(const char* who, int32_t dtype, int32_t index_bytes, int64_
                      const int32_t* status) {
   if (dtype < CASTLE_BF16 || dtype > CASTLE_F32) return reject("%s: unknown dtype", who);
   if (index_bytes != 4 && index_bytes != 8) return reject("%s: tokens must be 32- or 64-bit integers", who);
-  if (tokens <= 0 || tokens > 2147483647 || vocab <= 0 || vocab > kSortRows * kMaxOwners || dim <= 0 || dim > (1 << 24))
+  if (tokens <= 0 || tokens > kMostTokens || vocab <= 0 || vocab > kMostRows || dim <= 0 || dim > (1 << 24))
     return reject("%s: %lld tokens, vocabulary %lld, dim %d not supported", who, (long long)tokens, (long long)vocab, dim);
   if (!index || (uintptr_t)index % index_bytes || !status) return reject("%s: tokens (aligned to their size) and a status word are needed", who);
   if (stride < 0) return reject("%s: negative strides are not supported", who);
@@ -478,7 +479,7 @@ extern "C" int castle_embedding_fwd(int32_t dtype, int32_t index_bytes, int64_t 
 }
 
 extern "C" size_t castle_embedding_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int32_t dim) {
-  return tokens <= 0 || vocab <= 0 || dim <= 0 ? 0 : emb_scratch(tokens, vocab, dim).bytes;
+  return tokens <= 0 || tokens > kMostTokens || vocab <= 0 || vocab > kMostRows || dim <= 0 ? 0 : emb_scratch(tokens, vocab, dim).bytes;
 }
 
 extern "C" int castle_embedding_bwd(int32_t dtype, int32_t index_bytes, int64_t tokens, int64_t vocab, int32_t dim, const void* index, int64_t padding_idx,

@@ -36,6 +36,9 @@ void need_plain(const Tensor& t, const char* who) {
 void need_type(const Tensor& t, const char* who) {
   if (dtype_code(t.scalar_type()) < 0) throw std::runtime_error(std::string(who) + ": bf16, fp16 or fp32 expected");
 }
+void need_dim(int64_t dim, const char* who) {   // the C ABI takes a row's length as 32 bits
+  if (dim > std::numeric_limits<int32_t>::max()) throw std::runtime_error(std::string(who) + ": rows of " + std::to_string(dim) + " elements are not supported");
+}
 void need_gradient(const Tensor& g, at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev, const char* who) {
   if (g.sizes() != sizes || g.scalar_type() != type || g.device() != dev || !own_memory(g))
     throw std::runtime_error(std::string(who) + ": the gradient's shape, type or device is not the output's");
@@ -92,6 +95,7 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, int64
   need(weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) > 0, "castle_embedding: a (vocabulary, dim) weight expected");
   need(weight.device() == tokens.device(), "castle_embedding: tokens and weight must be on one device");
   const int64_t n = tokens.numel(), vocab = weight.size(0), dim = weight.size(1);
+  need_dim(dim, who);
   std::vector<int64_t> sizes = tokens.sizes().vec();
   sizes.push_back(dim);
   Tensor y;
@@ -177,6 +181,7 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, dou
   need_type(x, who);
   need(x.dim() >= 1 && x.size(-1) > 0, "castle_layer_norm: (..., dim) rows expected");
   const int64_t dim = x.size(-1), rows = x.numel() / dim;
+  need_dim(dim, who);
   for (const Tensor* t : {&weight, &bias}) {
     if (!t->defined()) continue;
     need_plain(*t, who);
@@ -269,6 +274,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
   need(targets.scalar_type() == at::kLong || targets.scalar_type() == at::kInt, "castle_linear_cross_entropy: targets must be int64 or int32");
   need(targets.sizes() == x.sizes().slice(0, x.dim() - 1), "castle_linear_cross_entropy: a target for each row of the input expected");
   const int64_t dim = x.size(-1), rows = targets.numel(), vocab = weight.size(0);
+  need_dim(dim, who);
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()), each = reduction == CASTLE_REDUCE_NONE;
   Tensor loss, lse;
   {

@@ -328,6 +328,15 @@ def test_offsets_beyond_32_bits():
     release_workspaces()
 
 
+def test_rows_longer_than_32_bits_are_refused():
+    dim = 2 ** 32 + 8          # (8 in 32 bits; nothing of this size is laid out)
+    x = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16).expand(4, dim)
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for call in (lambda: castle_embedding(t, x), lambda: castle_layer_norm(x), lambda: castle_linear_cross_entropy(x, x, t)):
+        with pytest.raises(RuntimeError, match="4294967304 elements are not supported"):
+            call()
+
+
 def test_another_device_than_the_current_one():
     if torch.cuda.device_count() < 2:
         pytest.skip("needs two GPUs")

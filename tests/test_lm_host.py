@@ -39,6 +39,18 @@ def test_embedding_arguments():
         assert bwd(**bad) < 0 and "castle_embedding_bwd" in L.last_error(), bad
 
 
+def test_embedding_limits():
+    """Places in the sorted list are 32 bits: 2^30 tokens at most, and no scratch is named for what would be refused."""
+    L, lib = _lib()
+    size = lib.castle_embedding_bwd_workspace_bytes
+    assert size(2 ** 30, 1536 * 2048, 1) > 2 ** 32
+    assert size(2 ** 30 + 1, 10, 1) == size(2 ** 31 - 1, 10, 1) == size(4, 1536 * 2048 + 1, 1) == size(4, 2 ** 62, 1) == 0
+    for n in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert lib.castle_embedding_fwd(L.BF16, 8, n, 10, 1, 32, 32, 1, 1.0, 32, 32, None) < 0
+        assert lib.castle_embedding_bwd(L.BF16, 8, n, 10, 1, 32, -1, 32, 1, 1.0, 32, 32, 2 ** 40, 32, None) < 0
+        assert "castle_embedding_bwd" in L.last_error()
+
+
 def test_cpu_tensors_are_refused():
     from lookahead_keys_attention_b200 import castle_embedding, castle_layer_norm
     with pytest.raises(RuntimeError, match="no CPU path"):
