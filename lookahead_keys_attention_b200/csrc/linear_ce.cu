@@ -144,6 +144,43 @@ __device__ __forceinline__ void copy_row(const T* src, uint16_t* dst, int64_t pl
     }
     return;
   }
+  if constexpr (sizeof(T) == 2) {
+    // A row at an odd place: 16-byte blocks of memory, of which each eight columns have parts of two (24989 rows of 5859
+    // 101 us, 5.8 TB/s read and written; by single elements 186).
+    const int lead = (int)(reinterpret_cast<uintptr_t>(src) % 16 / 2);   // columns of the first block that are not the row's
+    auto block = [&](int c) {                                            // columns [c, c + 8), a block of memory; those that are not there are zero
+      uint32_t w[4];
+      if (c >= 0 && c + 8 <= dim) {
+        const uint4 q = *reinterpret_cast<const uint4*>(src + c);
+        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+      } else {
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int k = c + 2 * j;
+          w[j] = (k >= 0 && k < dim ? from[k] : 0u) | (uint32_t)(k + 1 >= 0 && k + 1 < dim ? from[k + 1] : 0u) << 16;
+        }
+      }
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    auto shifted = [&](int c, const uint4& a, const uint4& b) {
+      uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 6; ++j) w[j] = lead & 4 ? w[j + 2] : w[j];
+#pragma unroll
+      for (int j = 0; j < 5; ++j) w[j] = lead & 2 ? w[j + 1] : w[j];
+      const int bits = lead % 2 * 16;
+      *reinterpret_cast<uint4*>(dst + c) = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                                                      __funnelshift_r(w[3], w[4], bits));
+    };
+    const int whole = dim + lead - 16;   // the last column whose two blocks are all the row's
+#pragma unroll 4
+    for (int c = 8 + lane * 8; c <= whole; c += 256)
+      shifted(c, *reinterpret_cast<const uint4*>(src + c - lead), *reinterpret_cast<const uint4*>(src + c - lead + 8));
+    const int end = lane == 0 ? 0 : max(8, whole / 8 * 8 + 8) + (lane - 1) * 8;   // the first, and three at most behind those
+    if (lane < 4 && end < pitch) shifted(end, block(end - lead), block(end - lead + 8));
+    return;
+  }
 #pragma unroll 4
   for (int c = lane * 2; c < pitch; c += 64) {
     float a[P], b[P];
@@ -413,36 +450,18 @@ template <typename OUT, int COUNT> __device__ __forceinline__ void ce_add_lost(c
   }
 }
 
-// Four or more values of a row of dx or dW go out: to the sums over the pieces of the vocabulary, or scaled to the result (`to`: its row).
-template <typename OUT, int COUNT>
-__device__ __forceinline__ void ce_emit(const CeProduct& p, float unit, int64_t row, int64_t to, int col, int have, float* v) {
-  if (p.acc) {
-    float* acc = p.acc + row * p.acc_ld + col;
+// Several pieces of the vocabulary: the sums of a row of dx so far are added, and kept unless this piece is the last.
+template <int COUNT> __device__ __forceinline__ void ce_accumulate(const CeProduct& p, int64_t row, int col, int have, float* v) {
+  float* acc = p.acc + row * p.acc_ld + col;
 #pragma unroll
-    for (int j = 0; j < COUNT; j += 4)
-      if (j < have) {   // (acc_ld is a multiple of 8)
-        if (p.acc_add) {
-          const float4 old = *reinterpret_cast<const float4*>(acc + j);
-          v[j] += old.x; v[j + 1] += old.y; v[j + 2] += old.z; v[j + 3] += old.w;
-        }
-        if (!p.acc_out) *reinterpret_cast<float4*>(acc + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  for (int j = 0; j < COUNT; j += 4)
+    if (j < have) {   // (acc_ld is a multiple of 8)
+      if (p.acc_add) {
+        const float4 old = *reinterpret_cast<const float4*>(acc + j);
+        v[j] += old.x; v[j + 1] += old.y; v[j + 2] += old.z; v[j + 3] += old.w;
       }
-    if (!p.acc_out) return;
-  }
-#pragma unroll
-  for (int j = 0; j < COUNT; ++j) v[j] *= unit;
-  OUT* out = static_cast<OUT*>(p.out) + to * p.ld + col;
-  if constexpr (COUNT % 8 == 0) {
-    if (p.vec) {
-#pragma unroll
-      for (int j = 0; j < COUNT; j += 8)
-        if (j < have) store8<OUT>(out + j, v + j);
-      return;
+      if (!p.acc_out) *reinterpret_cast<float4*>(acc + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
     }
-  }
-#pragma unroll
-  for (int j = 0; j < COUNT; ++j)
-    if (j < have) store1<OUT>(out + j, v[j]);
 }
 
 // T: the operands' type, OUT: the result's (kDx, kDw) or the caller's (kGrad: float means three planes of G).  REG: accumulators are emptied into
@@ -584,7 +603,7 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
       const int local = rank * kCeM + quarter * 32 + lane, row = m * PAIR * kCeM + local, c_base = n * p.bn + share * width;
       const int cols = min(width, p.n - c_base);   // that there are; of the others up to the next grain are computed
       const bool empty = k1 <= k0;
-      const bool on = row < (MODE == kDw ? p.m : head.rows), direct = slot < 0 && !p.acc && p.vec;
+      const bool on = row < (MODE == kDw ? p.m : head.rows), direct = slot < 0 && (!p.acc || p.acc_out);
       CeOut<OUT> dst{0, nullptr, 0.f};
       if constexpr (MODE == kDx || MODE == kDw) dst = ce_out<MODE, OUT>(p, row, on);
       float sums[REG ? WIDTH : 1];
@@ -747,12 +766,18 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
             float4* out = p.slab + ((int64_t)slot * (kCeN / 4) + (share * width + c0) / 4) * (kCeM * PAIR) + local;
 #pragma unroll
             for (int j = 0; j < 32; j += 4) out[(j / 4) * (kCeM * PAIR)] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-          } else if (direct) {
-            // through shared memory, so that four lanes store 64 bytes of a row
-            if constexpr (MODE == kDx) ce_add_lost<OUT, 32>(p, dst, c_base + c0, min(32, cols - c0), v);
+          } else {
+            if constexpr (MODE == kDx) {
+              ce_add_lost<OUT, 32>(p, dst, c_base + c0, min(32, cols - c0), v);
+              if (p.acc && on) ce_accumulate<32>(p, row, c_base + c0, min(32, cols - c0), v);
+            }
+            if (!direct) continue;
+            // Through shared memory, so that four lanes store 64 bytes of a row, or half a warp its words where rows are not
+            // at 16-byte boundaries (dW of 24989 x 5859 over 23 rows 168 us; by single elements of 32 rows at a time 1416, and with rows of 5856 63).
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= unit;
             constexpr int PIECE = 16 / (int)sizeof(OUT), PANEL = 4 * PIECE;   // columns of 16 bytes, and of 64
+            OUT* out = static_cast<OUT*>(p.out) + c_base;
 #pragma unroll
             for (int h = 0; h < 32; h += PANEL) {
 #pragma unroll
@@ -762,28 +787,61 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
                 else store8<OUT>(reinterpret_cast<OUT*>(staging + staging_off(lane, c)), f);
               }
               __syncwarp();
-              const int col = c0 + h + (lane & 3) * PIECE;
+              if (p.vec) {
+                const int col = c0 + h + (lane & 3) * PIECE;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int at = j * 8 + (lane >> 2);
-                int64_t row_to;
-                bool there;
-                if constexpr (MODE == kDw) {
-                  there = row - lane + at < p.m;
-                  row_to = to - lane + at;
-                } else {
-                  const int target = __shfl_sync(0xffffffffu, on ? (int)to : -1, at);
-                  there = target >= 0;
-                  row_to = target;
+                for (int j = 0; j < 4; ++j) {
+                  const int at = j * 8 + (lane >> 2);
+                  int64_t row_to;
+                  bool there;
+                  if constexpr (MODE == kDw) {
+                    there = row - lane + at < p.m;
+                    row_to = to - lane + at;
+                  } else {
+                    const int target = __shfl_sync(0xffffffffu, on ? (int)to : -1, at);
+                    there = target >= 0;
+                    row_to = target;
+                  }
+                  if (there && col < cols)
+                    *reinterpret_cast<uint4*>(out + row_to * p.ld + col) = *reinterpret_cast<const uint4*>(staging + staging_off(at, lane & 3));
                 }
-                if (there && col < cols)
-                  *reinterpret_cast<uint4*>(static_cast<OUT*>(p.out) + row_to * p.ld + c_base + col) = *reinterpret_cast<const uint4*>(staging + staging_off(at, lane & 3));
+              } else {
+                // Half a warp has a row, a lane a word of it; the single elements before and behind a row's words are stored by the row's own lane.
+                constexpr bool HALVES = sizeof(OUT) == 2;
+                const int k = lane % 16, side = lane / 16, have = min(PANEL, cols - c0 - h);
+                OUT* const panel = out + c0 + h;
+                auto lead = [](const OUT* row) { return HALVES ? (int)(reinterpret_cast<uintptr_t>(row) / 2 % 2) : 0; };
+                const uint8_t* const from = staging + side * 64;
+                auto word = [&](int j, int i) { return *reinterpret_cast<const uint32_t*>(from + j * 128 + (((i / 4) ^ (j & 3)) << 4) + i % 4 * 4); };   // (see staging_off)
+                auto store = [&](OUT* row, int off, int j) {   // the (2 j + side)-th row of the warp's
+                  *reinterpret_cast<uint32_t*>(row + (HALVES ? 2 * k + off : k)) = HALVES ? __funnelshift_r(word(j, k), word(j, (k + 1) % 16), off * 16) : word(j, k);
+                };
+                if constexpr (MODE == kDw) {
+                  OUT* row_at = panel + (to - lane + side) * p.ld;
+                  const int off = lead(row_at);   // (every second row begins alike)
+                  const int rows = (HALVES ? 2 * k + off + 1 : k) < have ? p.m - (row - lane) - side : 0;
+#pragma unroll 4
+                  for (int j = 0; j < 16; ++j, row_at += 2 * p.ld)
+                    if (2 * j < rows) store(row_at, off, j);
+                } else {
+#pragma unroll 4
+                  for (int j = 0; j < 16; ++j) {
+                    const int target = __shfl_sync(0xffffffffu, on ? (int)to : -1, 2 * j + side);
+                    OUT* row_at = panel + (int64_t)target * p.ld;
+                    const int off = lead(row_at);
+                    if (target >= 0 && (HALVES ? 2 * k + off + 1 : k) < have) store(row_at, off, j);
+                  }
+                }
+                if constexpr (HALVES) {
+                  OUT* mine = panel + to * p.ld;
+                  const int off = lead(mine);
+                  auto element = [&](int i) { return *reinterpret_cast<const OUT*>(staging + staging_off(lane, i / 8) + i % 8 * 2); };
+                  if (on && off) mine[0] = element(0);
+                  if (on && (have - off) % 2 == 1) mine[have - 1] = element(have - 1);   // (nothing for a row of its first element alone)
+                }
               }
               __syncwarp();
             }
-          } else if (on) {
-            if constexpr (MODE == kDx) ce_add_lost<OUT, 32>(p, dst, c_base + c0, min(32, cols - c0), v);
-            ce_emit<OUT, 32>(p, unit, row, to, c_base + c0, min(32, cols - c0), v);
           }
           __syncwarp();
         }
@@ -815,21 +873,54 @@ __global__ void __launch_bounds__(256) castle_ce_sum_kernel(const CeProduct p) {
   work.place(work.whole + tile, m, n);
   const int at = blockIdx.x * 256 + threadIdx.x, local = at % ROWS, first = at / ROWS * COLS;   // neighbouring threads: neighbouring rows
   const int row = m * ROWS + local, col = n * p.bn + first;
-  if (row >= (MODE == kDw ? p.m : head.rows) || col >= p.n) return;
+  const bool on = row < (MODE == kDw ? p.m : head.rows);
+  if (col >= p.n) return;   // (a whole warp: its threads have neighbouring rows)
   float t[COLS];
 #pragma unroll
   for (int j = 0; j < COLS; ++j) t[j] = 0.f;
+  const int slices = on ? work.slices : 0;
 #pragma unroll(COLS == 4 ? 8 : 2)
-  for (int s = 0; s < work.slices; ++s) {
+  for (int s = 0; s < slices; ++s) {
 #pragma unroll
     for (int j = 0; j < COLS; j += 4) {
       const float4 v = p.slab[((int64_t)(s * work.left + tile) * (kCeN / 4) + (first + j) / 4) * ROWS + local];
       t[j] += v.x; t[j + 1] += v.y; t[j + 2] += v.z; t[j + 3] += v.w;
     }
   }
-  const CeOut<OUT> dst = ce_out<MODE, OUT>(p, row, true);
-  if constexpr (MODE == kDx) ce_add_lost<OUT, COLS>(p, dst, col, min(COLS, p.n - col), t);
-  ce_emit<OUT, COLS>(p, head.unit, row, dst.to, col, min(COLS, p.n - col), t);
+  const int have = min(COLS, p.n - col);
+  const CeOut<OUT> dst = ce_out<MODE, OUT>(p, row, on);
+  if constexpr (MODE == kDx) {
+    ce_add_lost<OUT, COLS>(p, dst, col, have, t);
+    if (p.acc && on) ce_accumulate<COLS>(p, row, col, have, t);
+    if (p.acc && !p.acc_out) return;
+  }
+#pragma unroll
+  for (int j = 0; j < COLS; ++j) t[j] *= head.unit;
+  OUT* out = static_cast<OUT*>(p.out) + col;
+  if constexpr (COLS == 16) {
+    if (!p.vec) {   // rows at odd places: half a warp stores a row's 16 elements
+      __shared__ float stage[8][32][17];
+      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, in = lane % 16;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) stage[warp][lane][j] = t[j];
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 32; j += 2) {
+        const int at = j + lane / 16, to = __shfl_sync(0xffffffffu, on ? (int)dst.to : -1, at);
+        if (to >= 0 && in < have) store1<OUT>(out + to * p.ld + in, stage[warp][at][in]);
+      }
+      return;
+    }
+    if (!on) return;
+#pragma unroll
+    for (int j = 0; j < COLS; j += 8)
+      if (j < have) store8<OUT>(out + dst.to * p.ld + j, t + j);
+  } else {
+    if (!on) return;
+#pragma unroll
+    for (int j = 0; j < COLS; ++j)
+      if (j < have) store1<OUT>(out + dst.to * p.ld + j, t[j]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ the losses

@@ -118,6 +118,15 @@ def test_a_vocabulary_in_pieces(n, dim, vocab, dtype):
     check(*case(n, dim, vocab, dtype, 0.1))
 
 
+@pytest.mark.parametrize("dtype", TYPES.values(), ids=TYPES.keys())
+@pytest.mark.parametrize("n,dim,vocab", [(40, 21, 500), (300, 107, 513), (4200, 301, 1700), (1700, 301, 4200), (600, 260, 2000), (8200, 65, 70000)])
+def test_rows_at_odd_places(n, dim, vocab, dtype):
+    """Rows that begin at every place in 16 bytes: read and written in parts, whole tiles, shared ones and several pieces of a vocabulary."""
+    if vocab == 70000 and dtype == torch.float32:
+        vocab = 30000
+    check(*case(n, dim, vocab, dtype, 0.1))
+
+
 def test_nothing_to_learn():
     for reduction in ("mean", "sum", "none"):
         x, w, t = case(300, 64, 500, torch.bfloat16)
