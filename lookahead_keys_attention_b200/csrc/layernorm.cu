@@ -12,8 +12,8 @@
 // turn: the weight (and bias) is unpacked once, arithmetic is on packed pairs, and the rows ahead are on their way into shared memory,
 // each thread's columns into places of its own (asynchronous copies that it alone waits for, so nothing has to be synchronised).
 // The backward's groups keep their share of dw and db in registers; a CTA leaves one fp32 row of each, and a last launch adds
-// these in a fixed order.  Wider rows, and calls that want only some of the gradients, take a pass per result that reads its rows
-// from memory (or cache) as often as it needs them.
+// these in a fixed order.  Wider rows, and calls that want no dx, take a pass per result that reads its rows from memory (or
+// cache) as often as it needs them.
 #include <type_traits>
 
 #include "common.cuh"
@@ -154,8 +154,11 @@ template <int THREADS, bool VEC, int NV> __device__ __forceinline__ void ln_clea
     }
 }
 
+// Blocks of an SM.  Rows of more than 4096 columns: two of 256 threads with 32 elements each wait less for each other's sums than one of 512 with 16
+// (15063 rows of 8192 in bf16 78 us / 105, of 4824 62 / 97; 8000 of 5000 in fp32 82 / 98).
+template <int NV> constexpr int kLnFwdBlocks = NV > 2 ? 2 : 3;
 template <typename T, bool VEC, int THREADS, int NV>
-__global__ void __launch_bounds__(kLnBlock<THREADS>, THREADS > kLnThreads ? 1 : 3) castle_layernorm_fwd_kernel(
+__global__ void __launch_bounds__(kLnBlock<THREADS>, kLnFwdBlocks<NV>) castle_layernorm_fwd_kernel(
     const T* __restrict__ x, int64_t stride, const T* __restrict__ w, const T* __restrict__ b, float eps, T* __restrict__ y, float2* __restrict__ stats, int64_t rows,
     int dim) {
   constexpr int GROUPS = kLnBlock<THREADS> / THREADS;
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(kLnThreads) castle_layernorm_fwd_wide_kernel(c
   if (stats && t == 0) stats[r] = make_float2(mean, rstd);
 }
 
-// dx alone, rows of any width.
+// dx, rows of any width.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kLnThreads) castle_layernorm_dx_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t stride,
                                                                          const T* __restrict__ w, const float2* __restrict__ stats, T* __restrict__ dx, int dim) {
@@ -304,7 +307,7 @@ __global__ void __launch_bounds__(kLnThreads) castle_layernorm_dw_kernel(const T
   }
 }
 
-// All gradients in one pass over dy and x.
+// All gradients in one pass over dy and x, or dx alone (`partial` NULL: a thread's sums cost less than a pass without them in another kernel, 46882 x 256 in fp32 40 us, there 127).
 template <typename T, bool VEC, int THREADS, int NV>
 __global__ void __launch_bounds__(kLnBlock<THREADS>, THREADS > kLnThreads ? 1 : 2)
     castle_layernorm_bwd_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t stride, const T* __restrict__ w,
@@ -353,6 +356,7 @@ __global__ void __launch_bounds__(kLnBlock<THREADS>, THREADS > kLnThreads ? 1 : 
       for (int j = 0; j < 4; ++j) v[1].v[q][j] = mul2(fma2(v[0].v[q][j], mgh, add2(v[1].v[q][j], mg)), splat(st.y));
     ln_store<T, VEC, THREADS, NV>(dx + r * dim, t, dim, v[1]);
   }
+  if (!partial) return;   // dx alone
   // the groups' sums, in order
   for (int side = 0; side < 2; ++side) {
     if constexpr (GROUPS > 1) {
@@ -412,7 +416,7 @@ constexpr int kLnWhole = 8192;   // widest row that a group's registers hold
 
 // CTAs of the backward's one pass, or row ranges of dw's own: two per SM, but no more than there are rows for.
 static int ln_parts(int64_t rows, int dim) {
-  const int64_t most = dim > 4096 ? 148 : 296, have = (rows + 7) / 8;
+  const int64_t most = dim > 4096 ? 148 : 296, have = (rows + 3) / 4;
   return (int)(have < most ? have : most);
 }
 
@@ -441,12 +445,14 @@ static cudaError_t ln_fwd(int64_t rows, int dim, const T* x, int64_t stride, con
     castle_layernorm_fwd_wide_kernel<T, VEC><<<(unsigned)rows, kLnThreads, 0, st>>>(x, stride, w, b, eps, y, stats, dim);
     return cudaGetLastError();
   }
-  return ln_group(dim, [&](auto threads, auto nv) {
+  auto go = [&](auto threads, auto nv) {
     constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value, G = kLnBlock<TH> / TH;
-    const int64_t have = (rows + G - 1) / G, most = 148 * (TH > kLnThreads ? 1 : 3);
+    const int64_t have = (rows + G - 1) / G, most = 148 * kLnFwdBlocks<NV>;
     return ln_launch(castle_layernorm_fwd_kernel<T, VEC, TH, NV>, have < most ? have : most, kLnBlock<TH>, LnRows<T, VEC, TH, NV, 1>::kBytes, st, x, stride, w, b, eps, y,
                      stats, rows, dim);
-  });
+  };
+  using std::integral_constant;
+  return dim > 4096 ? go(integral_constant<int, 256>(), integral_constant<int, 4>()) : ln_group(dim, go);
 }
 
 template <typename T, bool VEC>
@@ -454,11 +460,11 @@ static cudaError_t ln_bwd(int64_t rows, int dim, const T* dy, int64_t dy_stride,
                           float* ws, cudaStream_t st) {
   const int parts = ln_parts(rows, dim);
   const bool params = dw || db;
-  if (dx && params && dim <= kLnWhole) {
+  if (dx && dim <= kLnWhole) {
     const cudaError_t e = ln_group(dim, [&](auto threads, auto nv) {
       constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value;
-      return ln_launch(castle_layernorm_bwd_kernel<T, VEC, TH, NV>, parts, kLnBlock<TH>, LnRows<T, VEC, TH, NV, 2>::kBytes, st, dy, dy_stride, x, stride, w, stats, dx, ws,
-                       rows, dim);
+      return ln_launch(castle_layernorm_bwd_kernel<T, VEC, TH, NV>, parts, kLnBlock<TH>, LnRows<T, VEC, TH, NV, 2>::kBytes, st, dy, dy_stride, x, stride, w, stats, dx,
+                       params ? ws : (float*)nullptr, rows, dim);
     });
     if (e != cudaSuccess) return e;
   } else {
