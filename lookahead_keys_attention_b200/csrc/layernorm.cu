@@ -8,7 +8,7 @@
 //
 // Both directions should be bound by memory (x in and y out; x and dy in and dx out), but 4096 columns of bf16 at 6.5 TB/s leave an SM
 // some seven instructions per element: one kernel per row with single arithmetic was bound by instruction issue (32768 rows: 135
-// and 174 us, where the bytes take 82 and 123).  So groups of threads (16 elements each; 32 to 512 threads) stay and take rows in
+// and 174 us, where the bytes take 82 and 123).  So groups of threads (16 elements each, 32 in the widest forward; 32 to 512 threads) stay and take rows in
 // turn: the weight (and bias) is unpacked once, arithmetic is on packed pairs, and the rows ahead are on their way into shared memory,
 // each thread's columns into places of its own (asynchronous copies that it alone waits for, so nothing has to be synchronised).
 // The backward's groups keep their share of dw and db in registers; a CTA leaves one fp32 row of each, and a last launch adds

@@ -124,13 +124,22 @@ __device__ __forceinline__ void copy_row(const T* src, uint16_t* dst, int64_t pl
   using Op = typename CePlanes<T>::Op;
   constexpr int P = CePlanes<T>::count;
   if (dim % 8 == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+    if constexpr (P == 1) {
 #pragma unroll 4
-    for (int c = lane * 8; c < dim; c += 256) {
-      if constexpr (P == 1) {
-        *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-      } else {
+      for (int c = lane * 8; c < dim; c += 256) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+      return;
+    }
+    for (int c0 = lane * 8; c0 < dim; c0 += 1024) {   // four loads on their way at a time
+      Raw8<T> raw[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c0 + u * 256 < dim) raw[u] = *reinterpret_cast<const Raw8<T>*>(src + c0 + u * 256);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int c = c0 + u * 256;
+        if (c >= dim) break;
         float v[8], w[P][8];
-        load8<T>(src + c, v);
+        load8<T>(reinterpret_cast<const T*>(&raw[u]), v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float a[P];
@@ -296,18 +305,19 @@ __global__ void __launch_bounds__(1024, 1) castle_ce_rows_kernel(const CeRowsPar
           copy_row<T>(src, p.copy + (int64_t)place[k] * p.pitch, plane, p.dim, p.pitch, lane);
         } else if (p.dx) {
           T* row = static_cast<T*>(p.dx) + (i0 + k) * p.dim;
+#pragma unroll 4
           for (int c = lane; c < p.dim; c += 32) store1<T>(row + c, 0.f);
         }
       }
     }
   }
-  // what the contraction over rows reads behind the last one
-  if ((gather || p.copy_always) && blockIdx.x == gridDim.x - 1) {
+  // what dW's contraction over rows reads behind the last one
+  if (!p.lse_out && (gather || p.copy_always) && blockIdx.x == gridDim.x - 1) {
     const int64_t plane = p.copy_rows * p.pitch;
     const int64_t end = min(p.copy_rows, ((int64_t)all + kCeK - 1) / kCeK * kCeK);
     for (int64_t k = all + warp; k < end; k += 32)
       for (int q = 0; q < p.planes; ++q)
-        for (int c = lane; c < p.pitch; c += 32) p.copy[q * plane + k * p.pitch + c] = 0;
+        for (int c = lane * 8; c < p.pitch; c += 256) *reinterpret_cast<uint4*>(p.copy + q * plane + k * p.pitch + c) = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -514,13 +524,15 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
       const CUtensorMap* mb = MODE == kDw && copy ? &map_copy : &map_b;
       // what a step brings, of the pair
       const uint32_t bytes = PAIR * ((A_MN ? 2 * p.k_rows : p.a_rows) * 128 + (MODE == kDw ? kCeN / PAIR / 64 * p.k_rows * 128 : p.bn / PAIR * kCeK * 2));
-      bool sent = false;
+      bool sent = false, ready = false;   // ready: the next stage was found free while this one's copies were sent (a wait takes 300 cycles even if it is over)
       for (int i = 0; work.at(worker, i, m, n, k0, k1, slot) && !*abortp; ++i) {
         const int m0 = (m * PAIR + rank) * kCeM, n0 = n * p.bn + (PAIR == 2 ? rank * (columns(n) / 2) : 0);
         for (int ks = k0; ks < k1; ++ks) {
-          for (int term = 6 - p.terms; term < 6; ++term, ring.next()) {
+          for (int term = 6 - p.terms; term < 6; ++term) {
             const int s = ring.s, k = ks * kCeK, pa = kTermA[term], pb = kTermB[term];
-            if (!mbar_wait_ok<true>(&bar_free[s], ring.phase ^ 1u, abortp)) { ks = k1; break; }
+            if (!ready && !mbar_wait_ok<true>(&bar_free[s], ring.phase ^ 1u, abortp)) { ks = k1; break; }
+            ring.next();
+            ready = mbar_test_wait(&bar_free[ring.s], ring.phase ^ 1u);
             uint8_t *a = smem + s * stage, *b = a + kCeA;
             if (rank == 0) mbar_expect_tx(&bar_full[s], bytes);
             sent = true;
@@ -554,6 +566,7 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
         else mma_commit(bar);
       };
       int turn = 0;
+      bool ready = false;   // the next stage was found filled (logits of 197 x 4096 against 256 in fp32 90 us, in bf16 17.3; without looking ahead 108 and 20)
       for (int i = 0; work.at(worker, i, m, n, k0, k1, slot) && !*abortp; ++i) {
         const uint32_t idesc = make_idesc(kCeM * PAIR, 16, Elem<T>::fmt, A_MN, B_MN, false) + ((uint32_t)((columns(n) - 16) >> 3) << 17);
         for (; k0 < k1 && !*abortp; k0 += p.flush, ++turn) {
@@ -562,10 +575,12 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
           const uint32_t phase = ((uint32_t)(turn >> 1) & 1u) ^ 1u;
           if (!(PAIR == 2 ? mbar_wait_ok_cluster(&bar_read[acc], phase, abortp) : mbar_wait_ok<true>(&bar_read[acc], phase, abortp))) break;
           tc_fence_after();
-          for (int j = 0; j < steps; ++j, ring.next()) {
+          for (int j = 0; j < steps; ++j) {
             const int s = ring.s;
-            if (!mbar_wait_ok<true>(&bar_full[s], ring.phase, abortp)) break;
+            if (!ready && !mbar_wait_ok<true>(&bar_full[s], ring.phase, abortp)) break;
             tc_fence_after();
+            ring.next();
+            ready = mbar_test_wait(&bar_full[ring.s], ring.phase);
             const uint32_t a = smem_u32(smem) + s * stage, b = a + kCeA;
             const uint64_t da = A_MN ? desc_mnmajor(a, 8192) : desc_kmajor(a), db = B_MN ? desc_mnmajor(b, 8192) : desc_kmajor(b);
 #pragma unroll
@@ -1153,9 +1168,9 @@ static cudaError_t ce_launch(const CeProduct& p, int pair, int64_t tiles, const 
   return pair == 2 ? ce_launch_as<T, OUT, MODE, F32, 2>(p, tiles, a, copy, b, st) : ce_launch_as<T, OUT, MODE, F32, 1>(p, tiles, a, copy, b, st);
 }
 
-static int ce_rows_per_cta(int64_t n) {   // a CTA per SM, at least 32 rows each
+static int ce_rows_per_cta(int64_t n) {   // a CTA per SM, at least eight rows each (197 x 4096 in fp32 9 us, with 32 rows 20)
   const int64_t r = (n + 147) / 148;
-  return (int)(r < 32 ? 32 : r);
+  return (int)(r < 8 ? 8 : r);
 }
 
 struct CeCall {
