@@ -512,7 +512,9 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
   const CeWork<MODE, PAIR> work(p, head.rows, gridDim.x / PAIR);
   const int worker = blockIdx.x / PAIR;
   int m, n, k0, k1, slot;
-  const uint32_t stage = kCeA + p.bn / PAIR * kCeK * 2;   // bytes
+  // fp32's parts: a stage has all of them where two such stages fit, and the six products of a step read them from there.
+  const bool together = CePlanes<OUT>::count > 1 && 2 * 3 * (kCeA + p.bn / PAIR * kCeK * 2) <= kCeRing;
+  const uint32_t parts = together ? 3 : 1, b_bytes = p.bn / PAIR * kCeK * 2, stage = parts * (kCeA + b_bytes);   // bytes
   CeTurn ring(min(kCeStages, (int)(kCeRing / stage)));
   // columns of a tile that are computed
   auto columns = [&](int n) { return min(p.bn, (p.n - n * p.bn + GRAIN - 1) / GRAIN * GRAIN); };
@@ -523,34 +525,37 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
       const CUtensorMap* ma = MODE != kDx && MODE != kDw && copy ? &map_copy : &map_a;
       const CUtensorMap* mb = MODE == kDw && copy ? &map_copy : &map_b;
       // what a step brings, of the pair
-      const uint32_t bytes = PAIR * ((A_MN ? 2 * p.k_rows : p.a_rows) * 128 + (MODE == kDw ? kCeN / PAIR / 64 * p.k_rows * 128 : p.bn / PAIR * kCeK * 2));
+      const uint32_t bytes = parts * PAIR * ((A_MN ? 2 * p.k_rows : p.a_rows) * 128 + (MODE == kDw ? kCeN / PAIR / 64 * p.k_rows * 128 : p.bn / PAIR * kCeK * 2));
       bool sent = false, ready = false;   // ready: the next stage was found free while this one's copies were sent (a wait takes 300 cycles even if it is over)
       for (int i = 0; work.at(worker, i, m, n, k0, k1, slot) && !*abortp; ++i) {
         const int m0 = (m * PAIR + rank) * kCeM, n0 = n * p.bn + (PAIR == 2 ? rank * (columns(n) / 2) : 0);
         for (int ks = k0; ks < k1; ++ks) {
-          for (int term = 6 - p.terms; term < 6; ++term) {
-            const int s = ring.s, k = ks * kCeK, pa = kTermA[term], pb = kTermB[term];
+          for (int term = together ? 5 : 6 - p.terms; term < 6; ++term) {
+            const int s = ring.s, k = ks * kCeK;
             if (!ready && !mbar_wait_ok<true>(&bar_free[s], ring.phase ^ 1u, abortp)) { ks = k1; break; }
             ring.next();
             ready = mbar_test_wait(&bar_free[ring.s], ring.phase ^ 1u);
-            uint8_t *a = smem + s * stage, *b = a + kCeA;
             if (rank == 0) mbar_expect_tx(&bar_full[s], bytes);
             sent = true;
             auto load = [&](void* dst, const CUtensorMap* map, int c0, int c1, int plane) {
               if constexpr (PAIR == 2) tma_load_4d_pair(dst, map, of_cta(&bar_full[s], 0), c0, c1, plane, 0);
               else tma_load_4d(dst, map, &bar_full[s], c0, c1, plane, 0);
             };
-            if (A_MN) {
-              load(a, ma, m0, k, pa);
-              load(a + kCeA / 2, ma, m0 + 64, k, pa);
-            } else {
-              load(a, ma, k, m0, pa);
-            }
-            if (B_MN) {
+            for (uint32_t part = 0; part < parts; ++part) {
+              uint8_t *a = smem + s * stage + part * kCeA, *b = smem + s * stage + parts * kCeA + part * b_bytes;
+              const int pa = together ? (int)part : kTermA[term], pb = together ? (int)part : kTermB[term];
+              if (A_MN) {
+                load(a, ma, m0, k, pa);
+                load(a + kCeA / 2, ma, m0 + 64, k, pa);
+              } else {
+                load(a, ma, k, m0, pa);
+              }
+              if (B_MN) {
 #pragma unroll
-              for (int j = 0; j < kCeN / PAIR / 64; ++j) load(b + j * 8192, mb, n0 + j * 64, k + (MODE == kDx ? p.b_row0 : 0), pb);
-            } else {
-              load(b, mb, k, p.b_row0 + n0, pb);
+                for (int j = 0; j < kCeN / PAIR / 64; ++j) load(b + j * 8192, mb, n0 + j * 64, k + (MODE == kDx ? p.b_row0 : 0), pb);
+              } else {
+                load(b, mb, k, p.b_row0 + n0, pb);
+              }
             }
           }
         }
@@ -570,7 +575,7 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
       for (int i = 0; work.at(worker, i, m, n, k0, k1, slot) && !*abortp; ++i) {
         const uint32_t idesc = make_idesc(kCeM * PAIR, 16, Elem<T>::fmt, A_MN, B_MN, false) + ((uint32_t)((columns(n) - 16) >> 3) << 17);
         for (; k0 < k1 && !*abortp; k0 += p.flush, ++turn) {
-          const int acc = turn & 1, steps = min(p.flush, k1 - k0) * p.terms;
+          const int acc = turn & 1, steps = min(p.flush, k1 - k0) * (together ? 1 : p.terms);
           const uint32_t d = tmem + acc * kCeN;
           const uint32_t phase = ((uint32_t)(turn >> 1) & 1u) ^ 1u;
           if (!(PAIR == 2 ? mbar_wait_ok_cluster(&bar_read[acc], phase, abortp) : mbar_wait_ok<true>(&bar_read[acc], phase, abortp))) break;
@@ -581,14 +586,18 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
             tc_fence_after();
             ring.next();
             ready = mbar_test_wait(&bar_full[ring.s], ring.phase);
-            const uint32_t a = smem_u32(smem) + s * stage, b = a + kCeA;
-            const uint64_t da = A_MN ? desc_mnmajor(a, 8192) : desc_kmajor(a), db = B_MN ? desc_mnmajor(b, 8192) : desc_kmajor(b);
+            for (int term = together ? 0 : 5; term < 6; ++term) {
+              const uint32_t a = smem_u32(smem) + s * stage + (together ? kTermA[term] * kCeA : 0),
+                             b = smem_u32(smem) + s * stage + parts * kCeA + (together ? kTermB[term] * b_bytes : 0);
+              const uint64_t da = A_MN ? desc_mnmajor(a, 8192) : desc_kmajor(a), db = B_MN ? desc_mnmajor(b, 8192) : desc_kmajor(b);
 #pragma unroll
-            for (int q = 0; q < kCeK / 16; ++q) {
-              if (MODE == kDw && q * 16 >= p.k_rows) break;
-              const uint64_t ao = da + (uint64_t)(((A_MN ? 2048 : 32) * q) >> 4), bo = db + (uint64_t)(((B_MN ? 2048 : 32) * q) >> 4);
-              if constexpr (PAIR == 2) mma_ss_pair(d, ao, bo, idesc, j > 0 || q > 0);
-              else mma_ss(d, ao, bo, idesc, j > 0 || q > 0);
+              for (int q = 0; q < kCeK / 16; ++q) {
+                if (MODE == kDw && q * 16 >= p.k_rows) break;
+                const uint64_t ao = da + (uint64_t)(((A_MN ? 2048 : 32) * q) >> 4), bo = db + (uint64_t)(((B_MN ? 2048 : 32) * q) >> 4);
+                const bool add = j > 0 || (together && term > 0) || q > 0;
+                if constexpr (PAIR == 2) mma_ss_pair(d, ao, bo, idesc, add);
+                else mma_ss(d, ao, bo, idesc, add);
+              }
             }
             commit(&bar_free[s]);
           }
