@@ -84,7 +84,8 @@ struct CeHead {          // at the start of the workspace, written by castle_ce_
 };
 struct CeRow { int target; float lse, coef; int row; };   // of the rows that take part, in order; coef: G's, row: in the caller's tensors
 
-__constant__ const int8_t kTermA[6] = {2, 0, 1, 1, 0, 0}, kTermB[6] = {0, 2, 1, 0, 1, 0};   // one term: the last
+__device__ __forceinline__ int term_a(int term) { return 0x001102 >> 4 * term & 3; }
+__device__ __forceinline__ int term_b(int term) { return 0x010120 >> 4 * term & 3; }   // one term: the last
 
 // ------------------------------------------------------------------------------------------------ rows that take part
 struct CeRowsParams {
@@ -512,7 +513,8 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
   const CeWork<MODE, PAIR> work(p, head.rows, gridDim.x / PAIR);
   const int worker = blockIdx.x / PAIR;
   int m, n, k0, k1, slot;
-  // fp32's parts: a stage has all of them where two such stages fit, and the six products of a step read them from there.
+  // fp32's parts: a stage has all of them where two such stages fit, and the six products of a step read them from there
+  // (logits of 197 x 4096 against 256 74 us, a stage for each product 90; forward and gradients of 9472 x 4096 against 8192 9.4 ms / 10.6).
   const bool together = CePlanes<OUT>::count > 1 && 2 * 3 * (kCeA + p.bn / PAIR * kCeK * 2) <= kCeRing;
   const uint32_t parts = together ? 3 : 1, b_bytes = p.bn / PAIR * kCeK * 2, stage = parts * (kCeA + b_bytes);   // bytes
   CeTurn ring(min(kCeStages, (int)(kCeRing / stage)));
@@ -543,7 +545,7 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
             };
             for (uint32_t part = 0; part < parts; ++part) {
               uint8_t *a = smem + s * stage + part * kCeA, *b = smem + s * stage + parts * kCeA + part * b_bytes;
-              const int pa = together ? (int)part : kTermA[term], pb = together ? (int)part : kTermB[term];
+              const int pa = together ? (int)part : term_a(term), pb = together ? (int)part : term_b(term);
               if (A_MN) {
                 load(a, ma, m0, k, pa);
                 load(a + kCeA / 2, ma, m0 + 64, k, pa);
@@ -571,14 +573,15 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
         else mma_commit(bar);
       };
       int turn = 0;
-      bool ready = false;   // the next stage was found filled (logits of 197 x 4096 against 256 in fp32 90 us, in bf16 17.3; without looking ahead 108 and 20)
+      bool read = false;    // the next accumulator was found free
+      bool ready = false;   // the next stage was found filled (logits of 197 x 4096 against 256 in bf16 17.3 us, without looking ahead 20)
       for (int i = 0; work.at(worker, i, m, n, k0, k1, slot) && !*abortp; ++i) {
         const uint32_t idesc = make_idesc(kCeM * PAIR, 16, Elem<T>::fmt, A_MN, B_MN, false) + ((uint32_t)((columns(n) - 16) >> 3) << 17);
         for (; k0 < k1 && !*abortp; k0 += p.flush, ++turn) {
           const int acc = turn & 1, steps = min(p.flush, k1 - k0) * (together ? 1 : p.terms);
           const uint32_t d = tmem + acc * kCeN;
           const uint32_t phase = ((uint32_t)(turn >> 1) & 1u) ^ 1u;
-          if (!(PAIR == 2 ? mbar_wait_ok_cluster(&bar_read[acc], phase, abortp) : mbar_wait_ok<true>(&bar_read[acc], phase, abortp))) break;
+          if ((PAIR == 2 || !read) && !(PAIR == 2 ? mbar_wait_ok_cluster(&bar_read[acc], phase, abortp) : mbar_wait_ok<true>(&bar_read[acc], phase, abortp))) break;
           tc_fence_after();
           for (int j = 0; j < steps; ++j) {
             const int s = ring.s;
@@ -587,8 +590,8 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
             ring.next();
             ready = mbar_test_wait(&bar_full[ring.s], ring.phase);
             for (int term = together ? 0 : 5; term < 6; ++term) {
-              const uint32_t a = smem_u32(smem) + s * stage + (together ? kTermA[term] * kCeA : 0),
-                             b = smem_u32(smem) + s * stage + parts * kCeA + (together ? kTermB[term] * b_bytes : 0);
+              const uint32_t a = smem_u32(smem) + s * stage + (together ? term_a(term) * kCeA : 0),
+                             b = smem_u32(smem) + s * stage + parts * kCeA + (together ? term_b(term) * b_bytes : 0);
               const uint64_t da = A_MN ? desc_mnmajor(a, 8192) : desc_kmajor(a), db = B_MN ? desc_mnmajor(b, 8192) : desc_kmajor(b);
 #pragma unroll
               for (int q = 0; q < kCeK / 16; ++q) {
@@ -602,6 +605,7 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
             commit(&bar_free[s]);
           }
           commit(&bar_done[acc]);
+          if (PAIR == 1) read = mbar_test_wait(&bar_read[acc ^ 1], ((uint32_t)((turn + 1) >> 1) & 1u) ^ 1u);
         }
       }
       commit(&bar_end);   // all products have read their operands
