@@ -565,6 +565,9 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
       // a copy that nobody waited for (after an abort) must not arrive in another CTA's shared memory
       if (*abortp && rank == 0 && sent)
         for (int j = 0; j < ring.stages; ++j, ring.next()) mbar_drain(&bar_full[ring.s], ring.phase ^ 1u);   // the last round of each
+      // nor must the other CTA's word that a stage is free: the second CTA of a pair waits for the last of each (stages never used are free)
+      if (rank == 1)
+        for (int j = 0; j < ring.stages && !*abortp; ++j, ring.next()) mbar_wait_ok<true>(&bar_free[ring.s], ring.phase ^ 1u, abortp);
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
@@ -880,7 +883,12 @@ __global__ void __launch_bounds__(kCeThreads<MODE>, 1) castle_ce_kernel(const Ce
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR == 2) cluster_sync();   // the other's products read this CTA's tiles, its warps arrive at this CTA's barriers
+  if constexpr (PAIR == 2) {
+    cluster_sync();   // the other's products read this CTA's tiles, its warps arrive at this CTA's barriers
+    // The issuing thread has seen its last commit at its own CTA's barrier, which says nothing of the arrival here: a CTA that ended before would
+    // have it in the shared memory of the next one on its SM.  (An issuer's commits arrive in order; this one comes after an abort, too.)
+    if (rank == 1 && tid == 0) mbar_drain(&bar_end, 0);
+  }
   if (warp == 1) {
     if constexpr (PAIR == 2) tmem_dealloc_pair(tmem, 512);
     else tmem_dealloc(tmem, 512);
