@@ -31,8 +31,9 @@
 //
 // What the tensor cores add to an accumulator loses more than rounding to nearest would, and the losses of a long sum add up (197 rows of 512,
 // fp32: losses 3.3e-6 off, gradients of longer sums 1.7e-5, where fp32 arithmetic has 2e-7).  Where the result has 32 bits
-// (the logits' statistics, and everything of fp32 tensors), accumulators are therefore emptied every `flush` steps into sums that
-// the working warps keep in registers.
+// (the logits, and everything of fp32 tensors), accumulators are therefore emptied every `flush` steps into sums that
+// the working warps keep in registers.  The logits formed again are the same sums, bit for bit, as those behind the log-sum-exp: summed in one go,
+// they made a row's probabilities add up to 1 + 1e-3 (logits of some 60 over 4096 to 8192, fp16), more than what a learnt row has to move by.
 //
 // G in 16 bits is taken in units of a power of two (the largest c_i's) with 2^14 on top, so that fp16 keeps probabilities down to 2^-28 in full
 // precision; the unit is multiplied back in fp32 at the end.  Where all rows have one coefficient (mean, sum) that is the unit and none
@@ -72,6 +73,7 @@ struct CeTurn {
 constexpr int64_t kCeScratch = (int64_t)1 << 30;   // bytes that a piece of the vocabulary may take
 // Steps between emptyings: of a 16-bit operand's logits (32 additions in the tensor cores), of fp32's parts (24).  With these the losses of
 // 197 x 512 in fp32 are 6.7e-8 of their norm off (emptied every second step 3.0e-7, and 8 % faster); not emptied 3.3e-6 and, of logits over 1024 in 16 bits, 8 % faster (166 us, 152).
+// (G's logits, too: 8192 x 4096 against 131072, forward and gradients, 28.2 ms for 27.5 without; 4096 x 1024 against 50021 1.49 ms for 1.45.)
 constexpr int kCeFlush = 8, kCeFlushF32 = 1, kCeNoFlush = 1 << 30;
 constexpr float kCeUnit = 16384.f;                 // of G: below 2 units
 
@@ -1182,7 +1184,7 @@ static cudaError_t ce_launch_as(const CeProduct& p, int64_t tiles, const CUtenso
 template <typename T, typename OUT, CeMode MODE>
 static cudaError_t ce_launch(const CeProduct& p, int pair, int64_t tiles, const CUtensorMap& a, const CUtensorMap& copy, const CUtensorMap& b, cudaStream_t st) {
   constexpr bool F32 = CePlanes<OUT>::count > 1;
-  if constexpr (MODE == kLse && !F32) {   // one emptying of an accumulator is none: it is read where it is
+  if constexpr ((MODE == kLse || MODE == kGrad) && !F32) {   // one emptying of an accumulator is none: it is read where it is
     if (p.k > p.flush * kCeK)
       return pair == 2 ? ce_launch_as<T, OUT, MODE, true, 2>(p, tiles, a, copy, b, st) : ce_launch_as<T, OUT, MODE, true, 1>(p, tiles, a, copy, b, st);
   }
@@ -1316,6 +1318,7 @@ static int ce_backward(const CeCall& c, const CePlan& q, const float* lse, const
     CeProduct p = base;
     p.n = (int)count; p.k = q.pitch; p.bn = cut.bn; p.b_row0 = q.copy_w ? 0 : (int)v0; p.vocab0 = (int)v0; p.group = 32 / cut.pair;
     p.g = gp; p.g_ld = pitch; p.g_plane = q.g_rows * pitch;
+    p.flush = q.terms > 1 ? kCeFlushF32 : kCeFlush;   // as in the forward: these are the logits that the log-sum-exp was formed of
     const int64_t tiles_m = (c.n + kCeM * cut.pair - 1) / (kCeM * cut.pair);
     CE_CUDA((ce_launch<T, OUT, kGrad>(p, cut.pair, tiles_m * ((count + cut.bn - 1) / cut.bn), x, copy, w, c.st)), what);
     if (dx) {
