@@ -163,7 +163,7 @@ int castle_layernorm_bwd(int32_t dtype, int64_t rows, int32_t dim, const void* d
  * y[i] = scale * weight[index[i]] for `tokens` indices of index_bytes (4 or 8) each; weight: `vocab` rows of `dim` elements,
  * row_stride elements apart (at most 3145728 rows, 2^30 indices); y contiguous.  An index outside the table gives a row of NaN and sets CASTLE_STATUS_BAD_INDEX.
  * Backward: dweight (vocab x dim, contiguous, every row written) = scale * the sum of each row's dy in the order of the
- * positions, in fp32; indices equal to padding_idx (-1: none) and those outside the table are left out, the latter set
+ * positions, in fp32; indices equal to padding_idx (a row of the table, or -1: none) and those outside the table are left out, the latter set
  * CASTLE_STATUS_BAD_INDEX.
  */
 int castle_embedding_fwd(int32_t dtype, int32_t index_bytes, int64_t tokens, int64_t vocab, int32_t dim, const void* index,

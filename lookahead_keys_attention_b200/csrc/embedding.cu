@@ -495,6 +495,8 @@ extern "C" int castle_embedding_bwd(int32_t dtype, int32_t index_bytes, int64_t 
   if (int rc = emb_check("castle_embedding_bwd", dtype, index_bytes, tokens, vocab, dim, index, dy_stride, status)) return rc;
   const int es = elem_size(dtype);
   if (!dy || !dweight || ((uintptr_t)dy | (uintptr_t)dweight) % es) return reject("castle_embedding_bwd: dy and dweight must be aligned to their elements");
+  if (padding_idx < -1 || padding_idx >= vocab)   // (the kernels compare 32 bits)
+    return reject("castle_embedding_bwd: padding_idx %lld is neither a row of the table nor -1", (long long)padding_idx);
   const EmbScratch s = emb_scratch(tokens, vocab, dim);
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < s.bytes) return reject("castle_embedding_bwd: workspace too small or not 16-byte aligned");
   EmbGrad p;

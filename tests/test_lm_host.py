@@ -39,6 +39,15 @@ def test_embedding_arguments():
         assert bwd(**bad) < 0 and "castle_embedding_bwd" in L.last_error(), bad
 
 
+@pytest.mark.parametrize("padding", [-2, 10, 2 ** 32 - 1, 2 ** 32 + 5, -2 ** 32 + 5, 2 ** 63 - 1, -2 ** 63])
+def test_padding_outside_the_table_is_refused(padding):
+    """Cut to 32 bits, 2^32 + 5 would be row 5, whose gradient would be left out."""
+    L, lib = _lib()
+    size = lib.castle_embedding_bwd_workspace_bytes(4, 10, 16)
+    assert lib.castle_embedding_bwd(L.BF16, 8, 4, 10, 16, 32, padding, 32, 16, 1.0, 32, 32, size, 32, None) < 0
+    assert f"padding_idx {padding}" in L.last_error()
+
+
 def test_embedding_limits():
     """Places in the sorted list are 32 bits: 2^30 tokens at most, and no scratch is named for what would be refused."""
     L, lib = _lib()
