@@ -10,6 +10,7 @@
 // Operators and their semantics: ops.py and castle.py.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/grad_mode.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -26,6 +27,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <array>
 #include <limits>
 #include <map>
@@ -40,6 +42,8 @@
 namespace {
 
 using at::Tensor;
+using torch::autograd::Edge;
+using torch::autograd::edge_list;
 using torch::autograd::Node;
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
@@ -440,6 +444,22 @@ Tensor restored(const Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype, co
 Tensor restored_contiguous(const Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype, const at::Device& dev) {
   restored(t, sizes, dtype, dev);
   return aligned_contiguous(t);
+}
+
+// The nodes compute gradients below autograd.  With create_graph they would come back as constants, and what a penalty on them adds to the
+// gradients would silently be missing; so they get a node that refuses to be differentiated, behind all that they depend on: the upstream
+// gradient and what `inputs` lead to.
+void refuse_second(variable_list& results, const char* who, const Tensor& upstream, edge_list inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  if (upstream.defined() && upstream.requires_grad()) inputs.push_back(torch::autograd::impl::gradient_edge(upstream));
+  if (std::none_of(inputs.begin(), inputs.end(), [](const Edge& e) { return e.is_valid(); })) return;
+  const auto node = std::make_shared<torch::autograd::Error>(std::string(who) + ": second derivatives are not implemented", std::move(inputs));
+  at::AutoDispatchBelowADInplaceOrView below;
+  for (Tensor& t : results)
+    if (t.defined()) {
+      t = t.detach();   // (no view of another gradient)
+      torch::autograd::set_history(t, node);
+    }
 }
 
 // What the core's backward needs of its forward.  Unpacking may run a user's hooks (checkpointing runs the whole forward

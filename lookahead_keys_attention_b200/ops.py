@@ -110,6 +110,7 @@ class _TracedCall(torch.autograd.Function):
         with torch.enable_grad():
             leaves = [t.detach().requires_grad_(t.requires_grad) if isinstance(t, torch.Tensor) else t for t in inputs]
             out = call(*leaves)
+            ctx.anchors = _anchors(inputs)
         ctx.graph = leaves, out
         return out.detach()
 
@@ -117,8 +118,23 @@ class _TracedCall(torch.autograd.Function):
     def backward(ctx, grad):
         leaves, out = ctx.graph
         wanted = [t for t in leaves if isinstance(t, torch.Tensor) and t.requires_grad]
-        grads = iter(torch.autograd.grad(out, wanted, grad, retain_graph=True))
+        grads = iter(_refuse_second(torch.autograd.grad(out, wanted, grad, retain_graph=True), (grad, *ctx.anchors)))
         return (None, *(next(grads) if isinstance(t, torch.Tensor) and t.requires_grad else None for t in leaves))
+
+
+def _anchors(inputs):
+    """Nothing of each differentiable input, by which its place in the graph can be kept."""
+    return [t.narrow(0, 0, 0) for t in inputs if isinstance(t, torch.Tensor) and t.requires_grad]
+
+
+def _refuse_second(grads, inputs):
+    """The gradients that a traced operator's own graph gave, under create_graph behind a node that refuses second derivatives
+    (what `refuse_second` of csrc/host.cpp does for the native nodes)."""
+    inputs = [t for t in inputs if t.requires_grad]
+    if not torch.is_grad_enabled() or not inputs:
+        return grads
+    refuse = torch._C._functions.DelayedError("castle: second derivatives are not implemented", len(grads) + len(inputs))
+    return refuse(*(g.detach() for g in grads), *inputs)[:len(grads)]
 
 
 def castle_attention_packed(packed, scale, return_U_for_cache=False, cache_out=None):
