@@ -448,9 +448,10 @@ Tensor restored_contiguous(const Tensor& t, at::IntArrayRef sizes, at::ScalarTyp
 
 // The nodes compute gradients below autograd.  With create_graph they would come back as constants, and what a penalty on them adds to the
 // gradients would silently be missing; so they get a node that refuses to be differentiated, behind all that they depend on: the upstream
-// gradient and what `inputs` lead to.
-void refuse_second(variable_list& results, const char* who, const Tensor& upstream, edge_list inputs) {
+// gradient and the first `count` inputs.
+void refuse_second(variable_list& results, const char* who, const Tensor& upstream, const Node& node_of, size_t count) {
   if (!at::GradMode::is_enabled()) return;
+  edge_list inputs(node_of.next_edges().begin(), node_of.next_edges().begin() + count);
   if (upstream.defined() && upstream.requires_grad()) inputs.push_back(torch::autograd::impl::gradient_edge(upstream));
   if (std::none_of(inputs.begin(), inputs.end(), [](const Edge& e) { return e.is_valid(); })) return;
   const auto node = std::make_shared<torch::autograd::Error>(std::string(who) + ": second derivatives are not implemented", std::move(inputs));
@@ -530,13 +531,16 @@ struct CastleBackward : public Node {
     variable_list result(packed ? 1 : 6);
     if (grads.empty() || !grads[0].defined()) return result;
     const SavedCore::Unpacked saved = core.unpack(shared_from_this());
-    at::NoGradGuard no_grad;
-    Tensor g = core.backward(saved, grads[0]);
-    if (packed) {
-      result[0] = std::move(g);
-    } else {
-      for (int i = 0; i < 6; ++i) result[i] = g.select(2, kPackedOrder[i]).permute({0, 2, 1, 3});
+    {
+      at::NoGradGuard no_grad;
+      Tensor g = core.backward(saved, grads[0]);
+      if (packed) {
+        result[0] = std::move(g);
+      } else {
+        for (int i = 0; i < 6; ++i) result[i] = g.select(2, kPackedOrder[i]).permute({0, 2, 1, 3});
+      }
     }
+    refuse_second(result, "castle_attention", grads[0], *this, num_outputs());
     return result;
   }
 };
@@ -752,6 +756,11 @@ struct LayerBackward : public Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list result(has_bias ? 5 : has_norm ? 4 : 3);
     if (grads.empty() || !grads[0].defined()) return result;
+    gradients(grads, result);
+    refuse_second(result, "Castle", grads[0], *this, num_outputs());
+    return result;
+  }
+  void gradients(const variable_list& grads, variable_list& result) {
     const bool need_x = task_should_compute_output(0), need_qkv = task_should_compute_output(1), need_combine = task_should_compute_output(2),
                need_weight = has_norm && task_should_compute_output(3), need_bias = has_bias && task_should_compute_output(4),
                need_norm = need_weight || need_bias;
@@ -777,15 +786,15 @@ struct LayerBackward : public Node {
     const Tensor g = grads[0].reshape({rows, grads[0].size(-1)});
     if (need_combine)
       result[2] = product(2, g, separate_merged ? ms : restored(saved.out16, {p.B, p.H, p.N, p.dp}, p.cdtype, dev).permute({0, 2, 1, 3}).reshape({rows, inner}), rows);
-    if (!need_core) return result;
+    if (!need_core) return;
     const Tensor dcore = product(1, g, wc, rows).view({p.B, p.N, p.H, p.d}).permute({0, 2, 1, 3});
     const Tensor dqkv = core.backward(saved, dcore).view({rows, 6 * inner});
     if (need_qkv) result[1] = product(2, dqkv, separate_h ? hs : xs.reshape({rows, dim}), rows);
-    if (!(need_x || need_norm)) return result;
+    if (!(need_x || need_norm)) return;
     Tensor dh = product(1, dqkv, wq, rows);
     if (!has_norm) {
       result[0] = dh.view(x_sizes);
-      return result;
+      return;
     }
     const Tensor xc = aligned_contiguous(xs), wn = restored_contiguous(ws_norm, {dim}, dtype, dev),
                  rs = layer_norm ? restored_contiguous(rs_norm, {rows, 2}, at::kFloat, dev) : restored_contiguous(rs_norm, {rows}, at::kFloat, dev);
@@ -794,7 +803,7 @@ struct LayerBackward : public Node {
     if (layer_norm) {
       if (need_bias) result[4] = at::empty({dim}, dh.options());
       launch_layernorm_bwd(as_rows(dh, rows, dim), as_rows(xc, rows, dim), dtype, wn, rs, result[0], result[3], has_bias ? result[4] : Tensor(), stream);
-      return result;
+      return;
     }
     const size_t bytes = api.rmsnorm_bwd_workspace_bytes(rows, (int32_t)dim);
     StreamUse use(stream);
@@ -802,7 +811,6 @@ struct LayerBackward : public Node {
     check(api.rmsnorm_bwd(dtype_code(dtype), rows, (int32_t)dim, dh.data_ptr(), xc.data_ptr(), wn.data_ptr(), rs.data_ptr<float>(),
                           need_x ? result[0].data_ptr() : nullptr, need_weight ? result[3].data_ptr() : nullptr, ws.data_ptr(), ws.numel(),
                           stream.stream()), "castle_rmsnorm_bwd");
-    return result;
   }
 };
 

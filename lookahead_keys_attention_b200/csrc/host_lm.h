@@ -83,7 +83,7 @@ struct EmbeddingBackward : public Node {
                             (float)scale, dw.data_ptr(), ws.data_ptr(), ws.numel(), status.data_ptr<int32_t>(), stream.stream()),
           "castle_embedding_bwd");
     variable_list result{dw};
-    refuse_second(result, "castle_embedding", grads[0], {});   // (it does not depend on the table)
+    refuse_second(result, "castle_embedding", grads[0], *this, 0);   // (it does not depend on the table)
     return result;
   }
 };
@@ -173,7 +173,7 @@ struct LayerNormBackward : public Node {   // of x, weight, bias
     const Tensor w = has_weight ? as_plain(restored(ws, {dim}, dtype, dev)) : Tensor();
     launch_layernorm_bwd(as_rows(grads[0], rows, dim), restored_rows(xs, sizes, dtype, dev, rows, dim), dtype, w,
                          restored_contiguous(ss, {rows, 2}, at::kFloat, dev), result[0], result[1], result[2], c10::cuda::getCurrentCUDAStream(dev.index()));
-    refuse_second(result, "castle_layer_norm", grads[0], {next_edge(0), next_edge(1)});
+    refuse_second(result, "castle_layer_norm", grads[0], *this, 2);
     return result;
   }
 };
@@ -262,7 +262,7 @@ struct LinearCrossEntropyBackward : public Node {   // of x, weight
                             reduction, l.data_ptr<float>(), g.data_ptr<float>(), result[0].defined() ? result[0].data_ptr() : nullptr,
                             result[1].defined() ? result[1].data_ptr() : nullptr, scratch.data_ptr(), scratch.numel(), status.data_ptr<int32_t>(), stream.stream()),
           "castle_linear_ce_bwd");
-    refuse_second(result, who, grads[0], {next_edge(0), next_edge(1)});
+    refuse_second(result, who, grads[0], *this, 2);
     return result;
   }
 };

@@ -88,6 +88,7 @@ class _Traced(torch.autograd.Function):
             limits = (scale, return_U, None, MAX_WORKSPACE_BYTES, LONG_SEQ_FP16)
             host = _lib.host()
             result = host.attention_packed(*leaves, *limits, None, True) if packed_op else host.attention(*leaves, *limits)
+            ctx.anchors = _anchors(inputs)
         out, *U = result if return_U else (result,)
         ctx.graph = leaves, out
         if return_U:
@@ -98,7 +99,7 @@ class _Traced(torch.autograd.Function):
     def backward(ctx, grad, *_):
         leaves, out = ctx.graph
         wanted = [t for t in leaves if t.requires_grad]
-        grads = iter(torch.autograd.grad(out, wanted, grad, retain_graph=True))
+        grads = iter(_refuse_second(torch.autograd.grad(out, wanted, grad, retain_graph=True), (grad, *ctx.anchors)))
         return (None, None, None, *(next(grads) if t.requires_grad else None for t in leaves))
 
 

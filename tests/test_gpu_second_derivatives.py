@@ -3,7 +3,7 @@ silently lose its share of the operator's inputs.  First derivatives under creat
 import pytest
 import torch
 
-from lookahead_keys_attention_b200 import castle_embedding, castle_layer_norm, castle_linear_cross_entropy
+from lookahead_keys_attention_b200 import Castle, castle_attention, castle_attention_packed, castle_embedding, castle_layer_norm, castle_linear_cross_entropy
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,36 @@ def test_a_traced_operator_refuses_them_too():
     assert torch.equal(dx, torch.autograd.grad(castle_linear_cross_entropy(x, w, t), [x])[0])
     with pytest.raises(RuntimeError, match="second derivatives"):
         ((dx ** 2).sum() + w.sum()).backward()
+
+
+def test_attention_refuses_them():
+    six = [leaf(2, 2, 40, 64, seed=i) for i in range(6)]
+    packed = leaf(2, 40, 6, 2, 64)
+    for op, leaves in ((lambda *v: castle_attention(*v, 0.125), six), (lambda v: castle_attention_packed(v, 0.125), [packed])):
+        for up in (1.0, leaf(1, seed=9)):
+            def make():
+                out = op(*leaves)
+                return out, torch.ones_like(out) * up
+            refused(make, leaves, "castle_attention")
+
+
+@pytest.mark.parametrize("prenorm", [False, True, "layer"])
+def test_a_layer_refuses_them(prenorm):
+    torch.manual_seed(0)
+    m = Castle(64, heads=2, dim_head=64, prenorm=prenorm).cuda()
+    x = leaf(2, 40, 64)
+    def make():
+        out = m(x)
+        return out, torch.ones_like(out)
+    refused(make, [x, *m.parameters()], "Castle")
+    for p in m.parameters():                                     # one that learns is enough: another's gradient depends on it
+        p.requires_grad_(False)
+    refused(make, [x], "Castle")
+    handle = m.combine_heads.register_forward_hook(lambda *a: None)   # the submodules as modules, around the core's own node
+    (g,) = torch.autograd.grad(m(x).sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError, match="castle_attention: second derivatives"):
+        ((g ** 2).sum() + x.sum()).backward()
+    handle.remove()
+    out = m(x)
+    (g,) = torch.autograd.grad(out, [x], torch.ones_like(out))   # without create_graph nothing is added
+    assert not g.requires_grad
