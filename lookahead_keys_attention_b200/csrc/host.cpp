@@ -436,13 +436,13 @@ Tensor run_backward(const Problem& p, const castle_tensor_t* in, const Tensor& o
 
 // A tensor that went through saved-tensor hooks: whatever they gave back must be the tensor that was saved, since the
 // kernels get its address.  Its strides may be others (save_on_cpu gives contiguous ones).
-Tensor restored(const Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype, const at::Device& dev) {
+Tensor restored(const Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype, const at::Device& dev, const char* who = "castle_attention") {
   if (!t.defined() || t.sizes() != sizes || t.scalar_type() != dtype || t.device() != dev || t.layout() != at::kStrided)
-    throw std::runtime_error("castle_attention: a saved tensor came back from its hooks with another shape, type or device");
+    throw std::runtime_error(std::string(who) + ": a saved tensor came back from its hooks with another shape, type or device");
   return t;
 }
-Tensor restored_contiguous(const Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype, const at::Device& dev) {
-  restored(t, sizes, dtype, dev);
+Tensor restored_contiguous(const Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype, const at::Device& dev, const char* who = "castle_attention") {
+  restored(t, sizes, dtype, dev, who);
   return aligned_contiguous(t);
 }
 

@@ -43,8 +43,8 @@ void need_gradient(const Tensor& g, at::IntArrayRef sizes, at::ScalarType type, 
   if (g.sizes() != sizes || g.scalar_type() != type || g.device() != dev || !own_memory(g))
     throw std::runtime_error(std::string(who) + ": the gradient's shape, type or device is not the output's");
 }
-Rows restored_rows(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev, int64_t rows, int64_t dim) {
-  return as_rows(restored(t, sizes, type, dev), rows, dim);
+Rows restored_rows(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev, int64_t rows, int64_t dim, const char* who) {
+  return as_rows(restored(t, sizes, type, dev, who), rows, dim);
 }
 
 // ------------------------------------------------------------------------------------------------ token lookup
@@ -62,17 +62,18 @@ struct EmbeddingBackward : public Node {
   }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
+    const char* who = "castle_embedding";
     if (grads.empty() || !grads[0].defined()) return {Tensor()};
     const Tensor saved = tokens.unpack();
     at::AutoDispatchBelowADInplaceOrView below;
     const at::Device dev = grads[0].device();
     const c10::cuda::CUDAGuard guard(dev);
     const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
-    const Tensor t = restored(saved, token_sizes, token_type, dev).contiguous();
+    const Tensor t = restored(saved, token_sizes, token_type, dev, who).contiguous();
     const int64_t n = t.numel();
     std::vector<int64_t> out_sizes = token_sizes;
     out_sizes.push_back(dim);
-    need_gradient(grads[0], out_sizes, dtype, dev, "castle_embedding");
+    need_gradient(grads[0], out_sizes, dtype, dev, who);
     const auto options = at::TensorOptions().dtype(dtype).device(dev);
     if (n == 0) return {at::zeros({vocab, dim}, options)};
     const Rows g = as_rows(grads[0], n, dim);
@@ -83,7 +84,7 @@ struct EmbeddingBackward : public Node {
                             (float)scale, dw.data_ptr(), ws.data_ptr(), ws.numel(), status.data_ptr<int32_t>(), stream.stream()),
           "castle_embedding_bwd");
     variable_list result{dw};
-    refuse_second(result, "castle_embedding", grads[0], *this, 0);   // (it does not depend on the table)
+    refuse_second(result, who, grads[0], *this, 0);   // (it does not depend on the table)
     return result;
   }
 };
@@ -156,6 +157,7 @@ struct LayerNormBackward : public Node {   // of x, weight, bias
   }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
+    const char* who = "castle_layer_norm";
     variable_list result(3);
     if (grads.empty() || !grads[0].defined()) return result;
     const Tensor xs = x.unpack(), ws = has_weight ? weight.unpack() : Tensor(), ss = stats.unpack();
@@ -163,17 +165,17 @@ struct LayerNormBackward : public Node {   // of x, weight, bias
     const at::Device dev = grads[0].device();
     const c10::cuda::CUDAGuard guard(dev);
     const int64_t dim = sizes.back();
-    need_gradient(grads[0], sizes, dtype, dev, "castle_layer_norm");
+    need_gradient(grads[0], sizes, dtype, dev, who);
     const int64_t rows = grads[0].numel() / dim;
     const auto options = at::TensorOptions().dtype(dtype).device(dev);
     for (int i = 0; i < 3; ++i)
       if (task_should_compute_output(i)) result[i] = rows == 0 ? (i == 0 ? at::empty(sizes, options) : at::zeros({dim}, options))
                                                               : i == 0 ? at::empty(sizes, options) : at::empty({dim}, options);
     if (rows == 0 || !(result[0].defined() || result[1].defined() || result[2].defined())) return result;
-    const Tensor w = has_weight ? as_plain(restored(ws, {dim}, dtype, dev)) : Tensor();
-    launch_layernorm_bwd(as_rows(grads[0], rows, dim), restored_rows(xs, sizes, dtype, dev, rows, dim), dtype, w,
-                         restored_contiguous(ss, {rows, 2}, at::kFloat, dev), result[0], result[1], result[2], c10::cuda::getCurrentCUDAStream(dev.index()));
-    refuse_second(result, "castle_layer_norm", grads[0], *this, 2);
+    const Tensor w = has_weight ? as_plain(restored(ws, {dim}, dtype, dev, who)) : Tensor();
+    launch_layernorm_bwd(as_rows(grads[0], rows, dim), restored_rows(xs, sizes, dtype, dev, rows, dim, who), dtype, w,
+                         restored_contiguous(ss, {rows, 2}, at::kFloat, dev, who), result[0], result[1], result[2], c10::cuda::getCurrentCUDAStream(dev.index()));
+    refuse_second(result, who, grads[0], *this, 2);
     return result;
   }
 };
@@ -253,8 +255,8 @@ struct LinearCrossEntropyBackward : public Node {   // of x, weight
     }
     if (task_should_compute_output(0)) result[0] = at::empty(x_sizes, options);
     if (task_should_compute_output(1)) result[1] = at::empty({vocab, dim}, options);
-    const Rows xr = restored_rows(xs, x_sizes, dtype, dev, rows, dim), w = restored_rows(ws, {vocab, dim}, dtype, dev, vocab, dim);
-    const Tensor t = as_long(restored(ts, target_sizes, target_type, dev)), l = restored_contiguous(ls, {rows}, at::kFloat, dev), g = as_plain(grads[0]),
+    const Rows xr = restored_rows(xs, x_sizes, dtype, dev, rows, dim, who), w = restored_rows(ws, {vocab, dim}, dtype, dev, vocab, dim, who);
+    const Tensor t = as_long(restored(ts, target_sizes, target_type, dev, who)), l = restored_contiguous(ls, {rows}, at::kFloat, dev, who), g = as_plain(grads[0]),
                  status = status_word(dev.index());
     StreamUse use(stream);
     const Tensor scratch = use.scratch(api.linear_ce_workspace_bytes(dtype_code(dtype), rows, (int32_t)dim, vocab, 1));

@@ -232,6 +232,16 @@ def test_hooks_that_change_a_saved_tensor_are_refused():
             out.backward()
 
 
+def test_a_refused_saved_tensor_names_its_operator():
+    x, w, t = torch.randn(20, 64, device="cuda", requires_grad=True), torch.randn(30, 64, device="cuda", requires_grad=True), torch.arange(20, device="cuda")
+    for name, call in (("castle_layer_norm", lambda: castle_layer_norm(x, w[0]).sum()), ("castle_linear_cross_entropy", lambda: castle_linear_cross_entropy(x, w, t)),
+                       ("castle_embedding", lambda: castle_embedding(t, w).sum())):
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s, lambda s: s[:-1] if s.dim() else s):
+            out = call()
+        with pytest.raises(RuntimeError, match=name + ": a saved tensor came back"):
+            out.backward()
+
+
 def test_a_traced_forward():
     w = torch.randn(40, 64, device="cuda", requires_grad=True)
     def f(tokens, table):
