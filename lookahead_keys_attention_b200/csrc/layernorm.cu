@@ -420,15 +420,15 @@ static int ln_parts(int64_t rows, int dim) {
   return (int)(have < most ? have : most);
 }
 
-// f(THREADS, NV) with the group that holds a row of `dim` columns, 8 NV elements a thread.
-template <typename F> static cudaError_t ln_group(int dim, F&& f) {
+// f(THREADS, NV) with the group that holds a row of `dim` columns, 8 NV elements a thread; rows beyond 4096 columns have WIDE threads of 8 WIDE_NV elements.
+template <int WIDE, int WIDE_NV, typename F> static cudaError_t ln_group(int dim, F&& f) {
   using std::integral_constant;
   if (dim <= 256) return f(integral_constant<int, 32>(), integral_constant<int, 1>());
   if (dim <= 512) return f(integral_constant<int, 32>(), integral_constant<int, 2>());
   if (dim <= 1024) return f(integral_constant<int, 64>(), integral_constant<int, 2>());
   if (dim <= 2048) return f(integral_constant<int, 128>(), integral_constant<int, 2>());
   if (dim <= 4096) return f(integral_constant<int, 256>(), integral_constant<int, 2>());
-  return f(integral_constant<int, 512>(), integral_constant<int, 2>());
+  return f(integral_constant<int, WIDE>(), integral_constant<int, WIDE_NV>());
 }
 template <typename K, typename... A> static cudaError_t ln_launch(K kernel, int64_t grid, int threads, size_t ring, cudaStream_t st, A... args) {
   if (ring > 16384) {   // (beside up to 17 KB of the kernel's own)
@@ -445,14 +445,12 @@ static cudaError_t ln_fwd(int64_t rows, int dim, const T* x, int64_t stride, con
     castle_layernorm_fwd_wide_kernel<T, VEC><<<(unsigned)rows, kLnThreads, 0, st>>>(x, stride, w, b, eps, y, stats, dim);
     return cudaGetLastError();
   }
-  auto go = [&](auto threads, auto nv) {
+  return ln_group<256, 4>(dim, [&](auto threads, auto nv) {
     constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value, G = kLnBlock<TH> / TH;
     const int64_t have = (rows + G - 1) / G, most = 148 * kLnFwdBlocks<NV>;
     return ln_launch(castle_layernorm_fwd_kernel<T, VEC, TH, NV>, have < most ? have : most, kLnBlock<TH>, LnRows<T, VEC, TH, NV, 1>::kBytes, st, x, stride, w, b, eps, y,
                      stats, rows, dim);
-  };
-  using std::integral_constant;
-  return dim > 4096 ? go(integral_constant<int, 256>(), integral_constant<int, 4>()) : ln_group(dim, go);
+  });
 }
 
 template <typename T, bool VEC>
@@ -461,7 +459,7 @@ static cudaError_t ln_bwd(int64_t rows, int dim, const T* dy, int64_t dy_stride,
   const int parts = ln_parts(rows, dim);
   const bool params = dw || db;
   if (dx && dim <= kLnWhole) {
-    const cudaError_t e = ln_group(dim, [&](auto threads, auto nv) {
+    const cudaError_t e = ln_group<512, 2>(dim, [&](auto threads, auto nv) {
       constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value;
       return ln_launch(castle_layernorm_bwd_kernel<T, VEC, TH, NV>, parts, kLnBlock<TH>, LnRows<T, VEC, TH, NV, 2>::kBytes, st, dy, dy_stride, x, stride, w, stats, dx,
                        params ? ws : (float*)nullptr, rows, dim);

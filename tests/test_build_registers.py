@@ -1,4 +1,7 @@
 """A build whose dim_head-64 score kernel does not start with the registers that it shares out anew fails, and leaves the library as it was."""
+import re
+import shutil
+import subprocess
 import sys
 
 import pytest
@@ -35,3 +38,15 @@ def test_build_with_other_registers_fails(tmp_path, used, wrong):
         _lib._compile([(target, stamp, "digest", compiler)])
         assert target.read_text() == "new" and stamp.read_text() == "digest\n"
     assert [p.name for p in tmp_path.iterdir() if ".tmp." in p.name] == []
+
+
+@pytest.mark.skipif(shutil.which("nm") is None, reason="needs nm")
+def test_layer_norm_has_the_kernels_that_calls_reach_and_no_others():
+    """Threads and elements of a thread by the row's width: rows beyond 4096 columns have 256 threads of 32 elements forward, 512 of 16 backward."""
+    _lib.build()
+    names = subprocess.run(["nm", str(_lib.LIB_PATH)], capture_output=True, text=True, check=True).stdout
+    narrow = {(32, 1), (32, 2), (64, 2), (128, 2), (256, 2)}
+    for kernel, wide in (("fwd", (256, 4)), ("bwd", (512, 2))):
+        forms = re.findall(r"\w*castle_layernorm_" + kernel + r"_kernelI(\w+?)Lb([01])ELi(\d+)ELi(\d+)E", names)
+        by_type = {(t, v): {(int(a), int(b)) for s, w, a, b in forms if (s, w) == (t, v)} for t, v, _, _ in forms}
+        assert len(by_type) == 6 and all(found == narrow | {wide} for found in by_type.values()), by_type
