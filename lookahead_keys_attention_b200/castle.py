@@ -108,6 +108,8 @@ class Castle(nn.Module):
         self.scale = dim_head ** -0.5
         # prenorm: RMSNorm as in the reference, or "layer" for a layer norm.  (A layer norm that the caller puts in the place of
         # another norm is called as a module.)
+        if isinstance(prenorm, str) and prenorm != "layer":   # (any other true value is an RMSNorm)
+            raise ValueError(f'Castle: prenorm must be False, True (an RMSNorm) or "layer" (a layer norm), not {prenorm!r}')
         self._layer_norm = prenorm == "layer"
         self.norm = nn.LayerNorm(dim) if self._layer_norm else nn.RMSNorm(dim) if prenorm else nn.Identity()
         self.rotary_emb = _Rotary(dim_head) if rotary_emb else None

@@ -103,3 +103,13 @@ def test_reduction_names():
         castle_linear_cross_entropy(torch.zeros(2, 8), torch.zeros(3, 8), torch.zeros(2, dtype=torch.int64), reduction="avg")
     with pytest.raises(RuntimeError, match="no CPU path"):
         castle_linear_cross_entropy(torch.zeros(2, 8), torch.zeros(3, 8), torch.zeros(2, dtype=torch.int64))
+
+
+def test_prenorm_names():
+    from lookahead_keys_attention_b200 import Castle
+    for name in ("layernorm", "Layer", "rms", ""):          # not an RMSNorm, as any true value would give
+        with pytest.raises(ValueError, match="prenorm"):
+            Castle(16, heads=1, dim_head=16, prenorm=name)
+    for value, norm in ((False, torch.nn.Identity), (None, torch.nn.Identity), (0, torch.nn.Identity), (True, torch.nn.RMSNorm), (1, torch.nn.RMSNorm),
+                        ("layer", torch.nn.LayerNorm)):
+        assert type(Castle(16, heads=1, dim_head=16, prenorm=value).norm) is norm
