@@ -2,7 +2,7 @@
 // with its autograd node.  Part of host.cpp (inside its namespace, behind what it shares with the other operators).
 //
 // What the kernels take by address is checked here: device, type and shape; tensors whose last dimension is not contiguous, or
-// whose negation is still to be done, are copied first.  Nodes compute in the type of their inputs, under autocast too.
+// whose negation is still to be done, are copied first.  Operators and nodes compute in the type of their rows, under autocast too.
 
 // (..., dim) as rows that are `stride` elements apart.  A contiguous tensor is taken as it is: views made by the dispatcher cost as much as
 // a launch's half, and a token's norm or lookup is little more than its launch.
@@ -42,6 +42,14 @@ void need_dim(int64_t dim, const char* who) {   // the C ABI takes a row's lengt
 void need_gradient(const Tensor& g, at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev, const char* who) {
   if (g.sizes() != sizes || g.scalar_type() != type || g.device() != dev || !own_memory(g))
     throw std::runtime_error(std::string(who) + ": the gradient's shape, type or device is not the output's");
+}
+// Under autocast a layer gives rows of its type beside parameters of theirs: these are cast to the rows' type, as autocast casts a projection's
+// weight (their gradients come back in their own type).  Elsewhere other types are refused.
+Tensor in_type_of(const Tensor& x, const Tensor& t) {
+  return t.defined() && t.scalar_type() != x.scalar_type() && t.is_cuda() && own_memory(t) && dtype_code(t.scalar_type()) >= 0 && dtype_code(x.scalar_type()) >= 0 &&
+                 at::autocast::is_autocast_enabled(at::kCUDA)
+             ? t.to(x.scalar_type())
+             : t;
 }
 Rows restored_rows(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev, int64_t rows, int64_t dim, const char* who) {
   return as_rows(restored(t, sizes, type, dev, who), rows, dim);
@@ -180,8 +188,9 @@ struct LayerNormBackward : public Node {   // of x, weight, bias
   }
 };
 
-Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
+Tensor layer_norm(const Tensor& x, const Tensor& own_weight, const Tensor& own_bias, double eps) {
   const char* who = "castle_layer_norm";
+  const Tensor weight = in_type_of(x, own_weight), bias = in_type_of(x, own_bias);
   need_plain(x, who);
   need_type(x, who);
   need(x.dim() >= 1 && x.size(-1) > 0, "castle_layer_norm: (..., dim) rows expected");
@@ -269,8 +278,9 @@ struct LinearCrossEntropyBackward : public Node {   // of x, weight
   }
 };
 
-Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& targets, int64_t ignore, int reduction) {
+Tensor linear_cross_entropy(const Tensor& x, const Tensor& own_weight, const Tensor& targets, int64_t ignore, int reduction) {
   const char* who = "castle_linear_cross_entropy";
+  const Tensor weight = in_type_of(x, own_weight);
   for (const Tensor* t : {&x, &weight, &targets}) need_plain(*t, who);
   need_type(x, who);
   need(x.dim() >= 1 && x.size(-1) > 0 && weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) == x.size(-1),

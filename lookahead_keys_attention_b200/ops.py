@@ -186,7 +186,8 @@ def castle_embedding(tokens, weight, scale: float = 1.0, padding_idx: int | None
 
 def castle_layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """Layer norm over the last dimension of `x` (any size), with an optional weight and bias of its type: mean, variance and
-    all sums in fp32, one rounding.  `Castle(..., prenorm="layer")` has it in front of the layer."""
+    all sums in fp32, one rounding.  Under autocast weight and bias may have another type than `x` and are cast to its.
+    `Castle(..., prenorm="layer")` has it in front of the layer."""
     if torch._C._is_tracing():
         return _TracedCall.apply(lambda *t: _lib.host().layer_norm(*t, eps), x, weight, bias)
     return _lib.host().layer_norm(x, weight, bias, eps)
@@ -198,7 +199,7 @@ _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}   # CASTLE_REDUCE_* of the C ABI
 def castle_linear_cross_entropy(x, weight, targets, ignore_index: int = -100, reduction: str = "mean"):
     """Cross entropy of the logits `x @ weight.T` against `targets`, without the logits in memory: the head and the loss of a
     language model around these layers (the reference's training script, train_triton.py:73-175).  x (..., dim) and weight
-    (vocabulary, dim) of one type, targets (...) int64 or int32; the loss is fp32, logits and sums are, too.  Rows whose target is
+    (vocabulary, dim) of one type (under autocast weight is cast to x's), targets (...) int64 or int32; the loss is fp32, logits and sums are, too.  Rows whose target is
     `ignore_index` take no part, whatever x holds there, and cost nothing; `reduction`: the mean of the others (NaN if there are
     none, with gradients of zero), their "sum", or "none" for each row's loss (0 where ignored).  The gradients of x and weight are formed in the backward
     pass, from logits formed again, and are the same from call to call.  A target outside the vocabulary gives NaN, and `check_status()` raises."""

@@ -287,6 +287,35 @@ def test_under_autocast_and_inference_mode():
     assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, also))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_a_layers_rows_beside_parameters_of_32_bits_under_autocast(dtype):
+    """Parameters are cast to the rows' type: bit for bit what a caller's own casts give, with gradients in the parameters' type.  Outside of autocast
+    mixed types stay refused."""
+    torch.manual_seed(0)
+    layer, norm, table = Castle(64, heads=2, dim_head=32).cuda(), torch.nn.LayerNorm(64).cuda(), torch.randn(300, 64, device="cuda", requires_grad=True)
+    torch.nn.init.normal_(norm.weight)
+    x, t = torch.randn(2, 50, 64, device="cuda"), torch.randint(0, 300, (2, 50), device="cuda")
+    leaves = [norm.weight, norm.bias, table]
+    def loss(cast):
+        h = castle_layer_norm(layer(x), cast(norm.weight), cast(norm.bias), norm.eps)
+        assert h.dtype == dtype
+        return castle_linear_cross_entropy(h, cast(table), t)
+    with torch.autocast("cuda", dtype=dtype):
+        got, want = loss(lambda p: p), loss(lambda p: p.to(dtype))
+    assert torch.equal(got, want)
+    for a, b, p in zip(torch.autograd.grad(got * 64, leaves), torch.autograd.grad(want * 64, leaves), leaves):
+        assert a.dtype == p.dtype == torch.float32 and torch.equal(a, b) and bool(a.any())
+    with torch.autocast("cuda", dtype=dtype):
+        assert castle_layer_norm(x, norm.weight.to(dtype)).dtype == torch.float32      # rows of 32 bits stay so
+        with pytest.raises(RuntimeError, match="castle_layer_norm"):
+            castle_layer_norm(x, norm.weight.double())
+    h = x.to(dtype)
+    for call in (lambda: castle_layer_norm(h, norm.weight), lambda: castle_layer_norm(h, None, norm.bias), lambda: castle_linear_cross_entropy(h, table, t)):
+        with pytest.raises(RuntimeError, match="type"):
+            call()
+    check_status()
+
+
 def test_offsets_beyond_32_bits():
     """Elements behind the 2^31st of the table, of the rows and of the weight, against the same values in small tensors."""
     if torch.cuda.get_device_properties(0).total_memory < 60e9:
