@@ -35,7 +35,7 @@
 // the working warps keep in registers.  The logits formed again are the same sums, bit for bit, as those behind the log-sum-exp: summed in one go,
 // they made a row's probabilities add up to 1 + 1e-3 (logits of some 60 over 4096 to 8192, fp16), more than what a learnt row has to move by.
 //
-// G in 16 bits is taken in units of a power of two (the largest c_i's) with 2^14 on top, so that fp16 keeps probabilities down to 2^-28 in full
+// G in 16 bits is taken in units of a power of two (the largest c_i's), in fp16 with 2^14 on top, so that it keeps probabilities down to 2^-28 in full
 // precision; the unit is multiplied back in fp32 at the end.  Where all rows have one coefficient (mean, sum) that is the unit and none
 // of it is in G: -1 for a target that has no probability is exact, where c would be off by the same half step in every row (1789 rows
 // against 132536, bf16: gradients 3.2e-3 off in their norm, 1.7e-3 by rounding the result).  A row's largest entry by far is
@@ -75,7 +75,9 @@ constexpr int64_t kCeScratch = (int64_t)1 << 30;   // bytes that a piece of the 
 // 197 x 512 in fp32 are 6.7e-8 of their norm off (emptied every second step 3.0e-7, and 8 % faster); not emptied 3.3e-6 and, of logits over 1024 in 16 bits, 8 % faster (166 us, 152).
 // (G's logits, too: 8192 x 4096 against 131072, forward and gradients, 28.2 ms for 27.5 without; 4096 x 1024 against 50021 1.49 ms for 1.45.)
 constexpr int kCeFlush = 8, kCeFlushF32 = 1, kCeNoFlush = 1 << 30;
-constexpr float kCeUnit = 16384.f;                 // of G: below 2 units
+// What G's largest entries (below 2 units) are raised by.  The exponents of the other types reach, and products with rows near their largest number
+// must not be 2^14 times as large.
+template <typename OUT> constexpr float kCeUnit = std::is_same<OUT, __half>::value ? 16384.f : 1.f;
 
 struct CeHead {          // at the start of the workspace, written by castle_ce_rows_kernel
   int rows;              // that take part
@@ -111,11 +113,13 @@ template <typename T> struct CePlanes {
   using Op = T;
   static __device__ __forceinline__ void split(float v, float* p) { p[0] = v; }
 };
+constexpr float kCeMostBf16 = 3.38953139e38f;   // (2 - 2^-7) 2^127
 template <> struct CePlanes<float> {
   static constexpr int count = 3;
   using Op = __nv_bfloat16;
   static __device__ __forceinline__ void split(float v, float* p) {
     p[0] = __bfloat162float(__float2bfloat16_rn(v));
+    if (isinf(p[0]) && !isinf(v)) p[0] = copysignf(kCeMostBf16, v);   // a number beyond the largest bf16 one is that and a rest
     const float r = v - p[0];
     p[1] = isfinite(p[0]) ? __bfloat162float(__float2bfloat16_rn(r)) : 0.f;   // an infinity is its first part alone
     p[2] = isfinite(p[0]) ? r - p[1] : 0.f;
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(1024, 1) castle_ce_rows_kernel(const CeRowsPar
     h.gathered = gather || p.copy_always;
     h.bad = (int)(p.n - ignored) - all;
     h.done = 0;
-    h.unit = all > 0 ? (p.each ? unit : g_one) * (1.f / kCeUnit) : 0.f;   // (the mean over no rows is not a number, its gradients are zero)
+    h.unit = all > 0 ? (p.each ? unit : g_one) * (1.f / kCeUnit<T>) : 0.f;   // (the mean over no rows is not a number, its gradients are zero)
     *p.head = h;
     if (h.bad) atomicOr(p.status, CASTLE_STATUS_BAD_INDEX);
   }
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(1024, 1) castle_ce_rows_kernel(const CeRowsPar
       r.target = (int)t;
       r.row = (int)i;
       r.lse = p.lse ? p.lse[i] : 0.f;
-      r.coef = p.each ? p.dloss[i] / unit * kCeUnit : kCeUnit;
+      r.coef = p.each ? p.dloss[i] / unit * kCeUnit<T> : kCeUnit<T>;
       p.rows[at] = r;
     } else if (i < r1 && p.lse_out) {
       const float none = skip ? 0.f : __int_as_float(0x7fffffff);

@@ -43,3 +43,37 @@ def test_learnt_rows_have_probabilities_that_add_up(n, dim, vocab, dtype):
     tol = 2.0 ** -21 + 300 * U + U * lse.abs() + h * (1 - p) + (vocab / 16 * (6 if dtype == torch.float32 else 1) + 64) * 2.0 ** -22 * 2 * (1 - p)
     off = dx[:, 1].double().abs()
     assert bool((off <= tol).all()), f"{off.max().item():.2e} beyond {tol.min().item():.2e}"
+
+
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_rows_of_the_types_lowest_value(dtype, sign):
+    """Finite numbers however large have finite parts: a row with the type's lowest value in it (or the largest) has logits of some 1e37 and the loss and
+    gradients that go with them, and the other rows keep theirs.  Losses: (32 + 8) additions of 2 u and the largest logit's rounding, 2^-18
+    at most; gradients of such a row: one weight's row less another's, or the row itself, off by the type's rounding h and, in fp32, 4 u."""
+    n, dim, vocab = 200, 64, 300
+    gen = torch.Generator("cuda").manual_seed(0)
+    x = torch.randn(n, dim, device="cuda", generator=gen).to(dtype)
+    w = (torch.randn(vocab, dim, device="cuda", generator=gen) * 0.1).to(dtype)
+    t = torch.randint(0, vocab, (n,), device="cuda", generator=gen)
+    far = torch.finfo(dtype).max * sign
+    def call(x):
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = castle_linear_cross_entropy(xl, wl, t, reduction="none")
+        return (loss.detach(), *torch.autograd.grad(loss, [xl, wl], torch.ones(n, device="cuda")))
+    loss0, dx0, dw0 = call(x)
+    x[7, 5] = far
+    loss, dx, dw = call(x)
+    check_status()
+    z = x[7].double() @ w.double().t()
+    want = z.amax() - z[t[7]]
+    assert want > 1e36 and abs(loss[7].double() - want) <= 2.0 ** -18 * want
+    others = [i for i in range(n) if i != 7]
+    assert torch.equal(loss[others], loss0[others]) and torch.equal(dx[others], dx0[others])
+    h = max(torch.finfo(dtype).eps / 2, 4 * U)
+    top = int(z.argmax())
+    row = w[top].double() - w[t[7]].double()
+    assert bool(((dx[7].double() - row).abs() <= 2 * h * row.abs() + 4 * U * w[t[7]].double().abs()).all())
+    assert bool(dw.isfinite().all())
+    for v, g in ((top, 1.0), (int(t[7]), -1.0)):
+        assert abs(dw[v, 5].double() - g * far) <= 2 * h * abs(far)
