@@ -94,3 +94,34 @@ def test_losses_of_16_bit_rows(n, dim, vocab, dtype):
     check_status()
     z = x.double() @ w.double().t()
     assert far(loss, z.logsumexp(1) - z[torch.arange(n, device="cuda"), t]) <= LOSS_16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_a_forward_of_16_bit_rows_in_pieces(dtype):
+    """65536 rows leave a forward's scratch for 262144 columns at a time: the second piece reads the weight where it lies from its own first row on, and joins the
+    first one's maxima, sums and target logits.  Targets on either side of the border and next to it; the logits of a sample of rows in 64 bits.  (Eight
+    products make a logit: off by 2 u of it, a loss by 2^-21 of an exponential, 300 u of their sum and 4 u of the log-sum-exp.)"""
+    from lookahead_keys_attention_b200 import castle_linear_cross_entropy, check_status
+    n, dim, vocab, border = 65536, 8, 300001, 262144
+    x, w, t = case(n, dim, vocab, dtype, "cuda")
+    t[:6] = torch.tensor([border - 1, border, 0, vocab - 1, border + 255, border - 256], device="cuda")
+    t[100:200] = -100
+    xl, wl = x.requires_grad_(), w.requires_grad_()
+    loss = castle_linear_cross_entropy(xl, wl, t, reduction="none")
+    mean = castle_linear_cross_entropy(x.detach(), w.detach(), t)
+    check_status()
+    rows = torch.cat([torch.arange(6), torch.arange(200, n, 331)]).cuda()
+    assert bool((t[rows] < border).any()) and bool((t[rows] >= border).any())
+    z = x[rows].double() @ w.double().t()
+    lse = z.logsumexp(1)
+    want = lse - z[torch.arange(len(rows), device="cuda"), t[rows]]
+    tol = 4 * U * z.abs().amax(1) + 2.0 ** -21 + 300 * U + 4 * U * lse.abs() + 2 * U * want.abs()
+    assert bool(((loss[rows].double() - want).abs() <= tol).all())
+    assert not bool(loss[100:200].any())
+    assert abs(mean.double() - loss.double().sum() / (n - 100)) <= 2 * U * mean
+    (dx,) = torch.autograd.grad(loss, [xl], torch.ones_like(loss))      # (37 pieces)
+    check_status()
+    p = z.softmax(1)
+    p[torch.arange(len(rows), device="cuda"), t[rows]] -= 1
+    assert far(dx[rows], p @ w.double()) <= torch.finfo(dtype).eps / 2
