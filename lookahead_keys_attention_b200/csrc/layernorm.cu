@@ -155,7 +155,8 @@ template <int THREADS, bool VEC, int NV> __device__ __forceinline__ void ln_clea
 }
 
 // Blocks of an SM.  Rows of more than 4096 columns: two of 256 threads with 32 elements each wait less for each other's sums than one of 512 with 16
-// (15063 rows of 8192 in bf16 78 us / 105, of 4824 62 / 97; 8000 of 5000 in fp32 82 / 98).
+// (15063 rows of 8192 in bf16 78 us / 105, of 4824 62 / 97; 8000 of 5000 in fp32 82 / 98).  The registers that this leaves hold all but 8 to 48 bytes a thread
+// where single elements are read, with 32 elements 124 to 140; of the backward's, two blocks as well, 56 to 60.
 template <int NV> constexpr int kLnFwdBlocks = NV > 2 ? 2 : 3;
 template <typename T, bool VEC, int THREADS, int NV>
 __global__ void __launch_bounds__(kLnBlock<THREADS>, kLnFwdBlocks<NV>) castle_layernorm_fwd_kernel(

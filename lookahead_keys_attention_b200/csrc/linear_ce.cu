@@ -19,9 +19,9 @@
 // Alone, an SM's shared memory brings in and reads 24 KB in the 128 cycles of a product of 16, more than it can (78 % of the tensor cores' cycles
 // at a contraction of 50021); a pair shares B's tile (92 %).  All sums, the logits and the statistics are fp32.
 //
-// What bounds it: at 8192 x 4096 against 131072 forward and backward take 25.2 to 26.5 ms by the box for 35.2 TFLOP, 1330 to 1400 TFLOP/s: the
+// What bounds it: at 8192 x 4096 against 131072 forward and backward take 26.1 to 28.5 ms by the box for 35.2 TFLOP, 1240 to 1350 TFLOP/s: the
 // power limit (the library's product, back to back, 1406 of measured), at clocks of 1.3 to 1.5 GHz.  8.8 of the 35.2 are the logits formed again.  Few
-// rows: the weight is read three times and dW written, 8 x 4096 against 131072 790 us of kernels for 4.3 GB.
+// rows: the weight is read three times and dW written, 8 x 4096 against 131072 798 us of kernels for 4.3 GB.
 //
 // dx and dW can have few tiles and long contractions.  As many tiles as go evenly to the workers are theirs whole; of the others the
 // contraction is cut into slices, whose sums go to scratch and are added, in order, by castle_ce_sum_kernel.
@@ -39,7 +39,8 @@
 // precision; the unit is multiplied back in fp32 at the end.  Where all rows have one coefficient (mean, sum) that is the unit and none
 // of it is in G: -1 for a target that has no probability is exact, where c would be off by the same half step in every row (1789 rows
 // against 132536, bf16: gradients 3.2e-3 off in their norm, 1.7e-3 by rounding the result).  A row's largest entry by far is
-// mostly its target's.  What rounding took from it is kept in fp32, and dx gets its product with the target's row of W.
+// mostly its target's.  What rounding took from it is kept in fp32, and dx gets its product with the target's row of W.  With a coefficient per row
+// fp16 has half steps of 2^-39 of the largest for all rows: one whose own is 2^20 times smaller has its probabilities to 2^-19 only.
 #include <type_traits>
 
 #include "common.cuh"
@@ -52,6 +53,7 @@ enum CeMode { kLse, kGrad, kDx, kDw };
 constexpr int kCeM = 128, kCeN = 256, kCeK = 64;
 // The warps that work on tiles.  Sixteen hide what each waits for better where results are written (dW of 131072 x 4096 over 8 rows: 257 us,
 // with eight 319); with eight a row's statistics have fewer parts.
+// (Their 576 threads leave 96 registers.  The forms that keep sums spill some: G of fp32 140 to 164 bytes a thread, of 16 bits 56 to 68, dx and dW of fp32 16 to 52.)
 template <CeMode MODE> constexpr int kCeWarps = MODE == kLse ? 8 : 16;
 template <CeMode MODE> constexpr int kCeShares = kCeWarps<MODE> / 4;      // of a tile's columns
 template <CeMode MODE> constexpr int kCeThreads = (kCeWarps<MODE> + 2) * 32;
@@ -121,7 +123,7 @@ template <> struct CePlanes<float> {
     p[0] = __bfloat162float(__float2bfloat16_rn(v));
     if (isinf(p[0]) && !isinf(v)) p[0] = copysignf(kCeMostBf16, v);   // a number beyond the largest bf16 one is that and a rest
     const float r = v - p[0];
-    p[1] = isfinite(p[0]) ? __bfloat162float(__float2bfloat16_rn(r)) : 0.f;   // an infinity is its first part alone
+    p[1] = isfinite(p[0]) ? __bfloat162float(__float2bfloat16_rn(r)) : 0.f;   // an infinity is its first part alone (times a part of zero it gives NaN)
     p[2] = isfinite(p[0]) ? r - p[1] : 0.f;
   }
 };
@@ -1053,12 +1055,12 @@ __global__ void __launch_bounds__(256) castle_ce_join_kernel(const CeJoin p) {
 // ------------------------------------------------------------------------------------------------ host
 // How a result of m x n over a contraction of k (all terms of it) is cut.  Pairs of CTAs are faster per row where the contraction is long and
 // slower where it is short (the second CTA waits for the first's products at a tile's start and end), and pad the rows to 256 instead of
-// 128.  us, pairs / single: logits and their gradient of 4096 x 1024 against 50021 282, 289 / 296, 363; 197 x 4096 against 131072 214, 208 / 236, 240;
-// 300 x 1024 against 50021 48, 48 / 40, 40; 2000 x 512 against 8000 21, 26 / 19, 23.  dx of 4096 x 1024 312 / 340, of 600 x 1024 73 / 81, of 300 x 1024 56 / 51.
+// 128.  us, pairs / single: logits and their gradient of 4096 x 1024 against 50021 281, 340 / 299, 369; 197 x 4096 against 131072 216, 231 / 231, 245;
+// 300 x 1024 against 50021 48, 48 / 40, 42; 2000 x 512 against 8000 21, 26 / 19, 23.  dx of 4096 x 1024 312 / 340, of 600 x 1024 73 / 81, of 300 x 1024 56 / 51.
 // dW, whose rows are the vocabulary: over 300 tokens 48 / 44, 600 61 / 66, 1000 33 / 36.  Narrower tiles (of single ones with one product's
 // contraction each) as long as all of them run at once: logits of 130 x 512 against 256 6.0, with 256 columns 8.3; but two rounds of half
 // tiles are slower than one of whole ones (50 x 768 against 32000 in fp32 55 / 43).  With one tile of rows, half as wide ones also where their
-// rounds come out shorter (128 x 4096 against 131072, 7 of 128 columns for 4 of 256: logits 192 -> 189 us, their gradient 190 -> 184).
+// rounds come out shorter (128 x 4096 against 131072, 7 of 128 columns for 4 of 256: logits 194 -> 188 us, their gradient 195 -> 192).
 struct CeCut { int pair, bn; };
 static CeCut ce_cut(CeMode mode, int64_t m, int64_t n, int64_t k) {
   const int64_t single = (m + 127) / 128 * 128, pairs = (m + 255) / 256 * 256;
@@ -1095,7 +1097,7 @@ static CePlan ce_plan(int dtype, int64_t n, int dim, int64_t vocab, bool x_ok, b
   q.copy_x = f32 || !x_ok;
   q.copy_w = f32 || !w_ok;
   // A tile's rows behind the last one need not be loaded (their results go nowhere); of the contraction they have to be zero, 16 at a time.  Rows that
-  // TMA has to fill take it longer than rows that it reads (8 x 4096 against 131072: logits 241 -> 187 us, their gradient 243 -> 180, dW 257 -> 239).
+  // TMA has to fill take it longer than rows that it reads (8 x 4096 against 131072: logits 241 -> 187 us, their gradient 243 -> 180 (188 since its sums are emptied on the way), dW 257 -> 239).
   q.a_rows = (int)(n < kCeM ? up(n, 8) : kCeM);
   q.k_rows = (int)(n < kCeK ? up(n, 16) : kCeK);
   q.copy_rows = up(n, kCeK);
