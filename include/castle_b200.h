@@ -318,6 +318,52 @@ int castle_decode_step_static(const castle_problem_t* p, int32_t cache_len, int3
                               const castle_tensor_t* kc_cache, const castle_tensor_t* vc_cache,
                               const castle_tensor_t* out, int32_t* status, void* stream);
 
+/* ---- caches in pages ---------------------------------------------------------
+ * (no counterpart in the reference, whose caches are one tensor of all sequences and positions)  The rows of a cache lie in
+ * pages of page_size positions (a power of two from 16 to 1024) of a pool: (pages, heads, page_size, dim_head), a head's rows of
+ * a page adjacent.  Row k of sequence b is row k % page_size of page table[b * table_stride + k / page_size].  qu, kc and vc
+ * have one table (their rows never change, so sequences may share pages), U has one of its own (every token rewrites it, so
+ * each of its pages is one sequence's).  Tables and lengths are read on the device; entries of a table beyond a sequence's
+ * last row are not read.
+ */
+typedef struct {
+  void* ptr;
+  int64_t stride_page; /* elements between pages */
+  int64_t stride_h;    /* elements between heads of a page */
+} castle_pages_t;
+
+/* castle_decode_step_fused() for `batch` (at most 4096) sequences of lengths[b] positions each: row lengths[b] is appended, so its
+ * page has to be in the tables.  A length below zero: no sequence, its row of `out` is zero.  A length without places in the
+ * tables, or a page outside its pool: `out` is NaN, nothing is written for those rows, CASTLE_STATUS_BAD_INDEX is set.
+ * rotary->position0 is ignored (the new row's position is its length).  counters: batch * heads words that are zero
+ * before the call and zero again when its kernel has run.  The result does not depend on how the work was shared out.
+ */
+size_t castle_paged_decode_workspace_bytes(const castle_problem_t* p, int32_t page_size, int32_t table_width);
+int castle_paged_decode_step(const castle_problem_t* p, int32_t page_size, int32_t u_pages, int32_t pages, const castle_tensor_t* qc_new,
+                             const castle_tensor_t* kc_new, const castle_tensor_t* vc_new, const castle_tensor_t* qu_new,
+                             const castle_tensor_t* ku_new, const castle_tensor_t* vu_new, const castle_pages_t* u_cache,
+                             const castle_pages_t* qu_cache, const castle_pages_t* kc_cache, const castle_pages_t* vc_cache,
+                             const int32_t* u_table, int64_t u_table_stride, const int32_t* table, int64_t table_stride,
+                             int32_t table_width, const int32_t* lengths, const castle_tensor_t* out, const castle_rotary_t* rotary,
+                             uint32_t* counters, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
+/* Rows [0, lengths[b]) of four (batch, heads, seq_len, dim_head) caches, as castle_fwd_prefill() leaves them, into pages.  A length
+ * of more than seq_len rows or than the tables have places for, or a page outside its pool: nothing is written for that sequence
+ * or page, CASTLE_STATUS_BAD_INDEX is set.
+ */
+int castle_write_pages(const castle_problem_t* p, int32_t page_size, int32_t u_pages, int32_t pages, const castle_tensor_t* u,
+                       const castle_tensor_t* qu, const castle_tensor_t* kc, const castle_tensor_t* vc, const castle_pages_t* u_cache,
+                       const castle_pages_t* qu_cache, const castle_pages_t* kc_cache, const castle_pages_t* vc_cache,
+                       const int32_t* u_table, int64_t u_table_stride, const int32_t* table, int64_t table_stride, int32_t table_width,
+                       const int32_t* lengths, int32_t* status, void* stream);
+
+/* Pages source[i] to target[i] (i < count) of each of `pools` pools.  ptr[k]: pool k; a page is `blocks` blocks of block_bytes
+ * bytes, stride_page[k] bytes from page to page and stride_block[k] from block to block; all of them multiples of 16 bytes.
+ * All arrays are the host's and are read before the call returns.  No target may be a source or another target.
+ */
+int castle_copy_pages(int32_t pools, void* const* ptr, const int64_t* stride_page, const int64_t* stride_block, int64_t blocks,
+                      int64_t block_bytes, int64_t pages, const int32_t* source, const int32_t* target, int64_t count, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libcastle_b200.so"
-SOURCES = ["api.cu", "decode.cu", "selftest.cu", "convert.cu", "transform.cu", "token_linear.cu", "token_layer.cu", "linear.cu", "norm.cu", "layernorm.cu", "embedding.cu", "linear_ce.cu", "fwd.cu", "bwd.cu", "bwd128.cu"]
+SOURCES = ["api.cu", "decode.cu", "selftest.cu", "convert.cu", "transform.cu", "token_linear.cu", "token_layer.cu", "linear.cu", "norm.cu", "layernorm.cu", "embedding.cu", "linear_ce.cu", "paged.cu", "pages.cu", "fwd.cu", "bwd.cu", "bwd128.cu"]
 
 BF16, F16, F32 = 0, 1, 2
 
@@ -23,6 +23,10 @@ BF16, F16, F32 = 0, 1, 2
 class CastleTensor(ctypes.Structure):
     _fields_ = [("ptr", ctypes.c_void_p), ("stride_b", ctypes.c_int64), ("stride_h", ctypes.c_int64),
                 ("stride_n", ctypes.c_int64)]
+
+
+class CastlePages(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("stride_page", ctypes.c_int64), ("stride_h", ctypes.c_int64)]
 
 
 class CastleProblem(ctypes.Structure):
@@ -52,7 +56,7 @@ STAMP_PATH = PKG_DIR / "libcastle_b200.so.stamp"
 HOST_PATH = PKG_DIR / "_host.so"
 HOST_STAMP_PATH = PKG_DIR / "_host.so.stamp"
 HOST_SOURCE = CSRC / "host.cpp"
-HOST_PARTS = [HOST_SOURCE, CSRC / "host_lm.h"]
+HOST_PARTS = [HOST_SOURCE, CSRC / "host_lm.h", CSRC / "host_serve.h"]
 
 
 def _deps():
@@ -170,7 +174,7 @@ def build(force: bool = False, verbose: bool = False):
 _lib = None
 
 P = ctypes.POINTER
-_T, _PR = P(CastleTensor), P(CastleProblem)
+_T, _PR, _PG = P(CastleTensor), P(CastleProblem), P(CastlePages)
 _vp, _i32, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t
 
 _SIGNATURES = {
@@ -208,6 +212,10 @@ _SIGNATURES = {
                            [P(CastleRotary), _vp, _vp, _i32, _vp, _sz, _vp, _vp]),
     "castle_linear": (ctypes.c_int, [_i32] * 5 + [_vp, ctypes.c_int64] * 3 + [_vp, _vp]),
     "castle_decode_step_static": (ctypes.c_int, [_PR, _i32, _i32] + [_T] * 11 + [_vp, _vp]),
+    "castle_paged_decode_workspace_bytes": (_sz, [_PR, _i32, _i32]),
+    "castle_paged_decode_step": (ctypes.c_int, [_PR] + [_i32] * 3 + [_T] * 6 + [_PG] * 4 + [_vp, ctypes.c_int64] * 2 + [_i32, _vp, _T, P(CastleRotary), _vp, _vp, _sz, _vp, _vp]),
+    "castle_write_pages": (ctypes.c_int, [_PR] + [_i32] * 3 + [_T] * 4 + [_PG] * 4 + [_vp, ctypes.c_int64] * 2 + [_i32, _vp, _vp, _vp]),
+    "castle_copy_pages": (ctypes.c_int, [_i32] + [_vp] * 3 + [ctypes.c_int64] * 3 + [_vp, _vp, ctypes.c_int64, _vp]),
     "castle_set_kernel_events": (ctypes.c_int, [_i32, _vp, _vp]),
     "castle_selftest_mma_rate": (ctypes.c_int, [_i32, _i32, _i32, _vp, _vp, _vp]),
     "castle_selftest_mma": (ctypes.c_int, [_i32, _vp, _vp, _vp, _vp, _vp]),

@@ -80,6 +80,10 @@ struct Api {
   decltype(&castle_linear_ce_workspace_bytes) linear_ce_workspace_bytes;
   decltype(&castle_linear_ce_fwd) linear_ce_fwd;
   decltype(&castle_linear_ce_bwd) linear_ce_bwd;
+  decltype(&castle_paged_decode_workspace_bytes) paged_decode_workspace_bytes;
+  decltype(&castle_paged_decode_step) paged_decode_step;
+  decltype(&castle_write_pages) write_pages;
+  decltype(&castle_copy_pages) copy_pages;
 } api{};
 
 void check(int rc, const char* what) {
@@ -671,6 +675,7 @@ Tensor decode_step(const Tensor* news, const Tensor* caches, int64_t t, double s
 }
 
 #include "host_lm.h"
+#include "host_serve.h"
 
 // ------------------------------------------------------------------------------------------------ the plain module
 struct Layer {
@@ -1296,6 +1301,71 @@ PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// paged_decode_step(six new rows, four pools, U's table, table, lengths, scale)
+PyObject* py_paged_decode_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    arg_count(n, 14);
+    Tensor v[13], out;
+    for (int i = 0; i < 13; ++i) v[i] = arg_tensor(a[i]);
+    const double scale = arg_float(a[13]);
+    {
+      Unlocked u;
+      out = paged_decode_step(v, v + 6, v[10], v[11], v[12], scale);
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
+// paged_decode_packed(packed, scale, rotary freqs or None, four pools, U's table, table, lengths)
+PyObject* py_paged_decode_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    arg_count(n, 7);
+    const Tensor packed = arg_tensor(a[0]);
+    const double scale = arg_float(a[1]);
+    Rotary rotary;
+    rotary.freqs = arg_optional(a[2]);
+    const std::vector<Tensor> pools = arg_caches(a[3]);
+    if (pools.size() != 4) throw std::runtime_error("castle: four cache tensors expected");
+    const Tensor u_table = arg_tensor(a[4]), table = arg_tensor(a[5]), lengths = arg_tensor(a[6]);
+    Tensor out;
+    {
+      Unlocked u;
+      out = paged_decode_packed(packed, pools.data(), u_table, table, lengths, scale, rotary);
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
+// write_pages(four caches, four pools, U's table, table, lengths)
+PyObject* py_write_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arg_count(n, 11);
+    Tensor v[11];
+    for (int i = 0; i < 11; ++i) v[i] = arg_tensor(a[i]);
+    {
+      Unlocked u;
+      write_pages(v, v + 4, v[8], v[9], v[10]);
+    }
+    Py_RETURN_NONE;
+  });
+}
+
+// copy_pages(list of pools, source, target)
+PyObject* py_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arg_count(n, 3);
+    std::vector<Tensor> pools;
+    if (!PyList_Check(a[0])) throw std::runtime_error("castle: a list of pools expected");
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); ++i) pools.push_back(arg_tensor(PyList_GET_ITEM(a[0], i)));
+    const Tensor source = arg_tensor(a[1]), target = arg_tensor(a[2]);
+    {
+      Unlocked u;
+      copy_pages(pools, source, target);
+    }
+    Py_RETURN_NONE;
+  });
+}
+
 // forward_chunks(B, H, bytes per pair, limit): the rectangles of a forward's launches as (b0, b1, h0, h1)
 PyObject* py_forward_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -1395,6 +1465,7 @@ PyObject* py_bind(PyObject*, PyObject* d) {
     CASTLE_BIND(layernorm_fwd); CASTLE_BIND(layernorm_bwd_workspace_bytes); CASTLE_BIND(layernorm_bwd);
     CASTLE_BIND(embedding_fwd); CASTLE_BIND(embedding_bwd_workspace_bytes); CASTLE_BIND(embedding_bwd);
     CASTLE_BIND(linear_ce_workspace_bytes); CASTLE_BIND(linear_ce_fwd); CASTLE_BIND(linear_ce_bwd);
+    CASTLE_BIND(paged_decode_workspace_bytes); CASTLE_BIND(paged_decode_step); CASTLE_BIND(write_pages); CASTLE_BIND(copy_pages);
 #undef CASTLE_BIND
     PyObject* module = PyImport_ImportModule("torch.utils._device");
     Py_XDECREF(device_context);
@@ -1416,6 +1487,10 @@ PyMethodDef methods[] = {{"bind", py_bind, METH_O, nullptr},
                          {"embedding", FAST(py_embedding), nullptr},
                          {"layer_norm", FAST(py_layer_norm), nullptr},
                          {"linear_cross_entropy", FAST(py_linear_cross_entropy), nullptr},
+                         {"paged_decode_step", FAST(py_paged_decode_step), nullptr},
+                         {"paged_decode_packed", FAST(py_paged_decode_packed), nullptr},
+                         {"write_pages", FAST(py_write_pages), nullptr},
+                         {"copy_pages", FAST(py_copy_pages), nullptr},
                          {"forward_chunks", FAST(py_forward_chunks), nullptr},
                          {"first_rows", FAST(py_first_rows), nullptr},
                          {"new_caches", FAST(py_new_caches), nullptr},

@@ -37,7 +37,7 @@ def check_status(device=None):
         if v != 0:
             w.zero_()
             raise RuntimeError(f"castle kernels reported status {v} on cuda:{d} (1 = a bounded wait ran out, "
-                               "4 = a token or target outside the vocabulary)")
+                               "4 = a token or target outside the vocabulary, or a length or page outside its table or pool)")
 
 
 def release_workspaces():
@@ -209,3 +209,36 @@ def castle_linear_cross_entropy(x, weight, targets, ignore_index: int = -100, re
     if torch._C._is_tracing():
         return _TracedCall.apply(lambda x, w, t: _lib.host().linear_cross_entropy(x, w, t, ignore_index, code), x, weight, targets)
     return _lib.host().linear_cross_entropy(x, weight, targets, ignore_index, code)
+
+
+def castle_paged_decode_step(qc, kc, vc, qu, ku, vu, U_pages, qu_pages, kc_pages, vc_pages, U_table, table, lengths, scale: float):
+    """`castle_decode_step` for sequences of different lengths whose caches lie in pages.  The six new-token tensors are
+    (B, H, 1, d); the four pools (pages, H, page size, d), a head's rows of a page adjacent, page size a power of two from 16 to
+    1024 (U's pool may have another number of pages than the others).  `lengths` (B) int32: the positions of each sequence, of which
+    position k is row k % page size of page `table[b, k // page size]` (int32), for U of page `U_table[b, k // page size]`.  All
+    of them are read on the device: a captured step can be replayed as they change.
+
+    The pools are updated IN PLACE: U of every position rewritten, a row appended at position `lengths[b]`, whose page must be in the
+    tables (`lengths` stay as they are).  So a page of U, and the page that gets the new row, must belong to one sequence of the
+    batch; other pages of qu, kc and vc may be shared.  A negative length means no sequence: nothing is read or written for it, and its
+    row of the result is zero.  A length that the tables have no place for, or a page outside its pool, gives NaN, and `check_status()`
+    raises.  Returns out (B, H, 1, d)."""
+    return _lib.host().paged_decode_step(qc, kc, vc, qu, ku, vu, U_pages, qu_pages, kc_pages, vc_pages, U_table, table, lengths, scale)
+
+
+def castle_write_pages(U, qu, kc, vc, U_pages, qu_pages, kc_pages, vc_pages, U_table, table, lengths):
+    """A prompt's caches (B, H, N, d), as `Castle(..., return_next_cache=True)` returns them, into pages: the first `lengths[b]`
+    (int32, at most N; none where negative) rows of each sequence, pools and tables as in `castle_paged_decode_step`."""
+    _lib.host().write_pages(U, qu, kc, vc, U_pages, qu_pages, kc_pages, vc_pages, U_table, table, lengths)
+
+
+def _page_numbers(pages):
+    return pages if isinstance(pages, torch.Tensor) else torch.tensor(pages, dtype=torch.int64, device="cpu")
+
+
+def castle_copy_pages(pools, source, target):
+    """Pages `source[i]` to `target[i]` of a (pages, ...) pool, or of each of a list of pools of one shape, type and device, in place: what a
+    fork of a sequence or a compaction of its pages moves.  A page is a multiple of 16 bytes.  `source` and `target` are lists, or
+    int64 or int32 tensors on the host (a CUDA graph keeps the pages it was captured with); a target that is a source too, or a target twice, is refused."""
+    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    _lib.host().copy_pages(pools, _page_numbers(source), _page_numbers(target))
