@@ -123,7 +123,7 @@ def test_pools_and_rows_of_other_strides(layout, dtype, page):
 
 
 def test_many_sequences_of_many_pieces():
-    """More tiles than one round of pieces has (592 x 64), and batches beyond a CTA's threads."""
+    """More pairs than there are CTAs, whole and cut ones, and batches beyond a CTA's threads."""
     _run(Case(torch.bfloat16, [16000 - 131 * i for i in range(48)], 8, 16, 128, std=0.5))
     _run(Case(torch.float16, [(i * 7) % 50 - 2 for i in range(700)], 2, 64, 16))
 
