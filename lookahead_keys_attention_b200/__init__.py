@@ -5,8 +5,10 @@ replaces the reference's `castle_attention_triton` operator.
 """
 from .castle import Cache, Castle, ModuleCache, cache_from_buffers
 from .ops import (castle_attention, castle_attention_packed, castle_decode_step, castle_embedding, castle_layer_norm,
-                  castle_copy_pages, castle_linear_cross_entropy, castle_paged_decode_step, castle_write_pages, check_status,
+                  castle_copy_pages, castle_linear_4bit, castle_linear_cross_entropy, castle_pack_4bit, castle_paged_decode_step,
+                  castle_quantize_4bit, castle_write_pages, check_status,
                   release_workspaces)
 
 __all__ = ["Castle", "Cache", "ModuleCache", "cache_from_buffers", "release_workspaces", "castle_attention", "castle_attention_packed", "castle_decode_step", "castle_embedding", "castle_layer_norm",
-           "castle_linear_cross_entropy", "castle_paged_decode_step", "castle_write_pages", "castle_copy_pages", "check_status"]
+           "castle_linear_cross_entropy", "castle_paged_decode_step", "castle_write_pages", "castle_copy_pages", "castle_linear_4bit", "castle_pack_4bit",
+           "castle_quantize_4bit", "check_status"]

@@ -15,7 +15,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libcastle_b200.so"
-SOURCES = ["api.cu", "decode.cu", "selftest.cu", "convert.cu", "transform.cu", "token_linear.cu", "token_layer.cu", "linear.cu", "norm.cu", "layernorm.cu", "embedding.cu", "linear_ce.cu", "paged.cu", "pages.cu", "fwd.cu", "bwd.cu", "bwd128.cu"]
+SOURCES = ["api.cu", "decode.cu", "selftest.cu", "convert.cu", "transform.cu", "token_linear.cu", "token_layer.cu", "linear.cu", "norm.cu", "layernorm.cu", "embedding.cu", "linear_ce.cu", "paged.cu", "pages.cu", "linear_4bit.cu", "fwd.cu", "bwd.cu", "bwd128.cu"]
 
 BF16, F16, F32 = 0, 1, 2
 
@@ -56,7 +56,7 @@ STAMP_PATH = PKG_DIR / "libcastle_b200.so.stamp"
 HOST_PATH = PKG_DIR / "_host.so"
 HOST_STAMP_PATH = PKG_DIR / "_host.so.stamp"
 HOST_SOURCE = CSRC / "host.cpp"
-HOST_PARTS = [HOST_SOURCE, CSRC / "host_lm.h", CSRC / "host_serve.h"]
+HOST_PARTS = [HOST_SOURCE, CSRC / "host_lm.h", CSRC / "host_serve.h", CSRC / "host_4bit.h"]
 
 
 def _deps():
@@ -216,6 +216,9 @@ _SIGNATURES = {
     "castle_paged_decode_step": (ctypes.c_int, [_PR] + [_i32] * 3 + [_T] * 6 + [_PG] * 4 + [_vp, ctypes.c_int64] * 2 + [_i32, _vp, _T, P(CastleRotary), _vp, _vp, _sz, _vp, _vp]),
     "castle_write_pages": (ctypes.c_int, [_PR] + [_i32] * 3 + [_T] * 4 + [_PG] * 4 + [_vp, ctypes.c_int64] * 2 + [_i32, _vp, _vp, _vp]),
     "castle_copy_pages": (ctypes.c_int, [_i32] + [_vp] * 3 + [ctypes.c_int64] * 3 + [_vp, _vp, ctypes.c_int64, _vp]),
+    "castle_linear_4bit_fits": (ctypes.c_int, [_i32] * 3),
+    "castle_linear_4bit": (ctypes.c_int, [_i32] * 3 + [ctypes.c_int64, _i32, _vp, ctypes.c_int64] + [_vp] * 5),
+    "castle_expand_4bit": (ctypes.c_int, [_i32] * 2 + [ctypes.c_int64, _i32] + [_vp] * 4 + [ctypes.c_int64, _vp]),
     "castle_set_kernel_events": (ctypes.c_int, [_i32, _vp, _vp]),
     "castle_selftest_mma_rate": (ctypes.c_int, [_i32, _i32, _i32, _vp, _vp, _vp]),
     "castle_selftest_mma": (ctypes.c_int, [_i32, _vp, _vp, _vp, _vp, _vp]),

@@ -1,5 +1,5 @@
-// What the cached-step kernels (decode.cu, token_layer.cu, token_linear.cu) share: 16-byte vectors of a row as floats, the sums over the
-// lanes of a row, the rotation of the new rows.
+// What the kernels of single tokens (decode.cu, paged.cu, token_layer.cu, token_linear.cu, linear_4bit.cu) share: 16-byte vectors of a row as
+// floats, the sums over the lanes of a row, the rotation of the new rows, a warp's product.
 #pragma once
 #include "rotary.cuh"
 #include "sm100.cuh"
@@ -63,6 +63,15 @@ __device__ __forceinline__ void rotate_new(const RotaryParams& r, int64_t col, f
     rotate_pair<T>(b[i], b[i + 1], cs);
     if (c) rotate_pair<T>(c[i], c[i + 1], cs);
   }
+}
+
+template <typename T> __device__ __forceinline__ void mma_16x8x16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (Elem<T>::fmt == 1)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 }  // namespace castle

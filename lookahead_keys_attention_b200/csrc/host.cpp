@@ -84,6 +84,9 @@ struct Api {
   decltype(&castle_paged_decode_step) paged_decode_step;
   decltype(&castle_write_pages) write_pages;
   decltype(&castle_copy_pages) copy_pages;
+  decltype(&castle_linear_4bit_fits) linear_4bit_fits;
+  decltype(&castle_linear_4bit) linear_4bit;
+  decltype(&castle_expand_4bit) expand_4bit;
 } api{};
 
 void check(int rc, const char* what) {
@@ -1019,6 +1022,8 @@ Tensor layer_decode(const Tensor& x, const Layer& l, const Tensor* caches, int64
   return at::linear(decode_packed(project(x, l), caches, t, scale, rotary), l.combine);
 }
 
+#include "host_4bit.h"
+
 // ------------------------------------------------------------------------------------------------ Python
 template <typename F>
 PyObject* guarded(F&& f) {   // C++ exceptions become Python ones; `f` runs without the interpreter lock where it says so
@@ -1350,6 +1355,21 @@ PyObject* py_write_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// linear_4bit(x, codes, scales, zeros or None, group size)
+PyObject* py_linear_4bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    arg_count(n, 5);
+    const Tensor x = arg_tensor(a[0]), codes = arg_tensor(a[1]), scales = arg_tensor(a[2]), zeros = arg_optional(a[3]);
+    const int64_t group = arg_int(a[4]);
+    Tensor out;
+    {
+      Unlocked u;
+      out = linear_4bit(x, codes, scales, zeros, group);
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
 // copy_pages(list of pools, source, target)
 PyObject* py_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -1466,6 +1486,7 @@ PyObject* py_bind(PyObject*, PyObject* d) {
     CASTLE_BIND(embedding_fwd); CASTLE_BIND(embedding_bwd_workspace_bytes); CASTLE_BIND(embedding_bwd);
     CASTLE_BIND(linear_ce_workspace_bytes); CASTLE_BIND(linear_ce_fwd); CASTLE_BIND(linear_ce_bwd);
     CASTLE_BIND(paged_decode_workspace_bytes); CASTLE_BIND(paged_decode_step); CASTLE_BIND(write_pages); CASTLE_BIND(copy_pages);
+    CASTLE_BIND(linear_4bit_fits); CASTLE_BIND(linear_4bit); CASTLE_BIND(expand_4bit);
 #undef CASTLE_BIND
     PyObject* module = PyImport_ImportModule("torch.utils._device");
     Py_XDECREF(device_context);
@@ -1491,6 +1512,7 @@ PyMethodDef methods[] = {{"bind", py_bind, METH_O, nullptr},
                          {"paged_decode_packed", FAST(py_paged_decode_packed), nullptr},
                          {"write_pages", FAST(py_write_pages), nullptr},
                          {"copy_pages", FAST(py_copy_pages), nullptr},
+                         {"linear_4bit", FAST(py_linear_4bit), nullptr},
                          {"forward_chunks", FAST(py_forward_chunks), nullptr},
                          {"first_rows", FAST(py_first_rows), nullptr},
                          {"new_caches", FAST(py_new_caches), nullptr},

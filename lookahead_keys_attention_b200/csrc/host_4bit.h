@@ -1,0 +1,123 @@
+// Host side of the products with weights of 4 bits.  Part of host.cpp (inside its namespace, behind `product`).
+
+struct Codes {   // a weight's, as the kernels take them
+  Tensor codes, scales, zeros;
+  int64_t N = 0, K = 0, group = 0;
+};
+Codes check_codes(const Tensor& codes, const Tensor& scales, const Tensor& zeros, int64_t K, int64_t group, at::ScalarType dtype, const at::Device& dev) {
+  const char* who = "castle_linear_4bit";
+  need_plain(codes, who);
+  need(codes.dim() == 2 && codes.scalar_type() == at::kInt && codes.size(0) > 0 && codes.size(1) == (K + 127) / 128 * 16,
+       "castle_linear_4bit: codes of castle_pack_4bit for weights of the rows' length expected");
+  need(group >= 32 && group <= (1 << 24) && (group & (group - 1)) == 0, "castle_linear_4bit: the group size must be a power of two from 32 up");
+  Codes c;
+  c.N = codes.size(0); c.K = K; c.group = group;
+  const std::array<int64_t, 2> sizes{c.N, (K + group - 1) / group};
+  for (const Tensor* t : {&scales, &zeros}) {
+    if (!t->defined()) continue;
+    need_plain(*t, who);
+    need(t->sizes() == at::IntArrayRef(sizes) && t->scalar_type() == dtype && t->device() == dev,
+         "castle_linear_4bit: scales and zero points must be (out, groups) tensors of the rows' type and device");
+    need(!(t->requires_grad() && at::GradMode::is_enabled()), "castle_linear_4bit: scales and zero points have no gradient");
+  }
+  need(codes.device() == dev, "castle_linear_4bit: codes and rows must be on one device");
+  c.codes = aligned_contiguous(codes); c.scales = as_plain(scales); c.zeros = as_plain(zeros);
+  return c;
+}
+
+// The weights at full width.
+Tensor expand_4bit(const Codes& c, at::ScalarType dtype, const at::Device& dev) {
+  const int64_t unit = 16 / (int64_t)c10::elementSize(dtype), ld = (c.K + unit - 1) / unit * unit;
+  const Tensor w = at::empty({c.N, ld}, at::TensorOptions().dtype(dtype).device(dev));
+  check(api.expand_4bit(dtype_code(dtype), (int32_t)c.K, c.N, (int32_t)c.group, c.codes.data_ptr(), c.scales.data_ptr(), c.zeros.defined() ? c.zeros.data_ptr() : nullptr,
+                        w.data_ptr(), ld, c10::cuda::getCurrentCUDAStream(dev.index()).stream()), "castle_expand_4bit");
+  return w.narrow(1, 0, c.K);
+}
+
+struct Linear4bitBackward : public Node {   // of x: the weights are frozen
+  SavedVariable codes, scales, zeros;
+  std::vector<int64_t> x_sizes;
+  at::ScalarType dtype = at::kFloat;
+  int64_t out_features = 0, group = 0;
+  bool has_zeros = false;
+
+  std::string name() const override { return "CastleLinear4bitBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&codes, &scales, &zeros}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    const char* who = "castle_linear_4bit";
+    variable_list result(1);
+    if (grads.empty() || !grads[0].defined()) return result;
+    const Tensor cs = codes.unpack(), ss = scales.unpack(), zs = has_zeros ? zeros.unpack() : Tensor();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);   // the products keep the rows' type
+    const at::Device dev = grads[0].device();
+    const c10::cuda::CUDAGuard guard(dev);
+    std::vector<int64_t> y_sizes = x_sizes;
+    y_sizes.back() = out_features;
+    need_gradient(grads[0], y_sizes, dtype, dev, who);
+    const int64_t K = x_sizes.back(), rows = grads[0].numel() / out_features;
+    if (rows == 0) {
+      result[0] = at::empty(x_sizes, grads[0].options());
+      return result;
+    }
+    const Codes c = check_codes(restored(cs, {out_features, (K + 127) / 128 * 16}, at::kInt, dev, who), ss, zs, K, group, dtype, dev);
+    result[0] = product(1, as_plain(grads[0]).view({rows, out_features}), expand_4bit(c, dtype, dev), rows).view(x_sizes);
+    refuse_second(result, who, grads[0], *this, 0);   // (it does not depend on x)
+    return result;
+  }
+};
+
+Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& own_scales, const Tensor& own_zeros, int64_t group) {
+  const char* who = "castle_linear_4bit";
+  need_plain(x, who);
+  need_type(x, who);
+  need(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) <= (1 << 24), "castle_linear_4bit: (..., in) rows expected");
+  const int64_t K = x.size(-1), rows = x.numel() / K;
+  const Tensor scales = in_type_of(x, own_scales), zeros = in_type_of(x, own_zeros);
+  need(scales.defined(), "castle_linear_4bit: scales expected");
+  const at::Device dev = x.device();
+  const auto dtype = x.scalar_type();
+  std::vector<int64_t> sizes = x.sizes().vec();
+  Tensor y;
+  Codes c;
+  {
+    const c10::cuda::CUDAGuard guard(dev);
+    c = check_codes(codes, scales, zeros, K, group, dtype, dev);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
+    const at::NoGradGuard no_grad;
+    sizes.back() = c.N;
+    // The rows of a few tokens go through the codes, as many at a time as the kernel takes; more of them through the weights at full width.
+    const int64_t most = dtype == at::kFloat ? 10 : 32, turns = (rows + most - 1) / most, each = turns > 0 ? (rows + turns - 1) / turns : 0;
+    if (rows == 0) {
+      y = at::empty(sizes, x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+    } else if (turns <= 2 && api.linear_4bit_fits(dtype_code(dtype), (int32_t)each, (int32_t)K)) {
+      y = at::empty(sizes, x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+      const Rows r = as_rows(x, rows, K);
+      const int64_t es = x.element_size();
+      for (int64_t i = 0; i < rows; i += each)
+        check(api.linear_4bit(dtype_code(dtype), (int32_t)std::min(each, rows - i), (int32_t)K, c.N, (int32_t)group, static_cast<char*>(r.data) + i * r.stride * es, r.stride,
+                              c.codes.data_ptr(), c.scales.data_ptr(), c.zeros.defined() ? c.zeros.data_ptr() : nullptr, static_cast<char*>(y.data_ptr()) + i * c.N * es,
+                              c10::cuda::getCurrentCUDAStream(dev.index()).stream()), who);
+    } else {
+      y = product(0, as_plain(x).view({rows, K}), expand_4bit(c, dtype, dev), rows).view(sizes);
+    }
+  }
+  if (!(at::GradMode::is_enabled() && x.requires_grad())) return y;
+  auto node = std::shared_ptr<Linear4bitBackward>(new Linear4bitBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x));
+  torch::autograd::set_history(y, node);
+  node->codes = SavedVariable(codes, false);
+  node->scales = SavedVariable(scales, false);
+  node->has_zeros = zeros.defined();
+  if (node->has_zeros) node->zeros = SavedVariable(zeros, false);
+  node->x_sizes = x.sizes().vec();
+  node->dtype = dtype;
+  node->out_features = c.N;
+  node->group = group;
+  return y;
+}

@@ -242,3 +242,56 @@ def castle_copy_pages(pools, source, target):
     int64 or int32 tensors on the host (a CUDA graph keeps the pages it was captured with); a target that is a source too, or a target twice, is refused."""
     pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
     _lib.host().copy_pages(pools, _page_numbers(source), _page_numbers(target))
+
+
+def castle_pack_4bit(codes):
+    """(out, in) codes of 0 to 15, of any integer type and on any device, as `castle_linear_4bit` takes them: eight to an int32 (their order: the C
+    ABI's header), (out, ceil(in / 128) * 16)."""
+    if codes.dim() != 2 or codes.is_floating_point() or codes.dtype == torch.bool:
+        raise ValueError("castle_pack_4bit: (out, in) integer codes expected")
+    n, k = codes.shape
+    blocks = (k + 127) // 128
+    padded = torch.full((n, blocks * 128), 8, dtype=torch.int32, device=codes.device)
+    padded[:, :k] = codes & 15
+    padded = padded.view(n, blocks, 4, 4, 8)                                        # 32 k, 8 k of these, k
+    word = torch.zeros((n, blocks, 4, 4), dtype=torch.int32, device=codes.device)
+    for i in range(8):
+        word |= padded[..., i] << (4 * (i // 2) + 16 * (i % 2))
+    return word.transpose(2, 3).reshape(n, blocks * 16)
+
+
+def castle_quantize_4bit(weight, group_size: int = 64, zeros: bool = False):
+    """(out, in) weights to the nearest of 16 values for each group of `group_size` (a power of two from 32 up) weights of a row: (codes, scales, zero points)
+    for `castle_linear_4bit`.  Without zero points the values are scale * {-8 .. 7}, with them scale * ({0 .. 15} - zero), the least to the
+    largest weight of the group.  Scales and zero points have the weights' type."""
+    if weight.dim() != 2 or weight.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError("castle_quantize_4bit: (out, in) weights in bf16, fp16 or fp32 expected")
+    if group_size < 32 or group_size & (group_size - 1):
+        raise ValueError(f"castle_quantize_4bit: group_size {group_size} is not a power of two from 32 up")
+    with torch.no_grad():
+        n, k = weight.shape
+        groups = (k + group_size - 1) // group_size
+        w = weight.float()
+        padded = torch.nn.functional.pad(w, (0, groups * group_size - k))             # (a value of zero is among the others' range below)
+        inside = (torch.arange(groups * group_size, device=w.device) < k).view(groups, group_size)
+        grouped = padded.view(n, groups, group_size)
+        high = torch.where(inside, grouped, -torch.inf).amax(-1)
+        low = torch.where(inside, grouped, torch.inf).amin(-1)
+        scale = (high - low) / 15 if zeros else torch.maximum(high / 7, -low / 8)
+        scale = scale.to(weight.dtype)
+        scale = torch.where(scale > 0, scale, torch.ones_like(scale))                 # (all of a group alike, or too small for the type)
+        zero = (-low / scale.float()).to(weight.dtype) if zeros else None
+        codes = grouped / scale.float()[..., None] + (zero.float()[..., None] if zeros else 8.0)
+        codes = codes.round().clamp(0, 15).to(torch.uint8).view(n, groups * group_size)[:, :k]
+    return castle_pack_4bit(codes), scale, zero
+
+
+def castle_linear_4bit(x, codes, scales, zeros=None, group_size: int = 64):
+    """`x @ W.T` for weights of 4 bits: W[n, k] = scales[n, k // group_size] * (code[n, k] - zeros[n, k // group_size]), with zero points of 8 where there are
+    none.  x (..., in); `codes` of `castle_pack_4bit` or `castle_quantize_4bit`; scales and zero points (out, ceil(in / group_size)) of x's type (under autocast they
+    are cast to it), group_size a power of two from 32 up.  For a few rows the codes are read as they are, the weights are not rounded, and sums
+    are fp32; many rows are a product with the weights at full width, rounded to x's type.  The gradient of x is that product's; the
+    weights are frozen.  With zero points an infinity in x may give NaN."""
+    if torch._C._is_tracing():
+        return _TracedCall.apply(lambda *t: _lib.host().linear_4bit(*t, group_size), x, codes, scales, zeros)
+    return _lib.host().linear_4bit(x, codes, scales, zeros, group_size)

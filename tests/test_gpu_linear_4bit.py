@@ -1,0 +1,218 @@
+"""GPU: products with weights of 4 bits, against their definition in 64 bits.
+
+Tolerances.  The codes less eight are exact operands and so are the rows (fp32 rows in three parts), so a group's sum of products is off by its fp32
+additions alone: at most 2^-23 of the sum of the products' sizes for each of the k (128 products are added in sixteens, with some bits less than
+fp32's kept of the smaller ones: 2^-22), then the zero points' part, (8 - z) times the sum of x, by as much of its own, and
+the groups' sums another in + 16 roundings.  The result is rounded once: eps / 2.  Products with many rows have each weight rounded once as
+well: eps / 2 of the products' sizes, eps times sqrt(in) of them in bf16 accumulations being fp32, too."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+EPS = {torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -10, torch.float32: 2.0 ** -23}
+
+
+def _weight(out, inner, group, dtype, zeros, gen):
+    groups = (inner + group - 1) // group
+    codes = torch.randint(0, 16, (out, inner), device="cuda", generator=gen, dtype=torch.uint8)
+    scales = torch.empty(out, groups, device="cuda").uniform_(-0.2, 0.3, generator=gen).to(dtype)
+    zero = torch.empty(out, groups, device="cuda").uniform_(-1, 16, generator=gen).to(dtype) if zeros else None
+    at = torch.arange(inner, device="cuda") // group
+    w = (codes.double() - (zero.double()[:, at] if zeros else 8.0)) * scales.double()[:, at]
+    parts = codes.double() - 8, scales.double()[:, at], (8 - zero.double()[:, at]) if zeros else torch.zeros(1, 1, dtype=torch.float64, device="cuda")
+    return codes, scales, zero, w, parts
+
+
+def _check(y, x, w, parts, eps, rounded_weights):
+    exact = torch.einsum("rk,nk->rn", x.double(), w)
+    xa = x.double().abs()
+    code, scale, zero = parts
+    sizes = torch.einsum("rk,nk->rn", xa, ((code.abs() + zero.abs()) * scale.abs()).expand_as(w))
+    tol = eps / 2 * exact.abs() + (2.0 ** -22 + (x.shape[-1] / 32 + 16) * 2.0 ** -24) * sizes + 1e-30
+    if rounded_weights:
+        tol = tol + eps / 2 * torch.einsum("rk,nk->rn", xa, w.abs()) + x.shape[-1] * 2.0 ** -24 * sizes
+    off = (y.double() - exact).abs() - tol
+    assert off.max().item() <= 0, f"{off.max().item():.3e} above the tolerance, largest {exact.abs().max().item():.3e}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128, 512])
+def test_against_the_definition(dtype, zeros, group):
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
+    gen = torch.Generator("cuda").manual_seed(group)
+    for inner, out in ((512, 96), (64, 17), (1000, 333), (129, 2048), (4096, 40), (2176, 5000), (1, 1), (31, 16), (9000, 130)):
+        codes, scales, zero, w, parts = _weight(out, inner, group, dtype, zeros, gen)
+        packed = castle_pack_4bit(codes)
+        for rows in (1, 2, 3, 8, 9, 17, 32, 33, 50):
+            x = torch.randn(rows, inner, device="cuda", generator=gen).to(dtype)
+            x[:, ::7] *= 20
+            y = castle_linear_4bit(x, packed, scales, zero, group_size=group)
+            assert y.shape == (rows, out) and y.dtype == dtype
+            _check(y, x, w, parts, EPS[dtype], True)
+            if rows <= (2 if dtype == torch.float32 else 32) and inner <= 4096:
+                _check(y, x, w, parts, EPS[dtype], False)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_rows_and_tiles(dtype):
+    """More row tiles than a CTA leaves at a time, wide rows shared out among the CTAs of a cluster."""
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
+    gen = torch.Generator("cuda").manual_seed(1)
+    for inner, out, rows in ((512, 50021, 3), (128, 70000, 20), (16384, 512, 8), (16384, 2500, 17), (12000, 48, 1), (1024, 4096, 300), (40000, 100, 5), (40000, 64, 32)):
+        codes, scales, zero, w, parts = _weight(out, inner, 64, dtype, True, gen)
+        x = torch.randn(rows, inner, device="cuda", generator=gen).to(dtype)
+        y = castle_linear_4bit(x, castle_pack_4bit(codes), scales, zero)
+        _check(y, x, w, parts, EPS[dtype], True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_strides_and_shapes(dtype):
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
+    gen = torch.Generator("cuda").manual_seed(2)
+    codes, scales, zero, w, parts = _weight(70, 300, 64, dtype, True, gen)
+    packed = castle_pack_4bit(codes)
+    base = torch.randn(4, 3, 700, device="cuda", generator=gen).to(dtype)
+    for x in (base[0, 0, :300], base[:, 1, 5:305], base[..., ::2][..., :300], base[:, :, 399:699], base[:0, :, :300], base.transpose(0, 1)[:, :, 1:301]):
+        y = castle_linear_4bit(x, packed, scales, zero)
+        assert y.shape == (*x.shape[:-1], 70) and y.is_contiguous()
+        if x.numel():
+            _check(y.reshape(-1, 70), x.reshape(-1, 300), w, parts, EPS[dtype], False)
+    spread = torch.zeros(70, 2 * scales.shape[1], device="cuda", dtype=dtype)
+    spread[:, ::2] = scales
+    assert torch.equal(castle_linear_4bit(base[0, :, :300], packed, spread[:, ::2], zero), castle_linear_4bit(base[0, :, :300], packed, scales, zero))
+
+
+def test_fp32_rows_of_all_sizes():
+    """The three parts of a row hold all its bits, down to where the last part's leave the type's range, and infinities and NaN stay what they are."""
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
+    gen = torch.Generator("cuda").manual_seed(3)
+    codes, scales, _, w, parts = _weight(64, 256, 64, torch.float32, False, gen)
+    packed = castle_pack_4bit(codes)
+    for size in (1e-20, 1.0, 1e30):
+        x = torch.randn(2, 256, device="cuda", generator=gen) * size
+        _check(castle_linear_4bit(x, packed, scales), x, w, parts, EPS[torch.float32], False)
+    x = torch.zeros(3, 256, device="cuda")
+    x[0, 7], x[1, 9] = float("inf"), float("nan")
+    x[2, 5] = torch.finfo(torch.float32).max / 4096
+    y = castle_linear_4bit(x, packed, scales)
+    sign = (codes[:, 7].double() - 8) * scales[:, 0].double()
+    assert bool((y[0][sign != 0] == torch.where(sign > 0, torch.inf, -torch.inf)[sign != 0].float()).all()) and bool(y[0][sign == 0].isnan().all())
+    assert bool(y[1].isnan().all()) and bool(y[2].isfinite().all())
+    _check(y[2:], x[2:], w, parts, EPS[torch.float32], False)
+
+
+def test_a_row_does_not_change_another():
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
+    gen = torch.Generator("cuda").manual_seed(4)
+    codes, scales, zero, _, _ = _weight(500, 1024, 32, torch.bfloat16, True, gen)
+    packed = castle_pack_4bit(codes)
+    x = torch.randn(8, 1024, device="cuda", generator=gen).bfloat16()
+    y = castle_linear_4bit(x, packed, scales, zero, 32)
+    assert all(torch.equal(castle_linear_4bit(x, packed, scales, zero, 32), y) for _ in range(5))
+    z = x.clone()
+    z[3] = float("nan")
+    other = castle_linear_4bit(z, packed, scales, zero, 32)
+    keep = [i for i in range(8) if i != 3]
+    assert torch.equal(other[keep], y[keep]) and bool(other[3].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,inner,out,zeros", [(1, 128, 64, False), (5, 300, 130, True), (100, 1000, 513, True)])
+def test_gradient_of_the_rows(dtype, rows, inner, out, zeros):
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
+    gen = torch.Generator("cuda").manual_seed(5)
+    codes, scales, zero, w, _ = _weight(out, inner, 64, dtype, zeros, gen)
+    packed = castle_pack_4bit(codes)
+    x = torch.randn(rows, inner, device="cuda", generator=gen).to(dtype).requires_grad_()
+    g = torch.randn(rows, out, device="cuda", generator=gen).to(dtype)
+    y = castle_linear_4bit(x, packed, scales, zero)
+    (dx,) = torch.autograd.grad(y, [x], g, retain_graph=True)
+    exact = g.double() @ w
+    tol = EPS[dtype] / 2 * exact.abs() + (EPS[dtype] / 2 + (out + 8) * 2.0 ** -24) * (g.double().abs() @ w.abs()) + 1e-30
+    assert bool(((dx.double() - exact).abs() <= tol).all()) and dx.dtype == dtype
+    (again,) = torch.autograd.grad(y, [x], g.t().contiguous().t())
+    assert torch.equal(again, dx)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, [x], g)      # (released)
+    if dtype == torch.float32:              # differences: the product is linear, so they are the gradient
+        d = torch.randn_like(x)
+        with torch.no_grad():
+            change = (castle_linear_4bit(x + d, packed, scales, zero) - castle_linear_4bit(x - d, packed, scales, zero)).double()
+        assert torch.allclose((change / 2 * g.double()).sum(), (dx.double() * d.double()).sum(), rtol=1e-4, atol=1e-3)
+
+
+def test_second_derivatives_are_refused():
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_quantize_4bit
+    codes, scales, _ = castle_quantize_4bit(torch.randn(64, 64, device="cuda"))
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    (dx,) = torch.autograd.grad(castle_linear_4bit(x, codes, scales).square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        dx.sum().backward()
+
+
+def test_under_autocast():
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_quantize_4bit
+    w = torch.randn(200, 256, device="cuda")
+    codes, scales, zeros = castle_quantize_4bit(w, zeros=True)
+    for rows in (4, 200):
+        x = torch.randn(rows, 256, device="cuda").bfloat16().requires_grad_()
+        with torch.autocast("cuda", dtype=torch.float16):
+            y = castle_linear_4bit(x, codes, scales, zeros)
+            (dx,) = torch.autograd.grad(y.float().sum(), [x])
+        want = castle_linear_4bit(x.detach(), codes, scales.bfloat16(), zeros.bfloat16())
+        assert y.dtype == dx.dtype == torch.bfloat16 and torch.equal(y, want)
+
+
+def test_quantized_weights_are_the_nearest():
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_quantize_4bit
+    for zeros in (False, True):
+        for k, group in ((256, 64), (200, 64), (100, 128)):
+            w = torch.randn(40, k, device="cuda") * torch.rand(40, 1, device="cuda")
+            w[3, :64] = 0
+            w[4, :64] = 0.25
+            codes, scales, zp = castle_quantize_4bit(w, group, zeros)
+            back = castle_linear_4bit(torch.eye(k, device="cuda"), codes, scales, zp, group).t()
+            at = torch.arange(k, device="cuda") // group
+            step = scales[:, at]
+            # half a step inside the range, plus what the zero point's or the extremes' rounding takes (fp32: 16 units of 2^-23 of 15 steps)
+            assert bool(((back - w).abs() <= step * (0.5 + 1e-4)).all())
+
+
+def test_refusals():
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit, castle_quantize_4bit
+    codes, scales, zeros = castle_quantize_4bit(torch.randn(32, 128, device="cuda").bfloat16(), zeros=True)
+    x = torch.randn(2, 128, device="cuda").bfloat16()
+    for call in (lambda: castle_linear_4bit(x[:, :60], codes, scales), lambda: castle_linear_4bit(x.float(), codes, scales), lambda: castle_linear_4bit(x, codes, scales, zeros[:, :1]),
+                 lambda: castle_linear_4bit(x, codes.long(), scales), lambda: castle_linear_4bit(x, codes, scales, group_size=48), lambda: castle_linear_4bit(x, codes, scales, group_size=128),
+                 lambda: castle_linear_4bit(x.cpu(), codes, scales), lambda: castle_linear_4bit(x, codes.cpu(), scales), lambda: castle_linear_4bit(x.double(), codes, scales),
+                 lambda: castle_linear_4bit(x, codes, scales.requires_grad_())):
+        with pytest.raises(RuntimeError, match="castle_linear_4bit"):
+            call()
+    for call in (lambda: castle_pack_4bit(x), lambda: castle_pack_4bit(codes[0]), lambda: castle_quantize_4bit(x, 48), lambda: castle_quantize_4bit(codes)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_captured_and_on_streams():
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_quantize_4bit
+    w = torch.randn(3000, 2048, device="cuda").bfloat16()
+    codes, scales, _ = castle_quantize_4bit(w)
+    xs = [torch.randn(r, 2048, device="cuda").bfloat16() for r in (1, 8, 20, 60, 500)]
+    want = [castle_linear_4bit(x, codes, scales) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    outs = []
+    for x, s in zip(xs, streams):
+        with torch.cuda.stream(s):
+            outs.append(castle_linear_4bit(x, codes, scales))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    for x, y in zip(xs[:4], want):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = castle_linear_4bit(x, codes, scales)
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, y)

@@ -1,0 +1,78 @@
+"""CPU: the codes' layout, the quantisation, and the arguments that products with weights of 4 bits refuse on the host."""
+import pytest
+import torch
+
+
+def _lib():
+    from lookahead_keys_attention_b200 import _lib
+    _lib.build()
+    return _lib, _lib.load()
+
+
+def _unpack(packed, k):
+    """By the layout's description in the C ABI's header, a code at a time."""
+    out = torch.empty(packed.shape[0], k, dtype=torch.int64)
+    for i in range(k):
+        block, rest = divmod(i, 128)
+        j, t, o = rest // 32, rest % 32 // 8, rest % 8
+        word = packed[:, block * 16 + 4 * t + j].long() & 0xffffffff
+        out[:, i] = word >> (4 * (o // 2) + 16 * (o % 2)) & 15
+    return out
+
+
+@pytest.mark.parametrize("n,k,dtype", [(3, 128, torch.uint8), (5, 1, torch.int64), (2, 300, torch.int32), (1, 127, torch.uint8)])
+def test_layout(n, k, dtype):
+    from lookahead_keys_attention_b200 import castle_pack_4bit
+    codes = torch.randint(0, 16, (n, k), generator=torch.Generator().manual_seed(k)).to(dtype)
+    packed = castle_pack_4bit(codes)
+    assert packed.dtype == torch.int32 and packed.shape == (n, (k + 127) // 128 * 16) and packed.is_contiguous()
+    assert torch.equal(_unpack(packed, k), codes.long())
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantised_weights(zeros, dtype):
+    """Every weight is at most half a step (and the rounding of scale and zero point: 16 steps times their half units) from its value."""
+    from lookahead_keys_attention_b200 import castle_quantize_4bit
+    gen = torch.Generator().manual_seed(1)
+    w = (torch.randn(20, 200, generator=gen) * torch.rand(20, 1, generator=gen)).to(dtype)
+    w[0], w[1, :64], w[2, 64:] = 0, 0.5, -w[2, 64:].abs()
+    codes, scales, zp = castle_quantize_4bit(w, 64, zeros)
+    assert scales.shape == (20, 4) and scales.dtype == dtype and (zp is None) == (not zeros)
+    at = torch.arange(200) // 64
+    back = (_unpack(codes, 200).double() - (zp.double()[:, at] if zeros else 8.0)) * scales.double()[:, at]
+    unit = torch.finfo(dtype).eps / 2
+    size = (15 + (zp.double().abs()[:, at] if zeros else 0)) * unit
+    assert bool(((back - w.double()).abs() <= scales.double()[:, at] * (0.5 + 2 * size)).all())
+
+
+def test_arguments():
+    L, lib = _lib()
+    good = dict(dtype=L.BF16, rows=2, k=200, n=10, group=64, x=256, stride=200, codes=256, scales=256, zeros=256, y=256)
+    def call(**kw):
+        a = {**good, **kw}
+        return lib.castle_linear_4bit(*a.values(), None)
+    for bad in [dict(dtype=3), dict(rows=0), dict(rows=33), dict(k=0), dict(k=(1 << 24) + 1), dict(n=0), dict(n=2 ** 31), dict(group=16), dict(group=48), dict(group=0), dict(x=None),
+                dict(x=257), dict(stride=-1), dict(codes=None), dict(codes=264), dict(scales=None), dict(scales=1), dict(zeros=3), dict(y=None), dict(y=255), dict(dtype=L.F32, rows=11)]:
+        assert call(**bad) < 0 and "castle_linear_4bit" in L.last_error(), bad
+    wide = dict(dtype=L.BF16, k=200, n=10, group=64, codes=256, scales=256, zeros=None, w=256, stride=200)
+    for bad in [dict(dtype=-1), dict(k=0), dict(n=-1), dict(group=33), dict(codes=8), dict(w=None), dict(w=264), dict(stride=192), dict(stride=204)]:
+        a = {**wide, **bad}
+        assert lib.castle_expand_4bit(*a.values(), None) < 0 and "castle_expand_4bit" in L.last_error(), bad
+
+
+def test_what_fits():
+    L, lib = _lib()
+    assert all(lib.castle_linear_4bit_fits(L.BF16, r, 4096) == 1 for r in (1, 8, 32)) and lib.castle_linear_4bit_fits(L.F32, 10, 4096) == 1
+    assert lib.castle_linear_4bit_fits(L.BF16, 32, 1 << 20) == 0 and lib.castle_linear_4bit_fits(L.F32, 11, 64) == 0 and lib.castle_linear_4bit_fits(7, 1, 64) == 0
+
+
+def test_refusals_of_the_host():
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit, castle_quantize_4bit
+    codes, scales, _ = castle_quantize_4bit(torch.randn(4, 64))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        castle_linear_4bit(torch.zeros(1, 64), codes, scales)
+    for bad in (lambda: castle_pack_4bit(torch.zeros(4)), lambda: castle_pack_4bit(torch.zeros(4, 4)), lambda: castle_quantize_4bit(torch.zeros(4, 4, dtype=torch.int32)),
+                lambda: castle_quantize_4bit(torch.zeros(4, 4), 40)):
+        with pytest.raises(ValueError):
+            bad()
