@@ -366,16 +366,17 @@ int castle_copy_pages(int32_t pools, void* const* ptr, const int64_t* stride_pag
 
 /* ---- products with weights of 4 bits -----------------------------------------
  * y = x W^T with W[n,k] = scales[n, k / group] * (code[n,k] - zeros[n, k / group]); group a power of two from 32 up; scales and zeros
- * (contiguous, out_features x ceil(in_features / group)) of `dtype`, zeros may be NULL (8 everywhere).  Codes: out_features rows of
- * ceil(in_features / 128) * 64 bytes; in the 64 bytes of 128 k the 32-bit word 4 t + j (t, j < 4) holds k = 32 j + 8 t + {0 .. 7}, its bits
- * 4 i .. 4 i + 3 k = 2 i of these and bits 16 + 4 i .. 16 + 4 i + 3 k = 2 i + 1 (i < 4); what k beyond in_features hold does not matter.  x: rows of
- * in_features elements, row_stride elements apart; y: contiguous (rows, out_features).  Sums in fp32; only y is rounded.
+ * (contiguous, out_features x ceil(in_features / group)) of `dtype`, zeros may be NULL (8 everywhere).  Codes: 2 KB for 16 rows and 256 k, those of 16
+ * rows one behind the other, then the next 16 (rows and k beyond the last hold anything): 16 bytes for each (g, t), g < 8, t < 4, t the faster, of row g and
+ * the first 128 k, the same of row g + 8, and both of the other 128 k; the 32-bit word j (j < 4) of the 16 bytes holds k = 32 j + 8 t + {0 .. 7}, its bits 4 i .. 4 i + 3 k = 2 i of these and bits
+ * 16 + 4 i .. 16 + 4 i + 3 k = 2 i + 1 (i < 4).  x: rows of in_features elements, row_stride elements apart; y: contiguous (rows, out_features).
+ * Sums in fp32; only y is rounded.
  * castle_linear_4bit_fits says whether a number of rows is supported (32 of 16 bits, 10 of 32, at the most).  castle_expand_4bit: W itself
  * in `dtype`, rows row_stride elements apart (a multiple of 16 bytes), for the products of more rows.
  */
 int castle_linear_4bit_fits(int32_t dtype, int32_t rows, int32_t in_features);
 int castle_linear_4bit(int32_t dtype, int32_t rows, int32_t in_features, int64_t out_features, int32_t group, const void* x,
-                       int64_t row_stride, const void* codes, const void* scales, const void* zeros, void* y, void* stream);
+                       int64_t row_stride, const void* codes, const void* scales, const void* zeros, void* y, int32_t* status, void* stream);
 int castle_expand_4bit(int32_t dtype, int32_t in_features, int64_t out_features, int32_t group, const void* codes, const void* scales,
                        const void* zeros, void* w, int64_t row_stride, void* stream);
 

@@ -217,7 +217,7 @@ _SIGNATURES = {
     "castle_write_pages": (ctypes.c_int, [_PR] + [_i32] * 3 + [_T] * 4 + [_PG] * 4 + [_vp, ctypes.c_int64] * 2 + [_i32, _vp, _vp, _vp]),
     "castle_copy_pages": (ctypes.c_int, [_i32] + [_vp] * 3 + [ctypes.c_int64] * 3 + [_vp, _vp, ctypes.c_int64, _vp]),
     "castle_linear_4bit_fits": (ctypes.c_int, [_i32] * 3),
-    "castle_linear_4bit": (ctypes.c_int, [_i32] * 3 + [ctypes.c_int64, _i32, _vp, ctypes.c_int64] + [_vp] * 5),
+    "castle_linear_4bit": (ctypes.c_int, [_i32] * 3 + [ctypes.c_int64, _i32, _vp, ctypes.c_int64] + [_vp] * 6),
     "castle_expand_4bit": (ctypes.c_int, [_i32] * 2 + [ctypes.c_int64, _i32] + [_vp] * 4 + [ctypes.c_int64, _vp]),
     "castle_set_kernel_events": (ctypes.c_int, [_i32, _vp, _vp]),
     "castle_selftest_mma_rate": (ctypes.c_int, [_i32, _i32, _i32, _vp, _vp, _vp]),

@@ -7,11 +7,12 @@ struct Codes {   // a weight's, as the kernels take them
 Codes check_codes(const Tensor& codes, const Tensor& scales, const Tensor& zeros, int64_t K, int64_t group, at::ScalarType dtype, const at::Device& dev) {
   const char* who = "castle_linear_4bit";
   need_plain(codes, who);
-  need(codes.dim() == 2 && codes.scalar_type() == at::kInt && codes.size(0) > 0 && codes.size(1) == (K + 127) / 128 * 16,
-       "castle_linear_4bit: codes of castle_pack_4bit for weights of the rows' length expected");
+  need(scales.defined() && scales.dim() == 2 && scales.size(0) > 0, "castle_linear_4bit: (out, groups) scales expected");
+  need(codes.dim() == 2 && codes.scalar_type() == at::kInt && codes.size(0) == (scales.size(0) + 15) / 16 && codes.size(1) == (K + 255) / 256 * 512,
+       "castle_linear_4bit: codes of castle_pack_4bit for weights of the rows' length and as many as the scales' expected");
   need(group >= 32 && group <= (1 << 24) && (group & (group - 1)) == 0, "castle_linear_4bit: the group size must be a power of two from 32 up");
   Codes c;
-  c.N = codes.size(0); c.K = K; c.group = group;
+  c.N = scales.size(0); c.K = K; c.group = group;
   const std::array<int64_t, 2> sizes{c.N, (K + group - 1) / group};
   for (const Tensor* t : {&scales, &zeros}) {
     if (!t->defined()) continue;
@@ -64,7 +65,7 @@ struct Linear4bitBackward : public Node {   // of x: the weights are frozen
       result[0] = at::empty(x_sizes, grads[0].options());
       return result;
     }
-    const Codes c = check_codes(restored(cs, {out_features, (K + 127) / 128 * 16}, at::kInt, dev, who), ss, zs, K, group, dtype, dev);
+    const Codes c = check_codes(restored(cs, {(out_features + 15) / 16, (K + 255) / 256 * 512}, at::kInt, dev, who), ss, zs, K, group, dtype, dev);
     result[0] = product(1, as_plain(grads[0]).view({rows, out_features}), expand_4bit(c, dtype, dev), rows).view(x_sizes);
     refuse_second(result, who, grads[0], *this, 0);   // (it does not depend on x)
     return result;
@@ -78,7 +79,6 @@ Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& own_scale
   need(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) <= (1 << 24), "castle_linear_4bit: (..., in) rows expected");
   const int64_t K = x.size(-1), rows = x.numel() / K;
   const Tensor scales = in_type_of(x, own_scales), zeros = in_type_of(x, own_zeros);
-  need(scales.defined(), "castle_linear_4bit: scales expected");
   const at::Device dev = x.device();
   const auto dtype = x.scalar_type();
   std::vector<int64_t> sizes = x.sizes().vec();
@@ -99,9 +99,10 @@ Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& own_scale
       y = at::empty(sizes, x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
       const Rows r = as_rows(x, rows, K);
       const int64_t es = x.element_size();
+      const Tensor status = status_word(dev.index());
       for (int64_t i = 0; i < rows; i += each)
         check(api.linear_4bit(dtype_code(dtype), (int32_t)std::min(each, rows - i), (int32_t)K, c.N, (int32_t)group, static_cast<char*>(r.data) + i * r.stride * es, r.stride,
-                              c.codes.data_ptr(), c.scales.data_ptr(), c.zeros.defined() ? c.zeros.data_ptr() : nullptr, static_cast<char*>(y.data_ptr()) + i * c.N * es,
+                              c.codes.data_ptr(), c.scales.data_ptr(), c.zeros.defined() ? c.zeros.data_ptr() : nullptr, static_cast<char*>(y.data_ptr()) + i * c.N * es, status.data_ptr<int32_t>(),
                               c10::cuda::getCurrentCUDAStream(dev.index()).stream()), who);
     } else {
       y = product(0, as_plain(x).view({rows, K}), expand_4bit(c, dtype, dev), rows).view(sizes);

@@ -246,18 +246,18 @@ def castle_copy_pages(pools, source, target):
 
 def castle_pack_4bit(codes):
     """(out, in) codes of 0 to 15, of any integer type and on any device, as `castle_linear_4bit` takes them: eight to an int32 (their order: the C
-    ABI's header), (out, ceil(in / 128) * 16)."""
+    ABI's header), (ceil(out / 16), ceil(in / 256) * 512)."""
     if codes.dim() != 2 or codes.is_floating_point() or codes.dtype == torch.bool:
         raise ValueError("castle_pack_4bit: (out, in) integer codes expected")
     n, k = codes.shape
-    blocks = (k + 127) // 128
-    padded = torch.full((n, blocks * 128), 8, dtype=torch.int32, device=codes.device)
-    padded[:, :k] = codes & 15
-    padded = padded.view(n, blocks, 4, 4, 8)                                        # 32 k, 8 k of these, k
-    word = torch.zeros((n, blocks, 4, 4), dtype=torch.int32, device=codes.device)
+    tiles, blocks = (n + 15) // 16, (k + 255) // 256 * 2                               # (of 128 k)
+    padded = torch.full((tiles * 16, blocks * 128), 8, dtype=torch.int32, device=codes.device)
+    padded[:n, :k] = codes & 15
+    padded = padded.view(tiles, 2, 8, blocks, 4, 4, 8)                              # half, row; block, 32 k, 8 k of these, k
+    word = torch.zeros((tiles, 2, 8, blocks, 4, 4), dtype=torch.int32, device=codes.device)
     for i in range(8):
         word |= padded[..., i] << (4 * (i // 2) + 16 * (i % 2))
-    return word.transpose(2, 3).reshape(n, blocks * 16)
+    return word.permute(0, 3, 1, 2, 5, 4).reshape(tiles, blocks * 256)
 
 
 def castle_quantize_4bit(weight, group_size: int = 64, zeros: bool = False):

@@ -9,24 +9,26 @@ def _lib():
     return _lib, _lib.load()
 
 
-def _unpack(packed, k):
+def _unpack(packed, n, k):
     """By the layout's description in the C ABI's header, a code at a time."""
-    out = torch.empty(packed.shape[0], k, dtype=torch.int64)
-    for i in range(k):
-        block, rest = divmod(i, 128)
-        j, t, o = rest // 32, rest % 32 // 8, rest % 8
-        word = packed[:, block * 16 + 4 * t + j].long() & 0xffffffff
-        out[:, i] = word >> (4 * (o // 2) + 16 * (o % 2)) & 15
+    out = torch.empty(n, k, dtype=torch.int64)
+    for r in range(n):
+        tile, half, g = r // 16, r % 16 // 8, r % 8
+        for i in range(k):
+            block, rest = divmod(i, 128)
+            j, t, o = rest // 32, rest % 32 // 8, rest % 8
+            word = int(packed[tile, block * 256 + half * 128 + (g * 4 + t) * 4 + j]) & 0xffffffff
+            out[r, i] = word >> (4 * (o // 2) + 16 * (o % 2)) & 15
     return out
 
 
-@pytest.mark.parametrize("n,k,dtype", [(3, 128, torch.uint8), (5, 1, torch.int64), (2, 300, torch.int32), (1, 127, torch.uint8)])
+@pytest.mark.parametrize("n,k,dtype", [(3, 128, torch.uint8), (5, 1, torch.int64), (33, 300, torch.int32), (1, 127, torch.uint8)])
 def test_layout(n, k, dtype):
     from lookahead_keys_attention_b200 import castle_pack_4bit
     codes = torch.randint(0, 16, (n, k), generator=torch.Generator().manual_seed(k)).to(dtype)
     packed = castle_pack_4bit(codes)
-    assert packed.dtype == torch.int32 and packed.shape == (n, (k + 127) // 128 * 16) and packed.is_contiguous()
-    assert torch.equal(_unpack(packed, k), codes.long())
+    assert packed.dtype == torch.int32 and packed.shape == ((n + 15) // 16, (k + 255) // 256 * 512) and packed.is_contiguous()
+    assert torch.equal(_unpack(packed, n, k), codes.long())
 
 
 @pytest.mark.parametrize("zeros", [False, True])
@@ -40,7 +42,7 @@ def test_quantised_weights(zeros, dtype):
     codes, scales, zp = castle_quantize_4bit(w, 64, zeros)
     assert scales.shape == (20, 4) and scales.dtype == dtype and (zp is None) == (not zeros)
     at = torch.arange(200) // 64
-    back = (_unpack(codes, 200).double() - (zp.double()[:, at] if zeros else 8.0)) * scales.double()[:, at]
+    back = (_unpack(codes, 20, 200).double() - (zp.double()[:, at] if zeros else 8.0)) * scales.double()[:, at]
     unit = torch.finfo(dtype).eps / 2
     size = (15 + (zp.double().abs()[:, at] if zeros else 0)) * unit
     assert bool(((back - w.double()).abs() <= scales.double()[:, at] * (0.5 + 2 * size)).all())
@@ -48,12 +50,12 @@ def test_quantised_weights(zeros, dtype):
 
 def test_arguments():
     L, lib = _lib()
-    good = dict(dtype=L.BF16, rows=2, k=200, n=10, group=64, x=256, stride=200, codes=256, scales=256, zeros=256, y=256)
+    good = dict(dtype=L.BF16, rows=2, k=200, n=10, group=64, x=256, stride=200, codes=256, scales=256, zeros=256, y=256, status=256)
     def call(**kw):
         a = {**good, **kw}
         return lib.castle_linear_4bit(*a.values(), None)
     for bad in [dict(dtype=3), dict(rows=0), dict(rows=33), dict(k=0), dict(k=(1 << 24) + 1), dict(n=0), dict(n=2 ** 31), dict(group=16), dict(group=48), dict(group=0), dict(x=None),
-                dict(x=257), dict(stride=-1), dict(codes=None), dict(codes=264), dict(scales=None), dict(scales=1), dict(zeros=3), dict(y=None), dict(y=255), dict(dtype=L.F32, rows=11)]:
+                dict(x=257), dict(stride=-1), dict(codes=None), dict(codes=264), dict(scales=None), dict(scales=1), dict(zeros=3), dict(y=None), dict(y=255), dict(status=None), dict(status=2), dict(dtype=L.F32, rows=11)]:
         assert call(**bad) < 0 and "castle_linear_4bit" in L.last_error(), bad
     wide = dict(dtype=L.BF16, k=200, n=10, group=64, codes=256, scales=256, zeros=None, w=256, stride=200)
     for bad in [dict(dtype=-1), dict(k=0), dict(n=-1), dict(group=33), dict(codes=8), dict(w=None), dict(w=264), dict(stride=192), dict(stride=204)]:
