@@ -18,6 +18,8 @@ Pass `inplace_cache=False` to get the reference's functional behaviour (each
 step then copies the caches first, and any cache can be decoded from again).
 Only caches this module returned (or took over through `cache_from_buffers`)
 are ever written; a cache made of the caller's own tensors is copied first.
+A layer of a batch over paged caches (`serve.py`) is another `cache=` of a single
+token: sequences of different lengths, whose pages the step updates in place.
 """
 from __future__ import annotations
 
@@ -28,6 +30,7 @@ from torch import nn
 from torch.nn.modules.module import _has_any_global_hook
 
 from . import _lib, ops
+from .serve import Linear4bit, PagedLayer
 
 Cache = namedtuple("Cache", ("U", "qu_cache", "kc_cache", "vc_cache"))
 
@@ -117,6 +120,13 @@ class Castle(nn.Module):
         self.combine_heads = nn.Linear(dim_inner, dim, bias=False)
         self.inplace_cache = inplace_cache
         self.cache_headroom = cache_headroom
+
+    def quantize_4bit(self, group_size=64, zeros=False):
+        """The projections' weights to 4 bits, for serving (`Linear4bit`: frozen, with a gradient for the layer's input)."""
+        for name in ("to_all_qkv", "combine_heads"):
+            if type(getattr(self, name)) is nn.Linear:
+                setattr(self, name, Linear4bit.from_linear(getattr(self, name), group_size, zeros))
+        return self
 
     def _split(self, qkvs):
         b, n, _ = qkvs.shape
@@ -215,7 +225,25 @@ class Castle(nn.Module):
         state = self._buffers_for_step((U, qu, kc, vc), seq_len, qu)
         return self._merge(out), ModuleCache(state, seq_len)
 
-    def forward(self, x, cache: Cache | None = None, return_next_cache=None):
+    def _forward_paged(self, x, layer: PagedLayer):
+        """A token of each sequence of a batch over paged caches."""
+        rotary, freqs, batch = self.rotary_emb, None, layer.batch
+        if x.shape[1] != 1 or x.shape[0] != batch.lengths.shape[0]:
+            raise ValueError(f"Castle: a paged cache takes one token of each of its batch's {batch.lengths.shape[0]} rows, not {tuple(x.shape[:2])}")
+        if torch._C._is_tracing():
+            raise RuntimeError("Castle: a step over paged caches cannot be traced")
+        if rotary is not None:
+            if type(rotary) is not _Rotary or "rotate" in rotary.__dict__:
+                raise RuntimeError("Castle: a rotary embedding of the caller's own has no place for sequences of different lengths")
+            freqs = rotary._buffers["freqs"]
+        host, plain, places = _lib.host(), self._plain_layer(), (layer.pools, batch.u_table, batch.table, batch.lengths)
+        out = None if plain is None else host.paged_layer_decode(x, *plain, self.scale, freqs, *places)
+        return self.combine_heads(host.paged_decode_packed(self._project(x), self.scale, freqs, *places)) if out is None else out
+
+    def forward(self, x, cache: Cache | PagedLayer | None = None, return_next_cache=None):
+        if isinstance(cache, PagedLayer):
+            out = self._forward_paged(x, cache)
+            return out if return_next_cache is False else (out, cache)
         host = _lib.host()
         seq_len = x.shape[1]
         is_inference = seq_len == 1

@@ -1022,6 +1022,46 @@ Tensor layer_decode(const Tensor& x, const Layer& l, const Tensor* caches, int64
   return at::linear(decode_packed(project(x, l), caches, t, scale, rotary), l.combine);
 }
 
+// A token of each sequence of a batch over paged caches: norm, projection, step and output projection as in token_layer.
+Tensor paged_token_layer(const Tensor& x, const Layer& l, const Tensor* pools, const Tensor& u_table, const Tensor& table, const Tensor& lengths, double scale,
+                         const Rotary& rotary) {
+  const at::Device dev = x.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
+  const auto dtype = x.scalar_type();
+  const int code = dtype_code(dtype);
+  const int64_t B = x.size(0), dim = x.size(2), H = l.heads, d = l.dim_head, inner = H * d, es = x.element_size(), N = l.combine.size(0);
+  const auto options = x.options().requires_grad(false).memory_format(c10::nullopt);
+  Tensor h = aligned_contiguous(x);
+  if (l.layer_norm) {
+    const Tensor y = at::empty({B, 1, dim}, options);
+    launch_layernorm(as_rows(h, B, dim), dtype, l.norm, l.norm_bias, *l.eps, y, Tensor(), stream);
+    h = y;
+  }
+  const bool rms = l.norm.defined() && !l.layer_norm;
+  Tensor packed = at::empty({B, 6 * inner}, options);
+  if (own_projection(code, B, dim, 6 * inner, es)) {
+    check(api.token_linear(code, (int32_t)B, (int32_t)dim, (int32_t)(6 * inner), h.data_ptr(), dim, rms ? l.norm.data_ptr() : nullptr, norm_eps(l), l.to_qkv.data_ptr(),
+                           packed.data_ptr(), 0, stream.stream()), "castle_token_linear");
+  } else {
+    if (rms) {
+      const Tensor y = at::empty({B, dim}, options);
+      check(api.rmsnorm_fwd(code, B, (int32_t)dim, h.data_ptr(), l.norm.data_ptr(), norm_eps(l), y.data_ptr(), nullptr, stream.stream()), "castle_rmsnorm_fwd");
+      h = y;
+    }
+    packed = at::mm(h.view({B, dim}), l.to_qkv.t());
+  }
+  castle_tensor_t news[6];
+  for (int i = 0; i < 6; ++i) news[i] = {static_cast<char*>(packed.data_ptr()) + kPackedOrder[i] * inner * es, 6 * inner, d, 6 * inner};
+  const Tensor o = paged_core(news, pools, u_table, table, lengths, B, H, d, dtype, scale, rotary, dev);
+  if (!own_projection(code, B, inner, N, es)) return at::mm(o.view({B, inner}), l.combine.t()).view({B, 1, N});
+  Tensor y = at::empty({B, 1, N}, options);
+  check(api.token_linear(code, (int32_t)B, (int32_t)inner, (int32_t)N, o.data_ptr(), inner, nullptr, 0.f, l.combine.data_ptr(), y.data_ptr(), 1, stream.stream()),
+        "castle_token_linear");
+  return y;
+}
+
 #include "host_4bit.h"
 
 // ------------------------------------------------------------------------------------------------ Python
@@ -1341,6 +1381,30 @@ PyObject* py_paged_decode_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// paged_layer_decode(x, <layer: 8>, scale, rotary freqs or None, four pools, U's table, table, lengths); None where it is watched(), or no plain layer
+PyObject* py_paged_layer_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arg_count(n, 15);
+    if (watched(a)) Py_RETURN_NONE;
+    const Tensor x = arg_tensor(a[0]);
+    const Layer l = arg_layer(a + 1);
+    const double scale = arg_float(a[9]);
+    Rotary rotary;
+    rotary.freqs = arg_optional(a[10]);
+    const std::vector<Tensor> pools = arg_caches(a[11]);
+    if (pools.size() != 4) throw std::runtime_error("castle: four cache tensors expected");
+    const Tensor u_table = arg_tensor(a[12]), table = arg_tensor(a[13]), lengths = arg_tensor(a[14]);
+    // no gradient flows through the cached step, so only the last projection could need a graph
+    if (!plain_layer(x, l) || x.size(1) != 1 || x.size(0) == 0 || (at::GradMode::is_enabled() && l.combine.requires_grad())) Py_RETURN_NONE;
+    Tensor out;
+    {
+      Unlocked u;
+      out = paged_token_layer(x, l, pools.data(), u_table, table, lengths, scale, rotary);
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
 // write_pages(four caches, four pools, U's table, table, lengths)
 PyObject* py_write_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -1510,6 +1574,7 @@ PyMethodDef methods[] = {{"bind", py_bind, METH_O, nullptr},
                          {"linear_cross_entropy", FAST(py_linear_cross_entropy), nullptr},
                          {"paged_decode_step", FAST(py_paged_decode_step), nullptr},
                          {"paged_decode_packed", FAST(py_paged_decode_packed), nullptr},
+                         {"paged_layer_decode", FAST(py_paged_layer_decode), nullptr},
                          {"write_pages", FAST(py_write_pages), nullptr},
                          {"copy_pages", FAST(py_copy_pages), nullptr},
                          {"linear_4bit", FAST(py_linear_4bit), nullptr},

@@ -211,6 +211,12 @@ def castle_linear_cross_entropy(x, weight, targets, ignore_index: int = -100, re
     return _lib.host().linear_cross_entropy(x, weight, targets, ignore_index, code)
 
 
+def _not_traced(who):
+    """Operators that write their caller's tensors: of the call a tracer would record nothing."""
+    if torch._C._is_tracing():
+        raise RuntimeError(f"{who}: cannot be traced")
+
+
 def castle_paged_decode_step(qc, kc, vc, qu, ku, vu, U_pages, qu_pages, kc_pages, vc_pages, U_table, table, lengths, scale: float):
     """`castle_decode_step` for sequences of different lengths whose caches lie in pages.  The six new-token tensors are
     (B, H, 1, d); the four pools (pages, H, page size, d), a head's rows of a page adjacent, page size a power of two from 16 to
@@ -223,12 +229,14 @@ def castle_paged_decode_step(qc, kc, vc, qu, ku, vu, U_pages, qu_pages, kc_pages
     batch; other pages of qu, kc and vc may be shared.  A negative length means no sequence: nothing is read or written for it, and its
     row of the result is zero.  A length that the tables have no place for, or a page outside its pool, gives NaN, and `check_status()`
     raises.  Returns out (B, H, 1, d)."""
+    _not_traced("castle_paged_decode_step")
     return _lib.host().paged_decode_step(qc, kc, vc, qu, ku, vu, U_pages, qu_pages, kc_pages, vc_pages, U_table, table, lengths, scale)
 
 
 def castle_write_pages(U, qu, kc, vc, U_pages, qu_pages, kc_pages, vc_pages, U_table, table, lengths):
     """A prompt's caches (B, H, N, d), as `Castle(..., return_next_cache=True)` returns them, into pages: the first `lengths[b]`
     (int32, at most N; none where negative) rows of each sequence, pools and tables as in `castle_paged_decode_step`."""
+    _not_traced("castle_write_pages")
     _lib.host().write_pages(U, qu, kc, vc, U_pages, qu_pages, kc_pages, vc_pages, U_table, table, lengths)
 
 
@@ -240,6 +248,7 @@ def castle_copy_pages(pools, source, target):
     """Pages `source[i]` to `target[i]` of a (pages, ...) pool, or of each of a list of pools of one shape, type and device, in place: what a
     fork of a sequence or a compaction of its pages moves.  A page is a multiple of 16 bytes.  `source` and `target` are lists, or
     int64 or int32 tensors on the host (a CUDA graph keeps the pages it was captured with); a target that is a source too, or a target twice, is refused."""
+    _not_traced("castle_copy_pages")
     pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
     _lib.host().copy_pages(pools, _page_numbers(source), _page_numbers(target))
 
