@@ -371,12 +371,15 @@ int castle_copy_pages(int32_t pools, void* const* ptr, const int64_t* stride_pag
  * the first 128 k, the same of row g + 8, and both of the other 128 k; the 32-bit word j (j < 4) of the 16 bytes holds k = 32 j + 8 t + {0 .. 7}, its bits 4 i .. 4 i + 3 k = 2 i of these and bits
  * 16 + 4 i .. 16 + 4 i + 3 k = 2 i + 1 (i < 4).  x: rows of in_features elements, row_stride elements apart; y: contiguous (rows, out_features).
  * Sums in fp32; only y is rounded.
- * castle_linear_4bit_fits says whether a number of rows is supported (32 of 16 bits, 10 of 32, at the most).  castle_expand_4bit: W itself
- * in `dtype`, rows row_stride elements apart (a multiple of 16 bytes), for the products of more rows.
+ * castle_linear_4bit_fits says whether a number of rows is supported (32 of 16 bits, 10 of 32, at the most).  castle_linear_4bit_tile: any number of
+ * rows of bf16 or fp16, at 16-byte boundaries, with W rounded to their type on its way to the tensor cores.  castle_expand_4bit: W itself in
+ * `dtype`, rows row_stride elements apart (a multiple of 16 bytes).
  */
 int castle_linear_4bit_fits(int32_t dtype, int32_t rows, int32_t in_features);
 int castle_linear_4bit(int32_t dtype, int32_t rows, int32_t in_features, int64_t out_features, int32_t group, const void* x,
                        int64_t row_stride, const void* codes, const void* scales, const void* zeros, void* y, int32_t* status, void* stream);
+int castle_linear_4bit_tile(int32_t dtype, int64_t rows, int32_t in_features, int64_t out_features, int32_t group, const void* x,
+                            int64_t row_stride, const void* codes, const void* scales, const void* zeros, void* y, int32_t* status, void* stream);
 int castle_expand_4bit(int32_t dtype, int32_t in_features, int64_t out_features, int32_t group, const void* codes, const void* scales,
                        const void* zeros, void* w, int64_t row_stride, void* stream);
 

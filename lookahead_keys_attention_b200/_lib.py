@@ -15,7 +15,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libcastle_b200.so"
-SOURCES = ["api.cu", "decode.cu", "selftest.cu", "convert.cu", "transform.cu", "token_linear.cu", "token_layer.cu", "linear.cu", "norm.cu", "layernorm.cu", "embedding.cu", "linear_ce.cu", "paged.cu", "pages.cu", "linear_4bit.cu", "fwd.cu", "bwd.cu", "bwd128.cu"]
+SOURCES = ["api.cu", "decode.cu", "selftest.cu", "convert.cu", "transform.cu", "token_linear.cu", "token_layer.cu", "linear.cu", "norm.cu", "layernorm.cu", "embedding.cu", "linear_ce.cu", "paged.cu", "pages.cu", "linear_4bit.cu", "linear_4bit_tile.cu", "fwd.cu", "bwd.cu", "bwd128.cu"]
 
 BF16, F16, F32 = 0, 1, 2
 
@@ -218,6 +218,7 @@ _SIGNATURES = {
     "castle_copy_pages": (ctypes.c_int, [_i32] + [_vp] * 3 + [ctypes.c_int64] * 3 + [_vp, _vp, ctypes.c_int64, _vp]),
     "castle_linear_4bit_fits": (ctypes.c_int, [_i32] * 3),
     "castle_linear_4bit": (ctypes.c_int, [_i32] * 3 + [ctypes.c_int64, _i32, _vp, ctypes.c_int64] + [_vp] * 6),
+    "castle_linear_4bit_tile": (ctypes.c_int, [_i32, ctypes.c_int64, _i32, ctypes.c_int64, _i32, _vp, ctypes.c_int64] + [_vp] * 6),
     "castle_expand_4bit": (ctypes.c_int, [_i32] * 2 + [ctypes.c_int64, _i32] + [_vp] * 4 + [ctypes.c_int64, _vp]),
     "castle_set_kernel_events": (ctypes.c_int, [_i32, _vp, _vp]),
     "castle_selftest_mma_rate": (ctypes.c_int, [_i32, _i32, _i32, _vp, _vp, _vp]),

@@ -86,6 +86,7 @@ struct Api {
   decltype(&castle_copy_pages) copy_pages;
   decltype(&castle_linear_4bit_fits) linear_4bit_fits;
   decltype(&castle_linear_4bit) linear_4bit;
+  decltype(&castle_linear_4bit_tile) linear_4bit_tile;
   decltype(&castle_expand_4bit) expand_4bit;
 } api{};
 
@@ -1550,7 +1551,7 @@ PyObject* py_bind(PyObject*, PyObject* d) {
     CASTLE_BIND(embedding_fwd); CASTLE_BIND(embedding_bwd_workspace_bytes); CASTLE_BIND(embedding_bwd);
     CASTLE_BIND(linear_ce_workspace_bytes); CASTLE_BIND(linear_ce_fwd); CASTLE_BIND(linear_ce_bwd);
     CASTLE_BIND(paged_decode_workspace_bytes); CASTLE_BIND(paged_decode_step); CASTLE_BIND(write_pages); CASTLE_BIND(copy_pages);
-    CASTLE_BIND(linear_4bit_fits); CASTLE_BIND(linear_4bit); CASTLE_BIND(expand_4bit);
+    CASTLE_BIND(linear_4bit_fits); CASTLE_BIND(linear_4bit); CASTLE_BIND(linear_4bit_tile); CASTLE_BIND(expand_4bit);
 #undef CASTLE_BIND
     PyObject* module = PyImport_ImportModule("torch.utils._device");
     Py_XDECREF(device_context);

@@ -72,6 +72,15 @@ struct Linear4bitBackward : public Node {   // of x: the weights are frozen
   }
 };
 
+// Whether 9 to 32 rows of 16 bits go through the codes rather than through tiles, by what either took (us, codes / tiles, bf16: 16 x 4096 -> 16384
+// 22.6 / 19.2, 16 x 4096 -> 4096 10.8 / 20.7, 32 x 4096 -> 16384 46.7 / 19.4, 32 x 4096 -> 4096 17.6 / 20.7, 32 x 512 -> 2048 5.9 / 6.6, 24 x 16384 -> 1024
+// 23.8 / 56.8, 24 x 1000 -> 50021 with zero points 36.4 / 34.6): the one by the number of weights, the other by steps of 128 k and rounds of 148 tiles.
+bool few_rows(int64_t rows, int64_t K, int64_t N) {
+  const double weights = 1e-6 * (double)K * (double)N, codes = rows <= 16 ? 3.3 + 0.29 * weights : 5.0 + 0.64 * weights;
+  const double tiles = (double)(((N + 127) / 128 + 147) / 148) * (5.0 + 0.45 * (double)((K + 127) / 128));
+  return codes <= tiles;
+}
+
 Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& own_scales, const Tensor& own_zeros, int64_t group) {
   const char* who = "castle_linear_4bit";
   need_plain(x, who);
@@ -91,11 +100,13 @@ Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& own_scale
     const c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
     const at::NoGradGuard no_grad;
     sizes.back() = c.N;
-    // The rows of a few tokens go through the codes, as many at a time as the kernel takes; more of them through the weights at full width.
+    // The rows of a few tokens go through the codes, fp32 ones as many at a time as the kernel takes; more rows of 16 bits through tiles of weights that
+    // are unpacked on their way to the tensor cores, and of 32 through the weights at full width (their products are FMA).
     const int64_t most = dtype == at::kFloat ? 10 : 32, turns = (rows + most - 1) / most, each = turns > 0 ? (rows + turns - 1) / turns : 0;
+    const bool few = dtype == at::kFloat ? turns <= 2 : rows <= 8 || (turns == 1 && few_rows(rows, K, c.N));
     if (rows == 0) {
       y = at::empty(sizes, x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
-    } else if (turns <= 2 && api.linear_4bit_fits(dtype_code(dtype), (int32_t)each, (int32_t)K)) {
+    } else if (few && api.linear_4bit_fits(dtype_code(dtype), (int32_t)each, (int32_t)K)) {
       y = at::empty(sizes, x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
       const Rows r = as_rows(x, rows, K);
       const int64_t es = x.element_size();
@@ -104,6 +115,19 @@ Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& own_scale
         check(api.linear_4bit(dtype_code(dtype), (int32_t)std::min(each, rows - i), (int32_t)K, c.N, (int32_t)group, static_cast<char*>(r.data) + i * r.stride * es, r.stride,
                               c.codes.data_ptr(), c.scales.data_ptr(), c.zeros.defined() ? c.zeros.data_ptr() : nullptr, static_cast<char*>(y.data_ptr()) + i * c.N * es, status.data_ptr<int32_t>(),
                               c10::cuda::getCurrentCUDAStream(dev.index()).stream()), who);
+    } else if (dtype != at::kFloat) {
+      y = at::empty(sizes, x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+      Rows r = as_rows(x, rows, K);
+      if (reinterpret_cast<uintptr_t>(r.data) % 16 != 0 || r.stride % 8 != 0 || (r.stride < K && rows > 1)) {   // rows at 16-byte boundaries, one behind the other
+        const int64_t ld = (K + 7) / 8 * 8;
+        const Tensor t = at::empty({rows, ld}, x.options().requires_grad(false).memory_format(c10::nullopt));
+        t.narrow(1, 0, K).copy_(r.keep.reshape({rows, K}));
+        r = {t, t.data_ptr(), rows, K, ld};
+      }
+      const Tensor status = status_word(dev.index());
+      check(api.linear_4bit_tile(dtype_code(dtype), rows, (int32_t)K, c.N, (int32_t)group, r.data, r.stride, c.codes.data_ptr(), c.scales.data_ptr(),
+                                 c.zeros.defined() ? c.zeros.data_ptr() : nullptr, y.data_ptr(), status.data_ptr<int32_t>(),
+                                 c10::cuda::getCurrentCUDAStream(dev.index()).stream()), who);
     } else {
       y = product(0, as_plain(x).view({rows, K}), expand_4bit(c, dtype, dev), rows).view(sizes);
     }

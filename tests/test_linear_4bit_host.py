@@ -57,6 +57,11 @@ def test_arguments():
     for bad in [dict(dtype=3), dict(rows=0), dict(rows=33), dict(k=0), dict(k=(1 << 24) + 1), dict(n=0), dict(n=2 ** 31), dict(group=16), dict(group=48), dict(group=0), dict(x=None),
                 dict(x=257), dict(stride=-1), dict(codes=None), dict(codes=264), dict(scales=None), dict(scales=1), dict(zeros=3), dict(y=None), dict(y=255), dict(status=None), dict(status=2), dict(dtype=L.F32, rows=11)]:
         assert call(**bad) < 0 and "castle_linear_4bit" in L.last_error(), bad
+    tile = dict(dtype=L.BF16, rows=100, k=200, n=10, group=64, x=256, stride=200, codes=256, scales=256, zeros=None, y=256, status=256)
+    for bad in [dict(dtype=L.F32), dict(rows=0), dict(rows=2 ** 31), dict(k=0), dict(n=0), dict(group=24), dict(x=None), dict(x=264), dict(stride=196), dict(stride=192), dict(codes=8),
+                dict(scales=None), dict(scales=1), dict(zeros=3), dict(y=None), dict(y=1), dict(status=None)]:
+        a = {**tile, **bad}
+        assert lib.castle_linear_4bit_tile(*a.values(), None) < 0 and "castle_linear_4bit_tile" in L.last_error(), bad
     wide = dict(dtype=L.BF16, k=200, n=10, group=64, codes=256, scales=256, zeros=None, w=256, stride=200)
     for bad in [dict(dtype=-1), dict(k=0), dict(n=-1), dict(group=33), dict(codes=8), dict(w=None), dict(w=264), dict(stride=192), dict(stride=204)]:
         a = {**wide, **bad}
