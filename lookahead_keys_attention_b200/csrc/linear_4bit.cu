@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) castle_linear_4bit_kernel(const
   if (bulk) {
     const int rest = blocks * 256 - have;                                      // the last block's k that there are not
     for (int e = threadIdx.x; e < cols * rest; e += kL4Threads) xs[(int64_t)(e / rest) * p.ldk + have + e % rest] = Elem<E>::from_f(0.f);
-    mbar_wait(&bar, 0, &abort_flag);
+    if (!mbar_wait_ok(&bar, 0, &abort_flag)) mbar_drain(&bar, 0);
   } else {
     const int eights = blocks * 32;
     for (int e = threadIdx.x; e < cols * eights; e += kL4Threads) {

@@ -308,6 +308,56 @@ def test_a_quantised_layer_trains_what_is_in_front_of_it():
     assert not any(p.requires_grad for p in q.to_all_qkv.parameters())
 
 
+def test_threads_on_one_stream():
+    """Steps and products of several host threads: what a call's launches share is the stream's, so they must not mix."""
+    import threading
+    from lookahead_keys_attention_b200 import PagedCache, check_status
+
+    def server(seed, dtype, heads, quantised):
+        layers = _layers(2, dtype, heads=heads, prenorm=True)
+        if quantised:
+            for m in layers:
+                m.quantize_4bit(32, zeros=True)
+        gen = torch.Generator("cuda").manual_seed(seed)
+        xs = torch.randn(60, 3, 1, 256, device="cuda", generator=gen).to(dtype)
+
+        @torch.no_grad()
+        def go():
+            cache = PagedCache(2, 60, heads, 64, 16, dtype=dtype)
+            prompt = torch.ones(3, 37, 256, device="cuda", dtype=dtype)
+            seqs = [cache.add() for _ in range(3)]
+            for i, c in enumerate(_prompt(layers, prompt)[1]):
+                cache.write(seqs, i, c)
+            batch, outs = cache.batch(seqs), []
+            for x in xs:
+                outs.append(_paged_token(layers, x, batch))
+                batch.advance()
+            return torch.cat(outs, 1)
+
+        return go
+
+    work = [server(1, torch.bfloat16, 4, True), server(2, torch.float32, 8, False), server(3, torch.float16, 2, True), server(4, torch.bfloat16, 6, False)]
+    want = [w() for w in work]
+    torch.cuda.synchronize()
+    got, errors = [None] * len(work), []
+
+    def run(i):
+        try:
+            got[i] = work[i]()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(work))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    check_status()
+    assert not errors, errors
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_traced_calls():
     from lookahead_keys_attention_b200 import Castle, Linear4bit, PagedCache, castle_copy_pages
     m = Linear4bit.from_linear(nn.Linear(64, 32).cuda(), 32)
