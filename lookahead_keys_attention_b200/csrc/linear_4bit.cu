@@ -409,7 +409,9 @@ template <typename T, bool ZEROS> __global__ void __launch_bounds__(256) castle_
   }
 }
 
-// How K is shared out: the largest number of blocks that a warp walks through decides.
+// How K is shared out: the longest walk of a warp decides, its blocks and three tenths of one for each row tile that it begins and leaves (us with 16 / 8 /
+// 4 warps to a tile, bf16: 1 x 4096 -> 4096 5.5 / 5.3 / 6.1, 8 x 4096 -> 16384 13.6 / 14.7 / 13.1, 1 x 8192 -> 32768 34.4 / 33.2 / 34.7, 1 x 16384 -> 1024 6.6 / 12.5 /
+// 12.3).  Two CTAs of eight warps on an SM instead of one of sixteen: the same within 5 %.
 static bool linear_4bit_plan(Linear4Params& p, int cols, size_t& smem) {
   int64_t best = -1;
   for (int kc = 1; kc <= 8 && kc <= p.blocks; kc *= 2) {
@@ -420,7 +422,7 @@ static bool linear_4bit_plan(Linear4Params& p, int cols, size_t& smem) {
     for (int ks = 16; ks >= 1; ks /= 2) {
       if (ks > least) continue;   // (every warp has a block)
       const int side = kL4Warps / ks;
-      const int64_t walk = (int64_t)((per + side - 1) / side) * ((most + ks - 1) / ks);
+      const int64_t walk = (int64_t)((per + side - 1) / side) * (10 * ((most + ks - 1) / ks) + 3);
       // larger clusters end with a barrier of theirs and loads from each other: for a tenth and more
       if (best < 0 || walk * 10 < best * (kc > p.kc ? 9 : 10)) {
         best = walk;
