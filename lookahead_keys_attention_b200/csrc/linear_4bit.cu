@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) castle_linear_4bit_kernel(const
   const int cols = p.rows * parts;
   float* red = reinterpret_cast<float*>(raw);                                  // [warp][tile][16][8]
   E* xs = reinterpret_cast<E*>(raw + (size_t)kL4Warps * kL4Tiles * 128 * sizeof(float));   // [column][ldk]
-  float* sums = reinterpret_cast<float*>(xs + (size_t)cols * p.ldk);           // [stretch][column], with zero points
+  float* sums = reinterpret_cast<float*>(xs + (size_t)cols * p.ldk);           // [stretch][pair of columns][4]
   if (threadIdx.x == 0) {
     mbar_init(&bar, 1);
     mbar_fence_init();
@@ -254,7 +254,11 @@ __global__ void __launch_bounds__(kL4Threads, 1) castle_linear_4bit_kernel(const
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-      if (e < cols * stretches && lane8 == 0) sums[k * NT * 8 + col] = sum;
+      // twice, as the sums of a lane's two rows begin with them; without zero points times -24, the codes' offset
+      if (e < cols * stretches && lane8 == 0) {
+        float* dst = sums + (k * NT * 4 + (col >> 1)) * 4 + (col & 1);
+        dst[0] = dst[2] = ZEROS ? sum : -24.f * sum;
+      }
     }
     __syncthreads();
   }
@@ -267,7 +271,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) castle_linear_4bit_kernel(const
   const E* column[NT];   // (columns that there are not repeat the last one; nobody reads their results)
 #pragma unroll
   for (int i = 0; i < NT; ++i) column[i] = xs + (int64_t)min(i * 8 + g, cols - 1) * p.ldk + 8 * t;
-  const int x0 = (b0 - first) * 256, sum0 = (b0 - first) * SPS * NT * 8 + 2 * t;
+  const int x0 = (b0 - first) * 256, sum0 = (b0 - first) * SPS * NT * 16 + 4 * t;
   int left = nb, x_at = x0, sum_at = sum0;
   for (int batch = tile_begin; batch < tile_end; batch += side * GM) {
     const int batch_end = min(batch + side * GM, tile_end);
@@ -285,11 +289,14 @@ __global__ void __launch_bounds__(kL4Threads, 1) castle_linear_4bit_kernel(const
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
             if constexpr (SUMS) {
-              const float2 sum = *reinterpret_cast<const float2*>(sums + sum_at + span * NT * 8 + i * 8);
-              constexpr float offset = sizeof(T) == 2 ? -16.f : 8.f;
-              const float z0 = ZEROS ? offset - group_value<T, SPB>(zero[ZEROS ? s : 0][0], span / per) : -24.f,
-                          z1 = ZEROS ? offset - group_value<T, SPB>(zero[ZEROS ? s : 0][1], span / per) : -24.f;
-              c[h][i][0] = z0 * sum.x; c[h][i][1] = z0 * sum.y; c[h][i][2] = z1 * sum.x; c[h][i][3] = z1 * sum.y;
+              const float4 sum = *reinterpret_cast<const float4*>(sums + sum_at + span * NT * 16 + i * 16);
+              if constexpr (ZEROS) {
+                constexpr float offset = sizeof(T) == 2 ? -16.f : 8.f;
+                const float z0 = offset - group_value<T, SPB>(zero[s][0], span / per), z1 = offset - group_value<T, SPB>(zero[s][1], span / per);
+                c[h][i][0] = z0 * sum.x; c[h][i][1] = z0 * sum.y; c[h][i][2] = z1 * sum.z; c[h][i][3] = z1 * sum.w;
+              } else {
+                c[h][i][0] = sum.x; c[h][i][1] = sum.y; c[h][i][2] = sum.z; c[h][i][3] = sum.w;
+              }
             } else {
 #pragma unroll
               for (int q = 0; q < 4; ++q) c[h][i][q] = 0.f;
@@ -347,7 +354,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) castle_linear_4bit_kernel(const
         }
         fetch(s);
         x_at += 256;
-        sum_at += SPS * NT * 8;
+        sum_at += SPS * NT * 16;
         if (--left == 0) {
           left = nb; x_at = x0; sum_at = sum0;
 #pragma unroll
@@ -409,20 +416,20 @@ template <typename T, bool ZEROS> __global__ void __launch_bounds__(256) castle_
   }
 }
 
-// How K is shared out: the longest walk of a warp decides, its blocks and three tenths of one for each row tile that it begins and leaves (us with 16 / 8 /
+// How K is shared out: the longest walk of a warp decides, its blocks and a fifth of one for each row tile that it begins and leaves (us with 16 / 8 /
 // 4 warps to a tile, bf16: 1 x 4096 -> 4096 5.5 / 5.3 / 6.1, 8 x 4096 -> 16384 13.6 / 14.7 / 13.1, 1 x 8192 -> 32768 34.4 / 33.2 / 34.7, 1 x 16384 -> 1024 6.6 / 12.5 /
 // 12.3).  Two CTAs of eight warps on an SM instead of one of sixteen: the same within 5 %.
 static bool linear_4bit_plan(Linear4Params& p, int cols, size_t& smem) {
   int64_t best = -1;
   for (int kc = 1; kc <= 8 && kc <= p.blocks; kc *= 2) {
     const int most = (p.blocks + kc - 1) / kc, least = p.blocks / kc, ldk = most * 256 + 32;   // (columns 64 bytes apart in the banks)
-    const size_t bytes = (size_t)kL4Warps * kL4Tiles * 128 * sizeof(float) + (size_t)cols * ldk * 2 + (size_t)most * 8 * (cols <= 8 ? 8 : cols <= 16 ? 16 : 32) * sizeof(float);
+    const size_t bytes = (size_t)kL4Warps * kL4Tiles * 128 * sizeof(float) + (size_t)cols * ldk * 2 + (size_t)most * 8 * (cols <= 8 ? 16 : cols <= 16 ? 32 : 64) * sizeof(float);
     if (bytes > kL4Smem) continue;
     const int clusters = std::min(p.tiles, kc == 8 ? 15 : kc == 4 ? 36 : 148 / kc), per = (p.tiles + clusters - 1) / clusters;
     for (int ks = 16; ks >= 1; ks /= 2) {
       if (ks > least) continue;   // (every warp has a block)
       const int side = kL4Warps / ks;
-      const int64_t walk = (int64_t)((per + side - 1) / side) * (10 * ((most + ks - 1) / ks) + 3);
+      const int64_t walk = (int64_t)((per + side - 1) / side) * (10 * ((most + ks - 1) / ks) + 2);
       // larger clusters end with a barrier of theirs and loads from each other: for a tenth and more
       if (best < 0 || walk * 10 < best * (kc > p.kc ? 9 : 10)) {
         best = walk;
