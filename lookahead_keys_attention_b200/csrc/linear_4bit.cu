@@ -9,6 +9,8 @@
 //     y[n] = sum over groups of  scale * (sum of (16 + code) x  -  (16 + zero) * sum of x)
 // (the fp32 sums are some six times larger that way than with code - 8, which costs them less than three of 24 bits where y has 8 or 11).
 // fp32 rows enter as three columns each, the bf16 parts of their 24 bits (8 bits each, exact), and codes as code - 8 (exact).
+// For the types with fp32's range the codes enter as 2^-16 of that, and y is 2^16 of the sums: a group's sum is some hundred times larger than what
+// its scale leaves of it, and would be infinite for rows near the type's largest number.
 // (tcgen05 products want 128 rows of x or of W a step in shared memory, written there by the threads that unpack them: at a
 // few columns the unpacking is the work, and a warp has its operand in registers already.)
 //
@@ -47,18 +49,30 @@ struct Linear4Params {
 template <typename T> struct CodeType { using type = T; static constexpr int parts = 1; };
 template <> struct CodeType<float> { using type = __nv_bfloat16; static constexpr int parts = 3; };
 
-// Codes 2 i and 2 i + 1 of the eight in a word as a pair of 16-bit numbers: 16 + code for rows of 16 bits, code - 8 for the parts of fp32 ones.  `mask`
-// and `bits` are the kernel's arguments: with constants in their place the and and the or became an operation each, and moves of the constants.
+// Codes 2 i and 2 i + 1 of the eight in a word as a pair of 16-bit numbers: `unit` times 16 + code for rows of 16 bits, code - 8 for the parts of fp32 ones.
+// `mask` and `bits` are the kernel's arguments: with constants in their place the and and the or became an operation each, and moves of the constants.
 template <typename T> struct CodeBits;
-template <> struct CodeBits<__nv_bfloat16> { static constexpr int at = 3; static constexpr uint32_t mask = 0x00780078u, bits = 0x41804180u; };   // at: the top four
-template <> struct CodeBits<__half> { static constexpr int at = 6; static constexpr uint32_t mask = 0x03c003c0u, bits = 0x4c004c00u; };          // of the mantissa's bits
-template <> struct CodeBits<float> { static constexpr int at = 0; static constexpr uint32_t mask = 0x000f000fu, bits = 0x43004300u; };           // 128 + code in bf16
+template <> struct CodeBits<__nv_bfloat16> {   // at: the top four of the mantissa's bits
+  static constexpr int at = 3;
+  static constexpr uint32_t mask = 0x00780078u, bits = 0x39803980u;
+  static constexpr float unit = 1.f / 65536.f;
+};
+template <> struct CodeBits<__half> {
+  static constexpr int at = 6;
+  static constexpr uint32_t mask = 0x03c003c0u, bits = 0x4c004c00u;
+  static constexpr float unit = 1.f;
+};
+template <> struct CodeBits<float> {           // 128 + code in bf16
+  static constexpr int at = 0;
+  static constexpr uint32_t mask = 0x000f000fu, bits = 0x3b003b00u;
+  static constexpr float unit = 1.f / 65536.f;
+};
 template <typename T> __device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, uint32_t mask, uint32_t bits) {
   const int right = 4 * i - CodeBits<T>::at;
   uint32_t v = right >= 0 ? w >> right : w << -right;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(v), "r"(mask), "r"(bits));   // v & mask | bits
   if constexpr (sizeof(T) == 4) {
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(136.f));
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(136.f * CodeBits<T>::unit));
     v = *reinterpret_cast<const uint32_t*>(&d);
   }
   return v;
@@ -247,7 +261,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) castle_linear_4bit_kernel(const
             float v[8];
             load8<E>(xs + (int64_t)col * p.ldk + (k * SPAN + i) * 32 + lane8 * 8, v);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) sum += v[q];
+            for (int q = 0; q < 8; ++q) sum = fmaf(v[q], CodeBits<T>::unit, sum);
           }
         }
       }
@@ -384,7 +398,7 @@ __global__ void __launch_bounds__(kL4Threads, 1) castle_linear_4bit_kernel(const
           for (int w = 0; w < p.ks; ++w) sum += p.kc > 1 ? cluster_load(src + w * GM * NT * 128, r) : src[w * GM * NT * 128];
         }
       }
-      if (n < p.N) store1<T>(reinterpret_cast<T*>(p.y) + (int64_t)token * p.N + n, sum);
+      if (n < p.N) store1<T>(reinterpret_cast<T*>(p.y) + (int64_t)token * p.N + n, sum * (1.f / CodeBits<T>::unit));
     }
     if (p.kc > 1) cluster_sync(); else __syncthreads();
   }

@@ -300,7 +300,8 @@ def castle_linear_4bit(x, codes, scales, zeros=None, group_size: int = 64):
     none.  x (..., in); `codes` of `castle_pack_4bit` or `castle_quantize_4bit`; scales and zero points (out, ceil(in / group_size)) of x's type (under autocast they
     are cast to it), group_size a power of two from 32 up.  For a few rows (up to 8, and up to 32 where that is faster) the codes are read as they are, the weights are not rounded, and sums
     are fp32; many rows are products with the weights rounded to x's type (and code - zero before that, where it is no whole number).  The gradient of x
-    is a product with the weights at full width; the weights are frozen.  With zero points an infinity in x may give NaN."""
+    is a product with the weights at full width; the weights are frozen.  An infinity in x may give NaN in place of
+    an infinity (for 16-bit rows, and with zero points)."""
     if torch._C._is_tracing():
         return _TracedCall.apply(lambda *t: _lib.host().linear_4bit(*t, group_size), x, codes, scales, zeros)
     return _lib.host().linear_4bit(x, codes, scales, zeros, group_size)

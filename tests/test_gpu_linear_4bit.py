@@ -107,6 +107,24 @@ def test_fp32_rows_of_all_sizes():
     _check(y[2:], x[2:], w, parts, EPS[torch.float32], False)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_rows_near_the_types_ends(dtype, zeros):
+    """Finite results of rows whose groups' sums, before their scales, are beyond fp32's range; and rows far below one.  (Small ones: what products with codes
+    lose below fp32's smallest normal number, 2^-149 each of 2^-16 of them, is 2^-133 of a scale a product.)"""
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
+    gen = torch.Generator("cuda").manual_seed(6)
+    codes, scales, zero, w, parts = _weight(100, 640, 64, dtype, zeros, gen)
+    for top, factor in ((torch.finfo(dtype).max, 2.0 ** -16), (1e-32, 1.0)):
+        small, part = (scales.float() * factor).to(dtype), (parts[0], parts[1] * factor, parts[2])   # (exact: a power of two)
+        for rows in (1, 3, 8):
+            x = ((torch.rand(rows, 640, device="cuda", generator=gen) * 0.5 + 0.5) * top).to(dtype)
+            y = castle_linear_4bit(x, castle_pack_4bit(codes), small, zero)
+            assert bool(y.isfinite().all())
+            lift = 1.0 / (x.double().abs().max() * factor)                                           # (the tolerance's constant is for results near one)
+            _check(y.double() * lift, x.double() * lift, w * factor, part, EPS[dtype], rows > 2)
+
+
 def test_a_row_does_not_change_another():
     from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
     gen = torch.Generator("cuda").manual_seed(4)
