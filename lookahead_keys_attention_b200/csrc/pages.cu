@@ -150,6 +150,7 @@ extern "C" int castle_write_pages(const castle_problem_t* p, int32_t page_size, 
   if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return reject("%s: page size %d is not a power of two from 16 to 1024", who, page_size);
   if (u_pages <= 0 || pages <= 0 || table_width <= 0) return reject("%s: empty pools or tables", who);
   if ((int64_t)table_width * page_size > INT32_MAX - 1024) return reject("%s: %d pages of %d positions are too many", who, table_width, page_size);
+  if (p->seq_len > INT32_MAX - 1024) return reject("%s: %d positions are too many", who, p->seq_len);   // (a tile's rows past the last one are counted in 32 bits)
   if (!u_table || !table || !lengths || !status) return reject("%s: null table, lengths or status", who);
   if (((uintptr_t)u_table | (uintptr_t)table | (uintptr_t)lengths | (uintptr_t)status) % 4) return reject("%s: tables, lengths and status must be 4-byte aligned", who);
   if (u_table_stride < 0 || table_stride < 0) return reject("%s: negative table strides", who);

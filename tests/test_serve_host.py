@@ -52,6 +52,11 @@ def test_write_arguments(bad):
     assert _paged(L, lib, "castle_write_pages", **bad) < 0 and L.last_error()
 
 
+def test_write_of_positions_at_the_end_of_32_bits():
+    L, lib = _lib()
+    assert _paged(L, lib, "castle_write_pages", batch=1, heads=1, seq_len=2 ** 31 - 1000) < 0 and "too many" in L.last_error()
+
+
 def test_workspace_grows_with_what_a_call_may_hold():
     L, lib = _lib()
     size = lambda width, **kw: lib.castle_paged_decode_workspace_bytes(ctypes.byref(_problem(L, **kw)), 64, width)  # noqa: E731
