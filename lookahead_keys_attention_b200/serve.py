@@ -89,6 +89,7 @@ class PagedCache:
         self._kv, self._u = _Pool(pages), _Pool(u_pages)
         self._sequences, self._next, self._batches = {}, 0, weakref.WeakSet()
 
+    @torch.inference_mode(False)   # (what a cache made in inference mode holds is written outside it as well)
     def _allocate(self, pages, u_pages):
         new = lambda n: torch.empty(self.layers, n, self.heads, self.page_size, self.dim_head, dtype=self.dtype, device=self.device)  # noqa: E731
         self.U, self.qu, self.kc, self.vc = new(u_pages), new(pages), new(pages), new(pages)
@@ -142,6 +143,7 @@ class PagedCache:
             raise ValueError(f"PagedCache: there is no layer {layer}")
         return self.U[layer], self.qu[layer], self.kc[layer], self.vc[layer]
 
+    @torch.inference_mode(False)
     def _to_device(self, values):
         t = torch.tensor(values, dtype=torch.int32)
         return (t.pin_memory() if self.device.type == "cuda" else t).to(self.device, non_blocking=True)
@@ -162,13 +164,21 @@ class PagedCache:
         pools, sequences = self._pools(layer), [self._of(q) for q in seqs]
         if any(s.length not in (0, n) for s in sequences) or any(s.batch and s.batch() for s in sequences):
             raise ValueError("PagedCache: a prompt can be written only to a sequence without positions that is in no batch")
-        if n == 0:
+        if any(self._kv.held[p] > 1 for s in sequences for p in s.pages):
+            raise ValueError("PagedCache: a prompt cannot be written to pages that a fork shares")
+        if n == 0 or not seqs:
             return
         self._reserve([(s, n) for s in sequences])
+        before = [s.length for s in sequences]
         for s in sequences:
             s.length = n
-        u, kv, lengths = self._tables(sequences, max(len(s.pages) for s in sequences))
-        ops.castle_write_pages(U, qu, kc, vc, *pools, u, kv, lengths)
+        try:
+            u, kv, lengths = self._tables(sequences, max(len(s.pages) for s in sequences))
+            ops.castle_write_pages(U, qu, kc, vc, *pools, u, kv, lengths)
+        except BaseException:
+            for s, k in zip(sequences, before):   # (the pages stay theirs)
+                s.length = k
+            raise
 
     def fork(self, seq, count: int = 1):
         """`count` more sequences with the positions of `seq` (between two tokens of all layers): its full pages of qu, kc and vc are shared, the last one, if it is not full, and U's are copied,
@@ -267,6 +277,7 @@ class PagedBatch:
     def _sequences(self):
         return [None if q is None else self.cache._of(q) for q in self.seqs]
 
+    @torch.inference_mode(False)
     def _upload(self):
         sequences = self._sequences()
         self._width = max([self._width] + [len(s.pages) for s in sequences if s])

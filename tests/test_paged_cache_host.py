@@ -165,6 +165,56 @@ def test_a_forked_prompt_shares_its_full_pages(plain):
     assert cache.free_pages() == (40 - 2 - 4, 40 - 4 * 3)
 
 
+def test_pages_that_forks_share_take_no_prompt(plain):
+    cache = _cache()
+    a = cache.add()
+    z = torch.zeros(1, 1, 40, 16, dtype=torch.float64)
+    cache.write([a], 0, (z, z, z, z))
+    (b,) = cache.fork(a)
+    for q in (a, b):
+        with pytest.raises(ValueError, match="shares"):
+            cache.write([q], 1, (z, z, z, z))
+    cache.free(b)
+    cache.write([a], 1, (z, z, z, z))
+
+
+def test_a_prompt_that_was_not_written_is_not_counted(plain, monkeypatch):
+    cache = _cache()
+    a = cache.add()
+    z = torch.zeros(1, 1, 40, 16, dtype=torch.float64)
+    with monkeypatch.context() as m:
+        def refuse(*_):
+            raise RuntimeError("refused")
+        m.setattr(ops, "castle_write_pages", refuse)
+        with pytest.raises(RuntimeError, match="refused"):
+            cache.write([a], 0, (z, z, z, z))
+    assert cache.length(a) == 0
+    cache.write([a], 0, (z[:, :, :20], z[:, :, :20], z[:, :, :20], z[:, :, :20]))
+    assert cache.length(a) == 20
+    cache.free(a)
+    assert cache.free_pages() == (40, 40)
+
+
+def test_made_in_inference_mode_and_used_outside(plain):
+    with torch.inference_mode():
+        cache = _cache()
+        a = cache.add()
+        z = torch.ones(1, 1, 15, 16, dtype=torch.float64)
+        cache.write([a], 0, (z, z, z, z))
+        batch = cache.batch([a])
+    for _ in range(3):                                                  # over the end of a page
+        batch.advance()
+    assert batch.lengths.tolist() == [18]
+    b = cache.fork(a)[0]
+    batch.replace([b])
+    with torch.inference_mode():
+        batch.advance()
+    assert batch.lengths.tolist() == [19] and cache.length(b) == 19 and cache.length(a) == 18
+    cache.free(a)
+    cache.compact()
+    cache.resize(10)
+
+
 def test_refusals(plain):
     for bad in (dict(layers=0), dict(pages=0), dict(u_pages=0), dict(page_size=8), dict(page_size=48), dict(dim_head=48)):
         with pytest.raises(ValueError):
