@@ -281,12 +281,14 @@ def castle_quantize_4bit(weight, group_size: int = 64, zeros: bool = False):
         n, k = weight.shape
         groups = (k + group_size - 1) // group_size
         w = weight.float()
+        if not bool(w.isfinite().all()):
+            raise ValueError("castle_quantize_4bit: a weight is not finite")
         padded = torch.nn.functional.pad(w, (0, groups * group_size - k))             # (a value of zero is among the others' range below)
         inside = (torch.arange(groups * group_size, device=w.device) < k).view(groups, group_size)
         grouped = padded.view(n, groups, group_size)
         high = torch.where(inside, grouped, -torch.inf).amax(-1)
         low = torch.where(inside, grouped, torch.inf).amin(-1)
-        scale = (high - low) / 15 if zeros else torch.maximum(high / 7, -low / 8)
+        scale = high / 15 - low / 15 if zeros else torch.maximum(high / 7, -low / 8)
         scale = scale.to(weight.dtype)
         scale = torch.where(scale > 0, scale, torch.ones_like(scale))                 # (all of a group alike, or too small for the type)
         zero = (-low / scale.float()).to(weight.dtype) if zeros else None

@@ -48,6 +48,24 @@ def test_quantised_weights(zeros, dtype):
     assert bool(((back - w.double()).abs() <= scales.double()[:, at] * (0.5 + 2 * size)).all())
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+def test_weights_at_the_types_ends(zeros):
+    """The largest weights have finite scales; weights that are not finite are refused."""
+    from lookahead_keys_attention_b200 import castle_quantize_4bit
+    top = torch.finfo(torch.float32).max
+    w = torch.linspace(-1, 1, 64).repeat(2, 1) * top
+    codes, scales, zp = castle_quantize_4bit(w, 64, zeros)
+    assert bool(scales.isfinite().all())
+    back = (_unpack(codes, 2, 64).double() - (zp.double() if zeros else 8.0)) * scales.double()
+    # (half a step, and the roundings of 15 steps)
+    assert bool(((back - w.double()).abs() <= scales.double() * (0.5 + 1e-4)).all())
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        w = torch.zeros(2, 64)
+        w[1, 5] = bad
+        with pytest.raises(ValueError, match="finite"):
+            castle_quantize_4bit(w, 64, zeros)
+
+
 def test_arguments():
     L, lib = _lib()
     good = dict(dtype=L.BF16, rows=2, k=200, n=10, group=64, x=256, stride=200, codes=256, scales=256, zeros=256, y=256, status=256)
