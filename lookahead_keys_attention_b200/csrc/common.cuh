@@ -101,7 +101,7 @@ inline int make_tmap_16bit(CUtensorMap* m, const castle_tensor_t* t, int dtype, 
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)N, (cuuint64_t)H, (cuuint64_t)B};
   // a size-1 dimension may carry any stride; give it a legal one
   cuuint64_t sn = (cuuint64_t)t->stride_n * 2, sh = (cuuint64_t)t->stride_h * 2, sb = (cuuint64_t)t->stride_b * 2;
-  if (N == 1) sn = (cuuint64_t)D * 2;
+  if (N == 1) sn = ((cuuint64_t)D * 2 + 15) / 16 * 16;
   if (H == 1) sh = sn * (cuuint64_t)N;
   if (B == 1) sb = sh * (cuuint64_t)H;
   cuuint64_t strides[3] = {sn, sh, sb};

@@ -21,6 +21,7 @@ namespace castle {
 // a phase, and a group that came to a stage on every fourth use of three took the phase before last for the last one.
 constexpr int kTileGroups = 3, kTileWarps = 4 * kTileGroups, kTileThreads = 32 * (kTileWarps + 2), kTileMaxStages = 6;
 constexpr uint32_t kTileSmem = 3 * 2 * 256 * 128;   // three stages of 256 rows of x, or six of 128
+constexpr int64_t kTileLaunchRows = 65535 * 32;      // of a launch: a grid's second dimension and the fewest rows of a tile
 
 struct Linear4TileParams {
   const uint4* codes;
@@ -237,19 +238,24 @@ extern "C" int castle_linear_4bit_tile(int32_t dtype, int64_t rows, int32_t in_f
   p.vec_groups = p.groups % 8 == 0 && ((uintptr_t)scales | (uintptr_t)zeros) % 16 == 0;
   while ((32 << p.shift) < group) ++p.shift;
   const int64_t n_tiles = (out_features + 127) / 128;
-  p.bn = linear_4bit_tile_rows(rows, n_tiles);
-  p.stages = p.bn <= 128 ? 6 : 3;
-  const int64_t r_tiles = (rows + p.bn - 1) / p.bn;
-  if (r_tiles > 65535) return reject("%s: too many rows", who);
-  CUtensorMap m_x;
-  const castle_tensor_t t{const_cast<void*>(x), rows * row_stride, rows * row_stride, row_stride};
-  if (const int rc = make_tmap_16bit(&m_x, &t, dtype, 1, 1, (int)rows, in_features, p.bn, "x")) return rc;
   p.mask = dtype == CASTLE_BF16 ? Pair<__nv_bfloat16>::mask : Pair<__half>::mask;
   p.bits = dtype == CASTLE_BF16 ? Pair<__nv_bfloat16>::bits : Pair<__half>::bits;
   auto launch = [&](auto kernel) {
-    cudaError_t e = allow_smem(kernel, kTileSmem + 1024);
-    if (e == cudaSuccess) e = launch_kernel(kernel, dim3((unsigned)n_tiles, (unsigned)r_tiles), kTileThreads, kTileSmem + 1024, (cudaStream_t)stream, true, p, m_x);
-    return e == cudaSuccess ? 0 : cuda_fail(e, "castle_linear_4bit_tile launch");
+    for (int64_t done = 0; done < rows; done += kTileLaunchRows) {
+      Linear4TileParams q = p;
+      q.rows = (int)std::min(rows - done, kTileLaunchRows);
+      q.y = static_cast<char*>(y) + done * out_features * 2;
+      q.bn = linear_4bit_tile_rows(q.rows, n_tiles);
+      q.stages = q.bn <= 128 ? 6 : 3;
+      CUtensorMap m_x;
+      const castle_tensor_t t{static_cast<char*>(const_cast<void*>(x)) + done * row_stride * 2, q.rows * row_stride, q.rows * row_stride, row_stride};
+      if (const int rc = make_tmap_16bit(&m_x, &t, dtype, 1, 1, q.rows, in_features, q.bn, "x")) return rc;
+      cudaError_t e = allow_smem(kernel, kTileSmem + 1024);
+      const dim3 grid((unsigned)n_tiles, (unsigned)((q.rows + q.bn - 1) / q.bn));
+      if (e == cudaSuccess) e = launch_kernel(kernel, grid, kTileThreads, kTileSmem + 1024, (cudaStream_t)stream, true, q, m_x);
+      if (e != cudaSuccess) return cuda_fail(e, "castle_linear_4bit_tile launch");
+    }
+    return 0;
   };
   if (dtype == CASTLE_BF16) return zeros ? launch(castle_linear_4bit_tile_kernel<__nv_bfloat16, true>) : launch(castle_linear_4bit_tile_kernel<__nv_bfloat16, false>);
   return zeros ? launch(castle_linear_4bit_tile_kernel<__half, true>) : launch(castle_linear_4bit_tile_kernel<__half, false>);

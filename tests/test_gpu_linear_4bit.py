@@ -68,6 +68,20 @@ def test_many_rows_and_tiles(dtype):
         _check(y, x, w, parts, EPS[dtype], True)
 
 
+def test_more_rows_than_a_launch_has_and_the_widest():
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
+    gen = torch.Generator("cuda").manual_seed(7)
+    codes, scales, zero, w, parts = _weight(40, 16, 64, torch.bfloat16, True, gen)
+    x = torch.randn(65535 * 32 * 2 + 77, 16, device="cuda", generator=gen).bfloat16()
+    y = castle_linear_4bit(x, castle_pack_4bit(codes), scales, zero)
+    for part in (slice(0, 1000), slice(65535 * 32 - 500, 65535 * 32 + 500), slice(65535 * 64 - 500, None)):
+        _check(y[part], x[part], w, parts, EPS[torch.bfloat16], True)
+    codes, scales, zero, w, parts = _weight(20, 600_001, 64, torch.bfloat16, False, gen)
+    for rows in (1, 3, 40):
+        x = torch.randn(rows, 600_001, device="cuda", generator=gen).bfloat16()
+        _check(castle_linear_4bit(x, castle_pack_4bit(codes), scales), x, w, parts, EPS[torch.bfloat16], True)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_strides_and_shapes(dtype):
     from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
