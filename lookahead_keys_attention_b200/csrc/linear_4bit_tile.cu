@@ -234,25 +234,25 @@ extern "C" int castle_linear_4bit_tile(int32_t dtype, int64_t rows, int32_t in_f
   if (!x || !codes || !scales || !y || !status) return reject("%s: null tensor", who);
   if (((uintptr_t)x | (uintptr_t)codes) % 16 || row_stride * 2 % 16 || row_stride < in_features) return reject("%s: rows and codes must be 16-byte aligned, rows of a multiple of 16 bytes", who);
   if (((uintptr_t)scales | (uintptr_t)zeros | (uintptr_t)y) % 2 || (uintptr_t)status % 4) return reject("%s: scales, zero points and results must be aligned to their type", who);
-  Linear4TileParams p{static_cast<const uint4*>(codes), scales, zeros, y, (int)rows, in_features, (int)out_features, (in_features + 255) / 256, 0, (in_features + group - 1) / group, 0, 0, false, status};
-  p.vec_groups = p.groups % 8 == 0 && ((uintptr_t)scales | (uintptr_t)zeros) % 16 == 0;
-  while ((32 << p.shift) < group) ++p.shift;
+  Linear4TileParams whole{static_cast<const uint4*>(codes), scales, zeros, y, (int)rows, in_features, (int)out_features, (in_features + 255) / 256, 0, (in_features + group - 1) / group, 0, 0, false, status};
+  whole.vec_groups = whole.groups % 8 == 0 && ((uintptr_t)scales | (uintptr_t)zeros) % 16 == 0;
+  while ((32 << whole.shift) < group) ++whole.shift;
   const int64_t n_tiles = (out_features + 127) / 128;
-  p.mask = dtype == CASTLE_BF16 ? Pair<__nv_bfloat16>::mask : Pair<__half>::mask;
-  p.bits = dtype == CASTLE_BF16 ? Pair<__nv_bfloat16>::bits : Pair<__half>::bits;
+  whole.mask = dtype == CASTLE_BF16 ? Pair<__nv_bfloat16>::mask : Pair<__half>::mask;
+  whole.bits = dtype == CASTLE_BF16 ? Pair<__nv_bfloat16>::bits : Pair<__half>::bits;
   auto launch = [&](auto kernel) {
     for (int64_t done = 0; done < rows; done += kTileLaunchRows) {
-      Linear4TileParams q = p;
-      q.rows = (int)std::min(rows - done, kTileLaunchRows);
-      q.y = static_cast<char*>(y) + done * out_features * 2;
-      q.bn = linear_4bit_tile_rows(q.rows, n_tiles);
-      q.stages = q.bn <= 128 ? 6 : 3;
+      Linear4TileParams p = whole;
+      p.rows = (int)std::min(rows - done, kTileLaunchRows);
+      p.y = static_cast<char*>(y) + done * out_features * 2;
+      p.bn = linear_4bit_tile_rows(p.rows, n_tiles);
+      p.stages = p.bn <= 128 ? 6 : 3;
       CUtensorMap m_x;
-      const castle_tensor_t t{static_cast<char*>(const_cast<void*>(x)) + done * row_stride * 2, q.rows * row_stride, q.rows * row_stride, row_stride};
-      if (const int rc = make_tmap_16bit(&m_x, &t, dtype, 1, 1, q.rows, in_features, q.bn, "x")) return rc;
+      const castle_tensor_t t{static_cast<char*>(const_cast<void*>(x)) + done * row_stride * 2, p.rows * row_stride, p.rows * row_stride, row_stride};
+      if (const int rc = make_tmap_16bit(&m_x, &t, dtype, 1, 1, p.rows, in_features, p.bn, "x")) return rc;
       cudaError_t e = allow_smem(kernel, kTileSmem + 1024);
-      const dim3 grid((unsigned)n_tiles, (unsigned)((q.rows + q.bn - 1) / q.bn));
-      if (e == cudaSuccess) e = launch_kernel(kernel, grid, kTileThreads, kTileSmem + 1024, (cudaStream_t)stream, true, q, m_x);
+      const dim3 grid((unsigned)n_tiles, (unsigned)((p.rows + p.bn - 1) / p.bn));
+      if (e == cudaSuccess) e = launch_kernel(kernel, grid, kTileThreads, kTileSmem + 1024, (cudaStream_t)stream, true, p, m_x);
       if (e != cudaSuccess) return cuda_fail(e, "castle_linear_4bit_tile launch");
     }
     return 0;
