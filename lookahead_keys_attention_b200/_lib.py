@@ -56,7 +56,7 @@ STAMP_PATH = PKG_DIR / "libcastle_b200.so.stamp"
 HOST_PATH = PKG_DIR / "_host.so"
 HOST_STAMP_PATH = PKG_DIR / "_host.so.stamp"
 HOST_SOURCE = CSRC / "host.cpp"
-HOST_PARTS = [HOST_SOURCE, CSRC / "host_lm.h", CSRC / "host_serve.h", CSRC / "host_4bit.h"]
+HOST_PARTS = [HOST_SOURCE, CSRC / "host_lm.h", CSRC / "host_serve.h", CSRC / "host_4bit.h", CSRC / "linear_4bit_plan.cuh"]
 
 
 def _deps():

@@ -38,6 +38,7 @@
 #include <vector>
 
 #include "../../include/castle_b200.h"
+#include "linear_4bit_plan.cuh"
 
 namespace {
 

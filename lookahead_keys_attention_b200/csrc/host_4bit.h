@@ -72,13 +72,13 @@ struct Linear4bitBackward : public Node {   // of x: the weights are frozen
   }
 };
 
-// Whether 9 to 32 rows of 16 bits go through the codes rather than through tiles, by what either took (us, codes / tiles, bf16: 16 x 4096 -> 16384
-// 22.6 / 19.2, 16 x 4096 -> 4096 10.8 / 20.7, 32 x 4096 -> 16384 46.7 / 19.4, 32 x 4096 -> 4096 17.6 / 20.7, 32 x 512 -> 2048 5.9 / 6.6, 24 x 16384 -> 1024
-// 23.8 / 56.8, 24 x 1000 -> 50021 with zero points 36.4 / 34.6): the one by the number of weights, the other by steps of 128 k and rounds of 148 tiles.
+// Whether 9 to 32 rows of 16 bits go through the codes rather than through tiles, by what either takes: the one by the number of weights (us, bf16: 16 x 4096 ->
+// 16384 22.6, 32 x 4096 -> 16384 46.7, 16 x 4096 -> 4096 10.8, 32 x 4096 -> 4096 17.6, 32 x 512 -> 2048 5.9) and, where the rows are wide, what their share of a CTA's
+// shared memory costs (12 x 16384 -> 1024 20.0, by tiles 12), the other by its plan.
 bool few_rows(int64_t rows, int64_t K, int64_t N) {
-  const double weights = 1e-6 * (double)K * (double)N, codes = rows <= 16 ? 3.3 + 0.29 * weights : 5.0 + 0.64 * weights;
-  const double tiles = (double)(((N + 127) / 128 + 147) / 148) * (5.0 + 0.45 * (double)((K + 127) / 128));
-  return codes <= tiles;
+  const double weights = 1e-6 * (double)K * (double)N, wide = 7e-4 * (double)std::max<int64_t>(0, K - 4096);
+  const double codes = (rows <= 16 ? 3.3 + 0.29 * weights : 5.0 + 0.64 * weights) + wide;
+  return codes <= castle::linear_4bit_tile_plan(rows, K, N).us;
 }
 
 Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& own_scales, const Tensor& own_zeros, int64_t group) {

@@ -125,11 +125,6 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {   // read once: n
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
-__device__ __forceinline__ float cluster_load(const float* p, uint32_t rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(of_cta(p, rank)) : "memory");
-  return v;
-}
 
 // Eight k of a column of x: a row's own values, or one of the three parts of fp32 ones.
 template <typename T> __device__ __forceinline__ void stage8(const Linear4Params& p, int col, int k, float* v) {

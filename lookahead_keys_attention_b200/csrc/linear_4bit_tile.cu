@@ -1,6 +1,7 @@
 // y = x W^T with weights of 4 bits, for the rows of prompts and batches of them (16-bit types; linear_4bit.cu has the few rows of tokens).
 //
-// A CTA owns 128 weight rows and up to 256 rows of x.  The weights are the first operand of its tcgen05 products and come from tensor memory:
+// A CTA owns 128 weight rows and up to 256 rows of x (and where that leaves SMs without a tile, a share of K: the CTAs of a cluster add up their results through
+// each other's shared memory, in order).  The weights are the first operand of its tcgen05 products and come from tensor memory:
 // a thread owns a weight row, loads the 64 bytes of its codes for 128 k, unpacks and scales them, and stores the pairs to its lane, so that the weights at
 // full width are never in memory of any kind but that.  The rows of x come by TMA into shared memory, the results are formed in 128 x 256
 // fp32 accumulators.  A weight is (code - zero) * scale, rounded to the rows' type (with zero points that are no whole numbers, code - zero
@@ -10,6 +11,7 @@
 // operations a thread and step, by three groups of four warps in turn.
 #include <algorithm>
 #include "common.cuh"
+#include "linear_4bit_plan.cuh"
 #include "sm100.cuh"
 #include "vec.cuh"
 
@@ -28,6 +30,7 @@ struct Linear4TileParams {
   const void *scales, *zeros;
   void* y;
   int rows, K, N, blocks, shift, groups, bn;   // bn: rows of x in a tile, a multiple of 16
+  int ks;                                              // CTAs of a cluster, which share K out
   int stages;                                          // six up to 128 rows, three above: tensor memory has bn and 64 columns a stage, rounded up
   bool vec_groups;                                     // eight groups of a row can be loaded at once
   int32_t* status;
@@ -72,7 +75,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
   __shared__ int abort_flag;
   volatile int* abortp = &abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n0 = blockIdx.x * 128, r0 = blockIdx.y * p.bn, chunks = (p.K + 127) / 128;
+  const int rank = p.ks > 1 ? (int)cluster_rank() : 0, all = (p.K + 127) / 128;
+  const int n0 = blockIdx.x / p.ks * 128, r0 = blockIdx.y * p.bn;
+  const int first = all * rank / p.ks, chunks = all * (rank + 1) / p.ks - first;   // this CTA's steps of 128 k
   const uint32_t panel = (uint32_t)p.bn * 128;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kTileMaxStages; ++i) { mbar_init(&full[i], 5); mbar_init(&free_[i], 1); }   // four warps' weights and x
@@ -94,8 +99,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
         if (*abortp) break;
         mbar_expect_tx(&full[s], 2 * panel);
         uint8_t* x = smem + s * 2 * panel;
-        tma_load_4d(x, &m_x, &full[s], c * 128, r0, 0, 0);
-        tma_load_4d(x + panel, &m_x, &full[s], c * 128 + 64, r0, 0, 0);
+        tma_load_4d(x, &m_x, &full[s], (first + c) * 128, r0, 0, 0);
+        tma_load_4d(x + panel, &m_x, &full[s], (first + c) * 128 + 64, r0, 0, 0);
         if (++s == p.stages) { s = 0; ++turn; }
       }
       // (after an abort: what is on its way arrives before the CTA leaves; the weights' arrivals are made in any case)
@@ -122,14 +127,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
     // ---- a weight row for each thread of a group of four warps, the groups in turn
     const int group = warp >> 2, m = (warp & 3) * 32 + lane;
     const int n = min(n0 + m, p.N - 1);
-    const uint4* codes = p.codes + (int64_t)(n >> 4) * p.blocks * 128 + (n >> 3 & 1) * 32 + (n & 7) * 4;
+    const uint4* codes = p.codes + (int64_t)(n >> 4) * p.blocks * 128 + (int64_t)first * 64 + (n >> 3 & 1) * 32 + (n & 7) * 4;
     const T *scales = reinterpret_cast<const T*>(p.scales) + (int64_t)n * p.groups, *zeros = reinterpret_cast<const T*>(p.zeros) + (int64_t)n * p.groups;
     const uint32_t at = weights + ((uint32_t)((warp & 3) * 32) << 16);
     uint4 next[4];             // the codes of this group's next step
     // Scales and zero points eight groups of the row at a time, the next eight on their way: single ones of 32 rows are 32 lines of the cache each,
     // which was the time (777 x 4096 -> 4096, groups of 64: 50 us, with zero points 79).
     uint4 scale8, next_scale8, zero8, next_zero8;
-    int window = 0;
+    int window = first * 4 >> p.shift >> 3;
     auto load8 = [&](const T* row, int w) {
       uint4 v = make_uint4(0, 0, 0, 0);
       if (p.vec_groups) {
@@ -142,9 +147,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
       }
       return v;
     };
-    scale8 = load8(scales, 0);
-    next_scale8 = load8(scales, 1);
-    if constexpr (ZEROS) { zero8 = load8(zeros, 0); next_zero8 = load8(zeros, 1); }
+    scale8 = load8(scales, window);
+    next_scale8 = load8(scales, window + 1);
+    if constexpr (ZEROS) { zero8 = load8(zeros, window); next_zero8 = load8(zeros, window + 1); }
     auto pick = [&](const uint4& v, int g) {   // element g of eight, twice
       const uint32_t w = g & 4 ? (g & 2 ? v.w : v.z) : (g & 2 ? v.y : v.x), r = __byte_perm(w, w, g & 1 ? 0x3232 : 0x1010);
       return *reinterpret_cast<const typename Pair<T>::type*>(&r);
@@ -157,7 +162,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
     fetch(group);
     for (int c = group, s = group, turn = 0; c < chunks; c += kTileGroups) {
       const uint4 q[4] = {next[0], next[1], next[2], next[3]};
-      while (c * 4 >> p.shift >> 3 > window) {   // (a step's four stretches of 32 k are in one window)
+      while ((first + c) * 4 >> p.shift >> 3 > window) {   // (a step's four stretches of 32 k are in one window)
         ++window;
         scale8 = next_scale8;
         next_scale8 = load8(scales, window + 1);
@@ -170,7 +175,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
 #pragma unroll
       for (int j = 0; j < 4; ++j) {   // 32 k, 16 columns
         uint32_t v[16];
-        const typename Pair<T>::type scale = pick(scale8, (c * 4 + j) >> p.shift & 7), zero = ZEROS ? pick(zero8, (c * 4 + j) >> p.shift & 7) : scale;
+        const int g = ((first + c) * 4 + j) >> p.shift & 7;
+        const typename Pair<T>::type scale = pick(scale8, g), zero = ZEROS ? pick(zero8, g) : scale;
 #pragma unroll
         for (int t = 0; t < 4; ++t) unpack_word<T, ZEROS>(j == 0 ? q[t].x : j == 1 ? q[t].y : j == 2 ? q[t].z : q[t].w, scale, zero, p.mask, p.bits, v + t * 4);
         tmem_st16(at + s * 64 + j * 16, v);
@@ -189,13 +195,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
     tc_fence_after();
     if (*abortp == 0) {
       T* y = reinterpret_cast<T*>(p.y) + n0 + m;
+      float* part = reinterpret_cast<float*>(smem) + m;   // [row of x][weight row], over the stages
       for (int c0 = group * 32; c0 < p.bn; c0 += 32 * kTileGroups) {
         float v[32];
         tmem_ld32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
         tmem_ld_wait();
+        if (p.ks > 1) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (c0 + i < p.bn && r0 + c0 + i < p.rows && n0 + m < p.N) y[(int64_t)(r0 + c0 + i) * p.N] = Elem<T>::from_f(v[i]);
+          for (int i = 0; i < 32; ++i)
+            if (c0 + i < p.bn) part[(c0 + i) * 128] = v[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c0 + i < p.bn && r0 + c0 + i < p.rows && n0 + m < p.N) y[(int64_t)(r0 + c0 + i) * p.N] = Elem<T>::from_f(v[i]);
+        }
       }
     }
     tc_fence_before();
@@ -204,20 +217,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+    __syncwarp();
+  }
+  if (p.ks > 1) {   // the CTAs' shares of K, in order; each adds up some of the rows of x
+    cluster_sync();
+    const int count = min(p.bn, p.rows - r0) * 128;
+    for (int e = rank * kTileThreads + threadIdx.x; e < count; e += p.ks * kTileThreads) {
+      float sum = 0.f;
+      for (int r = 0; r < p.ks; ++r) sum += cluster_load(reinterpret_cast<const float*>(smem) + e, r);
+      const int n = n0 + (e & 127);
+      if (n < p.N) reinterpret_cast<T*>(p.y)[(int64_t)(r0 + (e >> 7)) * p.N + n] = Elem<T>::from_f(sum);
+    }
+    __syncwarp();
+    cluster_sync();
   }
   if (threadIdx.x == 0 && abort_flag) atomicOr(p.status, CASTLE_STATUS_WAIT_TIMEOUT);
-}
-
-// Rows of x in a tile: a step costs the products 4 cycles a row of x, and their issue and the unpacking some 500 whatever there are; as many CTAs as there are SMs
-// work at a time.
-static int linear_4bit_tile_rows(int64_t rows, int64_t n_tiles) {
-  int best = 256;
-  int64_t least = INT64_MAX;
-  for (int bn = 256; bn >= 32; bn -= 16) {
-    const int64_t tiles = (rows + bn - 1) / bn * n_tiles, cost = (tiles + 147) / 148 * std::max(4 * bn, 500);
-    if (cost < least) { least = cost; best = bn; }
-  }
-  return best;
 }
 
 }  // namespace castle
@@ -234,7 +248,7 @@ extern "C" int castle_linear_4bit_tile(int32_t dtype, int64_t rows, int32_t in_f
   if (!x || !codes || !scales || !y || !status) return reject("%s: null tensor", who);
   if (((uintptr_t)x | (uintptr_t)codes) % 16 || row_stride * 2 % 16 || row_stride < in_features) return reject("%s: rows and codes must be 16-byte aligned, rows of a multiple of 16 bytes", who);
   if (((uintptr_t)scales | (uintptr_t)zeros | (uintptr_t)y) % 2 || (uintptr_t)status % 4) return reject("%s: scales, zero points and results must be aligned to their type", who);
-  Linear4TileParams whole{static_cast<const uint4*>(codes), scales, zeros, y, (int)rows, in_features, (int)out_features, (in_features + 255) / 256, 0, (in_features + group - 1) / group, 0, 0, false, status};
+  Linear4TileParams whole{static_cast<const uint4*>(codes), scales, zeros, y, (int)rows, in_features, (int)out_features, (in_features + 255) / 256, 0, (in_features + group - 1) / group, 0, 1, 0, false, status};
   whole.vec_groups = whole.groups % 8 == 0 && ((uintptr_t)scales | (uintptr_t)zeros) % 16 == 0;
   while ((32 << whole.shift) < group) ++whole.shift;
   const int64_t n_tiles = (out_features + 127) / 128;
@@ -245,14 +259,23 @@ extern "C" int castle_linear_4bit_tile(int32_t dtype, int64_t rows, int32_t in_f
       Linear4TileParams p = whole;
       p.rows = (int)std::min(rows - done, kTileLaunchRows);
       p.y = static_cast<char*>(y) + done * out_features * 2;
-      p.bn = linear_4bit_tile_rows(p.rows, n_tiles);
+      const TilePlan plan = linear_4bit_tile_plan(p.rows, in_features, out_features);
+      p.bn = plan.bn;
+      p.ks = plan.ks;
       p.stages = p.bn <= 128 ? 6 : 3;
       CUtensorMap m_x;
       const castle_tensor_t t{static_cast<char*>(const_cast<void*>(x)) + done * row_stride * 2, p.rows * row_stride, p.rows * row_stride, row_stride};
       if (const int rc = make_tmap_16bit(&m_x, &t, dtype, 1, 1, p.rows, in_features, p.bn, "x")) return rc;
       cudaError_t e = allow_smem(kernel, kTileSmem + 1024);
-      const dim3 grid((unsigned)n_tiles, (unsigned)((p.rows + p.bn - 1) / p.bn));
-      if (e == cudaSuccess) e = launch_kernel(kernel, grid, kTileThreads, kTileSmem + 1024, (cudaStream_t)stream, true, p, m_x);
+      cudaLaunchConfig_t c = {};
+      cudaLaunchAttribute attr[2];
+      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[0].val.programmaticStreamSerializationAllowed = 1;
+      attr[1].id = cudaLaunchAttributeClusterDimension;
+      attr[1].val.clusterDim = {(unsigned)p.ks, 1, 1};
+      c.gridDim = dim3((unsigned)(n_tiles * p.ks), (unsigned)((p.rows + p.bn - 1) / p.bn)); c.blockDim = dim3(kTileThreads);
+      c.dynamicSmemBytes = kTileSmem + 1024; c.stream = (cudaStream_t)stream; c.attrs = attr; c.numAttrs = p.ks > 1 ? 2 : 1;
+      if (e == cudaSuccess) e = cudaLaunchKernelEx(&c, kernel, p, m_x);
       if (e != cudaSuccess) return cuda_fail(e, "castle_linear_4bit_tile launch");
     }
     return 0;

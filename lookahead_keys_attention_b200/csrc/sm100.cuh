@@ -288,6 +288,11 @@ __device__ __forceinline__ uint32_t of_cta(const void* p, uint32_t rank) {   // 
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
+__device__ __forceinline__ float cluster_load(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(of_cta(p, rank)) : "memory");
+  return v;
+}
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {   // of another CTA's barrier, see of_cta
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }

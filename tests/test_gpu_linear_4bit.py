@@ -68,6 +68,21 @@ def test_many_rows_and_tiles(dtype):
         _check(y, x, w, parts, EPS[dtype], True)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_the_width_shared_out(dtype, zeros):
+    """Weights of few tiles, whose width the CTAs of clusters share out: of two, four and eight, in even and odd shares, groups that end inside one."""
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
+    gen = torch.Generator("cuda").manual_seed(8)
+    for inner, out, rows, group in ((4096, 4096, 40, 64), (8000, 200, 500, 32), (7997, 1000, 500, 256), (16384, 512, 48, 64), (16384, 17, 33, 4096), (8192, 1024, 100, 128),
+                                    (1153, 130, 70, 32), (1100, 100, 1000, 64), (4096, 4096, 200, 64), (5000, 2100, 300, 64), (6000, 8192, 60, 128)):
+        codes, scales, zero, w, parts = _weight(out, inner, group, dtype, zeros, gen)
+        packed, x = castle_pack_4bit(codes), torch.randn(rows, inner, device="cuda", generator=gen).to(dtype)
+        y = castle_linear_4bit(x, packed, scales, zero, group)
+        _check(y, x, w, parts, EPS[dtype], True)
+        assert all(torch.equal(castle_linear_4bit(x, packed, scales, zero, group), y) for _ in range(3))
+
+
 def test_more_rows_than_a_launch_has_and_the_widest():
     from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
     gen = torch.Generator("cuda").manual_seed(7)
