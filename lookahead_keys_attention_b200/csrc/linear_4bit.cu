@@ -400,21 +400,35 @@ __global__ void __launch_bounds__(kL4Threads, 1) castle_linear_4bit_kernel(const
   if (threadIdx.x == 0 && abort_flag) atomicOr(p.status, CASTLE_STATUS_WAIT_TIMEOUT);
 }
 
-// The weights at full width, in the rows' type (rounded once): for the products of many rows and for the gradient of x.
+// The weights at full width, in the rows' type (rounded once): for the products of many fp32 rows and for the gradient of x.  A warp has 4 rows and 128 k, two words a
+// thread, so that a store is 128 (fp32: 256) adjacent bytes of each row.  4096 x 4096 in us, bf16 and fp32: 15.2, 23.5 (the bytes take 6.4 and 11.6); a word a
+// thread along a row 15.8, 27.2; 16 bytes of codes a thread, 64 bytes of a row at once, 15.7, 27.0, more of them a thread 17.2, 26.5.  What bounds it now: a thread's
+// only loads are on their way while nothing is stored (not tried: CTAs that stay, with the next codes loaded ahead of the stores).
 template <typename T, bool ZEROS> __global__ void __launch_bounds__(256) castle_expand_4bit_kernel(const Linear4Params p, int64_t ldw) {
-  const int words = p.blocks * 32;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < (int64_t)p.N * words; e += (int64_t)gridDim.x * 256) {
-    const int64_t n = e / words;
-    const int word = (int)(e % words), j = word % 4, t = word / 4 % 4, part = word / 16, k0 = part * 128 + j * 32 + t * 8;   // (neighbours share a row)
-    if (k0 >= p.K) continue;
-    const uint32_t w = reinterpret_cast<const uint32_t*>(p.codes)[(((n >> 4) * p.blocks * 2 + part) * 2 + (n >> 3 & 1)) * 128 + ((n & 7) * 4 + t) * 4 + j];
-    const int64_t at = n * p.groups + (k0 / 32 >> p.shift);
-    const float s = load1<T>(reinterpret_cast<const T*>(p.scales) + at), z = ZEROS ? load1<T>(reinterpret_cast<const T*>(p.zeros) + at) : 8.f;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = (warp & 1) * 4 + (lane >> 3), h = lane >> 2 & 1, t = lane & 3;
+  const int part = blockIdx.y * 4 + (warp >> 1);   // of 128 k
+  const int64_t n = (int64_t)blockIdx.x * 8 + g;
+  if (n >= p.N || part * 128 >= p.K) return;
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(p.codes + (((n >> 4) * p.blocks * 2 + part) * 2 + (n >> 3 & 1)) * 32 + g * 4 + t);
+  uint32_t w[2];
+  float s[2], z[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int j = 2 * u + h;
+    w[u] = __ldg(src + j);
+    const int64_t at = n * p.groups + min((part * 4 + j) >> p.shift, p.groups - 1);
+    s[u] = load1<T>(reinterpret_cast<const T*>(p.scales) + at);
+    z[u] = ZEROS ? load1<T>(reinterpret_cast<const T*>(p.zeros) + at) : 8.f;
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int k0 = part * 128 + (2 * u + h) * 32 + t * 8;
+    if (k0 >= p.K) break;
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = s * ((float)(w >> (4 * i) & 15u) - z);
-      v[2 * i + 1] = s * ((float)(w >> (4 * i + 16) & 15u) - z);
+    for (int i = 0; i < 8; ++i) {   // 2^23 + code, less 2^23
+      const float code = __uint_as_float((w[u] >> (4 * (i >> 1) + 16 * (i & 1)) & 15u) | 0x4b000000u) - 8388608.f;
+      v[i] = s[u] * (code - z[u]);
     }
     T* dst = reinterpret_cast<T*>(p.y) + n * ldw + k0;
     if (k0 + 8 <= p.K) {
@@ -541,12 +555,11 @@ extern "C" int castle_expand_4bit(int32_t dtype, int32_t in_features, int64_t ou
   if (const int rc = linear_4bit_check(who, dtype, in_features, out_features, group, codes, scales, zeros, p)) return rc;
   if (!w || (uintptr_t)w % 16 || row_stride < in_features || row_stride * elem_size(dtype) % 16) return reject("%s: the weights must be 16-byte aligned, rows of a multiple of 16 bytes", who);
   p.y = w;
-  const int64_t words = (int64_t)p.N * p.blocks * 32;
-  const int ctas = (int)std::min<int64_t>((words + 255) / 256, 148 * 16);
+  const dim3 grid((unsigned)((p.N + 7) / 8), (unsigned)((p.K + 511) / 512));
   cudaError_t e = by_type(dtype, [&](auto v) {
     using T = decltype(v);
-    return zeros ? launch_kernel(castle_expand_4bit_kernel<T, true>, dim3(ctas), 256, 0, (cudaStream_t)stream, false, p, row_stride)
-                 : launch_kernel(castle_expand_4bit_kernel<T, false>, dim3(ctas), 256, 0, (cudaStream_t)stream, false, p, row_stride);
+    return zeros ? launch_kernel(castle_expand_4bit_kernel<T, true>, grid, 256, 0, (cudaStream_t)stream, false, p, row_stride)
+                 : launch_kernel(castle_expand_4bit_kernel<T, false>, grid, 256, 0, (cudaStream_t)stream, false, p, row_stride);
   });
   return e == cudaSuccess ? 0 : cuda_fail(e, "castle_expand_4bit launch");
 }
