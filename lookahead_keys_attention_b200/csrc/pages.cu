@@ -2,7 +2,7 @@
 // what bounds them is HBM, and for a few pages a launch.
 #include <algorithm>
 #include <new>
-#include <unordered_set>
+#include <vector>
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -39,6 +39,32 @@ __global__ void __launch_bounds__(kCopyThreads) castle_copy_pages_kernel(const _
     if (at < bytes) *reinterpret_cast<uint4*>(dst + at) = v[i];
   }
 }
+
+// A set of pages, on the host: places of a table that is at most half full, one behind the other from where a page's number leads.  (Of the standard
+// library's sets a call with 1000 pairs took 47 us.)
+class PageSet {
+ public:
+  explicit PageSet(int64_t count) {
+    while (((int64_t)1 << bits_) < 2 * count) ++bits_;
+    places_.assign((size_t)1 << bits_, -1);
+  }
+  bool insert(int32_t page) {
+    size_t at = find(page);
+    if (places_[at] == page) return false;
+    places_[at] = page;
+    return true;
+  }
+  bool has(int32_t page) const { return places_[find(page)] == page; }
+
+ private:
+  size_t find(int32_t page) const {   // the page's place, or the free one where it would be
+    size_t at = (size_t)(((uint64_t)(uint32_t)page * 0x9e3779b97f4a7c15ull) >> (64 - bits_));
+    while (places_[at] != -1 && places_[at] != page) at = (at + 1) & (places_.size() - 1);
+    return at;
+  }
+  int bits_ = 1;
+  std::vector<int32_t> places_;
+};
 
 struct WriteParams {
   castle_tensor_t src[4];          // U, qu, kc, vc
@@ -108,16 +134,14 @@ extern "C" int castle_copy_pages(int32_t pools, void* const* ptr, const int64_t*
       if (ptr[j] == ptr[k]) return reject("%s: pool %d is pool %d again", who, k, j);
   }
   try {
-    std::unordered_set<int32_t> from, to;
-    from.reserve(count); to.reserve(count);
+    PageSet targets(count);
     for (int64_t i = 0; i < count; ++i) {
       if (source[i] < 0 || source[i] >= pages || target[i] < 0 || target[i] >= pages)
         return reject("%s: pair %lld (%d to %d) is outside the %lld pages", who, (long long)i, source[i], target[i], (long long)pages);
-      from.insert(source[i]);
-      if (!to.insert(target[i]).second) return reject("%s: page %d is a target twice", who, target[i]);
+      if (!targets.insert(target[i])) return reject("%s: page %d is a target twice", who, target[i]);
     }
     for (int64_t i = 0; i < count; ++i)
-      if (from.count(target[i])) return reject("%s: page %d is a target and a source", who, target[i]);
+      if (targets.has(source[i])) return reject("%s: page %d is a target and a source", who, source[i]);
   } catch (const std::bad_alloc&) {
     return reject("%s: out of host memory", who);
   }

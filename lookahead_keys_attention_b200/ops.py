@@ -12,6 +12,8 @@ argument order (causal triple first), unscaled inputs, returns `out` or
 """
 from __future__ import annotations
 
+from array import array
+
 import torch
 
 from . import _lib
@@ -241,7 +243,10 @@ def castle_write_pages(U, qu, kc, vc, U_pages, qu_pages, kc_pages, vc_pages, U_t
 
 
 def _page_numbers(pages):
-    return pages if isinstance(pages, torch.Tensor) else torch.tensor(pages, dtype=torch.int64, device="cpu")
+    if isinstance(pages, torch.Tensor):
+        return pages
+    numbers = array("q", pages)   # (torch.tensor takes 43 us for a list of 900, this 14)
+    return torch.frombuffer(numbers, dtype=torch.int64) if numbers else torch.empty(0, dtype=torch.int64, device="cpu")
 
 
 def castle_copy_pages(pools, source, target):

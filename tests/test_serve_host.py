@@ -81,6 +81,30 @@ def test_copy_arguments(bad):
     assert _copy(lib, **bad) < 0 and "castle_copy_pages" in L.last_error()
 
 
+def test_copies_of_many_pages():
+    """A target twice and a target that is a source are found among any number of pairs, and named."""
+    import random
+    L, lib = _lib()
+    for seed, count in enumerate((1, 2, 3, 17, 64, 65, 1000, 5000)):
+        rng = random.Random(seed)
+        pages = rng.sample(range(2 ** 31 - 1 if seed % 2 else 3 * count), 2 * count)
+        source, target = [rng.choice(pages[:count]) for _ in range(count)], pages[count:]
+        at, both = rng.randrange(count), rng.choice(source)
+        assert _copy(lib, pages=2 ** 31 - 1, source=source, target=target[:at] + [both] + target[at + 1:]) < 0 and f"page {both} is a target and a source" in L.last_error()
+        if count > 1:
+            twice = rng.choice(target[:-1])
+            assert _copy(lib, pages=2 ** 31 - 1, source=source, target=target[:-1] + [twice]) < 0 and f"page {twice} is a target twice" in L.last_error()
+
+
+def test_page_numbers():
+    from lookahead_keys_attention_b200.ops import _page_numbers
+    for pages in ([3, 1, 2 ** 31], (5,), range(4), [True], [torch.tensor(7)], []):
+        t = _page_numbers(pages)
+        assert t.dtype == torch.int64 and t.device.type == "cpu" and t.tolist() == [int(p) for p in pages]
+    with pytest.raises(TypeError):
+        _page_numbers([1.5])
+
+
 def test_nothing_to_copy_is_fine():
     L, lib = _lib()
     assert _copy(lib, source=(), target=()) == 0 and _copy(lib, pools=0) == 0
