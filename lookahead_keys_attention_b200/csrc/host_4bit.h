@@ -81,6 +81,16 @@ bool few_rows(int64_t rows, int64_t K, int64_t N) {
   return codes <= castle::linear_4bit_tile_plan(rows, K, N).us;
 }
 
+// Rows of 32 bits go through the codes ten at a time, or five where ten are wider than two CTAs' shared memory (us: 10 x 4096 -> 4096 18.9, 5 14.1, 10 x 8136 -> 5307
+// 111, 5 31.3), or through the weights at full width, whose making and products take some 12 + 5.5 for each million of them up to 64 rows (in turns / at full width:
+// 45 x 4096 -> 4096 88 / 121, 64 x 1000 -> 50021 167 / 251, 30 x 8136 -> 5307 180 / 277, 45 x 1024 -> 4096 44 / 29).
+constexpr int64_t kWholeF32 = 4096;
+bool few_rows_f32(int64_t rows, int64_t turns, int64_t K, int64_t N) {
+  const double weights = 1e-6 * (double)K * (double)N;
+  const double turn = K <= kWholeF32 ? 5.5 + 0.0021 * (double)K + 0.38 * weights : 4.0 + 0.0018 * (double)K + 0.23 * weights;
+  return rows <= 10 || (double)turns * turn <= 12.0 + 5.5 * weights;
+}
+
 Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& own_scales, const Tensor& own_zeros, int64_t group) {
   const char* who = "castle_linear_4bit";
   need_plain(x, who);
@@ -102,8 +112,8 @@ Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& own_scale
     sizes.back() = c.N;
     // The rows of a few tokens go through the codes, fp32 ones as many at a time as the kernel takes; more rows of 16 bits through tiles of weights that
     // are unpacked on their way to the tensor cores, and of 32 through the weights at full width (their products are FMA).
-    const int64_t most = dtype == at::kFloat ? 10 : 32, turns = (rows + most - 1) / most, each = turns > 0 ? (rows + turns - 1) / turns : 0;
-    const bool few = dtype == at::kFloat ? turns <= 2 : rows <= 8 || (turns == 1 && few_rows(rows, K, c.N));
+    const int64_t most = dtype != at::kFloat ? 32 : K <= kWholeF32 ? 10 : 5, turns = (rows + most - 1) / most, each = turns > 0 ? (rows + turns - 1) / turns : 0;
+    const bool few = dtype == at::kFloat ? few_rows_f32(rows, turns, K, c.N) : rows <= 8 || (turns == 1 && few_rows(rows, K, c.N));
     if (rows == 0) {
       y = at::empty(sizes, x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
     } else if (few && api.linear_4bit_fits(dtype_code(dtype), (int32_t)each, (int32_t)K)) {

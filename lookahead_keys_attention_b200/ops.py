@@ -305,7 +305,7 @@ def castle_quantize_4bit(weight, group_size: int = 64, zeros: bool = False):
 def castle_linear_4bit(x, codes, scales, zeros=None, group_size: int = 64):
     """`x @ W.T` for weights of 4 bits: W[n, k] = scales[n, k // group_size] * (code[n, k] - zeros[n, k // group_size]), with zero points of 8 where there are
     none.  x (..., in); `codes` of `castle_pack_4bit` or `castle_quantize_4bit`; scales and zero points (out, ceil(in / group_size)) of x's type (under autocast they
-    are cast to it), group_size a power of two from 32 up.  For a few rows (up to 8, and up to 32 where that is faster) the codes are read as they are, the weights are not rounded, and sums
+    are cast to it), group_size a power of two from 32 up.  For a few rows (up to 8, and up to 32, of 32 bits any number, where that is faster) the codes are read as they are, the weights are not rounded, and sums
     are fp32; many rows are products with the weights rounded to x's type (and code - zero before that, where it is no whole number).  The gradient of x
     is a product with the weights at full width; the weights are frozen.  An infinity in x may give NaN in place of
     an infinity (for 16-bit rows, and with zero points)."""

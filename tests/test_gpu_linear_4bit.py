@@ -83,6 +83,18 @@ def test_the_width_shared_out(dtype, zeros):
         assert all(torch.equal(castle_linear_4bit(x, packed, scales, zero, group), y) for _ in range(3))
 
 
+def test_fp32_rows_in_turns():
+    """Five or ten at a time, the last turn with fewer, and from how many on at full width."""
+    from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
+    gen = torch.Generator("cuda").manual_seed(9)
+    for inner, out, group in ((4097, 3000, 64), (4096, 2000, 32), (9000, 1100, 128), (1000, 9000, 64)):
+        codes, scales, zero, w, parts = _weight(out, inner, group, torch.float32, True, gen)
+        packed = castle_pack_4bit(codes)
+        for rows in (5, 6, 10, 11, 21, 33, 47, 90):
+            x = torch.randn(rows, inner, device="cuda", generator=gen)
+            _check(castle_linear_4bit(x, packed, scales, zero, group), x, w, parts, EPS[torch.float32], True)
+
+
 def test_more_rows_than_a_launch_has_and_the_widest():
     from lookahead_keys_attention_b200 import castle_linear_4bit, castle_pack_4bit
     gen = torch.Generator("cuda").manual_seed(7)
