@@ -145,7 +145,7 @@ class PagedCache:
 
     @torch.inference_mode(False)
     def _to_device(self, values):
-        t = torch.tensor(values, dtype=torch.int32)
+        t = torch.tensor(values, dtype=torch.int32, device="cpu")   # (whatever the default device is)
         return (t.pin_memory() if self.device.type == "cuda" else t).to(self.device, non_blocking=True)
 
     def _tables(self, sequences, width):

@@ -372,3 +372,33 @@ def test_traced_calls():
         torch.jit.trace(lambda v: layer(v, cache=batch.layer(0))[0], (torch.randn(1, 1, 64, device="cuda"),), check_trace=False)
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda v: castle_copy_pages(v, [0], [1]) or v, (torch.randn(4, 2, 16, 64, device="cuda"),), check_trace=False)
+
+
+@torch.no_grad()
+def test_under_a_default_device():
+    """A server that makes everything on the GPU by default: the same tokens."""
+    from lookahead_keys_attention_b200 import PagedCache, check_status
+    layers = _layers(2, torch.bfloat16, prenorm=True)
+    prompt, tokens = torch.randn(2, 30, 256, device="cuda").bfloat16(), torch.randn(5, 3, 1, 256, device="cuda").bfloat16()
+
+    def serve():
+        cache = PagedCache(2, 40, 4, 64, 16)
+        a, b = cache.add(), cache.add()
+        for i, c in enumerate(_prompt(layers, prompt)[1]):
+            cache.write([a, b], i, c)
+        c = cache.fork(b)[0]
+        batch, outs = cache.batch([a, b, c]), []
+        for x in tokens:
+            outs.append(_paged_token(layers, x, batch))
+            batch.advance()
+        cache.free(a)
+        cache.compact()
+        cache.resize(30)
+        outs.append(_paged_token(layers, tokens[0], batch))
+        return torch.cat(outs, 1)
+
+    want = serve()
+    with torch.device("cuda"):
+        got = serve()
+    check_status()
+    assert torch.equal(got, want)

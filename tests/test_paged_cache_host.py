@@ -215,6 +215,29 @@ def test_made_in_inference_mode_and_used_outside(plain):
     cache.resize(10)
 
 
+def test_under_another_default_device(plain):
+    """Lists on their way to the cache's device begin on the host, whatever the default device is ("meta": one without values, which cannot be copied from)."""
+    cache = _cache()
+    a = cache.add()
+    z = torch.ones(1, 1, 15, 16, dtype=torch.float64)
+    with torch.device("meta"):
+        cache.write([a], 0, (z, z, z, z))
+        batch = cache.batch([a])
+        for _ in range(3):                                              # over the end of a page
+            batch.advance()
+        (b,) = cache.fork(a)
+        batch.replace([b, a])
+        cache.free(b)
+        cache.compact()
+        cache.resize(10)
+    assert batch.lengths.tolist() == [-1, 18] and all(t.device.type == "cpu" for t in (batch.u_table, batch.table, batch.lengths, cache.U, cache.kc))
+    other = _cache()
+    q = other.add()
+    with torch.device("meta"):
+        made = other.batch([q], size=2, width=3)
+    assert made.table.device.type == made.lengths.device.type == "cpu" and made.lengths.tolist() == [0, -1]
+
+
 def test_refusals(plain):
     for bad in (dict(layers=0), dict(pages=0), dict(u_pages=0), dict(page_size=8), dict(page_size=48), dict(dim_head=48)):
         with pytest.raises(ValueError):
