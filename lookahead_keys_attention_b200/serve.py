@@ -332,7 +332,7 @@ class PagedLayer:
 
 class Linear4bit(nn.Module):
     """A linear layer with frozen weights of 4 bits (`castle_linear_4bit`); `Linear4bit.from_linear(m)` quantises an `nn.Linear`.  It can take the place
-    of any, a `Castle`'s projections among them (`Castle.quantize_4bit`)."""
+    of any, a `Castle`'s projections among them (`Castle.quantize_4bit`).  Under autocast it takes its rows in autocast's type, as a linear layer does."""
 
     def __init__(self, in_features, out_features, bias=False, group_size=64, zeros=False, device=None, dtype=None):
         super().__init__()
@@ -355,6 +355,8 @@ class Linear4bit(nn.Module):
         return m.train(linear.training)
 
     def forward(self, x):
+        if x.is_cuda and torch.is_autocast_enabled("cuda") and x.is_floating_point() and x.dtype is not torch.float64:
+            x = x.to(torch.get_autocast_dtype("cuda"))
         y = ops.castle_linear_4bit(x, self.codes, self.scales, self.zeros, self.group_size)
         return y if self.bias is None else y + self.bias.to(y.dtype)
 

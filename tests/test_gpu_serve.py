@@ -402,3 +402,49 @@ def test_under_a_default_device():
         got = serve()
     check_status()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("other", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_quantised_linear_under_autocast(dtype, other):
+    """The types that a linear layer takes and gives; bit for bit the operator's result for rows and parameters in autocast's type."""
+    from lookahead_keys_attention_b200 import Linear4bit, castle_linear_4bit
+    torch.manual_seed(3)
+    full = nn.Linear(192, 96).cuda().to(dtype)
+    m = Linear4bit.from_linear(full, 64, zeros=True)
+    for rows in ((3,), (2, 150)):
+        for x_type in (torch.float32, torch.bfloat16, torch.float16):
+            x, g = torch.randn(*rows, 192, device="cuda").to(x_type), torch.randn(*rows, 96, device="cuda").to(other)
+            outs = []
+            for layer in (full, m):
+                v = x.clone().requires_grad_()
+                with torch.autocast("cuda", dtype=other):
+                    y = layer(v)
+                outs.append((y, torch.autograd.grad(y, [v], g)[0]))
+            (y0, dx0), (y1, dx1) = outs
+            assert y1.dtype == y0.dtype == other and dx1.dtype == dx0.dtype == x_type and y1.shape == y0.shape
+            want = castle_linear_4bit(x.to(other), m.codes, m.scales.to(other), m.zeros.to(other), 64) + m.bias.to(other)
+            assert torch.equal(y1, want)
+
+
+@torch.no_grad()
+def test_a_quantised_model_under_autocast():
+    """fp32 parameters, autocast's rows: caches of autocast's type, into pages and on from there, beside the same layers over contiguous caches."""
+    from lookahead_keys_attention_b200 import PagedCache, check_status
+    layers = _layers(2, torch.float32, prenorm=True)
+    for m in layers:
+        m.quantize_4bit(32)
+    cache = PagedCache(2, 20, 4, 64, 16)
+    a = cache.add()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        _, caches = _prompt(layers, torch.randn(1, 21, 256, device="cuda"))
+        for i, c in enumerate(caches):
+            assert all(t.dtype == torch.bfloat16 for t in c)
+            cache.write([a], i, c)
+        batch = cache.batch([a])
+        for t in range(12):
+            x = torch.randn(1, 1, 256, device="cuda")
+            got, want = _paged_token(layers, x, batch), _token(layers, x, caches)
+            batch.advance()
+            assert got.dtype == want.dtype and (got - want).abs().max() <= CLOSE[torch.bfloat16] * want.abs().max()
+    check_status()
