@@ -260,13 +260,17 @@ def castle_copy_pages(pools, source, target):
 
 def castle_pack_4bit(codes):
     """(out, in) codes of 0 to 15, of any integer type and on any device, as `castle_linear_4bit` takes them: eight to an int32 (their order: the C
-    ABI's header), (ceil(out / 16), ceil(in / 256) * 512)."""
-    if codes.dim() != 2 or codes.is_floating_point() or codes.dtype == torch.bool:
+    ABI's header), (ceil(out / 16), ceil(in / 256) * 512).  Other codes are refused (to signed ones, -8 to 7, add 8)."""
+    if codes.dim() != 2 or codes.is_floating_point() or codes.is_complex() or codes.dtype == torch.bool:
         raise ValueError("castle_pack_4bit: (out, in) integer codes expected")
+    if codes.numel():
+        low, high = (int(v) for v in codes.aminmax())
+        if low < 0 or high > 15:
+            raise ValueError(f"castle_pack_4bit: codes from {low} to {high}, where 0 to 15 are expected")
     n, k = codes.shape
     tiles, blocks = (n + 15) // 16, (k + 255) // 256 * 2                               # (of 128 k)
     padded = torch.full((tiles * 16, blocks * 128), 8, dtype=torch.int32, device=codes.device)
-    padded[:n, :k] = codes & 15
+    padded[:n, :k] = codes
     padded = padded.view(tiles, 2, 8, blocks, 4, 4, 8)                              # half, row; block, 32 k, 8 k of these, k
     word = torch.zeros((tiles, 2, 8, blocks, 4, 4), dtype=torch.int32, device=codes.device)
     for i in range(8):

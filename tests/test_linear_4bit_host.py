@@ -101,3 +101,19 @@ def test_refusals_of_the_host():
                 lambda: castle_quantize_4bit(torch.zeros(4, 4), 40)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_codes_of_more_or_other_bits_are_refused(dtype):
+    """Signed codes, or ones of five bits, are not wrapped into others; the ends of 0 to 15 are taken."""
+    from lookahead_keys_attention_b200 import castle_pack_4bit
+    codes = torch.tensor([[0, 15], [15, 0], [7, 8]], dtype=dtype)
+    assert torch.equal(_unpack(castle_pack_4bit(codes), 3, 2), codes.long())
+    for bad in ([16, 255, 31] if dtype == torch.uint8 else [16, -1, -8, 127]):
+        wrong = codes.clone()
+        wrong[1, 1] = bad
+        with pytest.raises(ValueError, match="0 to 15"):
+            castle_pack_4bit(wrong)
+    assert castle_pack_4bit(codes[:0]).shape == (0, 512) and castle_pack_4bit(codes[:, :0]).shape == (1, 0)
+    with pytest.raises(ValueError):
+        castle_pack_4bit(codes.to(torch.complex64))
