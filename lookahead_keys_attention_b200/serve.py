@@ -108,9 +108,13 @@ class PagedCache:
         """(pages of qu, kc and vc, pages of U) that no sequence holds."""
         return len(self._kv.free), len(self._u.free)
 
+    def _missing(self, wanted):
+        """How many pages each of `wanted` = [(sequence, positions)] lacks."""
+        return [max(0, -(-n // self.page_size) - len(s.pages)) for s, n in wanted]
+
     def _reserve(self, wanted):
         """Pages for `wanted` = [(sequence, positions)]: all of them, or none and an error.  How many each got."""
-        need = [max(0, -(-n // self.page_size) - len(s.pages)) for s, n in wanted]
+        need = self._missing(wanted)
         if sum(need) > min(len(self._kv.free), len(self._u.free)):
             raise RuntimeError(f"PagedCache: {sum(need)} more pages needed, {len(self._kv.free)} and {len(self._u.free)} (U) are free")
         for (s, _), k in zip(wanted, need):
@@ -296,24 +300,38 @@ class PagedBatch:
     def layer(self, index) -> "PagedLayer":
         return PagedLayer(self, index)
 
-    def advance(self):
+    def advance(self, leave: bool = False):
         """Every sequence has its token in all layers: count it, and have a place for the next.  Where no page is free for one nothing is counted: free a
-        sequence and advance again."""
+        sequence and advance again.  With `leave` every token is counted, one that fills the last free page too, and the sequences that no page is free for leave
+        the batch: they stay the cache's, their rows take no part from then on, and `replace` takes them back once there are pages.  Returns those that left."""
         sequences = self._sequences()
         rows = [i for i, s in enumerate(sequences) if s]
-        grown = self.cache._reserve([(sequences[i], sequences[i].length + 2) for i in rows])
+        stay, left = rows, []
+        if leave:
+            stay, room = [], min(self.cache.free_pages())
+            for i, k in zip(rows, self.cache._missing([(sequences[i], sequences[i].length + 2) for i in rows])):
+                (stay if k <= room else left).append(i)
+                room -= k if k <= room else 0
+        grown = self.cache._reserve([(sequences[i], sequences[i].length + 2) for i in stay])
         for i in rows:
             sequences[i].length += 1
-        grown = [i for i, k in zip(rows, grown) if k]
+        gone = [self.seqs[i] for i in left]
+        for i in left:
+            sequences[i].batch = self.seqs[i] = None
+        grown = [i for i, k in zip(stay, grown) if k]
         if any(len(sequences[i].pages) > self._width for i in grown):
             self._upload()
-            return
+            return gone
         self.lengths += self._taking
         if grown:   # the new pages alone
             at, column, u, kv = self.cache._to_device([grown, [len(sequences[i].pages) - 1 for i in grown], [sequences[i].u_pages[-1] for i in grown],
                                                        [sequences[i].pages[-1] for i in grown]])
             self.u_table[at, column] = u
             self.table[at, column] = kv
+        if left:
+            at = self.cache._to_device(left)
+            self.lengths[at], self._taking[at] = -1, 0
+        return gone
 
 
 class PagedLayer:

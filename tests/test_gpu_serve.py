@@ -448,3 +448,42 @@ def test_a_quantised_model_under_autocast():
             batch.advance()
             assert got.dtype == want.dtype and (got - want).abs().max() <= CLOSE[torch.bfloat16] * want.abs().max()
     check_status()
+
+
+@torch.no_grad()
+def test_sequences_leave_a_full_cache():
+    """A captured token: the row of a sequence that no page is free for takes no part, the other goes on, and the first comes back with all its positions."""
+    from lookahead_keys_attention_b200 import PagedCache, check_status
+    layers = _layers(2, torch.bfloat16, prenorm=True)
+    cache = PagedCache(2, 3, 4, 64, 16)
+    a, b = cache.add(), cache.add()
+    batch, alone, x = cache.batch([a, b], width=2), [[None] * 2, [None] * 2], torch.zeros(2, 1, 256, device="cuda").bfloat16()
+    _paged_token(layers, x, batch)                                       # (not counted: nothing of it stays)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = _paged_token(layers, x, batch)
+
+    def token(rows):
+        x.copy_(torch.randn(2, 1, 256, device="cuda"))
+        graph.replay()
+        for row, who in enumerate(rows):
+            if who is None:
+                assert torch.equal(out[row], x[row])                     # (the layers' outputs are zero)
+            else:
+                want = _token(layers, x[row:row + 1], alone[who])
+                assert (out[row] - want[0]).abs().max() <= CLOSE[torch.bfloat16] * want.abs().max()
+
+    for t in range(16):
+        token([0, 1])
+        assert batch.advance(leave=True) == ([b] if t == 15 else [])
+    for _ in range(4):
+        token([0, None])
+        assert batch.advance(leave=True) == []
+    cache.free(a)
+    batch.replace([None, b])
+    for _ in range(9):
+        token([None, 1])
+        assert batch.advance(leave=True) == []
+    check_status()
+    assert cache.length(b) == 25

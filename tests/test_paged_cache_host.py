@@ -215,6 +215,77 @@ def test_made_in_inference_mode_and_used_outside(plain):
     cache.resize(10)
 
 
+def test_a_token_that_fills_the_last_page_is_counted(plain):
+    """With `leave`: one page of 16 holds 16 positions, and only the sequence that has no place for its next token leaves the batch."""
+    cache = _cache(pages=1)
+    a = cache.add()
+    batch = cache.batch([a])
+    for t in range(16):
+        _step(batch, [t + 1])
+        assert batch.advance(leave=True) == ([a] if t == 15 else [])
+    # a token's value is added to U of every row before it
+    model = {a: ([sum(range(t + 2, 17)) for t in range(16)], list(range(1, 17)))}
+    _check(cache, model)
+    assert cache.length(a) == 16 and batch.seqs == [None] and batch.lengths.tolist() == [-1] and batch.advance(leave=True) == []
+    with pytest.raises(RuntimeError, match="more pages needed"):
+        batch.replace([a])
+    cache.resize(2)
+    batch.replace([a])
+    _step(batch, [100])
+    assert batch.advance() == [] and batch.lengths.tolist() == [17]
+    model[a] = ([u + 100 for u in model[a][0]] + [0], model[a][1] + [100])
+    _check(cache, model)
+
+
+def test_the_others_go_on(plain):
+    """Three sequences, pages for two of them: the third leaves with all its positions and comes back to the pages of one that is freed."""
+    cache = _cache(pages=5)
+    seqs = [cache.add() for _ in range(3)]
+    model = {q: ([], []) for q in seqs}
+    batch = cache.batch(seqs, size=4, width=3)
+    tensors = batch.u_table, batch.table, batch.lengths
+
+    def token(value, gone):
+        who = list(batch.seqs)
+        _step(batch, [value + i for i in range(4)])
+        assert batch.advance(leave=True) == gone
+        for i, q in enumerate(who):
+            if q is not None:
+                u, rows = model[q]
+                model[q] = ([v + value + i for v in u] + [0], rows + [value + i])
+        _check(cache, model)
+        assert batch.lengths.tolist() == [-1 if q is None else len(model[q][0]) for q in batch.seqs]
+
+    for t in range(15):
+        token(t, [])
+    token(15, [seqs[2]])                                                # 16 each; the two free pages are the first two's
+    for t in range(5):
+        token(20 + t, [])
+    cache.free(seqs[0])
+    del model[seqs[0]]
+    batch.replace([seqs[2], seqs[1]])
+    for t in range(12):
+        token(30 + t, [])
+    assert all(a is b for a, b in zip(tensors, (batch.u_table, batch.table, batch.lengths)))
+    assert [cache.length(q) for q in seqs[1:]] == [33, 28]
+
+
+def test_a_sequence_that_leaves_as_another_outgrows_the_tables(plain):
+    cache = _cache(pages=4)
+    a, b = cache.add(), cache.add()
+    z = torch.zeros(1, 1, 31, 16, dtype=torch.float64)
+    cache.write([a], 0, (z, z, z, z))
+    z = z[:, :, :15]
+    cache.write([b], 0, (z, z, z, z))
+    batch = cache.batch([a, b])
+    assert batch.table.shape == (2, 2) and cache.free_pages() == (1, 1)
+    assert batch.advance(leave=True) == [b]
+    assert batch.table.shape == (2, 3) and batch.lengths.tolist() == [32, -1] and batch.table[1].tolist() == [-1] * 3
+    assert cache.length(a) == 32 and cache.length(b) == 16 and cache.batch([None], width=1).seqs == [None]
+    cache.free(a)
+    assert cache.batch([b]).lengths.tolist() == [16]
+
+
 def test_under_another_default_device(plain):
     """Lists on their way to the cache's device begin on the host, whatever the default device is ("meta": one without values, which cannot be copied from)."""
     cache = _cache()
