@@ -204,7 +204,12 @@ class PagedCache:
             q = self.add()
             self._sequences[q] = _Sequence(s.length, s.pages[:full] + tail, u)
             new.append(q)
-        self._copy(kv_copies, u_copies)
+        try:
+            self._copy(kv_copies, u_copies)
+        except BaseException:
+            for q in new:
+                self.free(q)
+            raise
         return new
 
     def _copy(self, kv, u):

@@ -195,6 +195,22 @@ def test_a_prompt_that_was_not_written_is_not_counted(plain, monkeypatch):
     assert cache.free_pages() == (40, 40)
 
 
+def test_a_fork_that_was_not_copied_keeps_no_pages(plain, monkeypatch):
+    cache = _cache()
+    a = cache.add()
+    z = torch.zeros(1, 1, 40, 16, dtype=torch.float64)
+    cache.write([a], 0, (z, z, z, z))
+    before = cache.free_pages(), list(cache._kv.held), list(cache._u.held), list(cache._sequences)
+    with monkeypatch.context() as m:
+        def refuse(*_):
+            raise RuntimeError("refused")
+        m.setattr(ops, "castle_copy_pages", refuse)
+        with pytest.raises(RuntimeError, match="refused"):
+            cache.fork(a, 3)
+    assert before == (cache.free_pages(), cache._kv.held, cache._u.held, list(cache._sequences))
+    assert len(cache.fork(a, 3)) == 3
+
+
 def test_made_in_inference_mode_and_used_outside(plain):
     with torch.inference_mode():
         cache = _cache()
