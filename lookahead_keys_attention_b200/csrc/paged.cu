@@ -328,58 +328,57 @@ __global__ void __launch_bounds__(kPagedThreads + 32, kPagedCtas) castle_paged_s
   int count = 0, segments = 0;                                                 // stages and segments so far
   if (warp == kPagedWarps) {
     const int which = lane & 3, nth = lane >> 2, page_size = 1 << p.page_shift;
-    {
-      for (int at = begin; at < end;) {
-        const PagedSegment s = paged_segment<ROWS>(p, start, lengths, at, end);
-        at = s.next;
-        if (s.tiles == 0) continue;
-        const int32_t* table = which == 1 ? p.u_table + s.b * p.u_table_stride : p.table + s.b * p.table_stride;
-        const castle_pages_t pool = which == 0 ? p.quc : which == 1 ? p.U : which == 2 ? p.kcc : p.vcc;
-        const int r_end = min(s.length, (s.tile0 + s.tiles) * ROWS);
-        auto look_up = [&](int r0) {                                           // the page of this lane's copy, of the tile that begins with row r0
-          const int r = r0 + nth * page_size;
-          return r < min(r_end, r0 + ROWS) ? __ldg(table + (r >> p.page_shift)) : -1;
-        };
-        int page = look_up(s.tile0 * ROWS);
-        const int last = __ldg(table + (s.length >> p.page_shift)), slot = segments & 1;   // (the new rows need not wait for the pages)
-        if (segments >= 2) mbar_wait(&new_empty[slot], (uint32_t)((segments >> 1) - 1) & 1, abortp);
-        {
-          const castle_tensor_t t = lane == 0 ? p.qc : lane == 1 ? p.ku : lane == 2 ? p.vu : lane == 3 ? p.kc : lane == 4 ? p.vc : p.qu;
-          const bool over = __any_sync(0xffffffffu, *abortp != 0);
-          if (lane == 0) mbar_expect_tx(&new_full[slot], over ? 0 : 6 * ROWB);
-          __syncwarp();
-          if (lane < 6 && !over) bulk_g2s(smem + kPagedStages * 4 * TENB + (slot * 6 + lane) * ROWB, new_row<T>(t, s.b, s.h), ROWB, &new_full[slot]);
-        }
-        for (int r0 = s.tile0 * ROWS; r0 < r_end; r0 += ROWS, ++count) {
-          const int st = count % kPagedStages, next = look_up(r0 + ROWS);
-          if (count >= kPagedStages) mbar_wait(&empty[st], (uint32_t)(count / kPagedStages - 1) & 1, abortp);
-          const int r = r0 + nth * page_size, rows = min(min(page_size, ROWS), r_end - r);   // of this lane's copy
-          const bool mine = nth * page_size < ROWS && rows > 0;
-          const bool good = (uint32_t)page < (uint32_t)(which == 1 ? p.u_pages : p.pages);
-          const uint32_t all = __ballot_sync(0xffffffffu, good);
-          const bool over = __any_sync(0xffffffffu, *abortp != 0);              // after which nothing is fetched, and the stage's rows are not there
-          const bool copy = mine && (all >> (lane & ~3) & 15u) == 15u && !over;
-          const uint32_t bytes = copy ? rows * ROWB : 0, sum = __reduce_add_sync(0xffffffffu, bytes);
-          T* rows_at = page_row<T>(pool, copy ? page : 0, s.h, r & (page_size - 1), D);
-          if (mine && which == 1) s_u[st][nth] = copy ? rows_at : nullptr;
-          __syncwarp();
-          if (lane == 0) mbar_expect_tx(&full[st], sum);
-          __syncwarp();
-          if (copy) bulk_g2s(smem + st * 4 * TENB + which * TENB + nth * page_size * ROWB, rows_at, bytes, &full[st]);
-          page = next;
-        }
-        const uint32_t good = __ballot_sync(0xffffffffu, (uint32_t)last < (uint32_t)(which == 1 ? p.u_pages : p.pages));
-        if (lane < 4) s_new[slot][lane] = (good & 15u) == 15u ? page_row<T>(pool, last, s.h, s.length & (page_size - 1), D) : nullptr;
+    bool over = false;   // a wait of this CTA ran out: what was waited for has not ended, so nothing more is fetched and no barrier is arrived at again
+    for (int at = begin; at < end && !over;) {
+      const PagedSegment s = paged_segment<ROWS>(p, start, lengths, at, end);
+      at = s.next;
+      if (s.tiles == 0) continue;
+      const int32_t* table = which == 1 ? p.u_table + s.b * p.u_table_stride : p.table + s.b * p.table_stride;
+      const castle_pages_t pool = which == 0 ? p.quc : which == 1 ? p.U : which == 2 ? p.kcc : p.vcc;
+      const int r_end = min(s.length, (s.tile0 + s.tiles) * ROWS);
+      auto look_up = [&](int r0) {                                           // the page of this lane's copy, of the tile that begins with row r0
+        const int r = r0 + nth * page_size;
+        return r < min(r_end, r0 + ROWS) ? __ldg(table + (r >> p.page_shift)) : -1;
+      };
+      int page = look_up(s.tile0 * ROWS);
+      const int last = __ldg(table + (s.length >> p.page_shift)), slot = segments & 1;   // (the new rows need not wait for the pages)
+      if (segments >= 2) mbar_wait(&new_empty[slot], (uint32_t)((segments >> 1) - 1) & 1, abortp);
+      if ((over = __any_sync(0xffffffffu, *abortp != 0))) break;
+      {
+        const castle_tensor_t t = lane == 0 ? p.qc : lane == 1 ? p.ku : lane == 2 ? p.vu : lane == 3 ? p.kc : lane == 4 ? p.vc : p.qu;
+        if (lane == 0) mbar_expect_tx(&new_full[slot], 6 * ROWB);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&new_place[slot]);
+        if (lane < 6) bulk_g2s(smem + kPagedStages * 4 * TENB + (slot * 6 + lane) * ROWB, new_row<T>(t, s.b, s.h), ROWB, &new_full[slot]);
         ++segments;
       }
+      for (int r0 = s.tile0 * ROWS; r0 < r_end; r0 += ROWS, ++count) {
+        const int st = count % kPagedStages, next = look_up(r0 + ROWS);
+        if (count >= kPagedStages) mbar_wait(&empty[st], (uint32_t)(count / kPagedStages - 1) & 1, abortp);
+        if ((over = __any_sync(0xffffffffu, *abortp != 0))) break;
+        const int r = r0 + nth * page_size, rows = min(min(page_size, ROWS), r_end - r);   // of this lane's copy
+        const bool mine = nth * page_size < ROWS && rows > 0;
+        const bool good = (uint32_t)page < (uint32_t)(which == 1 ? p.u_pages : p.pages);
+        const uint32_t all = __ballot_sync(0xffffffffu, good);
+        const bool copy = mine && (all >> (lane & ~3) & 15u) == 15u;
+        const uint32_t bytes = copy ? rows * ROWB : 0, sum = __reduce_add_sync(0xffffffffu, bytes);
+        T* rows_at = page_row<T>(pool, copy ? page : 0, s.h, r & (page_size - 1), D);
+        if (mine && which == 1) s_u[st][nth] = copy ? rows_at : nullptr;
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(&full[st], sum);
+        __syncwarp();
+        if (copy) bulk_g2s(smem + st * 4 * TENB + which * TENB + nth * page_size * ROWB, rows_at, bytes, &full[st]);
+        page = next;
+      }
+      if (over) break;
+      const uint32_t good = __ballot_sync(0xffffffffu, (uint32_t)last < (uint32_t)(which == 1 ? p.u_pages : p.pages));
+      if (lane < 4) s_new[slot][lane] = (good & 15u) == 15u ? page_row<T>(pool, last, s.h, s.length & (page_size - 1), D) : nullptr;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&new_place[slot]);
     }
     paged_outside<T, D>(p, lengths);
-    if (*abortp) {   // nobody may have waited for the last copies
-      for (int i = max(0, count - kPagedStages); i < count; ++i) mbar_drain(&full[i % kPagedStages], (uint32_t)(i / kPagedStages) & 1);
-      for (int i = max(0, segments - 2); i < segments; ++i) mbar_drain(&new_full[i & 1], (uint32_t)(i >> 1) & 1);
-    }
+    // Its own last copies have ended when it leaves, whoever else waited for them or gave up.
+    for (int i = max(0, count - kPagedStages); i < count; ++i) mbar_drain(&full[i % kPagedStages], (uint32_t)(i / kPagedStages) & 1);
+    for (int i = max(0, segments - 2); i < segments; ++i) mbar_drain(&new_full[i & 1], (uint32_t)(i >> 1) & 1);
     return;
   }
   const int sub = lane % LPR, grp = lane / LPR, col = sub * VEC, mask = (1 << p.page_shift) - 1, row = warp * RPW + grp;
