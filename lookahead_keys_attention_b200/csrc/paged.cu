@@ -383,6 +383,7 @@ __global__ void __launch_bounds__(kPagedThreads + 32, kPagedCtas) castle_paged_s
   }
   const int sub = lane % LPR, grp = lane / LPR, col = sub * VEC, mask = (1 << p.page_shift) - 1, row = warp * RPW + grp;
   const bool odd = lane & 1;
+  bool there = true;   // until a wait of this warp has run out: its later ones would see the phases of others, so that it makes none and stores nothing any more
   {
     for (int at = begin; at < end;) {
       const PagedSegment s = paged_segment<ROWS>(p, start, lengths, at, end);
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(kPagedThreads + 32, kPagedCtas) castle_paged_s
       if (s.tiles == 0) continue;
       const int slot = segments & 1;
       const uint32_t turn = (uint32_t)(segments++ >> 1) & 1;
-      const bool there = !mbar_wait_failed(&new_full[slot], turn, abortp);
+      there = there && !mbar_wait_failed(&new_full[slot], turn, abortp);
       const T* rows = reinterpret_cast<const T*>(smem + kPagedStages * 4 * TENB + slot * 6 * ROWB) + col;
       RotaryParams rot = p.rot;
       rot.position0 = (float)s.length;
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(kPagedThreads + 32, kPagedCtas) castle_paged_s
       for (int r0 = s.tile0 * ROWS; r0 < r_end; r0 += ROWS, ++count) {
         const int st = count % kPagedStages;
         // A wait that ran out means that the stage never arrived: U is persistent state, so nothing computed from it may be stored.
-        const bool arrived = there && !mbar_wait_failed(&full[st], (uint32_t)(count / kPagedStages) & 1, abortp);
+        there = there && !mbar_wait_failed(&full[st], (uint32_t)(count / kPagedStages) & 1, abortp);
         // A thread has two rows, side by side: each is a chain of dot products, shuffles and exponentials, which is the time where few warps are
         // resident.  The lanes of a row share them out: even ones sum up the first row's products and work out its gate, odd ones the second's.
         const T* src = reinterpret_cast<const T*>(smem + st * 4 * TENB) + row * D + col;
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(kPagedThreads + 32, kPagedCtas) castle_paged_s
         for (int k = 0; k < 2; ++k) {
           const int in = row + k * HALF;   // row of the tile
           u[k] = nullptr;
-          if (arrived && in < r_end - r0) {
+          if (there && in < r_end - r0) {
             u[k] = s_u[st][in >> p.page_shift];
             bad |= u[k] == nullptr;
             if (u[k]) u[k] += (in & mask) * D + col;
@@ -475,9 +476,9 @@ __global__ void __launch_bounds__(kPagedThreads + 32, kPagedCtas) castle_paged_s
         Vec<T>::load(rows + 4 * D, vn);
         Vec<T>::load(rows + 5 * D, qn);
         rotate_new<T>(rot, col, kn, qn, nullptr);
-        const bool placed = there && !mbar_wait_failed(&new_place[slot], turn, abortp);
-        bad |= placed && s_new[slot][0] == nullptr;
-        if (grp == 0 && placed && s_new[slot][0] && *abortp == 0) {   // a step that ran out of time leaves the caches as they were
+        there = there && !mbar_wait_failed(&new_place[slot], turn, abortp);
+        bad |= there && s_new[slot][0] == nullptr;
+        if (grp == 0 && there && s_new[slot][0] && *abortp == 0) {   // a step that ran out of time leaves the caches as they were
           Vec<T>::store(s_new[slot][0] + col, qn);
           *reinterpret_cast<uint4*>(s_new[slot][1] + col) = make_uint4(0, 0, 0, 0);
           Vec<T>::store(s_new[slot][2] + col, kn);

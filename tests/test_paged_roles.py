@@ -1,6 +1,6 @@
 """CPU: the roles of the paged step's CTA (csrc/paged.cu) around its barriers where waits run out: the warp that copies and the four that work, in any order, with
-copies that take any time.  A barrier takes as many arrivals a phase as it was made for and no more, nobody waits for good, and
-none of the CTA's copies is on its way when its last warp has left."""
+copies that take any time.  A barrier takes as many arrivals a phase as it was made for and no more, what is read has arrived and is not written meanwhile, nobody waits for
+good, and none of the CTA's copies is on its way when its last warp has left."""
 import random
 import re
 
@@ -37,13 +37,18 @@ class Barrier:
 
 class Cta:
     """`patience`: polls after which a wait of the working warps runs out; `former`: the copying warp goes on arriving after that, and waits for its copies only if
-    it has seen it."""
+    it has seen it; `forgets`: a working warp waits again after one of its waits ran out."""
 
-    def __init__(self, rng, patience, former=False):
-        self.rng, self.patience, self.former, self.abort, self.flight = rng, patience, former, False, []
+    def __init__(self, rng, patience, former=False, forgets=False):
+        self.rng, self.patience, self.former, self.forgets, self.abort, self.flight = rng, patience, former, forgets, False, []
         self.full, self.empty = [Barrier(1) for _ in range(STAGES)], [Barrier(WARPS) for _ in range(STAGES)]
         self.new_full, self.new_place, self.new_empty = [Barrier(1) for _ in range(2)], [Barrier(1) for _ in range(2)], [Barrier(WARPS) for _ in range(2)]
         self.segments = [(rng.randint(0, 5), rng.random() < 0.5) for _ in range(rng.randint(1, 6))]   # tiles with rows; whether the pair ends with it
+        self.content, self.reading = [None] * STAGES, [0] * STAGES
+        self.seen = [[] for _ in range(WARPS)]
+
+    def copy(self, bar, stage=None, what=None):
+        self.flight.append((bar, stage, what))
 
     def wait(self, bar, parity, patience):
         """What the wait's caller is told: whether the phase ended."""
@@ -70,7 +75,7 @@ class Cta:
                 break
             self.new_full[slot].arrive(0 if over else 1)
             if not over:
-                self.flight.append(self.new_full[slot])
+                self.copy(self.new_full[slot])
             if not self.former:
                 segments += 1
             yield
@@ -82,9 +87,12 @@ class Cta:
                 if over and not self.former:
                     break
                 yield
+                if not over:
+                    assert self.reading[st] == 0, "a stage is written while it is read"
+                    self.content[st] = None
                 self.full[st].arrive(0 if over else 1)
                 if not over:
-                    self.flight.append(self.full[st])
+                    self.copy(self.full[st], st, count)
                 count += 1
                 yield
             if over and not self.former:
@@ -101,20 +109,29 @@ class Cta:
 
     def works(self, warp):
         segments = count = 0
+        there = True
         for tiles, ends in self.segments:
             slot, turn = segments & 1, (segments >> 1) & 1
             segments += 1
-            there = yield from self.wait(self.new_full[slot], turn, self.patience)
-            for tile in range(tiles):
+            there = (there or self.forgets) and (yield from self.wait(self.new_full[slot], turn, self.patience))
+            whole = there
+            for _ in range(tiles):
                 st = count % STAGES
-                if there:
-                    yield from self.wait(self.full[st], (count // STAGES) & 1, self.patience)
+                arrived = there and (yield from self.wait(self.full[st], (count // STAGES) & 1, self.patience))
+                there = arrived or (there and self.forgets)
+                whole = whole and arrived
+                if arrived:
+                    assert self.content[st] == count, "what is read has not arrived"
+                    self.reading[st] += 1
+                    yield
+                    self.reading[st] -= 1
                 self.empty[st].arrive()
                 count += 1
                 yield
             if ends and warp == 0 and there:
-                yield from self.wait(self.new_place[slot], turn, self.patience)
+                there = whole = whole and (yield from self.wait(self.new_place[slot], turn, self.patience))
             self.new_empty[slot].arrive()
+            self.seen[warp].append((whole, there))
             yield
 
     def run(self):
@@ -124,7 +141,10 @@ class Cta:
             steps += 1
             assert steps < 100000, "a wait without an end"
             if self.flight and self.rng.random() < slow:
-                self.flight.pop(self.rng.randrange(len(self.flight))).landed()
+                bar, stage, what = self.flight.pop(self.rng.randrange(len(self.flight)))
+                if stage is not None:
+                    self.content[stage] = what
+                bar.landed()
             role = self.rng.choice(roles)
             for _ in range(self.rng.randint(1, 6)):
                 try:
@@ -139,7 +159,7 @@ def test_without_one_that_runs_out():
     for seed in range(300):
         cta = Cta(random.Random(seed), 10 ** 9)
         cta.run()
-        assert not cta.abort
+        assert not cta.abort and all(all(whole for whole, _ in seen) for seen in cta.seen)
 
 
 def test_where_waits_run_out():
@@ -149,6 +169,8 @@ def test_where_waits_run_out():
         cta = Cta(rng, rng.choice([0, 1, 3, 10, 30, 100]))
         cta.run()
         aborted += cta.abort
+        # a warp that has not got all of a segment's rows knows it at the segment's end
+        assert all(whole or not there for seen in cta.seen for whole, there in seen)
     assert aborted > 500
 
 
@@ -163,6 +185,17 @@ def test_arrivals_after_it_would_be_more_than_a_phase_takes_and_copies_outlive_t
     assert found >= {"an arrival that the phase has no place for", "the CTA has left while its copies are on their way"}
 
 
+def test_a_warp_that_forgets_would_read_what_has_not_arrived():
+    found = set()
+    for seed in range(1500):
+        rng = random.Random(seed)
+        try:
+            Cta(rng, rng.choice([0, 1, 3, 10, 30, 100]), forgets=True).run()
+        except AssertionError as e:
+            found.add(str(e).splitlines()[0])
+    assert found == {"what is read has not arrived"}
+
+
 def test_the_source_plays_these_roles():
     """The copying warp looks at the flag behind each wait and leaves its loops, and its last waits are made in any case."""
     start = SOURCE.index("castle_paged_step_kernel(const")
@@ -173,3 +206,6 @@ def test_the_source_plays_these_roles():
     assert re.search(r"if \(over\) break;[^}]*mbar_arrive\(&new_place", body)
     end = body[body.index("paged_outside<T, D>(p, lengths);"):]
     assert end.count("mbar_drain(") == 2 and "abortp" not in end
+    works = SOURCE[SOURCE.index("const int sub = lane % LPR", start):]
+    waits = re.findall(r"(.*)mbar_wait_failed\(", works)
+    assert len(waits) == 3 and all(w.strip() == "there = there && !" for w in waits)
