@@ -334,7 +334,9 @@ typedef struct {
 
 /* castle_decode_step_fused() for `batch` (at most 4096) sequences of lengths[b] positions each: row lengths[b] is appended, so its
  * page has to be in the tables.  A length below zero: no sequence, its row of `out` is zero.  A length without places in the
- * tables, or a page outside its pool: `out` is NaN, nothing is written for those rows, CASTLE_STATUS_BAD_INDEX is set.
+ * tables, or a page outside its pool: `out` is NaN, nothing is written for those rows, CASTLE_STATUS_BAD_INDEX is set.  Where a bounded wait ran out
+ * (CASTLE_STATUS_WAIT_TIMEOUT), `out` is NaN for the (sequence, head) pairs that missed rows by it, and U of those that had arrived is rewritten: the caches of such
+ * a sequence are void.
  * rotary->position0 is ignored (the new row's position is its length).  counters: batch * heads words that are zero
  * before the call and zero again when its kernel has run.  The result does not depend on how the work was shared out.
  */

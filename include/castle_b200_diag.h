@@ -58,6 +58,10 @@ int castle_selftest_wait_timeout(int32_t poll_limit, int32_t* polls, int32_t* st
  * all the same and the kernel ends.  result[0] receives whether the tile came, result[1] the events taken (device int32[2]). */
 int castle_selftest_event_timeout(int32_t poll_limit, int32_t rounds, int32_t form, int32_t* result, int32_t* status, void* stream);
 
+/* The failure path of the paged step itself (no counterpart in the reference): its waits for rows in later calls of this host thread give up after `limit` (0 .. 65536)
+ * polls; -1: after as many as ever.  What it misses by that is NaN and CASTLE_STATUS_WAIT_TIMEOUT; its copies end before the kernel does. */
+int castle_selftest_paged_polls(int32_t limit);
+
 /* y[i] = 2^x[i] for `count` (even, at most 2^26) values as the score passes at dim_head 64 compute a part of their
  * exponentials, without the special-function unit (no counterpart in the reference). */
 int castle_selftest_exp2(const float* x, float* y, int32_t count, void* stream);

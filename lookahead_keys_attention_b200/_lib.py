@@ -225,6 +225,7 @@ _SIGNATURES = {
     "castle_selftest_mma": (ctypes.c_int, [_i32, _vp, _vp, _vp, _vp, _vp]),
     "castle_selftest_wait_timeout": (ctypes.c_int, [_i32, _vp, _vp, _vp]),
     "castle_selftest_event_timeout": (ctypes.c_int, [_i32, _i32, _i32, _vp, _vp, _vp]),
+    "castle_selftest_paged_polls": (ctypes.c_int, [_i32]),
     "castle_selftest_exp2": (ctypes.c_int, [_vp, _vp, _i32, _vp]),
 }
 

@@ -43,6 +43,7 @@ struct PagedParams {
   float* part;                      // [2 per piece][4 + D]: D sums, the maximum, the sum of the weights
   uint32_t* counters;               // [B * H], zero
   int32_t* status;
+  uint32_t row_polls;               // of a wait for rows, see castle_selftest_paged_polls
 };
 
 // Where a pair's rows lie and what a piece has of them.
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(kPagedThreads + 32, kPagedCtas) castle_paged_s
       for (int r0 = s.tile0 * ROWS; r0 < r_end; r0 += ROWS, ++count) {
         const int st = count % kPagedStages;
         // A wait that ran out means that the stage never arrived: U is persistent state, so nothing computed from it may be stored.
-        there = there && !mbar_wait_failed(&full[st], (uint32_t)(count / kPagedStages) & 1, abortp);
+        there = there && !mbar_wait_failed(&full[st], (uint32_t)(count / kPagedStages) & 1, abortp, p.row_polls);
         // A thread has two rows, side by side: each is a chain of dot products, shuffles and exponentials, which is the time where few warps are
         // resident.  The lanes of a row share them out: even ones sum up the first row's products and work out its gate, odd ones the second's.
         const T* src = reinterpret_cast<const T*>(smem + st * 4 * TENB) + row * D + col;
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(kPagedThreads + 32, kPagedCtas) castle_paged_s
         rotate_new<T>(rot, col, kn, qn, nullptr);
         there = there && !mbar_wait_failed(&new_place[slot], turn, abortp);
         bad |= there && s_new[slot][0] == nullptr;
-        if (grp == 0 && there && s_new[slot][0] && *abortp == 0) {   // a step that ran out of time leaves the caches as they were
+        if (grp == 0 && there && s_new[slot][0]) {   // (rows that arrived before a wait that ran out are rewritten and this one is not: such a sequence's caches are void)
           Vec<T>::store(s_new[slot][0] + col, qn);
           *reinterpret_cast<uint4*>(s_new[slot][1] + col) = make_uint4(0, 0, 0, 0);
           Vec<T>::store(s_new[slot][2] + col, kn);
@@ -498,15 +499,15 @@ __global__ void __launch_bounds__(kPagedThreads + 32, kPagedCtas) castle_paged_s
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&new_empty[slot]);
-      if (bad) {
-        x.l = __int_as_float(0x7fc00000);
-        if (*abortp == 0) atomicOr(p.status, CASTLE_STATUS_BAD_INDEX);
-      }
+      if (bad || !there) x.l = __int_as_float(0x7fc00000);   // (a mean of some of the rows would look like a result)
+      if (bad) atomicOr(p.status, CASTLE_STATUS_BAD_INDEX);
       paged_finish<T, D>(p, plan, s, piece, x);
     }
   }
   if (threadIdx.x == 0 && abort_flag) atomicOr(p.status, CASTLE_STATUS_WAIT_TIMEOUT);
 }
+
+static thread_local uint32_t paged_row_polls = kWaitPollLimit;   // (for the tests)
 
 template <typename T, int D> static int launch_paged(const PagedParams& p, cudaStream_t st) {
   constexpr size_t fixed = kPagedStages * 4 * kPagedTensor<T, D> + 2 * 6 * D * sizeof(T);
@@ -540,7 +541,6 @@ static int64_t paged_most_units(const castle_problem_t* p, int32_t page_size, in
   const int64_t each = (capacity + rows - 1) / rows + kPagedPair;
   return each > INT32_MAX / pairs ? -1 : each * pairs;
 }
-
 
 }  // namespace castle
 
@@ -596,11 +596,17 @@ extern "C" int castle_paged_decode_step(const castle_problem_t* p, int32_t page_
     if (rotary->dtype < CASTLE_BF16 || rotary->dtype > CASTLE_F32) return reject("%s: unknown rotary dtype", who);
     q.rot = RotaryParams{rotary->freqs, rotary->dtype, rotary->inverse, 0.f};
   }
-  q.part = (float*)workspace; q.counters = counters; q.status = status;
+  q.part = (float*)workspace; q.counters = counters; q.status = status; q.row_polls = paged_row_polls;
   const cudaStream_t st = (cudaStream_t)stream;
   switch (p->dtype) {
     case CASTLE_BF16: return launch_paged_d<__nv_bfloat16>(q, p->dim_head, st);
     case CASTLE_F16: return launch_paged_d<__half>(q, p->dim_head, st);
     default: return launch_paged_d<float>(q, p->dim_head, st);
   }
+}
+
+extern "C" int castle_selftest_paged_polls(int32_t limit) {
+  if (limit < -1 || limit > 65536) return reject("castle_selftest_paged_polls: -1 or 0..65536 polls expected");
+  paged_row_polls = limit < 0 ? kWaitPollLimit : (uint32_t)limit;
+  return 0;
 }

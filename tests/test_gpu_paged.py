@@ -211,6 +211,45 @@ def test_values_that_are_not_finite_stay_in_their_sequence():
     assert bool(out[2].isfinite().all())
 
 
+@pytest.mark.parametrize("limit", [0, 1, 2, 5, 20, 100])
+def test_rows_that_do_not_arrive_in_time(limit):
+    """Waits for rows that give up after some polls: every pair has its whole result or NaN, the status says so, rows that did not arrive stay as they were, and the next
+    step is right."""
+    from lookahead_keys_attention_b200 import _lib, check_status
+    lib = _lib.load()
+    shape = torch.bfloat16, [900, 0, 40, 2500, 333], 4, 64, 32
+    c, good = Case(*shape, seed=13), Case(*shape, seed=13)
+    before = [p.clone() for p in c.pools]
+    want = good.step()
+    check_status()
+    _lib.check(lib.castle_selftest_paged_polls(limit), "paged_polls")
+    try:
+        out = c.step()
+    finally:
+        _lib.check(lib.castle_selftest_paged_polls(-1), "paged_polls")
+    lost = out.isnan().flatten(2)
+    assert bool((lost.all(-1) == lost.any(-1)).all()) and torch.equal(out[~lost.any(-1)], want[~lost.any(-1)])
+    if bool(lost.any()):
+        with pytest.raises(RuntimeError, match="status 1"):
+            check_status()
+    if limit == 0:                                                       # none arrives
+        rows = [0, 2, 3, 4]
+        assert bool(lost[rows].all())
+        spare = c.u_table[1, 0].long(), c.table[1, 0].long()
+        for i, (p, q) in enumerate(zip(c.pools, before)):
+            keep = torch.ones(len(p), dtype=torch.bool, device="cuda")
+            keep[spare[min(i, 1)]] = False
+            assert torch.equal(p[keep], q[keep])
+    for p, q, w in zip(c.pools, before, good.pools):                     # a row is the one before or the one of the whole step
+        assert bool(((p == q) | (p == w)).all())
+        p.copy_(q)
+    for _ in range(2):
+        assert torch.equal(c.step(), want) and all(torch.equal(p, q) for p, q in zip(c.pools, good.pools))
+        for p, q in zip(c.pools, before):
+            p.copy_(q)
+    check_status()
+
+
 def test_places_beyond_32_bits():
     """Pools of more than 2^31 elements, pages at their ends."""
     from lookahead_keys_attention_b200 import castle_paged_decode_step, check_status

@@ -119,3 +119,10 @@ def test_cpu_tensors_are_refused():
         castle_write_pages(*[rows] * 4, *[pool] * 4, table, table, table[:, 0])
     with pytest.raises(RuntimeError, match="no CPU path"):
         castle_copy_pages(pool, [0], [1])
+
+
+def test_polls_of_the_self_test():
+    L, lib = _lib()
+    for bad in (-2, 65537):
+        assert lib.castle_selftest_paged_polls(bad) < 0 and "castle_selftest_paged_polls" in L.last_error()
+    assert lib.castle_selftest_paged_polls(0) == 0 and lib.castle_selftest_paged_polls(-1) == 0
