@@ -94,7 +94,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
   const uint32_t tmem = tmem_base_s, weights = tmem + (p.stages == 3 ? 256 : 128);   // columns from 0 on: the results; from `weights` on: the stages of the weights
   if (warp == kTileWarps) {
     if (elect_one()) {
-      for (int c = 0, s = 0, turn = 0; c < chunks; ++c) {
+      int c = 0;
+      for (int s = 0, turn = 0; c < chunks; ++c) {
         if (turn > 0) mbar_wait(&free_[s], (uint32_t)(turn - 1) & 1, abortp);
         if (*abortp) break;
         mbar_expect_tx(&full[s], 2 * panel);
@@ -103,9 +104,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
         tma_load_4d(x + panel, &m_x, &full[s], (first + c) * 128 + 64, r0, 0, 0);
         if (++s == p.stages) { s = 0; ++turn; }
       }
-      // (after an abort: what is on its way arrives before the CTA leaves; the weights' arrivals are made in any case)
-      if (*abortp)
-        for (int i = 0; i < p.stages; ++i) { mbar_drain(&full[i], 0); mbar_drain(&full[i], 1); }
+      // What is on its way arrives before this thread leaves, whoever else waits for it or gave up.  (Where a wait ran out the weights of a stage may be missing, and
+      // these end with their polls.)
+      for (int i = max(0, c - p.stages); i < c; ++i) mbar_drain(&full[i % p.stages], (uint32_t)(i / p.stages) & 1);
     }
   } else if (warp == kTileWarps + 1) {
     if (elect_one()) {
@@ -169,8 +170,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) castle_linear_4bit_tile_kerne
         if constexpr (ZEROS) { zero8 = next_zero8; next_zero8 = load8(zeros, window + 1); }
       }
       fetch(c + kTileGroups);
-      if (turn > 0) mbar_wait(&free_[s], (uint32_t)(turn - 1) & 1, abortp);
-      __syncwarp();
+      // (a wait that ran out: the stage may be in use, and its barrier takes no second arrival in a phase)
+      if (turn > 0 && mbar_wait_failed(&free_[s], (uint32_t)(turn - 1) & 1, abortp)) break;
       tc_fence_after();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {   // 32 k, 16 columns
