@@ -338,7 +338,8 @@ typedef struct {
  * (CASTLE_STATUS_WAIT_TIMEOUT), `out` is NaN for the (sequence, head) pairs that missed rows by it, and U of those that had arrived is rewritten: the caches of such
  * a sequence are void.
  * rotary->position0 is ignored (the new row's position is its length).  counters: batch * heads words that are zero
- * before the call and zero again when its kernel has run.  The result does not depend on how the work was shared out.
+ * before the call and zero again when its kernel has run.  The same call gives the same bits; the other sequences' lengths move the places where a pair is cut, and
+ * with them the last places of its result (not of U).
  */
 size_t castle_paged_decode_workspace_bytes(const castle_problem_t* p, int32_t page_size, int32_t table_width);
 int castle_paged_decode_step(const castle_problem_t* p, int32_t page_size, int32_t u_pages, int32_t pages, const castle_tensor_t* qc_new,

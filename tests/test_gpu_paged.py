@@ -168,6 +168,29 @@ def test_same_bits_every_time_and_whatever_the_batch():
         assert torch.equal(c.step(), first) and all(torch.equal(p, q) for p, q in zip(c.pools, after))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_one_sequence_in_different_batches(dtype):
+    """Who else is in the batch decides where a sequence is cut: its result is within the tolerance in each of them, its lookahead keys are the same bits."""
+    from lookahead_keys_attention_b200 import check_status
+    c = Case(dtype, [5000, 12, 900, 4097, 64], 8, 64, 64, seed=14)
+    before, everyone, keys, outs = [p.clone() for p in c.pools], list(c.lengths), [], []
+    for there in ([0, 1, 2, 3, 4], [0], [0, 1], [0, 3], [0, 2, 4]):
+        c.lengths = [n if b in there else -1 for b, n in enumerate(everyone)]
+        c.lens.copy_(torch.tensor(c.lengths, dtype=torch.int32))
+        for p, q in zip(c.pools, before):
+            p.copy_(q)
+        out = c.step()
+        check_status()
+        c.check(before, out)
+        keys.append(c.rows(0, 0, everyone[0], c.pools))
+        outs.append(out[0])
+    assert all(torch.equal(k, keys[0]) for k in keys)
+    # fp32: two results of one sequence are apart by what joining in another order rounds, n + 16 roundings of each, and twice the weights' error, 2^-19 of the largest value
+    largest = c.rows(3, 0, everyone[0] + 1, c.pools).abs().amax().item()
+    if dtype == torch.float32:
+        assert all((o - outs[0]).abs().max().item() <= 2 * (2.0 ** -19 + (everyone[0] + 16) * 2.0 ** -24) * largest for o in outs)
+
+
 @pytest.mark.parametrize("bad", ["u", "kv", "new", "length"])
 def test_places_outside_the_pools(bad):
     """NaN for the sequence, the others as they should be, nothing written outside; then the status, which is clear again after it."""
