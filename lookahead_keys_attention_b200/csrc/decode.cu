@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 4) castle_decode_ring_kernel(c
     rotate_new<T>(p.rot, col, kn, qn, nullptr);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) zero[i] = 0.f;
-    if (grp == 0 && *abortp == 0) {   // a timed-out step leaves the caches as they were
+    if (grp == 0 && *abortp == 0) {   // (after a wait that ran out this row is not appended; U of rows that had arrived is rewritten)
       Vec<T>::store(row_ptr(p.kcc, p.t), kn);
       Vec<T>::store(row_ptr(p.vcc, p.t), vn);
       Vec<T>::store(row_ptr(p.quc, p.t), qn);

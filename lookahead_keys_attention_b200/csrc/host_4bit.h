@@ -83,7 +83,8 @@ bool few_rows(int64_t rows, int64_t K, int64_t N) {
 
 // Rows of 32 bits go through the codes ten at a time, or five where ten are wider than two CTAs' shared memory (us: 10 x 4096 -> 4096 18.9, 5 14.1, 10 x 8136 -> 5307
 // 111, 5 31.3), or through the weights at full width, whose making and products take some 12 + 5.5 for each million of them up to 64 rows (in turns / at full width:
-// 45 x 4096 -> 4096 88 / 121, 64 x 1000 -> 50021 167 / 251, 30 x 8136 -> 5307 180 / 277, 45 x 1024 -> 4096 44 / 29).
+// 45 x 4096 -> 4096 88 / 121, 64 x 1000 -> 50021 167 / 251, 30 x 8136 -> 5307 180 / 277, 45 x 1024 -> 4096 44 / 29).  The latter is a line through few shapes: 45 x 4096 -> 1024
+// take 63 where it says 35, 45 x 8136 -> 5307 309 where it says 250, a little less than nine turns.
 constexpr int64_t kWholeF32 = 4096;
 bool few_rows_f32(int64_t rows, int64_t turns, int64_t K, int64_t N) {
   const double weights = 1e-6 * (double)K * (double)N;

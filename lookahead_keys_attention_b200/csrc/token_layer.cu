@@ -334,7 +334,7 @@ __global__ void __cluster_dims__(kTlCluster, 1, 1) __launch_bounds__(kTlThreads,
       new_row(0, qn);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) zero[i] = 0.f;
-      if (grp == 0 && *abortp == 0) {   // a timed-out step leaves the caches as they were
+      if (grp == 0 && *abortp == 0) {   // (after a wait that ran out this row is not appended; U of rows that had arrived is rewritten)
         Vec<T>::store(row_ptr(p.kcc, p.t) + col, kn);
         Vec<T>::store(row_ptr(p.vcc, p.t) + col, vn);
         Vec<T>::store(row_ptr(p.quc, p.t) + col, qn);
